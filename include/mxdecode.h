@@ -1,7 +1,8 @@
 /*
  * mxdecode - MI355X (gfx950) decode-step hot path: weight-only int8 linear
- * layers, paged-attention decode and the per-layer glue around them (KV append,
- * rotary embedding, residual + RMSNorm, SwiGLU). C ABI of libmxdecode.so.
+ * layers, paged-attention decode over a 16-bit or 8-bit KV cache and the per-layer
+ * glue around them (KV append, rotary embedding, residual + RMSNorm, SwiGLU). C ABI
+ * of libmxdecode.so.
  *
  * Conventions
  *   - fp16 tensors are passed as `uint16_t*` (IEEE binary16 bit patterns).
@@ -23,7 +24,7 @@
 extern "C" {
 #endif
 
-#define MX_ABI_VERSION 20
+#define MX_ABI_VERSION 21
 
 typedef enum mx_status {
     MX_OK = 0,
@@ -544,6 +545,108 @@ int mx_swiglu_interleaved(const uint16_t* gate_up, int64_t gu_stride, const floa
  * reached from worker_server.py:771-775). */
 int mx_silu_mul(const uint16_t* gate_up, int64_t gu_stride, int32_t M, int32_t I, uint16_t* out,
                 int64_t out_stride, void* stream);
+
+/* ----------------------------------------------------------------------------
+ * 8-bit KV cache.
+ *
+ * A layer of the cache is data: uint8 [num_blocks, Hkv, 2, block_size * D] (K,
+ * then V, of a page) and codes: uint8 [num_blocks, Hkv, 2]. A value is
+ * q * 2^(code - 127), q = byte - 128 in [-127, 127]; K bytes are ordered
+ * [D / 64][block_size][64], V bytes [D][block_size]. code is the smallest whose
+ * page keeps |q| <= 127 after rounding to nearest even, within [103, 136] for
+ * fp16 and [1, 248] for bf16 (MX_PA_BF16 in flags), so every value is a number
+ * of the 16-bit type; 255: a value that is not finite was written to the page,
+ * which stands for NaN; 0: nothing was written, the page stands for 0. Fill data
+ * with 128 and codes with 0 at allocation (a byte is never 0 after that).
+ * D in {64, 128}, block_size in {4, 8, 16, 32}; data 16-byte aligned. A page
+ * occurs in at most one row's written range per call.
+ * ------------------------------------------------------------------------- */
+
+/* k_new / v_new [B, Hkv, T, D] (16-bit, strides new_sb, new_sh, new_st, 1:
+ * multiples of 8, 16-byte aligned) quantised at positions start_pos[b] + t. A
+ * write that begins at slot 0 of a page starts the page anew; one that begins
+ * inside a page keeps the tokens before it, whose q are rounded to the page's new
+ * scale when that grows; what stood behind the written tokens is lost. Slots
+ * outside the table or the pool are skipped and set bit 0 of the nullable err
+ * word; used (nullable, uint8 [num_blocks]) gets 1 at every page written. The
+ * 8-bit form of mx_kv_append: GpuKVBlockPool.write_tokens_batch
+ * (runtime/phase2/paged_kv_kernel.py:176-227). */
+int mx_kv8_write(const uint16_t* k_new, const uint16_t* v_new, int64_t new_sb, int64_t new_sh, int64_t new_st,
+                 int32_t B, int32_t T, int32_t Hkv, int32_t D, const int32_t* block_tables, int64_t bt_sb,
+                 int32_t max_blocks, const int32_t* start_pos, uint8_t* data, uint8_t* codes, int32_t block_size,
+                 int32_t num_blocks, int32_t* err, uint8_t* used, uint32_t flags, void* stream);
+
+/* The first S tokens of B rows as k_out and v_out [B, Hkv, S, D] (16-bit,
+ * contiguous), exact; zero past seq_lens[b] (nullable) and where a block is
+ * outside the table or the pool (bit 0 of the nullable err word). The 8-bit form
+ * of mx_kv_gather: GpuKVBlockPool.gather_layer / gather_layer_batch
+ * (runtime/phase2/paged_kv_kernel.py:252-309). */
+int mx_kv8_gather(const uint8_t* data, const uint8_t* codes, const int32_t* block_tables, int64_t bt_sb,
+                  int32_t max_blocks, const int32_t* seq_lens, int32_t B, int32_t S, int32_t Hkv, int32_t D,
+                  int32_t block_size, int32_t num_blocks, uint16_t* k_out, uint16_t* v_out, int32_t* err,
+                  uint32_t flags, void* stream);
+
+/* mx_qkv_rope_append (qkv: 16-bit rows of (Hq + 2 Hkv) * D) or
+ * mx_qkv_rope_append_splits (partials: fp32 [splits][B][(Hq + 2 Hkv) * D], plus
+ * the nullable bias) over the 8-bit cache: q rotated to q_out, k rotated and v
+ * written as by mx_kv8_write with T = 1. Exactly one of qkv and partials is given.
+ * Bit 1 of err: a position outside the rope table (its q are zero, nothing is
+ * written). lens_out (nullable) gets positions + 1. No reference counterpart in
+ * 8 bits; it covers HF's apply_rotary_pos_emb and BlockPagedBatchLayer.update
+ * (runtime/phase2/paged_kv_cache.py:121-157). */
+int mx_kv8_rope_append(const uint16_t* qkv, int64_t qkv_stride, const float* partials, int32_t splits,
+                       const uint16_t* bias, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, const float* rope,
+                       int32_t max_pos, const int32_t* positions, uint16_t* q_out, int64_t q_stride,
+                       const int32_t* block_tables, int64_t bt_sb, int32_t max_blocks, uint8_t* data, uint8_t* codes,
+                       int32_t block_size, int32_t num_blocks, int32_t* err, int32_t* lens_out, uint8_t* used,
+                       uint32_t flags, void* stream);
+
+/* Decode attention over the 8-bit cache: out[b, h] = softmax(scale q[b, h] K^T) V
+ * over the row's min(seq_lens[b], max_blocks * block_size) tokens, K and V the
+ * values of pages block_tables[b] for kv-head h / (Hq / Hkv). q, out: 16-bit
+ * [B, Hq, D] with strides (sb, sh, 1). Empty rows give zeros; a block outside the
+ * pool is skipped and sets bit 2 of the nullable err word; a page that stands for
+ * NaN makes its heads' outputs NaN. Any GQA group. workspace: at least
+ * mx_kv8_attn_workspace_bytes, 256-byte aligned, not shared by calls that overlap
+ * (its contents need not be kept or cleared). The 8-bit form of
+ * mx_paged_attn_decode (runtime/phase2/paged_attention_triton.py:745-775). */
+size_t mx_kv8_attn_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_blocks,
+                                   int32_t block_size);
+int mx_kv8_attn_decode(const uint16_t* q, int64_t q_sb, int64_t q_sh, const uint8_t* data, const uint8_t* codes,
+                       const int32_t* block_tables, int64_t bt_sb, int32_t max_blocks, const int32_t* seq_lens,
+                       int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t block_size, int32_t num_blocks,
+                       float scale, uint16_t* out, int64_t o_sb, int64_t o_sh, void* workspace,
+                       size_t workspace_bytes, int32_t* err, uint32_t flags, void* stream);
+
+/* ----------------------------------------------------------------------------
+ * Pages of a pool: one or two device regions (base2 NULL: one) of layers x
+ * num_pages runs of page_bytes, layer_stride bytes between layers. The id lists
+ * are HOST memory, read during the call. 16-byte aligned where page_bytes is a
+ * multiple of 16.
+ * ------------------------------------------------------------------------- */
+
+/* Page dst[i] = page src[i] in every layer and region, for all i at once: every
+ * source is read as it was before the call, in whatever order the pairs stand.
+ * Of several pairs with one dst the last counts. used (nullable, uint8
+ * [num_pages]) gets 1 at every dst; with move != 0 no page may be both a src and
+ * a dst, and used gets 0 at every src. More than 256 pairs that depend on each
+ * other (a page that is a src and a dst) are refused (MX_ERR_UNSUPPORTED).
+ * GpuKVBlockPool.copy_blocks (runtime/phase2/paged_kv_kernel.py:233-250). */
+int mx_kv_copy_pages(void* base, int64_t page_bytes, int64_t layer_stride, void* base2, int64_t page_bytes2,
+                     int64_t layer_stride2, int32_t layers, int32_t num_pages, const int32_t* src, const int32_t* dst,
+                     int32_t n, uint8_t* used, int32_t move, void* stream);
+
+/* out[r, c] = to[i] where tables[r, c] == from[i], else tables[r, c] (int32
+ * [rows, width]; out may be tables). from holds no id twice and none of to's.
+ * No reference counterpart: its pages never move. */
+int mx_kv_rename_pages(const int32_t* tables, int64_t in_stride, int32_t* out, int64_t out_stride, int32_t rows,
+                       int32_t width, const int32_t* from, const int32_t* to, int32_t n, void* stream);
+
+/* Freed pages: codes (an 8-bit pool's, nullable) and used (nullable) set to 0 at
+ * every id. No reference counterpart: GpuKVBlockPool only ever adds to its used
+ * blocks. */
+int mx_kv_clear_pages(uint8_t* codes, int64_t page_bytes, int64_t layer_stride, int32_t layers, uint8_t* used,
+                      int32_t num_pages, const int32_t* ids, int32_t n, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,7 @@ import threading
 import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "libmxdecode.so")
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 MX_OK = 0
 MX_ERR_INVALID = -1
@@ -107,6 +107,30 @@ SIGNATURES = {
         [_p, _i32, _p, _p, _i64, _p, _i32, _i32, ctypes.c_float, _p, _i64, _p, _i64, _p],
     ),
     "mx_silu_mul": (ctypes.c_int, [_p, _i64, _i32, _i32, _p, _i64, _p]),
+    "mx_kv8_write": (
+        ctypes.c_int,
+        [_p, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _p, _i64, _i32, _p, _p, _p, _i32, _i32, _p, _p, _u32, _p],
+    ),
+    "mx_kv8_gather": (
+        ctypes.c_int,
+        [_p, _p, _p, _i64, _i32, _p, _i32, _i32, _i32, _i32, _i32, _i32, _p, _p, _p, _u32, _p],
+    ),
+    "mx_kv8_rope_append": (
+        ctypes.c_int,
+        [_p, _i64, _p, _i32, _p, _i32, _i32, _i32, _i32, _p, _i32, _p, _p, _i64, _p, _i64, _i32, _p, _p, _i32, _i32,
+         _p, _p, _p, _u32, _p],
+    ),
+    "mx_kv8_attn_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "mx_kv8_attn_decode": (
+        ctypes.c_int,
+        [_p, _i64, _i64, _p, _p, _p, _i64, _i32, _p, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _p, _i64,
+         _i64, _p, _sz, _p, _u32, _p],
+    ),
+    "mx_kv_copy_pages": (
+        ctypes.c_int, [_p, _i64, _i64, _p, _i64, _i64, _i32, _i32, _p, _p, _i32, _p, _i32, _p],
+    ),
+    "mx_kv_rename_pages": (ctypes.c_int, [_p, _i64, _p, _i64, _i32, _i32, _p, _p, _i32, _p]),
+    "mx_kv_clear_pages": (ctypes.c_int, [_p, _i64, _i64, _i32, _p, _i32, _p, _i32, _p]),
     "mx_stream_probe": (ctypes.c_int, [_p, _i64, _i64, _i64, _i32, _i32, _p, _p]),
     "mx_launch_probe": (ctypes.c_int, [_p, _i64, _i64, _i32, _p]),
     "mx_run_gather_probe": (ctypes.c_int, [_p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _i32, _p, _p]),
@@ -193,6 +217,12 @@ def linear_workspace_bytes(m: int, n: int, k: int) -> int:
 def attn_workspace_bytes(*key: int) -> int:
     """``mx_paged_attn_workspace_bytes``, a function of the shape alone."""
     return int(load().mx_paged_attn_workspace_bytes(*key))
+
+
+@functools.lru_cache(maxsize=4096)
+def kv8_attn_workspace_bytes(*key: int) -> int:
+    """``mx_kv8_attn_workspace_bytes``, a function of the shape alone."""
+    return int(load().mx_kv8_attn_workspace_bytes(*key))
 
 
 def require_device_tensor(t: torch.Tensor, name: str) -> None:

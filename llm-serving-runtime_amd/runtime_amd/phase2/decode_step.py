@@ -22,6 +22,9 @@ current stream:
     h += a Wdown^T                         mx_w8a16_linear (+ the next add_rmsnorm)
     logits = RMSNorm(h) Wlm^T; argmax      mx_add_rmsnorm, mx_w8a16_linear, mx_argmax_rows_split
 
+Over an ``Int8KVBlockPool`` the middle lines are mx_w8a16_linear (or its split partials),
+mx_kv8_rope_append and mx_kv8_attn_decode.
+
 The first norm gathers the embedding rows of the step's tokens itself, layer
 0's RoPE kernel writes the attention lengths (positions + 1) and the argmax
 kernel advances ``seq_lens``, so no torch kernel runs inside a step.
@@ -56,6 +59,7 @@ from .decode_glue import (QKV_ROPE_MAX_ROWS, add_rmsnorm, add_rmsnorm_splits, ar
 from .int8_linear import (MLP_SYNC_ERR, MLP_SYNC_WORDS, gateup_interleave, int8_gateup_swiglu, int8_linear,
                           int8_linear_partials, int8_mlp_fused_partials, linear_splits, mlp_fusable,
                           pack_weight, quantize_weight)
+from .kv8 import kv8_attention_decode, kv8_rope_append
 from .paged_attention_hip import MX_PA_PLAN_READ, MX_PA_PLAN_WRITE
 from .paged_attention_hip import _decode as _paged_decode
 from .roofline import linear_hbm_bytes
@@ -274,8 +278,8 @@ class Int8DecodeModel:
         return buf
 
     def error_flag(self) -> int:
-        """OR of the KV-append error bits since the buffers were created (one host sync each), with
-        bit 16 set if a fused MLP launch gave up waiting for its activations."""
+        """OR of the KV-append error bits since the buffers were created (one host sync each), 4 among them
+        where attention over an 8-bit pool met a block outside it, with bit 16 set if a fused MLP launch gave up waiting for its activations."""
         flag = 0
         for buf in self._buffers.values():
             flag |= int(buf.err.item())
@@ -297,6 +301,7 @@ class Int8DecodeModel:
             raise ValueError("seq_lens and block_tables must be int32 and tokens int64 device tensors")
         eps = s.rms_eps
         plan = self.attn_plan and not self.shared_kv_blocks and pool.block_size_tokens >= 16
+        kv8 = getattr(pool, "kv_bits", 16) == 8
         sp = buf.splits
         for li, layer in enumerate(self.layers):
             if li == 0:  # h = embed[tokens]; x = RMSNorm(h)
@@ -304,30 +309,11 @@ class Int8DecodeModel:
             else:
                 self._norm_after_down(buf, layer.ln_in)
             lens_out = buf.attn_lens if li == 0 else None
-            k_layer = pool.k_layer_view(li)
-            v_layer = pool.v_layer_view(li)
-            used = pool._used_map  # the pool's block-usage accounting, marked by the K/V append
-            if self.uses_fused_qkv(bsz):
-                ev = self._tick(timers, "qkv")
-                packed, scale, _, bias = layer.qkv
-                qkv_linear_rope_append(buf.x, packed, scale, bias, self.rope, seq_lens, buf.q, k_layer, v_layer,
-                                       block_tables, s.heads, s.kv_heads, err=buf.err, lens_out=lens_out,
-                                       used_blocks=used)
-                self._tock(timers, "qkv", ev)
-            elif sp["qkv"] > 1:
-                self._partials(buf.x, layer.qkv, buf.part, timers, "qkv")
-                qkv_rope_append_splits(buf.part, sp["qkv"], layer.qkv[3], self.rope, seq_lens, buf.q, k_layer,
-                                       v_layer, block_tables, s.heads, s.kv_heads, err=buf.err, lens_out=lens_out,
-                                       used_blocks=used)
+            if kv8:
+                self._attend_kv8(buf, layer, pool, li, block_tables, seq_lens, lens_out, timers)
             else:
-                self._lin(buf.x, layer.qkv, buf.qkv, timers, "qkv")
-                qkv_rope_append(buf.qkv, self.rope, seq_lens, buf.q, k_layer, v_layer, block_tables, s.heads,
-                                s.kv_heads, err=buf.err, lens_out=lens_out, used_blocks=used)
-            ev = self._tick(timers, "attn")
-            _paged_decode(buf.q.view(bsz, s.heads, 1, s.head_dim), k_layer, v_layer, block_tables, buf.attn_lens,
-                          s.head_dim ** -0.5, s.group, out=buf.attn, shared_blocks=self.shared_kv_blocks,
-                          plan=(MX_PA_PLAN_WRITE if li == 0 else MX_PA_PLAN_READ) if plan else 0)
-            self._tock(timers, "attn", ev)
+                self._attend(buf, layer, pool, li, block_tables, seq_lens, lens_out,
+                             (MX_PA_PLAN_WRITE if li == 0 else MX_PA_PLAN_READ) if plan else 0, timers)
             if sp["o"] > 1:
                 self._partials(buf.attn.view(bsz, -1), layer.o, buf.part, timers, "o")
                 add_rmsnorm_splits(buf.part, sp["o"], layer.o[3], layer.ln_post, eps, buf.x, residual=buf.h,
@@ -349,6 +335,55 @@ class Int8DecodeModel:
         self._lin(buf.x, self.lm_head, buf.logits, timers, "lm_head")
         nxt = argmax_rows(buf.logits, out=buf.next if out is None else out, seq_lens=seq_lens)
         return (nxt, buf.logits) if return_logits else nxt
+
+    def _attend(self, buf: _Buffers, layer: _Layer, pool, li: int, block_tables, seq_lens, lens_out, plan: int,
+                timers) -> None:
+        """buf.attn = attention of the step's tokens over the 16-bit pool, their K and V appended first."""
+        s, sp = self.shape, buf.splits
+        bsz = int(buf.q.shape[0])
+        k_layer = pool.k_layer_view(li)
+        v_layer = pool.v_layer_view(li)
+        used = pool._used_map  # the pool's block-usage accounting, marked by the K/V append
+        if self.uses_fused_qkv(bsz):
+            ev = self._tick(timers, "qkv")
+            packed, scale, _, bias = layer.qkv
+            qkv_linear_rope_append(buf.x, packed, scale, bias, self.rope, seq_lens, buf.q, k_layer, v_layer,
+                                   block_tables, s.heads, s.kv_heads, err=buf.err, lens_out=lens_out,
+                                   used_blocks=used)
+            self._tock(timers, "qkv", ev)
+        elif sp["qkv"] > 1:
+            self._partials(buf.x, layer.qkv, buf.part, timers, "qkv")
+            qkv_rope_append_splits(buf.part, sp["qkv"], layer.qkv[3], self.rope, seq_lens, buf.q, k_layer,
+                                   v_layer, block_tables, s.heads, s.kv_heads, err=buf.err, lens_out=lens_out,
+                                   used_blocks=used)
+        else:
+            self._lin(buf.x, layer.qkv, buf.qkv, timers, "qkv")
+            qkv_rope_append(buf.qkv, self.rope, seq_lens, buf.q, k_layer, v_layer, block_tables, s.heads,
+                            s.kv_heads, err=buf.err, lens_out=lens_out, used_blocks=used)
+        ev = self._tick(timers, "attn")
+        _paged_decode(buf.q.view(bsz, s.heads, 1, s.head_dim), k_layer, v_layer, block_tables, buf.attn_lens,
+                      s.head_dim ** -0.5, s.group, out=buf.attn, shared_blocks=self.shared_kv_blocks, plan=plan)
+        self._tock(timers, "attn", ev)
+
+    def _attend_kv8(self, buf: _Buffers, layer: _Layer, pool, li: int, block_tables, seq_lens, lens_out,
+                    timers) -> None:
+        """:meth:`_attend` over an ``Int8KVBlockPool``: the QKV projection (its split partials where the
+        shape splits K), rotary + write in 8 bits, attention over the pages."""
+        s, sp = self.shape, buf.splits
+        bsz = int(buf.q.shape[0])
+        store = pool.layer_store(li)
+        parts = sp["qkv"] > 1
+        if parts:
+            self._partials(buf.x, layer.qkv, buf.part, timers, "qkv")
+        else:
+            self._lin(buf.x, layer.qkv, buf.qkv, timers, "qkv")
+        kv8_rope_append(None if parts else buf.qkv, self.rope, seq_lens, buf.q, store, block_tables, s.heads,
+                        partials=buf.part if parts else None, splits=sp["qkv"], bias=layer.qkv[3] if parts else None,
+                        err=buf.err, lens_out=lens_out, used_blocks=pool._used_map)
+        ev = self._tick(timers, "attn")
+        kv8_attention_decode(buf.q.view(bsz, s.heads, 1, s.head_dim), store, block_tables, buf.attn_lens,
+                             s.head_dim ** -0.5, s.group, out=buf.attn, err=buf.err)
+        self._tock(timers, "attn", ev)
 
     def uses_fused_qkv(self, bsz: int) -> bool:
         """Whether the step's QKV projection and RoPE + append run as one launch at this batch."""

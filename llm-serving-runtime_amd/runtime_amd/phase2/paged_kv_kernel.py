@@ -38,16 +38,23 @@ MI355X-first differences:
   ``sync_write_checks`` (or ``PHASE2_KV_SYNC_CHECKS=1`` before the pool is
   built): every batched write then checks the word right away (one host sync
   per call, skipped while a HIP graph is being captured).
+* ``copy_blocks`` on a device pool is one ``mx_kv_copy_pages`` launch per 256
+  pages whose ids travel with it; beside it stand ``move_blocks`` (compaction:
+  pages to other ids, the block tables that name them renamed) and
+  ``free_blocks``. The reference has neither: its pool only ever adds to its
+  used blocks.
 """
 
 from __future__ import annotations
 
+import array
 import math
 import os
 from dataclasses import dataclass
 
 import torch
 
+from . import _hip
 
 KV_LAYOUTS = ("split", "interleaved")
 
@@ -61,8 +68,14 @@ class PoolShape:
     head_dim: int
 
 
+def _ids(block_ids) -> list[int]:
+    return list(map(int, block_ids))
+
+
 class GpuKVBlockPool:
     """Shared block pool; same constructor and methods as the reference's."""
+
+    kv_bits = 16  # of a stored K or V element (Int8KVBlockPool: 8)
 
     def __init__(self, *, num_blocks: int, block_size_tokens: int, num_layers: int, num_kv_heads: int, head_dim: int,
                  dtype: torch.dtype, device: str | torch.device, kv_layout: str = "interleaved") -> None:
@@ -83,6 +96,7 @@ class GpuKVBlockPool:
         self.device = torch.device(device)
         self._k_pool: torch.Tensor | None = None
         self._v_pool: torch.Tensor | None = None
+        self._regions: list[torch.Tensor] = []  # the tensors [L, num_blocks, ...] that hold the pages
         self._used_blocks: set[int] = set()
         self._peak_allocated_blocks = 0
         self._used_map: torch.Tensor | None = None    # uint8 [num_blocks]: blocks written on the device
@@ -142,10 +156,12 @@ class GpuKVBlockPool:
             kv = torch.zeros(s.num_layers, s.num_blocks, s.num_kv_heads, 2, s.block_size_tokens, s.head_dim,
                              dtype=self.dtype, device=self.device)
             self._k_pool, self._v_pool = kv[:, :, :, 0], kv[:, :, :, 1]
+            self._regions = [kv]
         else:
             shape = (s.num_layers, s.num_blocks, s.num_kv_heads, s.block_size_tokens, s.head_dim)
             self._k_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
             self._v_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
+            self._regions = [self._k_pool, self._v_pool]
         if self.device.type == "cuda":
             self._used_map = torch.zeros(s.num_blocks, dtype=torch.uint8, device=self.device)
             self._write_err = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -259,23 +275,108 @@ class GpuKVBlockPool:
             -1, value_states.shape[1], value_states.shape[3])
 
     def copy_blocks(self, src_block_ids: list[int], dst_block_ids: list[int]) -> None:
-        """Copy full physical blocks (all layers) from src ids to dst ids (``:233-250``)."""
+        """Copy full physical blocks (all layers) from src ids to dst ids (``:233-250``), every source as
+        it was before the call; of several pairs with one destination the last counts."""
         if len(src_block_ids) != len(dst_block_ids):
             raise ValueError(f"copy_blocks length mismatch: src={len(src_block_ids)} dst={len(dst_block_ids)}")
-        if not src_block_ids:
+        pairs = [(s, d) for s, d in zip(_ids(src_block_ids), _ids(dst_block_ids)) if s != d]
+        self._touch_ids([i for pair in pairs for i in pair])
+        if pairs:
+            self._copy_pages([s for s, _ in pairs], [d for _, d in pairs])
+
+    def move_blocks(self, src_block_ids: list[int], dst_block_ids: list[int],
+                    block_tables: torch.Tensor | None = None, out: torch.Tensor | None = None
+                    ) -> torch.Tensor | None:
+        """Move blocks (all layers) from src ids to dst ids, which leaves the src ids free: a pool's live
+        blocks brought together. Returns ``block_tables`` (int32 ``[B, max_blocks]`` on the pool's device)
+        with every src id replaced by its dst id, as a new tensor or in ``out`` (which may be
+        ``block_tables`` itself). No id may occur twice, neither among nor between the two lists.
+        """
+        src, dst = _ids(src_block_ids), _ids(dst_block_ids)
+        if len(src) != len(dst):
+            raise ValueError(f"move_blocks length mismatch: src={len(src)} dst={len(dst)}")
+        if len(set(src).union(dst)) != 2 * len(src):
+            raise ValueError("move_blocks takes every block id once")
+        if block_tables is None:
+            if out is not None:
+                raise ValueError("out goes with block_tables")
+        else:
+            if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.device.type != self.device.type:
+                raise ValueError("block_tables must be int32 [B, max_blocks] on the pool's device")
+            if out is None:
+                out = torch.empty(block_tables.shape, dtype=torch.int32, device=block_tables.device)
+            elif out.dtype != torch.int32 or out.shape != block_tables.shape or out.device != block_tables.device:
+                raise ValueError("out must be int32 of block_tables' shape and device")
+        self._touch_ids(src + dst)
+        if src:
+            self._copy_pages(src, dst, move=True)
+            self._used_blocks.difference_update(src)
+        if block_tables is not None:
+            self._rename(block_tables, out, src, dst)
+        return out
+
+    def free_blocks(self, block_ids: list[int]) -> None:
+        """Give blocks back: they no longer count as allocated (and an 8-bit pool's stand for 0). A block
+        written on the device and freed before the counts are read is not seen by the peak."""
+        ids = sorted(set(_ids(block_ids)))
+        if ids and (ids[0] < 0 or ids[-1] >= self.shape.num_blocks):
+            raise IndexError(f"physical block id out of range: {ids[0] if ids[0] < 0 else ids[-1]}")
+        self._used_blocks.difference_update(ids)
+        if not ids or self._used_map is None:
             return
+        codes = self._freed_codes()
+        arr = array.array("i", ids)
+        with _hip.on_device(self.device):
+            _hip.check(_hip.load().mx_kv_clear_pages(
+                codes.data_ptr() if codes is not None else None, codes[0, 0].numel() if codes is not None else 0,
+                codes.stride(0) if codes is not None else 0, self.shape.num_layers, self._used_map.data_ptr(),
+                self.shape.num_blocks, arr.buffer_info()[0], len(ids), _hip.stream_handle(self.device)),
+                "mx_kv_clear_pages")
+
+    def _freed_codes(self) -> torch.Tensor | None:
+        """What a freed block's bytes are cleared in (uint8 ``[L, num_blocks, ...]``); nothing in 16 bits."""
+        return None
+
+    def _page_regions(self) -> list[torch.Tensor]:
         self._ensure_pools()
-        assert self._k_pool is not None and self._v_pool is not None
-        pairs = [(int(s), int(d)) for s, d in zip(src_block_ids, dst_block_ids) if int(s) != int(d)]
-        for s, d in pairs:
-            self._touch_block(s)
-            self._touch_block(d)
-        if not pairs:
+        return self._regions
+
+    def _copy_pages(self, src: list[int], dst: list[int], move: bool = False) -> None:
+        """Page dst[i] = page src[i] (ids checked) in every layer, all at once."""
+        regions = self._page_regions()
+        if self.device.type == "cuda":
+            args: list = []
+            for t in (*regions, None)[:2]:
+                args += [None, 0, 0] if t is None else [t.data_ptr(), t[0, 0].numel() * t.element_size(),
+                                                        t.stride(0) * t.element_size()]
+            a, b = array.array("i", src), array.array("i", dst)
+            with _hip.on_device(self.device):
+                rc = _hip.load().mx_kv_copy_pages(
+                    *args, self.shape.num_layers, self.shape.num_blocks, a.buffer_info()[0], b.buffer_info()[0],
+                    len(src), self._used_map.data_ptr(), int(move), _hip.stream_handle(self.device))
+            if rc != _hip.MX_ERR_UNSUPPORTED:  # a chain of copies longer than a launch takes
+                _hip.check(rc, "mx_kv_copy_pages")
+                return
+        last = dict(zip(dst, src))
+        to = torch.tensor(list(last), device=self.device, dtype=torch.long)
+        of = torch.tensor(list(last.values()), device=self.device, dtype=torch.long)
+        for t in regions:
+            t[:, to] = t[:, of]
+
+    def _rename(self, tables: torch.Tensor, out: torch.Tensor, src: list[int], dst: list[int]) -> None:
+        if self.device.type != "cuda":
+            name = {s: d for s, d in zip(src, dst)}
+            out.copy_(torch.tensor([[name.get(i, i) for i in row] for row in tables.tolist()],
+                                   dtype=torch.int32).view(tables.shape))
             return
-        src = torch.tensor([s for s, _ in pairs], device=self.device, dtype=torch.long)
-        dst = torch.tensor([d for _, d in pairs], device=self.device, dtype=torch.long)
-        self._k_pool[:, dst] = self._k_pool[:, src]
-        self._v_pool[:, dst] = self._v_pool[:, src]
+        if tables.stride(1) != 1 or out.stride(1) != 1:
+            raise ValueError("block_tables and out must have unit inner stride")
+        a, b = array.array("i", src), array.array("i", dst)
+        with _hip.on_device(self.device):
+            _hip.check(_hip.load().mx_kv_rename_pages(
+                tables.data_ptr(), tables.stride(0), out.data_ptr(), out.stride(0), tables.shape[0], tables.shape[1],
+                a.buffer_info()[0], b.buffer_info()[0], len(src), _hip.stream_handle(self.device)),
+                "mx_kv_rename_pages")
 
     def gather_layer(self, layer_idx: int, block_ids: list[int], seq_len: int) -> tuple[torch.Tensor, torch.Tensor]:
         """Gather one row as ``[1, Hkv, seq_len, D]`` (prefill / parity, ``:252-283``)."""
@@ -286,12 +387,12 @@ class GpuKVBlockPool:
         if n_logical > len(block_ids):
             raise IndexError("block table underrun during gather")
         self._ensure_pools()
-        assert self._k_pool is not None and self._v_pool is not None
         ids_list = [int(b) for b in list(block_ids)[:n_logical]]
         self._touch_ids(ids_list)
         if self._gathers_on_device(seq_len):
             table = torch.tensor([ids_list], dtype=torch.int32).to(self.device)
             return self._gather_table(layer_idx, table, seq_len)
+        assert self._k_pool is not None and self._v_pool is not None
         ids = torch.tensor(ids_list, device=self.device, dtype=torch.long)
         s = self.shape
         k = self._k_pool[layer_idx, ids].permute(1, 0, 2, 3).reshape(s.num_kv_heads, n_logical * bs, s.head_dim)
@@ -338,6 +439,7 @@ class GpuKVBlockPool:
     def reset(self) -> None:
         self._k_pool = None
         self._v_pool = None
+        self._regions = []
         self._used_map = None
         self._write_err = None
         self._used_blocks.clear()

@@ -1,0 +1,143 @@
+"""Pages of a pool on the GPU: copies (with chains, cycles and fan-out), compaction, renamed tables, freed
+pages, for the 16-bit pool's two layouts and the 8-bit pool. Bar: bit-identical (nothing is computed)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+POOLS = ["interleaved", "split", "int8"]
+
+
+def _pool(kind, nb, layers=3, hkv=2, bs=16, d=64, seed=0):
+    from runtime_amd.phase2.kv8_pool import Int8KVBlockPool
+    from runtime_amd.phase2.paged_kv_kernel import GpuKVBlockPool
+
+    args = dict(num_blocks=nb, block_size_tokens=bs, num_layers=layers, num_kv_heads=hkv, head_dim=d,
+                dtype=torch.float16, device=DEV)
+    pool = Int8KVBlockPool(**args) if kind == "int8" else GpuKVBlockPool(**args, kv_layout=kind)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    for t in pool._page_regions():
+        t.copy_(torch.randint(1, 250, t.shape, generator=g, device=DEV).to(t.dtype))
+    return pool
+
+
+def _pages(pool):
+    return [t.clone() for t in pool._page_regions()]
+
+
+def _check(pool, was, of):
+    """Page i holds what page of.get(i, i) held."""
+    index = torch.tensor([of.get(i, i) for i in range(pool.shape.num_blocks)], device=DEV)
+    for now, old in zip(pool._page_regions(), was):
+        assert torch.equal(now, old[:, index])
+
+
+@pytest.mark.parametrize("kind", POOLS)
+@pytest.mark.parametrize("hkv,bs,d", [(2, 16, 64), (1, 4, 64), (8, 32, 128), (3, 8, 128)])
+def test_copies_of_independent_pages(kind, hkv, bs, d):
+    pool = _pool(kind, 40, hkv=hkv, bs=bs, d=d)
+    was = _pages(pool)
+    src, dst = [0, 0, 5, 39, 7, 9], [1, 2, 38, 3, 7, 4]
+    pool.copy_blocks(src, dst)
+    _check(pool, was, {d: s for s, d in zip(src, dst)})
+    assert pool.allocated_block_count() == 9  # 7 -> 7 is no copy
+
+
+@pytest.mark.parametrize("kind", POOLS)
+@pytest.mark.parametrize("src,dst", [
+    ([1, 2, 3], [2, 3, 4]), ([4, 3, 2], [5, 4, 3]), ([1, 2], [2, 1]), ([1, 2, 3, 6, 5], [2, 3, 1, 5, 6]),
+    ([1, 1, 2, 2], [2, 3, 4, 5]), ([1, 2, 1], [2, 1, 3]), ([0, 1, 2, 8], [1, 2, 0, 9]), ([4, 5, 6], [7, 7, 5])])
+def test_copies_that_depend_on_each_other(kind, src, dst):
+    pool = _pool(kind, 12)
+    was = _pages(pool)
+    pool.copy_blocks(src, dst)
+    _check(pool, was, {d: s for s, d in zip(src, dst)})
+
+
+@pytest.mark.parametrize("n", [256, 257, 700])
+def test_more_pages_than_a_launch_holds(n):
+    pool = _pool("int8", 2 * n + 5, layers=2, hkv=1, bs=4)
+    was = _pages(pool)
+    g = torch.Generator().manual_seed(n)
+    ids = torch.randperm(2 * n + 5, generator=g).tolist()
+    pool.copy_blocks(ids[:n], ids[n:2 * n])
+    _check(pool, was, dict(zip(ids[n:2 * n], ids[:n])))
+
+
+@pytest.mark.parametrize("kind", POOLS)
+def test_a_chain_and_a_cycle_longer_than_a_launch_holds(kind):
+    n = 300
+    pool = _pool(kind, n + 1, layers=1, hkv=1, bs=4)
+    was = _pages(pool)
+    pool.copy_blocks(list(range(n)), list(range(1, n + 1)))
+    _check(pool, was, {i + 1: i for i in range(n)})
+    was = _pages(pool)
+    pool.copy_blocks(list(range(n)), [*range(1, n), 0])
+    _check(pool, was, {(i + 1) % n: i for i in range(n)})
+
+
+@pytest.mark.parametrize("kind", POOLS)
+@pytest.mark.parametrize("n", [1, 37, 300])
+def test_move_blocks_renames_tables_and_frees_the_sources(kind, n):
+    nb = 3 * n + 4
+    pool = _pool(kind, nb, layers=2, hkv=1, bs=4)
+    was = _pages(pool)
+    g = torch.Generator().manual_seed(n)
+    ids = torch.randperm(nb, generator=g).tolist()
+    src, dst, rest = ids[:n], ids[n:2 * n], ids[2 * n:]
+    pool._touch_ids(src + rest)
+    pool._used_map[torch.tensor(src, device=DEV)] = 1
+    tables = torch.tensor(src + rest + src, dtype=torch.int32)[None].repeat(3, 1)
+    tables[1], tables[2, 0], tables[2, -1] = tables[1].flip(0), -1, nb + 7  # ids that name no page stay
+    name = dict(zip(src, dst))
+    want = [[name.get(i, i) for i in row] for row in tables.tolist()]
+    wide = torch.zeros(3, tables.shape[1] + 5, dtype=torch.int32, device=DEV)
+    wide[:, :tables.shape[1]] = tables.to(DEV)
+    view = wide[:, :tables.shape[1]]
+    got = pool.move_blocks(src, dst, view)
+    assert got.tolist() == want and torch.equal(view.cpu(), tables)
+    _check(pool, was, {d: s for s, d in name.items()})
+    assert pool.allocated_block_count() == n + len(rest) and pool.peak_allocated_block_count() == 2 * n + len(rest)
+    pool.move_blocks(dst, src, got, out=got)  # back again, in place
+    assert torch.equal(got.cpu()[:2], tables[:2])
+
+
+@pytest.mark.parametrize("kind", POOLS)
+def test_freed_blocks(kind):
+    pool = _pool(kind, 700, layers=2, hkv=1, bs=4)
+    was = _pages(pool)
+    pool._used_map.fill_(1)
+    assert pool.allocated_block_count() == 700
+    gone = list(range(0, 600)) + [5]
+    pool.free_blocks(gone)
+    assert pool.allocated_block_count() == 100 and pool.peak_allocated_block_count() == 700
+    if kind == "int8":
+        assert (pool._codes[:, :600] == 0).all() and torch.equal(pool._codes[:, 600:], was[1][:, 600:])
+        k, _ = pool.gather_layer(0, [3], 4)
+        assert (k == 0).all()
+    assert torch.equal(pool._page_regions()[0], was[0])
+
+
+def test_copies_in_a_captured_graph_and_on_a_side_stream():
+    pool = _pool("interleaved", 20)
+    tables = torch.arange(20, dtype=torch.int32, device=DEV).view(2, 10)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        out = pool.move_blocks([11], [1], tables)
+        with torch.cuda.graph(graph, stream=side):
+            pool.copy_blocks([3, 4, 5], [4, 3, 6])
+            pool.move_blocks([12], [2], tables, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(4):
+        was = _pages(pool)
+        out.zero_()
+        graph.replay()
+        _check(pool, was, {4: 3, 3: 4, 6: 5, 2: 12})
+        assert out.tolist()[1][2] == 2 and out.tolist()[1][1] == 11
+        pool.copy_blocks([i], [13 + i])
+        torch.cuda.synchronize()
