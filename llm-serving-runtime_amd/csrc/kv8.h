@@ -88,23 +88,47 @@ __device__ __forceinline__ float growth_factor(int old, int now) {
     return old == 0 || e <= 0 ? 0.0f : __uint_as_float((uint32_t)e << 23);
 }
 
-// 8 bytes -> 8 values of the element type, exact. s: the page's scale (scale_of).
+// 8 bytes -> their 8 integers q in the element type, exact.
 template <bool BF16>
-__device__ __forceinline__ half8v values8(uint32_t d0, uint32_t d1, float s) {
+__device__ __forceinline__ half8v integers8(uint32_t d0, uint32_t d1) {
     if constexpr (!BF16) {
-        return w8a16::dequant8(d0, d1) * (half8v)((_Float16)s);
+        return w8a16::dequant8(d0, d1);
+    } else {
+        uint32_t out[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = i < 2 ? d0 : d1;
+            const float lo = (float)((w >> (16 * (i & 1))) & 0xffu) - 128.0f;
+            const float hi = (float)((w >> (16 * (i & 1) + 8)) & 0xffu) - 128.0f;
+            out[i] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+        }
+        return __builtin_bit_cast(half8v, uint4{out[0], out[1], out[2], out[3]});
+    }
+}
+
+// 4 bytes at scale s0 and 4 at s1 (scale_of) -> 8 values of the element type, exact.
+template <bool BF16>
+__device__ __forceinline__ half8v values4x2(uint32_t d0, uint32_t d1, float s0, float s1) {
+    if constexpr (!BF16) {
+        const _Float16 a = (_Float16)s0, b = (_Float16)s1;
+        return w8a16::dequant8(d0, d1) * half8v{a, a, a, a, b, b, b, b};
     } else {
         // q s has at most 8 significant bits: the upper half of its fp32 pattern is the bf16 value.
         uint32_t out[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t w = i < 2 ? d0 : d1;
+            const float s = i < 2 ? s0 : s1;
             const float lo = ((float)((w >> (16 * (i & 1))) & 0xffu) - 128.0f) * s;
             const float hi = ((float)((w >> (16 * (i & 1) + 8)) & 0xffu) - 128.0f) * s;
             out[i] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
         }
         return __builtin_bit_cast(half8v, uint4{out[0], out[1], out[2], out[3]});
     }
+}
+template <bool BF16>
+__device__ __forceinline__ half8v values8(uint32_t d0, uint32_t d1, float s) {
+    return values4x2<BF16>(d0, d1, s, s);
 }
 
 // Largest 16-bit half of v over the wave (every lane gets it).

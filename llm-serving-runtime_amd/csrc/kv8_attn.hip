@@ -1,6 +1,30 @@
 // Decode attention over the 8-bit KV cache (kv8.h) on gfx950: out = softmax(scale q K^T) V per query
 // head, K and V the values that the pages stand for. The 8-bit form of paged_attn.hip, which replaces
 // paged_attention_decode_batched (runtime/phase2/paged_attention_triton.py:745-775).
+//
+// Work. A segment is one row and one group of at most 16 query heads of a kv-head (a larger GQA group is
+// cut into equal ones; each reads the head's pages again). Its tokens are chunks of 16. The chunks of all
+// segments, row after row, form one sequence that is cut into equal ranges, one per wave, so every wave
+// streams the same bytes whatever the mix of lengths; a segment that several waves share is joined by a
+// second, small launch from their (m, l, acc), all fp32. Tables of at most kDirectChunks chunks give every
+// segment to one wave instead: one launch.
+//
+// A wave takes 4 chunks a step, one per lane group g = lane / 16, so that what a lane scores is what it
+// weighs, and no score crosses lanes:
+//   * scores, 4 x D / 32 products v_mfma_f32_16x16x32: the A operand's row r of product j is token
+//     4 j + r % 4 of chunk r / 4, so lane group g receives tokens 4 j + i of chunk g, for head lane % 16
+//     (the B operand holds the query heads). K enters as the integers q, exact in 16 bits; the page's
+//     scale multiplies the fp32 score. The head dim is contracted in the order of the lane's 16-byte
+//     loads, the query's operand in the same order;
+//   * online softmax in fp32 on the exp2 scale; the reference maximum moves only when a score exceeds it
+//     by more than 2^8, so most steps neither rescale nor exchange maxima between lane groups;
+//   * P.V, 2 x D / 16 products over 32 tokens: lane group g supplies tokens 8 u .. 8 u + 7 of chunk g,
+//     which is what its scores gave (weights) and half of a 16-byte load of a dim's token row (V, times
+//     the page's scale: exact in 16 bits).
+// Weights are rounded to the 16-bit type before the product, as the 16-bit path's are; the denominator
+// sums the rounded ones.
+#include <algorithm>
+
 #include "common.h"
 #include "elt.h"
 #include "kv8.h"
@@ -8,7 +32,14 @@
 namespace mx {
 namespace kv8 {
 
-constexpr int kAttnWaves = 4;
+constexpr int kAttnWaves = 4;      // waves per workgroup
+constexpr int kChunk = 16;         // tokens per chunk
+constexpr int kStep = 4;           // chunks per step of a wave
+constexpr int kHeads = 16;         // query heads of a segment, at most
+constexpr int kWorkers = 2048;     // waves of a launch: 256 CUs x 8
+constexpr int kDirectChunks = 16;  // tables of at most this many chunks: one wave per segment
+constexpr int kMaxTokens = 1 << 30;  // of a table row, so that token and chunk numbers are 32-bit
+constexpr float kLazyLog2 = 8.0f;
 
 struct AttnParams {
     const uint16_t* q;
@@ -18,91 +49,397 @@ struct AttnParams {
     int64_t bt_sb;
     int max_blocks;
     const int32_t* seq_lens;
-    int Hq, G;
+    int B, G;      // rows; query heads per kv-head
+    int NG, GS;    // segments per kv-head, query heads of one (the last may have fewer)
+    int Hv;        // segments per row: Hkv * NG
+    int workers;   // 0: one wave per segment
     float scale_log2e;
     uint16_t* out;
     int64_t o_sb, o_sh;
     int32_t* err;
+    float* part_ml;   // [2 workers][GS][2]: a piece's maximum and denominator
+    float* part_acc;  // [2 workers][GS][D]: its unnormalised output
 };
 
-// One workgroup per (row, query head); its waves take the row's 64-token stretches in turn, a lane
-// scoring one token, then D / 64 output dims.
+// A row's tokens within its table, and their chunks.
+template <int BS>
+__device__ __forceinline__ int row_tokens(const AttnParams& p, int b) {
+    const int most = p.max_blocks * BS, s = p.seq_lens[b];  // at most kMaxTokens (checked on the host)
+    return s < 0 ? 0 : (s < most ? s : most);
+}
+__device__ __forceinline__ int chunks_of(int tokens) { return (tokens + kChunk - 1) / kChunk; }
+
+__device__ __forceinline__ int incl_scan(int v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(v, o);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+
+// Chunks of rows [0, b) and of all rows (every lane gets both).
+template <int BS>
+__device__ __forceinline__ void sum_rows(const AttnParams& p, int b, int lane, int& before, int& total) {
+    int s0 = 0, s1 = 0;
+    for (int i = lane; i < p.B; i += 64) {
+        const int n = chunks_of(row_tokens<BS>(p, i));
+        s1 += n;
+        if (i < b) s0 += n;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        s0 += __shfl_xor(s0, o);
+        s1 += __shfl_xor(s1, o);
+    }
+    before = s0;
+    total = s1;
+}
+
+// The cut of T chunks into W ranges: the first `rem` have base + 1 chunks, the others base.
+struct Cut {
+    int W, base, rem;
+    __device__ __forceinline__ Cut(int T, int workers) {
+        const int steps = (T + kStep - 1) / kStep;  // no range shorter than a step
+        W = steps < workers ? steps : workers;
+        base = W > 0 ? T / W : 0;
+        rem = T - base * W;
+    }
+    __device__ __forceinline__ int lo(int w) const { return w * base + (w < rem ? w : rem); }
+    __device__ __forceinline__ int worker_of(int x) const {
+        const int edge = rem * (base + 1);
+        return x < edge ? x / (base + 1) : rem + (x - edge) / base;
+    }
+};
+
+// The state of a piece: its heads' running maximum, this lane's part of the denominator, the
+// unnormalised output (acc[e][i]: dim 16 e + 4 g + i of head lane % 16).
+template <int D>
+struct Piece {
+    float m, l;
+    float4v acc[D / 16];
+};
+
+// One step's loads. NP pages stand in a chunk: 1, or 16 / BS.
+template <int D, int BS>
+struct Regs {
+    static constexpr int NP = BS >= kChunk ? 1 : kChunk / BS;
+    uint4 k[4][D / 64];
+    uint32_t v[D / 16][4];
+    uint32_t codes[NP];  // K code | V code << 8
+};
+
 template <int D, int BS, bool BF16>
-__global__ __launch_bounds__(kAttnWaves * 64) void kv8_attn_kernel(AttnParams p) {
-    constexpr int DP = D / 64;
-    __shared__ float qs[D];
-    __shared__ float ps[kAttnWaves][64];
-    __shared__ int pg[kAttnWaves][64];
-    __shared__ float red[kAttnWaves][D + 2];
-    const int h = blockIdx.x, b = blockIdx.y, kvh = h / p.G;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint16_t* q = p.q + (int64_t)b * p.q_sb + (int64_t)h * p.q_sh;
-    if (threadIdx.x < D) qs[threadIdx.x] = widen<BF16>(q[threadIdx.x]) * p.scale_log2e;
-    __syncthreads();
-    int64_t len = p.seq_lens[b];
-    const int64_t most = (int64_t)p.max_blocks * BS;
-    len = len < 0 ? 0 : (len < most ? len : most);
+__device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, int h0, int nh, int c0, int nc,
+                                          int tokens, int lane, Piece<D>& st) {
+    constexpr int NP = Regs<D, BS>::NP, KA = D / 64;
+    constexpr int PT = BS < kChunk ? BS : kChunk;  // tokens of a chunk in one page
+    const int g = lane >> 4, r = lane & 15;
     const float kNegInf = -__builtin_huge_valf();
-    float m = kNegInf, l = 0.0f, acc[DP];
-    for (int j = 0; j < DP; ++j) acc[j] = 0.0f;
-    for (int64_t t0 = wave * 64; t0 < len; t0 += kAttnWaves * 64) {
-        const int64_t t = t0 + lane;
-        int phys = -1;
-        float s = kNegInf;
-        if (t < len) {
-            phys = p.bt[(int64_t)b * p.bt_sb + t / BS];
-            if ((unsigned)phys >= (unsigned)p.pages.num_blocks) {
-                if (p.err) atomicOr(p.err, 4);
-                phys = -1;
+    const int32_t* bt = p.bt + (int64_t)b * p.bt_sb;
+    const int nblk = (tokens + BS - 1) / BS;
+
+    // Page ids of this lane's chunks in a step: of the chunk whose K row it loads (r / 4), and of the
+    // chunk whose V and scores it holds (g). -1: past the piece or the row, or outside the pool.
+    struct Ids {
+        int k[NP], v[NP];
+    };
+    auto load_ids = [&](int c, Ids& id) {  // c: first chunk of the step, relative to the piece
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int ck = c + (r >> 2), cv = c + g;
+            const int pk = (c0 + ck) * kChunk / BS + n, pv = (c0 + cv) * kChunk / BS + n;
+            id.k[n] = ck < nc && pk < nblk ? bt[pk] : -1;
+            id.v[n] = cv < nc && pv < nblk ? bt[pv] : -1;
+        }
+    };
+    auto in_pool = [&](int id) { return (unsigned)id < (unsigned)p.pages.num_blocks; };
+
+    half8v qf[2 * KA];
+    if (r < nh) {
+        const uint16_t* qp = p.q + (int64_t)b * p.q_sb + (int64_t)(h0 + r) * p.q_sh + 16 * g;
+#pragma unroll
+        for (int a = 0; a < KA; ++a)
+#pragma unroll
+            for (int hi = 0; hi < 2; ++hi)
+                qf[2 * a + hi] = __builtin_bit_cast(half8v, *reinterpret_cast<const uint4*>(qp + 64 * a + 8 * hi));
+    } else {
+#pragma unroll
+        for (int a = 0; a < 2 * KA; ++a) qf[a] = half8v{};
+    }
+
+    st.m = kNegInf;
+    st.l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) st.acc[e] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+
+    Regs<D, BS> rg{};  // lanes without a page keep what is there: any bytes, masked (K) or at scale 0 (V)
+    auto load_k = [&](int c, const Ids& id) {
+        // Token 4 j + r % 4 of chunk r / 4, dims 64 a + 16 g + [0, 16).
+        const int base = BS > kChunk ? (c0 + c + (r >> 2)) * kChunk % BS : 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = 4 * j / PT, slot = base + (4 * j) % PT + (r & 3);
+            const int id_ = id.k[n];
+            if (in_pool(id_)) {
+                const uint8_t* run = p.pages.data + run_offset<D, BS>(p.pages, id_, kvh, 0) + slot * 64 + 16 * g;
+#pragma unroll
+                for (int a = 0; a < KA; ++a) rg.k[j][a] = *reinterpret_cast<const uint4*>(run + a * (BS * 64));
             }
         }
-        if (phys >= 0) {
-            const uint8_t* run = p.pages.data + run_offset<D, BS>(p.pages, phys, kvh, 0) + (t % BS) * 64;
-            s = 0.0f;
-            for (int d = 0; d < D; ++d) s += qs[d] * ((float)run[(d / 64) * (BS * 64) + d % 64] - 128.0f);
-            s *= scale_of(p.pages.codes[code_offset(p.pages, phys, kvh, 0)]);
+    };
+    auto load_v = [&](int c, const Ids& id) {
+        // Token row of dim 16 e + r, chunk g; zero scale where there is no page.
+        const int base = BS > kChunk ? (c0 + c + g) * kChunk % BS : 0;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            rg.codes[n] = 0;
+            if (in_pool(id.v[n])) {
+                rg.codes[n] = *reinterpret_cast<const uint16_t*>(p.pages.codes + code_offset(p.pages, id.v[n], kvh, 0));
+                const uint8_t* run = p.pages.data + run_offset<D, BS>(p.pages, id.v[n], kvh, 1) + r * BS + base;
+#pragma unroll
+                for (int e = 0; e < D / 16; ++e) {
+                    const uint8_t* src = run + e * (16 * BS);
+                    if constexpr (PT == 16) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(src);
+                        rg.v[e][0] = w.x, rg.v[e][1] = w.y, rg.v[e][2] = w.z, rg.v[e][3] = w.w;
+                    } else if constexpr (PT == 8) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(src);
+                        rg.v[e][2 * n] = w.x, rg.v[e][2 * n + 1] = w.y;
+                    } else {
+                        rg.v[e][n] = *reinterpret_cast<const uint32_t*>(src);
+                    }
+                }
+            }
         }
-        float mx = s;
-        for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        const float mn = fmaxf(m, mx), ref = mn == kNegInf ? 0.0f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
-        const float pr = phys >= 0 ? __builtin_amdgcn_exp2f(s - ref) : 0.0f;
-        m = mn;
-        l = l * alpha + pr;
-        ps[wave][lane] = pr;
-        pg[wave][lane] = phys;
-        __builtin_amdgcn_wave_barrier();
-        for (int j = 0; j < DP; ++j) acc[j] *= alpha;
-        for (int i = 0; i < 64; ++i) {
-            const int ph = pg[wave][i];
-            if (ph < 0) continue;
-            const uint8_t* run = p.pages.data + run_offset<D, BS>(p.pages, ph, kvh, 1) + (t0 + i) % BS;
-            const float w = ps[wave][i] * scale_of(p.pages.codes[code_offset(p.pages, ph, kvh, 1)]);
-            for (int j = 0; j < DP; ++j) acc[j] += w * ((float)run[(lane * DP + j) * BS] - 128.0f);
+    };
+
+    Ids id, next;
+    load_ids(0, id);
+    load_k(0, id);
+    load_v(0, id);
+    load_ids(kStep, next);
+    for (int c = 0; c < nc; c += kStep) {
+        // Scores of tokens 4 j + i of chunk g.
+        float4v s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            s[j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int a = 0; a < KA; ++a) {
+                s[j] = Elt<BF16>::mma32(integers8<BF16>(rg.k[j][a].x, rg.k[j][a].y), qf[2 * a], s[j]);
+                s[j] = Elt<BF16>::mma32(integers8<BF16>(rg.k[j][a].z, rg.k[j][a].w), qf[2 * a + 1], s[j]);
+            }
         }
-        __builtin_amdgcn_wave_barrier();
+        if (c + kStep < nc) load_k(c + kStep, next);
+        bool live[NP];
+        float vs[NP];
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            live[n] = in_pool(id.v[n]);
+            if (!live[n] && r == 0 && p.err && c + g < nc && (c0 + c + g) * kChunk / BS + n < nblk) atomicOr(p.err, 4);
+            vs[n] = scale_of((int)(rg.codes[n] >> 8));
+        }
+        const int t0 = (c0 + c + g) * kChunk;
+        float mx = kNegInf;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = 4 * j / PT;
+            const float ks = scale_of((int)(rg.codes[n] & 0xffu)) * p.scale_log2e;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[j][i] = live[n] && t0 + 4 * j + i < tokens ? s[j][i] * ks : kNegInf;
+                mx = fmaxf(mx, s[j][i]);
+            }
+        }
+        if (__builtin_amdgcn_ballot_w64(mx > st.m + kLazyLog2) != 0) {
+            mx = xor_max_16_32(mx);  // all lane groups of a head move together
+            const bool grow = mx > st.m + kLazyLog2;
+            const float now = grow ? mx : st.m;
+            const float alpha = grow ? __builtin_amdgcn_exp2f(st.m - now) : 1.0f;  // 0 from -inf
+            st.l *= alpha;
+#pragma unroll
+            for (int e = 0; e < D / 16; ++e) st.acc[e] *= alpha;
+            st.m = now;
+        }
+        const float ref = st.m == kNegInf ? 0.0f : st.m;
+        half8v pv[2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const _Float16 w = Elt<BF16>::round(__builtin_amdgcn_exp2f(s[j][i] - ref));
+                pv[j / 2][4 * (j & 1) + i] = w;
+                st.l += Elt<BF16>::widen(w);
+            }
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const half8v a = values4x2<BF16>(rg.v[e][2 * u], rg.v[e][2 * u + 1], vs[8 * u / PT], vs[(8 * u + 4) / PT]);
+                st.acc[e] = Elt<BF16>::mma32(a, pv[u], st.acc[e]);
+            }
+        if (c + kStep < nc) load_v(c + kStep, next);
+        id = next;
+        load_ids(c + 2 * kStep, next);
     }
-    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    st.l = xor_sum_16_32(st.l);
+}
+
+// A finished segment's output.
+template <int D, bool BF16>
+__device__ __forceinline__ void write_out(const AttnParams& p, int b, int h0, int nh, int lane, const Piece<D>& st) {
+    const int g = lane >> 4, r = lane & 15;
+    if (r >= nh) return;
+    const float inv = st.l == 0.0f ? 0.0f : 1.0f / st.l;
+    uint16_t* o = p.out + (int64_t)b * p.o_sb + (int64_t)(h0 + r) * p.o_sh + 4 * g;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) {
+        half4v v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = Elt<BF16>::round(st.acc[e][i] * inv);
+        *reinterpret_cast<uint2*>(o + 16 * e) = __builtin_bit_cast(uint2, v);
+    }
+}
+
+__device__ __forceinline__ void heads_of(const AttnParams& p, int vh, int& kvh, int& h0, int& nh) {
+    kvh = vh / p.NG;
+    const int first = (vh - kvh * p.NG) * p.GS;
+    h0 = kvh * p.G + first;
+    nh = p.G - first < p.GS ? p.G - first : p.GS;
+}
+
+template <int D, int BS, bool BF16>
+__global__ __launch_bounds__(kAttnWaves * 64, 2) void kv8_attn_kernel(AttnParams p) {
+    const int lane = threadIdx.x & 63;
+    const int w = blockIdx.x * kAttnWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Piece<D> st;
+    int kvh, h0, nh;
+    if (p.workers == 0) {
+        if (w >= p.B * p.Hv) return;
+        const int b = w / p.Hv;
+        heads_of(p, w - b * p.Hv, kvh, h0, nh);
+        const int tokens = __builtin_amdgcn_readfirstlane(row_tokens<BS>(p, b));
+        run_piece<D, BS, BF16>(p, b, kvh, h0, nh, 0, chunks_of(tokens), tokens, lane, st);
+        write_out<D, BF16>(p, b, h0, nh, lane, st);
+        return;
+    }
+    // Up to 64 rows: one read of the lengths, a row a lane. More: their sum first, then 64 at a time.
+    const bool one_pass = p.B <= 64;
+    int at = 0, before = 0, tok = 0, incl = 0, total;  // rows [at, at + 64) in the lanes; chunks before them
+    if (!one_pass) sum_rows<BS>(p, 0, lane, before, total);
+    auto load_rows = [&]() {
+        tok = at + lane < p.B ? row_tokens<BS>(p, at + lane) : 0;
+        incl = incl_scan(chunks_of(tok), lane);
+    };
+    load_rows();
+    if (one_pass) total = __builtin_amdgcn_readlane(incl, 63);
+    const Cut cut(total * p.Hv, p.workers);
+    if (w >= cut.W) return;
+    int x = cut.lo(w);
+    const int x0 = x, hi = cut.lo(w + 1);
+    while (x < hi) {
+        while (!one_pass && (before + __builtin_amdgcn_readlane(incl, 63)) * p.Hv <= x && at + 64 < p.B) {
+            before += __builtin_amdgcn_readlane(incl, 63);
+            at += 64;
+            load_rows();
+        }
+        // The last row that begins at or before chunk x: a row without tokens ends where it begins.
+        const int first = before + incl - chunks_of(tok);
+        const int i = __builtin_popcountll(__builtin_amdgcn_ballot_w64(at + lane < p.B && first * p.Hv <= x)) - 1;
+        const int tokens = __builtin_amdgcn_readlane(tok, i), n = chunks_of(tokens), b = at + i;
+        const int rel = x - __builtin_amdgcn_readlane(first, i) * p.Hv;
+        const int vh = n > 0 ? rel / n : p.Hv, c0 = rel - vh * n;
+        const int nc = n - c0 < hi - x ? n - c0 : hi - x;
+        if (nc <= 0 || vh >= p.Hv) break;  // cannot happen for lengths that stay as they are
+        heads_of(p, vh, kvh, h0, nh);
+        run_piece<D, BS, BF16>(p, b, kvh, h0, nh, c0, nc, tokens, lane, st);
+        if (nc == n) {
+            write_out<D, BF16>(p, b, h0, nh, lane, st);
+        } else {
+            // A range holds at most two shared pieces: the one it begins with and the one it ends with.
+            const int64_t slot = 2 * (int64_t)w + (x == x0 ? 0 : 1);
+            const int g = lane >> 4, r = lane & 15;
+            if (r < nh) {
+                if (g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * p.GS + r) * 2) = float2{st.m, st.l};
+                float* a = p.part_acc + (slot * p.GS + r) * D + 4 * g;
+#pragma unroll
+                for (int e = 0; e < D / 16; ++e) *reinterpret_cast<float4v*>(a + 16 * e) = st.acc[e];
+            }
+        }
+        x += nc;
+    }
+}
+
+// Joins a segment's pieces and writes its heads; zeros for a row without tokens. One workgroup per query
+// head and row; its waves share the pieces, a lane D / 64 dims.
+constexpr int kMergeWaves = 4;
+template <int D, int BS, bool BF16>
+__global__ __launch_bounds__(kMergeWaves * 64) void kv8_merge_kernel(AttnParams p) {
+    constexpr int DP = D / 64;
+    typedef float VecT __attribute__((ext_vector_type(DP)));
+    __shared__ float red[kMergeWaves][D + 2];
+    const int h = blockIdx.x, b = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kvh = h / p.G, hg = h - kvh * p.G;
+    const int vh = kvh * p.NG + hg / p.GS, r = hg % p.GS;
+    int before, total;
+    sum_rows<BS>(p, b, lane, before, total);
+    const int n = chunks_of(row_tokens<BS>(p, b));
+    uint16_t* o = p.out + (int64_t)b * p.o_sb + (int64_t)h * p.o_sh;
+    if (n == 0) {
+        if (threadIdx.x < D) o[threadIdx.x] = 0;
+        return;
+    }
+    const Cut cut(total * p.Hv, p.workers);
+    const int x = before * p.Hv + vh * n;
+    const int w0 = cut.worker_of(x), np = cut.worker_of(x + n - 1) - w0 + 1;
+    if (np == 1) return;  // one wave had the whole segment and wrote it
+    const float kNegInf = -__builtin_huge_valf();
+    float m = kNegInf, l = 0.0f;
+    VecT acc = 0.0f;
+    const bool cut_first = cut.lo(w0) < x;  // the first piece is its range's last, not its first
+    for (int k = wave; k < np; k += kMergeWaves) {
+        const int64_t slot = (2 * (int64_t)(w0 + k) + (k == 0 && cut_first ? 1 : 0)) * p.GS + r;
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+        const VecT a = *reinterpret_cast<const VecT*>(p.part_acc + slot * D + lane * DP);
+        const float now = fmaxf(m, ml.x), ref = now == kNegInf ? 0.0f : now;
+        const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(ml.x - ref);
+        l = l * f0 + ml.y * f1;
+        acc = acc * f0 + a * f1;
+        m = now;
+    }
+#pragma unroll
     for (int j = 0; j < DP; ++j) red[wave][lane * DP + j] = acc[j];
     if (lane == 0) {
         red[wave][D] = m;
         red[wave][D + 1] = l;
     }
     __syncthreads();
-    if (threadIdx.x < D) {
-        float mx = kNegInf;
-        for (int w = 0; w < kAttnWaves; ++w) mx = fmaxf(mx, red[w][D]);
-        const float ref = mx == kNegInf ? 0.0f : mx;
-        float num = 0.0f, den = 0.0f;
-        for (int w = 0; w < kAttnWaves; ++w) {
-            const float a = __builtin_amdgcn_exp2f(red[w][D] - ref);
-            num += a * red[w][threadIdx.x];
-            den += a * red[w][D + 1];
-        }
-        const float o = den == 0.0f ? 0.0f : num / den;
-        uint16_t* dst = p.out + (int64_t)b * p.o_sb + (int64_t)h * p.o_sh + threadIdx.x;
-        *dst = __builtin_bit_cast(uint16_t, Elt<BF16>::round(o));
+    if (threadIdx.x >= D) return;
+    float mx = kNegInf;
+#pragma unroll
+    for (int i = 0; i < kMergeWaves; ++i) mx = fmaxf(mx, red[i][D]);
+    const float ref = mx == kNegInf ? 0.0f : mx;
+    float num = 0.0f, den = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMergeWaves; ++i) {
+        const float f = __builtin_amdgcn_exp2f(red[i][D] - ref);
+        num += f * red[i][threadIdx.x];
+        den += f * red[i][D + 1];
     }
+    o[threadIdx.x] = __builtin_bit_cast(uint16_t, Elt<BF16>::round(den == 0.0f ? 0.0f : num / den));
+}
+
+// Waves of a launch, by the table's width: 0 where every segment goes to one wave.
+static int workers_for(int64_t max_tokens) {
+    return ceil_div(max_tokens, kChunk) <= kDirectChunks ? 0 : kWorkers;
+}
+
+static void head_groups(int G, int& NG, int& GS) {
+    NG = (int)ceil_div(G, kHeads);
+    GS = (int)ceil_div(G, NG);
+    NG = (int)ceil_div(G, GS);
 }
 
 }  // namespace kv8
@@ -112,7 +449,10 @@ using namespace mx;
 
 extern "C" size_t mx_kv8_attn_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_blocks,
                                               int32_t block_size) {
-    return 0;
+    if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_blocks <= 0 || block_size <= 0 || Hq % Hkv != 0) return 0;
+    int NG, GS;
+    kv8::head_groups(Hq / Hkv, NG, GS);
+    return (size_t)2 * kv8::workers_for((int64_t)max_blocks * block_size) * GS * (D + 2) * sizeof(float);
 }
 
 extern "C" int mx_kv8_attn_decode(const uint16_t* q, int64_t q_sb, int64_t q_sh, const uint8_t* data,
@@ -134,15 +474,41 @@ extern "C" int mx_kv8_attn_decode(const uint16_t* q, int64_t q_sb, int64_t q_sh,
     if (flags & ~(uint32_t)MX_PA_BF16) return fail(MX_ERR_INVALID, "%s: unknown flags 0x%x", what, flags);
     if (!aligned(q, 16) || q_sb % 8 || q_sh % 8 || !aligned(out, 16) || o_sb % 8 || o_sh % 8)
         return fail(MX_ERR_ALIGNMENT, "%s: q and out rows must be 16-byte aligned", what);
-    kv8::AttnParams p{q, q_sb, q_sh, {const_cast<uint8_t*>(data), const_cast<uint8_t*>(codes), Hkv, num_blocks},
-                      block_tables, bt_sb, max_blocks, seq_lens, Hq, Hq / Hkv, scale * 1.4426950408889634f, out, o_sb,
-                      o_sh, err};
+    if (!aligned(codes, 2)) return fail(MX_ERR_ALIGNMENT, "%s: codes must be 2-byte aligned", what);
+    const int64_t max_tokens = (int64_t)max_blocks * block_size;
+    kv8::AttnParams p{};
+    p.q = q, p.q_sb = q_sb, p.q_sh = q_sh;
+    p.pages = {const_cast<uint8_t*>(data), const_cast<uint8_t*>(codes), Hkv, num_blocks};
+    p.bt = block_tables, p.bt_sb = bt_sb, p.max_blocks = max_blocks, p.seq_lens = seq_lens;
+    p.B = B, p.G = Hq / Hkv;
+    kv8::head_groups(p.G, p.NG, p.GS);
+    p.Hv = Hkv * p.NG;
+    if (max_tokens > kv8::kMaxTokens || (int64_t)B * p.Hv * ceil_div(max_tokens, kv8::kChunk) > (int64_t)1 << 30)
+        return fail(MX_ERR_UNSUPPORTED, "%s: more tokens than 32-bit numbers hold", what);
+    p.workers = kv8::workers_for(max_tokens);
+    p.scale_log2e = scale * 1.4426950408889634f;
+    p.out = out, p.o_sb = o_sb, p.o_sh = o_sh, p.err = err;
+    if (p.workers > 0) {
+        const size_t need = mx_kv8_attn_workspace_bytes(B, Hq, Hkv, D, max_blocks, block_size);
+        if (!workspace || workspace_bytes < need)
+            return fail(MX_ERR_WORKSPACE, "%s: workspace needs %zu bytes, got %zu", what, need, workspace_bytes);
+        if (!aligned(workspace, 256)) return fail(MX_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", what);
+        p.part_acc = static_cast<float*>(workspace);
+        p.part_ml = p.part_acc + (size_t)2 * p.workers * p.GS * D;
+    }
+    const int64_t waves = p.workers > 0 ? p.workers : (int64_t)B * p.Hv;
+    const dim3 grid((unsigned)ceil_div(waves, kv8::kAttnWaves)), block(kv8::kAttnWaves * 64);
     hipStream_t st = as_stream(stream);
-#define CALL(DD, BB)                                                                                                   \
-    if (flags & MX_PA_BF16)                                                                                            \
-        hipLaunchKernelGGL((kv8::kv8_attn_kernel<DD, BB, true>), dim3(Hq, B), dim3(kv8::kAttnWaves * 64), 0, st, p);    \
-    else                                                                                                               \
-        hipLaunchKernelGGL((kv8::kv8_attn_kernel<DD, BB, false>), dim3(Hq, B), dim3(kv8::kAttnWaves * 64), 0, st, p)
+#define CALL(DD, BB)                                                                                             \
+    if (flags & MX_PA_BF16) {                                                                                    \
+        hipLaunchKernelGGL((kv8::kv8_attn_kernel<DD, BB, true>), grid, block, 0, st, p);                         \
+        if (p.workers > 0)                                                                                       \
+            hipLaunchKernelGGL((kv8::kv8_merge_kernel<DD, BB, true>), dim3(Hq, B), dim3(kv8::kMergeWaves * 64), 0, st, p);  \
+    } else {                                                                                                     \
+        hipLaunchKernelGGL((kv8::kv8_attn_kernel<DD, BB, false>), grid, block, 0, st, p);                        \
+        if (p.workers > 0)                                                                                       \
+            hipLaunchKernelGGL((kv8::kv8_merge_kernel<DD, BB, false>), dim3(Hq, B), dim3(kv8::kMergeWaves * 64), 0, st, p); \
+    }
     MX_KV8_DISPATCH(D, block_size, CALL)
 #undef CALL
     return check_launch(what);
