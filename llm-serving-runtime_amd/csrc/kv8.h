@@ -64,16 +64,29 @@ __device__ __forceinline__ float widen(uint32_t bits) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
 
-// q + 128 of x at the scale whose inverse is inv (0 for a poisoned page: any byte will do).
-__device__ __forceinline__ uint32_t quant_byte(float x, float inv, bool poisoned) {
-    const float r = __builtin_amdgcn_fmed3f(__builtin_rintf(x * inv), -127.0f, 127.0f);
-    return poisoned ? 128u : (uint32_t)((int)r + 128);
-}
-__device__ __forceinline__ float inverse_of(int code) {
-    return __uint_as_float((uint32_t)(254 - code) << 23);  // unused for 255
-}
+// Quantising at a run's scale: q = rne(x / 2^e), at most 127 in magnitude. x is clamped to 127 * 2^e
+// first (only the largest fp16 numbers need it, where e has reached its cap; a NaN comes out finite), then
+// one fused multiply-add puts q + 128 into the low byte: its product is exact and its sum is rounded, to
+// nearest even, at the units' place. A poisoned run stores q = 0.
+struct Quant {
+    float inv, lim;
+    __device__ __forceinline__ explicit Quant(int code) {
+        const bool poisoned = code == kPoison;
+        inv = __uint_as_float(poisoned ? 0u : (uint32_t)(254 - code) << 23);
+        lim = poisoned ? 0.0f : 127.0f * __uint_as_float((uint32_t)code << 23);
+    }
+    __device__ __forceinline__ uint32_t byte(float x) const {  // in the low byte; the others are not 0
+        constexpr float kUnits = 12582912.0f + 128.0f;  // 1.5 * 2^23: units' place is the last bit
+        return __float_as_uint(__builtin_fmaf(__builtin_amdgcn_fmed3f(x, -lim, lim), inv, kUnits));
+    }
+    __device__ __forceinline__ uint32_t word(float x0, float x1, float x2, float x3) const {
+        const uint32_t lo = __builtin_amdgcn_perm(byte(x1), byte(x0), 0x00000400u);
+        const uint32_t hi = __builtin_amdgcn_perm(byte(x3), byte(x2), 0x00000400u);
+        return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+    }
+};
 
-// Four kept bytes at a page's new, larger scale: rne(q 2^(old - now)). old = 0: nothing was there.
+// Four kept bytes at a run's new, larger scale: rne(q 2^(old - now)). old = 0: nothing was there.
 __device__ __forceinline__ uint32_t requant4(uint32_t w, float factor) {
     uint32_t out = 0;
 #pragma unroll
@@ -131,15 +144,24 @@ __device__ __forceinline__ half8v values8(uint32_t d0, uint32_t d1, float s) {
     return values4x2<BF16>(d0, d1, s, s);
 }
 
-// Largest 16-bit half of v over the wave (every lane gets it).
+// Largest 16-bit half of v over the wave (every lane gets it): row rotations, then row exchanges.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t m) {
+    const uint32_t t = (uint32_t)__builtin_amdgcn_mov_dpp((int)m, CTRL, 0xf, 0xf, false);
+    return t > m ? t : m;
+}
 __device__ __forceinline__ uint32_t wave_max_u16x2(uint32_t v) {
     uint32_t m = (v & 0xffffu) > (v >> 16) ? (v & 0xffffu) : v >> 16;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t t = (uint32_t)__shfl_xor((int)m, o);
-        m = t > m ? t : m;
-    }
-    return m;
+    m = dpp_max<0x128>(m);  // row_ror:8, 4, 2, 1
+    m = dpp_max<0x124>(m);
+    m = dpp_max<0x122>(m);
+    m = dpp_max<0x121>(m);
+    float a = __uint_as_float(m), b = a;
+    row_swap16(a, b);
+    m = __float_as_uint(a) > __float_as_uint(b) ? __float_as_uint(a) : __float_as_uint(b);
+    a = b = __uint_as_float(m);
+    row_swap32(a, b);
+    return __float_as_uint(a) > __float_as_uint(b) ? __float_as_uint(a) : __float_as_uint(b);
 }
 typedef uint16_t u16x2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {

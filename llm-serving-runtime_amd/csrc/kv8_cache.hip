@@ -53,30 +53,39 @@ __device__ __forceinline__ void regrow_k(uint8_t* run, int o, Codes c, int lane)
     }
 }
 
+// Bytes [lo, hi) of the 4-byte word that begins at byte `at`.
+__device__ __forceinline__ uint32_t byte_mask(int lo, int hi, int at) {
+    const int a = lo - at < 0 ? 0 : (lo - at > 4 ? 4 : lo - at), b = hi - at < 0 ? 0 : (hi - at > 4 ? 4 : hi - at);
+    return (uint32_t)(((uint64_t)1 << (8 * b)) - ((uint64_t)1 << (8 * a)));  // 0 where a == b
+}
+
 // The whole V run: kept tokens below slot o, new ones in [o, e), zero from e on. x[s]: the lane's
 // D / 64 dims of slot s (16-bit patterns, low half first).
 template <int D, int BS, bool BF16>
 __device__ __forceinline__ void store_v(uint8_t* run, int o, int e, Codes c, const uint32_t (&x)[BS],
                                         const uint32_t (&kept)[D / 64][BS / 4], int lane) {
     constexpr int DP = D / 64, W = BS / 4;
-    const bool poisoned = c.now == kPoison;
-    const float inv = inverse_of(c.now), f = growth_factor(c.old, c.now);
+    const Quant quant(c.now);
     uint32_t row[DP * W];
 #pragma unroll
-    for (int j = 0; j < DP; ++j)
+    for (int w = 0; w < W; ++w) {
+        const uint32_t fresh = byte_mask(o, e, 4 * w), was = byte_mask(0, o, 4 * w);
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const uint32_t was = c.old == c.now ? kept[j][w] : requant4(kept[j][w], f);
-            uint32_t out = 0;
+        for (int j = 0; j < DP; ++j) {
+            float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int s = 4 * w + i;
-                const uint32_t fresh = quant_byte(widen<BF16>(j == 0 ? x[s] & 0xffffu : x[s] >> 16), inv, poisoned);
-                const uint32_t byte = s < o ? (was >> (8 * i)) & 0xffu : (s < e ? fresh : 128u);
-                out |= byte << (8 * i);
-            }
-            row[j * W + w] = out;
+            for (int i = 0; i < 4; ++i) v[i] = widen<BF16>(j == 0 ? x[4 * w + i] & 0xffffu : x[4 * w + i] >> 16);
+            row[j * W + w] = (quant.word(v[0], v[1], v[2], v[3]) & fresh) | (0x80808080u & ~(fresh | was));
         }
+    }
+    if (o > 0) {
+        const float f = growth_factor(c.old, c.now);
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int j = 0; j < DP; ++j)
+                row[j * W + w] |= (c.old == c.now ? kept[j][w] : requant4(kept[j][w], f)) & byte_mask(0, o, 4 * w);
+    }
     uint8_t* dst = run + lane * (DP * BS);
     if constexpr (DP * W % 4 == 0) {
 #pragma unroll
@@ -105,21 +114,21 @@ __device__ __forceinline__ void load_v(const uint8_t* run, int o, uint32_t (&kep
         for (int w = 0; w < W; ++w) kept[j][w] = src[j * W + w];
 }
 
-// Grows a run's scale to hold `bits` (the new tokens' largest magnitude) and stores it.
+// Grows a run's scale to hold `bits` (the new tokens' largest magnitude) and stores it. old: the scale it
+// had where tokens are kept, else 0.
 template <bool BF16>
-__device__ __forceinline__ Codes grow(uint8_t* code, int o, int old, uint32_t bits, int lane) {
+__device__ __forceinline__ Codes grow(uint8_t* code, int old, uint32_t bits, int lane) {
     const int need = code_of<BF16>(bits);
-    const int was = o > 0 ? old : 0;
-    const int now = was > need ? was : need;
+    const int now = old > need ? old : need;
     if (lane == 0) *code = (uint8_t)now;
-    return Codes{was, now};
+    return Codes{old, now};
 }
 
 template <int D, int BS, bool BF16>
 __global__ __launch_bounds__(kWaves * 64) void kv8_write_kernel(WriteParams p) {
     constexpr int CH = D / 8;        // 8-dim pieces of a token
     constexpr int TPI = 64 / CH;     // tokens of one K load
-    constexpr int NI = (BS + TPI - 1) / TPI;
+    constexpr int NI = (BS + TPI - 1) / TPI, DP = D / 64;
     const int lane = threadIdx.x & 63;
     int64_t u = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (u >= p.units) return;
@@ -139,64 +148,61 @@ __global__ __launch_bounds__(kWaves * 64) void kv8_write_kernel(WriteParams p) {
     const bool flags = lane == 0 && kind == 0 && h == 0 && p.err;
     if (start < 0 && j == 0 && flags) atomicOr(p.err, 1);
     if (lo >= hi) return;
+    const int o = (int)(lo - lb * BS), e = (int)(hi - lb * BS);
+    // The new tokens, all loads at once and ahead of the page's: slots outside [o, e) load a neighbour's
+    // token again, which a branch per slot would not be faster than.
+    const int64_t src = (int64_t)b * p.sb + (int64_t)h * p.sh + (lo - start) * p.st;
+    auto offset = [&](int s) { return (int64_t)((s < o ? o : (s < e ? s : e - 1)) - o) * p.st; };
+    uint4 xk[NI];
+    uint32_t xv[BS];
+    if (kind == 0) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            xk[i] = glue::ld16(p.k_new + src + offset(i * TPI + lane / CH) + (lane % CH) * 8);
+    } else {
+#pragma unroll
+        for (int s = 0; s < BS; ++s) {
+            const uint16_t* q = p.v_new + src + offset(s) + lane * DP;
+            xv[s] = DP == 2 ? *reinterpret_cast<const uint32_t*>(q) : (uint32_t)*q;
+        }
+    }
     const int phys = lb < p.max_blocks ? p.bt[(int64_t)b * p.bt_sb + lb] : -1;
     if ((unsigned)phys >= (unsigned)p.pages.num_blocks) {
         if (flags) atomicOr(p.err, 1);
         return;
     }
-    const int o = (int)(lo - lb * BS), e = (int)(hi - lb * BS);
-    const int64_t t0 = lb * BS - start;  // token of slot 0
     uint8_t* run = p.pages.data + run_offset<D, BS>(p.pages, phys, h, kind);
     uint8_t* code = p.pages.codes + code_offset(p.pages, phys, h, kind);
-    const int old = *code;
-    const int64_t src = (int64_t)b * p.sb + (int64_t)h * p.sh;
+    const int old = o > 0 ? *code : 0;
+    uint32_t m = 0;
     if (kind == 0) {
         if (p.used && h == 0 && lane == 0) p.used[phys] = 1;
-        const int c = lane % CH;
-        uint4 x[NI];
-        uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int s = i * TPI + lane / CH;
-            x[i] = uint4{0, 0, 0, 0};
-            if (s >= o && s < e) x[i] = glue::ld16(p.k_new + src + (t0 + s) * p.st + c * 8);
+            m = max_u16x2(m, max_u16x2(xk[i].x & 0x7fff7fffu, xk[i].y & 0x7fff7fffu));
+            m = max_u16x2(m, max_u16x2(xk[i].z & 0x7fff7fffu, xk[i].w & 0x7fff7fffu));
         }
+        const Codes cd = grow<BF16>(code, old, wave_max_u16x2(m), lane);
+        if (cd.now != cd.old && cd.now != kPoison) regrow_k<D, BS>(run, o, cd, lane);
+        const Quant quant(cd.now);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            m = max_u16x2(m, max_u16x2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu));
-            m = max_u16x2(m, max_u16x2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
-        }
-        const Codes cd = grow<BF16>(code, o, old, wave_max_u16x2(m), lane);
-        if (o > 0 && cd.now != cd.old && cd.now != kPoison) regrow_k<D, BS>(run, o, cd, lane);
-        const bool poisoned = cd.now == kPoison;
-        const float inv = inverse_of(cd.now);
+            const int s = i * TPI + lane / CH, d = (lane % CH) * 8;
+            const uint32_t w[4] = {xk[i].x, xk[i].y, xk[i].z, xk[i].w};
+            float v[8];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int s = i * TPI + lane / CH;
-            if (s < o || s >= e) continue;
-            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-            uint32_t out[2] = {0, 0};
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-                out[q / 4] |= quant_byte(widen<BF16>((w[q / 2] >> (16 * (q & 1))) & 0xffffu), inv, poisoned) << (8 * (q & 3));
-            *reinterpret_cast<uint2*>(run + (c * 8 / 64) * (BS * 64) + s * 64 + c * 8 % 64) = uint2{out[0], out[1]};
+            for (int q = 0; q < 8; ++q) v[q] = widen<BF16>(q & 1 ? w[q / 2] >> 16 : w[q / 2] & 0xffffu);
+            if (s >= o && s < e)
+                *reinterpret_cast<uint2*>(run + (d / 64) * (BS * 64) + s * 64 + d % 64) =
+                    uint2{quant.word(v[0], v[1], v[2], v[3]), quant.word(v[4], v[5], v[6], v[7])};
         }
     } else {
-        constexpr int DP = D / 64;
-        uint32_t x[BS], kept[DP][BS / 4], m = 0;
+        uint32_t kept[DP][BS / 4];
         load_v<D, BS>(run, o, kept, lane);
 #pragma unroll
-        for (int s = 0; s < BS; ++s) {
-            x[s] = 0;
-            if (s >= o && s < e) {
-                const uint16_t* q = p.v_new + src + (t0 + s) * p.st + lane * DP;
-                x[s] = DP == 2 ? *reinterpret_cast<const uint32_t*>(q) : (uint32_t)*q;
-            }
-        }
-#pragma unroll
-        for (int s = 0; s < BS; ++s) m = max_u16x2(m, x[s] & 0x7fff7fffu);
-        const Codes cd = grow<BF16>(code, o, old, wave_max_u16x2(m), lane);
-        store_v<D, BS, BF16>(run, o, e, cd, x, kept, lane);
+        for (int s = 0; s < BS; ++s) m = max_u16x2(m, xv[s] & 0x7fff7fffu);
+        const Codes cd = grow<BF16>(code, old, wave_max_u16x2(m), lane);
+        store_v<D, BS, BF16>(run, o, e, cd, xv, kept, lane);
     }
 }
 
@@ -375,21 +381,20 @@ __global__ __launch_bounds__(kWaves * 64) void kv8_token_kernel(TokenParams p) {
     }
     uint8_t* run = p.pages.data + run_offset<D, BS>(p.pages, phys, kvh, is_v);
     uint8_t* code = p.pages.codes + code_offset(p.pages, phys, kvh, is_v);
-    const int old = *code;
+    const int old = o > 0 ? *code : 0;
     uint32_t m = x[0];
     if constexpr (DP == 2) m |= x[1] << 16;
     if (!is_v) {
         if (p.used && kvh == 0 && lane == 0) p.used[phys] = 1;
-        const Codes cd = grow<BF16>(code, o, old, wave_max_u16x2(m & 0x7fff7fffu), lane);
-        if (o > 0 && cd.now != cd.old && cd.now != kPoison) regrow_k<D, BS>(run, o, cd, lane);
-        const float inv = inverse_of(cd.now);
+        const Codes cd = grow<BF16>(code, old, wave_max_u16x2(m & 0x7fff7fffu), lane);
+        if (cd.now != cd.old && cd.now != kPoison) regrow_k<D, BS>(run, o, cd, lane);
+        const Quant quant(cd.now);
 #pragma unroll
-        for (int j = 0; j < DP; ++j)
-            run[j * (BS * 64) + o * 64 + lane] = (uint8_t)quant_byte(widen<BF16>(x[j]), inv, cd.now == kPoison);
+        for (int j = 0; j < DP; ++j) run[j * (BS * 64) + o * 64 + lane] = (uint8_t)quant.byte(widen<BF16>(x[j]));
     } else {
         uint32_t kept[DP][BS / 4], xs[BS];
         load_v<D, BS>(run, o, kept, lane);
-        const Codes cd = grow<BF16>(code, o, old, wave_max_u16x2(m & 0x7fff7fffu), lane);
+        const Codes cd = grow<BF16>(code, old, wave_max_u16x2(m & 0x7fff7fffu), lane);
 #pragma unroll
         for (int s = 0; s < BS; ++s) xs[s] = m;
         store_v<D, BS, BF16>(run, o, o + 1, cd, xs, kept, lane);

@@ -15,7 +15,7 @@
 namespace mx {
 namespace pages {
 
-constexpr int kBatch = 256;    // page pairs per launch: 2 KiB of kernel arguments
+constexpr int kBatch = 448;    // page pairs per launch: 3.5 KiB of the 4 KiB of kernel arguments
 constexpr int kThreads = 256;
 
 struct Region {
@@ -121,6 +121,8 @@ struct ClearParams {
     int n;
     int id[2 * kBatch];
 };
+static_assert(sizeof(CopyParams) < 4000 && sizeof(RenameParams) < 4000 && sizeof(ClearParams) < 4000,
+              "kernel arguments");
 
 __global__ __launch_bounds__(kThreads) void clear_kernel(ClearParams p) {
     const int id = p.id[blockIdx.x];

@@ -38,7 +38,7 @@ MI355X-first differences:
   ``sync_write_checks`` (or ``PHASE2_KV_SYNC_CHECKS=1`` before the pool is
   built): every batched write then checks the word right away (one host sync
   per call, skipped while a HIP graph is being captured).
-* ``copy_blocks`` on a device pool is one ``mx_kv_copy_pages`` launch per 256
+* ``copy_blocks`` on a device pool is one ``mx_kv_copy_pages`` launch per 448
   pages whose ids travel with it; beside it stand ``move_blocks`` (compaction:
   pages to other ids, the block tables that name them renamed) and
   ``free_blocks``. The reference has neither: its pool only ever adds to its
@@ -96,6 +96,8 @@ class GpuKVBlockPool:
         self.device = torch.device(device)
         self._k_pool: torch.Tensor | None = None
         self._v_pool: torch.Tensor | None = None
+        self._k_views: tuple[torch.Tensor, ...] = ()  # k_layer_view's, made once: a step asks 2 L times
+        self._v_views: tuple[torch.Tensor, ...] = ()
         self._regions: list[torch.Tensor] = []  # the tensors [L, num_blocks, ...] that hold the pages
         self._used_blocks: set[int] = set()
         self._peak_allocated_blocks = 0
@@ -162,6 +164,7 @@ class GpuKVBlockPool:
             self._k_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
             self._v_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
             self._regions = [self._k_pool, self._v_pool]
+        self._k_views, self._v_views = self._k_pool.unbind(0), self._v_pool.unbind(0)
         if self.device.type == "cuda":
             self._used_map = torch.zeros(s.num_blocks, dtype=torch.uint8, device=self.device)
             self._write_err = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -193,14 +196,12 @@ class GpuKVBlockPool:
     def k_layer_view(self, layer_idx: int) -> torch.Tensor:
         """Per-layer K blocks: ``[num_blocks, num_kv_heads, block_size, head_dim]``."""
         self._ensure_pools()
-        assert self._k_pool is not None
-        return self._k_pool.select(0, layer_idx)
+        return self._k_views[layer_idx]
 
     def v_layer_view(self, layer_idx: int) -> torch.Tensor:
         """Per-layer V blocks: ``[num_blocks, num_kv_heads, block_size, head_dim]``."""
         self._ensure_pools()
-        assert self._v_pool is not None
-        return self._v_pool.select(0, layer_idx)
+        return self._v_views[layer_idx]
 
     def write_tokens(self, layer_idx: int, block_ids: list[int], start_pos: int, key_states: torch.Tensor,
                      value_states: torch.Tensor) -> None:
@@ -439,6 +440,7 @@ class GpuKVBlockPool:
     def reset(self) -> None:
         self._k_pool = None
         self._v_pool = None
+        self._k_views = self._v_views = ()
         self._regions = []
         self._used_map = None
         self._write_err = None

@@ -57,7 +57,7 @@ def test_copies_that_depend_on_each_other(kind, src, dst):
     _check(pool, was, {d: s for s, d in zip(src, dst)})
 
 
-@pytest.mark.parametrize("n", [256, 257, 700])
+@pytest.mark.parametrize("n", [448, 449, 1000])
 def test_more_pages_than_a_launch_holds(n):
     pool = _pool("int8", 2 * n + 5, layers=2, hkv=1, bs=4)
     was = _pages(pool)
@@ -68,8 +68,8 @@ def test_more_pages_than_a_launch_holds(n):
 
 
 @pytest.mark.parametrize("kind", POOLS)
-def test_a_chain_and_a_cycle_longer_than_a_launch_holds(kind):
-    n = 300
+@pytest.mark.parametrize("n", [400, 500])
+def test_a_long_chain_and_a_long_cycle(kind, n):  # within a launch, and beyond one
     pool = _pool(kind, n + 1, layers=1, hkv=1, bs=4)
     was = _pages(pool)
     pool.copy_blocks(list(range(n)), list(range(1, n + 1)))
@@ -80,7 +80,7 @@ def test_a_chain_and_a_cycle_longer_than_a_launch_holds(kind):
 
 
 @pytest.mark.parametrize("kind", POOLS)
-@pytest.mark.parametrize("n", [1, 37, 300])
+@pytest.mark.parametrize("n", [1, 37, 500])
 def test_move_blocks_renames_tables_and_frees_the_sources(kind, n):
     nb = 3 * n + 4
     pool = _pool(kind, nb, layers=2, hkv=1, bs=4)
@@ -107,15 +107,15 @@ def test_move_blocks_renames_tables_and_frees_the_sources(kind, n):
 
 @pytest.mark.parametrize("kind", POOLS)
 def test_freed_blocks(kind):
-    pool = _pool(kind, 700, layers=2, hkv=1, bs=4)
+    pool = _pool(kind, 1100, layers=2, hkv=1, bs=4)
     was = _pages(pool)
     pool._used_map.fill_(1)
-    assert pool.allocated_block_count() == 700
-    gone = list(range(0, 600)) + [5]
+    assert pool.allocated_block_count() == 1100
+    gone = list(range(0, 1000)) + [5]
     pool.free_blocks(gone)
-    assert pool.allocated_block_count() == 100 and pool.peak_allocated_block_count() == 700
+    assert pool.allocated_block_count() == 100 and pool.peak_allocated_block_count() == 1100
     if kind == "int8":
-        assert (pool._codes[:, :600] == 0).all() and torch.equal(pool._codes[:, 600:], was[1][:, 600:])
+        assert (pool._codes[:, :1000] == 0).all() and torch.equal(pool._codes[:, 1000:], was[1][:, 1000:])
         k, _ = pool.gather_layer(0, [3], 4)
         assert (k == 0).all()
     assert torch.equal(pool._page_regions()[0], was[0])

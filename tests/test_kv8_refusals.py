@@ -119,7 +119,7 @@ def test_page_entry_points_refuse_bad_arguments():
     _status(copy(src=(0, 8)), _hip.MX_ERR_INVALID)
     _status(copy(dst=(2, -1)), _hip.MX_ERR_INVALID)
     _status(copy(src=(0, 2), move=1), _hip.MX_ERR_INVALID)  # page 2 is a source and a destination
-    n = 300  # one chain of 300 copies
+    n = 500  # one chain, longer than a launch takes
     _status(copy(src=range(n), dst=range(1, n + 1), pages=n + 1), _hip.MX_ERR_UNSUPPORTED)
 
     def rename(tables=FAKE, rows=2, width=4, of=(1, 2), to=(3, 4)):
