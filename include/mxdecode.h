@@ -628,8 +628,8 @@ int mx_kv8_attn_decode(const uint16_t* q, int64_t q_sb, int64_t q_sh, const uint
 /* Page dst[i] = page src[i] in every layer and region, for all i at once: every
  * source is read as it was before the call, in whatever order the pairs stand.
  * Of several pairs with one dst the last counts. used (nullable, uint8
- * [num_pages]) gets 1 at every dst; with move != 0 no page may be both a src and
- * a dst, and used gets 0 at every src. More than 448 pairs that depend on each
+ * [num_pages]) gets 1 at every dst; with move != 0 no page may occur twice in the
+ * two lists, and used gets 0 at every src. More than 448 pairs that depend on each
  * other (a page that is a src and a dst) are refused (MX_ERR_UNSUPPORTED).
  * GpuKVBlockPool.copy_blocks (runtime/phase2/paged_kv_kernel.py:233-250). */
 int mx_kv_copy_pages(void* base, int64_t page_bytes, int64_t layer_stride, void* base2, int64_t page_bytes2,
@@ -637,7 +637,8 @@ int mx_kv_copy_pages(void* base, int64_t page_bytes, int64_t layer_stride, void*
                      int32_t n, uint8_t* used, int32_t move, void* stream);
 
 /* out[r, c] = to[i] where tables[r, c] == from[i], else tables[r, c] (int32
- * [rows, width]; out may be tables). from holds no id twice and none of to's.
+ * [rows, width]; out may be tables). from holds no id twice, none below 0 and none
+ * of to's.
  * No reference counterpart: its pages never move. */
 int mx_kv_rename_pages(const int32_t* tables, int64_t in_stride, int32_t* out, int64_t out_stride, int32_t rows,
                        int32_t width, const int32_t* from, const int32_t* to, int32_t n, void* stream);

@@ -134,61 +134,77 @@ __global__ __launch_bounds__(kThreads) void clear_kernel(ClearParams p) {
     }
 }
 
-// Splits pairs (one per dst, no src == dst) into independent ones and an ordered list for
-// copy_ordered: a pair that reads a page comes before the one that writes it, a cycle is opened by
-// keeping one page.
-static void order_pairs(const std::vector<int2>& in, std::vector<int2>& free_pairs, std::vector<int2>& ordered) {
-    std::vector<int> srcs, dsts;
-    for (const int2& p : in) {
-        srcs.push_back(p.x);
-        dsts.push_back(p.y);
+// Page id -> number, for n ids: open addressing over at least 4 n slots (a call's host work is a few
+// microseconds where sorts of the lists took 25 for 384 pairs).
+class IdMap {
+   public:
+    explicit IdMap(size_t n) {
+        while (((size_t)1 << bits_) < 4 * n) ++bits_;
+        slots_.assign((size_t)1 << bits_, int2{-1, -1});
     }
-    std::sort(srcs.begin(), srcs.end());
-    std::sort(dsts.begin(), dsts.end());
+    void set(int id, int value) { *find(id) = int2{id, value}; }
+    int get(int id) const {
+        const int2* s = const_cast<IdMap*>(this)->find(id);
+        return s->x == id ? s->y : -1;
+    }
+
+   private:
+    int2* find(int id) {
+        for (size_t i = ((uint32_t)id * 2654435761u) >> (32 - bits_);; i = (i + 1) & (slots_.size() - 1))
+            if (slots_[i].x == id || slots_[i].x == -1) return &slots_[i];
+    }
+    int bits_ = 3;
+    std::vector<int2> slots_;
+};
+
+// The pairs of (src, dst) that copy something, of several with one dst the last, split into independent
+// ones and an ordered list for copy_ordered: a pair that reads a page comes before the one that writes
+// it, a cycle is opened by keeping one page.
+static void order_pairs(const int32_t* src, const int32_t* dst, int n, std::vector<int2>& free_pairs,
+                        std::vector<int2>& ordered) {
+    IdMap writer(n), reader(n);  // a page's last pair in the lists; whether a counted pair reads it
+    for (int i = 0; i < n; ++i) writer.set(dst[i], i);
+    auto counts = [&](int i) { return src[i] != dst[i] && writer.get(dst[i]) == i; };
+    for (int i = 0; i < n; ++i)
+        if (counts(i)) reader.set(src[i], 1);
     std::vector<int2> rest;
-    for (const int2& p : in) {
-        const bool tied = std::binary_search(dsts.begin(), dsts.end(), p.x) ||
-                          std::binary_search(srcs.begin(), srcs.end(), p.y);
-        (tied ? rest : free_pairs).push_back(p);
+    for (int i = 0; i < n; ++i) {
+        if (!counts(i)) continue;
+        const int w = writer.get(src[i]);
+        const bool tied = (w >= 0 && counts(w)) || reader.get(dst[i]) >= 0;
+        (tied ? rest : free_pairs).push_back(int2{src[i], dst[i]});
     }
-    // readers[i]: pairs of rest not yet done that read rest[i]'s dst. A pair is ready at 0.
-    std::vector<int2> by_dst = rest;
-    std::sort(by_dst.begin(), by_dst.end(), [](int2 a, int2 b) { return a.y < b.y; });
-    auto writer_of = [&](int page) {
-        auto it = std::lower_bound(by_dst.begin(), by_dst.end(), page, [](int2 a, int v) { return a.y < v; });
-        return it != by_dst.end() && it->y == page ? (int)(it - by_dst.begin()) : -1;
-    };
-    std::vector<int> readers(by_dst.size(), 0), ready;
-    std::vector<char> done(by_dst.size(), 0);
-    for (const int2& p : by_dst) {
-        const int w = writer_of(p.x);
+    if (rest.empty()) return;
+    IdMap of(rest.size());  // page -> the pair of rest that writes it
+    for (size_t i = 0; i < rest.size(); ++i) of.set(rest[i].y, (int)i);
+    std::vector<int> readers(rest.size(), 0), ready;  // readers: pairs not yet done that read the pair's dst
+    std::vector<char> done(rest.size(), 0);
+    for (const int2& p : rest) {
+        const int w = of.get(p.x);
         if (w >= 0) ++readers[w];
     }
-    for (size_t i = 0; i < by_dst.size(); ++i)
+    for (size_t i = 0; i < rest.size(); ++i)
         if (readers[i] == 0) ready.push_back((int)i);
-    auto drain = [&]() {
-        while (!ready.empty()) {
-            const int i = ready.back();
-            ready.pop_back();
-            ordered.push_back(by_dst[i]);
-            done[i] = 1;
-            const int w = writer_of(by_dst[i].x);  // the pair that overwrites what was just read
-            if (w >= 0 && --readers[w] == 0) ready.push_back(w);
-        }
-    };
-    drain();
+    while (!ready.empty()) {
+        const int i = ready.back();
+        ready.pop_back();
+        ordered.push_back(rest[i]);
+        done[i] = 1;
+        const int w = of.get(rest[i].x);  // the pair that overwrites what was just read
+        if (w >= 0 && --readers[w] == 0) ready.push_back(w);
+    }
     // What is left are cycles, each page read once: a1 <- a0, a2 <- a1, ..., a0 <- ak.
-    for (size_t i = 0; i < by_dst.size(); ++i) {
+    for (size_t i = 0; i < rest.size(); ++i) {
         if (done[i]) continue;
-        const int kept = by_dst[i].y;
+        const int kept = rest[i].y;
         ordered.push_back(int2{kept, -1});
         int w = (int)i;
-        while (by_dst[w].x != kept) {  // write a page, then the one that was just read
-            ordered.push_back(by_dst[w]);
+        while (rest[w].x != kept) {  // write a page, then the one that was just read
+            ordered.push_back(rest[w]);
             done[w] = 1;
-            w = writer_of(by_dst[w].x);
+            w = of.get(rest[w].x);
         }
-        ordered.push_back(int2{-1, by_dst[w].y});
+        ordered.push_back(int2{-1, rest[w].y});
         done[w] = 1;
     }
 }
@@ -225,18 +241,17 @@ extern "C" int mx_kv_copy_pages(void* base, int64_t page_bytes, int64_t layer_st
         if (src[i] < 0 || src[i] >= num_pages || dst[i] < 0 || dst[i] >= num_pages)
             return fail(MX_ERR_INVALID, "%s: page id out of range: %d -> %d", what, src[i], dst[i]);
     try {
-        std::vector<int2> pairs, ordered, free_pairs;
-        {
-            std::vector<int> at(n);
-            for (int i = 0; i < n; ++i) at[i] = i;
-            std::stable_sort(at.begin(), at.end(), [&](int a, int b) { return dst[a] < dst[b]; });
+        std::vector<int2> ordered, free_pairs;
+        pages::order_pairs(src, dst, n, free_pairs, ordered);
+        if (move && free_pairs.size() != (size_t)n)
+            return fail(MX_ERR_INVALID, "%s: a moved page occurs twice in the lists", what);
+        if (move) {
+            pages::IdMap seen(n);
             for (int i = 0; i < n; ++i) {
-                const bool last = i + 1 == n || dst[at[i + 1]] != dst[at[i]];  // a page named twice: the last pair
-                if (last && src[at[i]] != dst[at[i]]) pairs.push_back(int2{src[at[i]], dst[at[i]]});
+                if (seen.get(src[i]) >= 0) return fail(MX_ERR_INVALID, "%s: page %d is moved twice", what, src[i]);
+                seen.set(src[i], 1);
             }
         }
-        pages::order_pairs(pairs, free_pairs, ordered);
-        if (move && !ordered.empty()) return fail(MX_ERR_INVALID, "%s: a moved page is also a destination", what);
         if (ordered.size() > (size_t)pages::kBatch)
             return fail(MX_ERR_UNSUPPORTED, "%s: more than %d copies depend on each other", what, pages::kBatch);
         p.layers = layers;
@@ -271,16 +286,19 @@ extern "C" int mx_kv_rename_pages(const int32_t* tables, int64_t in_stride, int3
     if ((int64_t)rows * width >= ((int64_t)1 << 32)) return fail(MX_ERR_UNSUPPORTED, "%s: tables too large", what);
     try {
         std::vector<int2> list(n);
-        for (int i = 0; i < n; ++i) list[i] = int2{from[i], to[i]};
-        std::sort(list.begin(), list.end(), [](int2 a, int2 b) { return a.x < b.x; });
+        pages::IdMap old(n);
         for (int i = 0; i < n; ++i) {
-            if (i > 0 && list[i].x == list[i - 1].x) return fail(MX_ERR_INVALID, "%s: id %d twice", what, list[i].x);
-            // Lists longer than a launch holds go one after another: no new name may be an old one.
-            const int to_id = list[i].y;
-            auto it = std::lower_bound(list.begin(), list.end(), to_id, [](int2 a, int v) { return a.x < v; });
-            if (it != list.end() && it->x == to_id)
-                return fail(MX_ERR_INVALID, "%s: id %d is both renamed and a new name", what, to_id);
+            if (from[i] < 0) return fail(MX_ERR_INVALID, "%s: id %d", what, from[i]);
+            if (old.get(from[i]) >= 0) return fail(MX_ERR_INVALID, "%s: id %d twice", what, from[i]);
+            old.set(from[i], 1);
+            list[i] = int2{from[i], to[i]};
         }
+        // Lists longer than a launch holds go one after another: no new name may be an old one.
+        for (int i = 0; i < n; ++i)
+            if (to[i] >= 0 && old.get(to[i]) >= 0)
+                return fail(MX_ERR_INVALID, "%s: id %d is both renamed and a new name", what, to[i]);
+        auto below = [](int2 a, int2 b) { return a.x < b.x; };
+        if (!std::is_sorted(list.begin(), list.end(), below)) std::sort(list.begin(), list.end(), below);
         pages::RenameParams p{tables, out, in_stride, out_stride, rows, width, 0, {}};
         int i = 0;
         do {

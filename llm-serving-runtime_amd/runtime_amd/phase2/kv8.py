@@ -44,6 +44,9 @@ class Kv8Layer:
     dtype: torch.dtype
     num_blocks: int = field(init=False)
     num_kv_heads: int = field(init=False)
+    device: torch.device = field(init=False)
+    pointers: tuple[int, int] = field(init=False)  # of data and codes
+    flags: int = field(init=False)                 # MX_PA_BF16 or 0
 
     def __post_init__(self) -> None:
         data, codes = self.data, self.codes
@@ -62,10 +65,9 @@ class Kv8Layer:
         _hip.require_device_tensor(data, "data")
         object.__setattr__(self, "num_blocks", int(data.shape[0]))
         object.__setattr__(self, "num_kv_heads", int(data.shape[1]))
-
-    @property
-    def device(self) -> torch.device:
-        return self.data.device
+        object.__setattr__(self, "device", data.device)
+        object.__setattr__(self, "pointers", (data.data_ptr(), codes.data_ptr()))
+        object.__setattr__(self, "flags", _DTYPE_FLAGS[self.dtype])
 
 
 def _tables(block_tables: torch.Tensor, rows: int, device: torch.device) -> torch.Tensor:
@@ -74,6 +76,14 @@ def _tables(block_tables: torch.Tensor, rows: int, device: torch.device) -> torc
     if block_tables.dtype != torch.int32 or block_tables.device != device or block_tables.stride(1) != 1:
         block_tables = block_tables.to(device=device, dtype=torch.int32).contiguous()
     return block_tables
+
+
+def _lengths(t: torch.Tensor, rows: int, device: torch.device) -> torch.Tensor:
+    """``rows`` lengths or positions as contiguous int32 on the device."""
+    t = _i32(t if t.dim() == 1 else t.reshape(-1), device)
+    if t.shape[0] != rows:
+        raise ValueError(f"{rows} rows but {t.shape[0]} lengths or positions")
+    return t
 
 
 def _err_ptr(err: torch.Tensor | None, device: torch.device):
@@ -114,9 +124,7 @@ def kv8_append(layer: Kv8Layer, block_tables: torch.Tensor, start_pos: torch.Ten
         raise ValueError("states do not match the cache's heads and head_dim")
     if key_states.device != dev or value_states.device != dev:
         raise ValueError("states must be on the cache's device")
-    starts = _i32(start_pos.reshape(-1), dev)
-    if starts.numel() != b:
-        raise ValueError(f"{b} rows but {starts.numel()} start positions")
+    starts = _lengths(start_pos, b, dev)
     tables = _tables(block_tables, b, dev)
     strides = _strides(key_states)
     if strides is None or strides != _strides(value_states):
@@ -127,9 +135,9 @@ def kv8_append(layer: Kv8Layer, block_tables: torch.Tensor, start_pos: torch.Ten
     with _hip.on_device(dev):
         rc = _hip.load().mx_kv8_write(
             key_states.data_ptr(), value_states.data_ptr(), *strides, b, t, hkv, d, tables.data_ptr(),
-            tables.stride(0), tables.shape[1], starts.data_ptr(), layer.data.data_ptr(), layer.codes.data_ptr(),
+            tables.stride(0), tables.shape[1], starts.data_ptr(), *layer.pointers,
             layer.block_size, layer.num_blocks, _err_ptr(err, dev), _used_ptr(used_blocks, layer.num_blocks, dev),
-            _DTYPE_FLAGS[layer.dtype], _hip.stream_handle(dev))
+            layer.flags, _hip.stream_handle(dev))
     if rc != _hip.MX_OK:
         _hip.check(rc, "mx_kv8_write")
 
@@ -142,21 +150,17 @@ def kv8_gather(layer: Kv8Layer, block_tables: torch.Tensor, tokens: int, seq_len
     dev = layer.device
     b = int(block_tables.shape[0]) if block_tables.dim() == 2 else -1
     tables = _tables(block_tables, b, dev)
-    lens = None
-    if seq_lens is not None:
-        lens = _i32(seq_lens.reshape(-1), dev)
-        if lens.numel() != b:
-            raise ValueError(f"{b} block-table rows but {lens.numel()} lengths")
+    lens = _lengths(seq_lens, b, dev) if seq_lens is not None else None
     if tokens < 0:
         raise ValueError("tokens must be >= 0")
     k = torch.empty((b, layer.num_kv_heads, tokens, layer.head_dim), dtype=layer.dtype, device=dev)
     v = torch.empty_like(k)
     with _hip.on_device(dev):
         rc = _hip.load().mx_kv8_gather(
-            layer.data.data_ptr(), layer.codes.data_ptr(), tables.data_ptr(), tables.stride(0), tables.shape[1],
+            *layer.pointers, tables.data_ptr(), tables.stride(0), tables.shape[1],
             lens.data_ptr() if lens is not None else None, b, tokens, layer.num_kv_heads, layer.head_dim,
             layer.block_size, layer.num_blocks, k.data_ptr(), v.data_ptr(), _err_ptr(err, dev),
-            _DTYPE_FLAGS[layer.dtype], _hip.stream_handle(dev))
+            layer.flags, _hip.stream_handle(dev))
     if rc != _hip.MX_OK:
         _hip.check(rc, "mx_kv8_gather")
     return k, v
@@ -207,18 +211,16 @@ def kv8_rope_append(qkv: torch.Tensor | None, rope: torch.Tensor, positions: tor
     if (rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[1:] != (d // 2, 2) or not rope.is_contiguous()
             or rope.device != dev):
         raise ValueError("rope must be a contiguous fp32 [max_pos, D/2, 2] table")
-    pos = _i32(positions.reshape(-1), dev)
-    if pos.numel() != b:
-        raise ValueError("batch dimension mismatch")
+    pos = _lengths(positions, b, dev)
     tables = _tables(block_tables, b, dev)
     with _hip.on_device(dev):
         rc = _hip.load().mx_kv8_rope_append(
             x.data_ptr() if x is not None else None, x.stride(0) if x is not None else 0,
             partials.data_ptr() if partials is not None else None, splits, bias.data_ptr() if bias is not None else None,
             b, num_heads, hkv, d, rope.data_ptr(), rope.shape[0], pos.data_ptr(), q2.data_ptr(), q2.stride(0),
-            tables.data_ptr(), tables.stride(0), tables.shape[1], layer.data.data_ptr(), layer.codes.data_ptr(),
+            tables.data_ptr(), tables.stride(0), tables.shape[1], *layer.pointers,
             layer.block_size, layer.num_blocks, _err_ptr(err, dev), _lens_ptr(lens_out, b),
-            _used_ptr(used_blocks, layer.num_blocks, dev), _DTYPE_FLAGS[layer.dtype], _hip.stream_handle(dev))
+            _used_ptr(used_blocks, layer.num_blocks, dev), layer.flags, _hip.stream_handle(dev))
     if rc != _hip.MX_OK:
         _hip.check(rc, "mx_kv8_rope_append")
     return q_out
@@ -251,9 +253,7 @@ def kv8_attention_decode(query: torch.Tensor, layer: Kv8Layer, block_tables: tor
     if hq != hkv * num_kv_groups:
         raise ValueError(f"num_heads {hq} != num_kv_heads {hkv} * num_kv_groups {num_kv_groups}")
     tables = _tables(block_tables, b, dev)
-    lens = _i32(seq_lens.reshape(-1), dev)
-    if lens.numel() != b:
-        raise ValueError(f"{b} rows but {lens.numel()} lengths")
+    lens = _lengths(seq_lens, b, dev)
     if not _aligned_heads(query):
         query = query.clone(memory_format=torch.contiguous_format)
     if out is None:
@@ -271,11 +271,11 @@ def kv8_attention_decode(query: torch.Tensor, layer: Kv8Layer, block_tables: tor
     one_row, one_head = b == 1, hq == 1
     with _hip.on_device(dev):
         rc = _hip.load().mx_kv8_attn_decode(
-            query.data_ptr(), 0 if one_row else q_sb, 0 if one_head else q_sh, layer.data.data_ptr(),
-            layer.codes.data_ptr(), tables.data_ptr(), tables.stride(0), width, lens.data_ptr(), b, hq, hkv, d,
+            query.data_ptr(), 0 if one_row else q_sb, 0 if one_head else q_sh, *layer.pointers, tables.data_ptr(),
+            tables.stride(0), width, lens.data_ptr(), b, hq, hkv, d,
             layer.block_size, layer.num_blocks, float(scaling), out.data_ptr(), 0 if one_row else o_sb,
             0 if one_head else o_sh, ws.data_ptr() if ws is not None else None, nbytes, _err_ptr(err, dev),
-            _DTYPE_FLAGS[layer.dtype], _hip.stream_handle(dev))
+            layer.flags, _hip.stream_handle(dev))
     if rc != _hip.MX_OK:
         _hip.check(rc, "mx_kv8_attn_decode")
     return out

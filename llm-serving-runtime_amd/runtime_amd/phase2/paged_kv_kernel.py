@@ -283,7 +283,7 @@ class GpuKVBlockPool:
         pairs = [(s, d) for s, d in zip(_ids(src_block_ids), _ids(dst_block_ids)) if s != d]
         self._touch_ids([i for pair in pairs for i in pair])
         if pairs:
-            self._copy_pages([s for s, _ in pairs], [d for _, d in pairs])
+            self._copy_pages(array.array("i", [s for s, _ in pairs]), array.array("i", [d for _, d in pairs]))
 
     def move_blocks(self, src_block_ids: list[int], dst_block_ids: list[int],
                     block_tables: torch.Tensor | None = None, out: torch.Tensor | None = None
@@ -293,28 +293,47 @@ class GpuKVBlockPool:
         with every src id replaced by its dst id, as a new tensor or in ``out`` (which may be
         ``block_tables`` itself). No id may occur twice, neither among nor between the two lists.
         """
-        src, dst = _ids(src_block_ids), _ids(dst_block_ids)
+        src, dst = list(src_block_ids), list(dst_block_ids)
         if len(src) != len(dst):
             raise ValueError(f"move_blocks length mismatch: src={len(src)} dst={len(dst)}")
-        if len(set(src).union(dst)) != 2 * len(src):
-            raise ValueError("move_blocks takes every block id once")
         if block_tables is None:
             if out is not None:
                 raise ValueError("out goes with block_tables")
         else:
-            if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.device.type != self.device.type:
-                raise ValueError("block_tables must be int32 [B, max_blocks] on the pool's device")
+            if (block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.stride(1) != 1
+                    or block_tables.device.type != self.device.type):
+                raise ValueError("block_tables must be int32 [B, max_blocks] with unit inner stride on the pool's device")
             if out is None:
                 out = torch.empty(block_tables.shape, dtype=torch.int32, device=block_tables.device)
-            elif out.dtype != torch.int32 or out.shape != block_tables.shape or out.device != block_tables.device:
-                raise ValueError("out must be int32 of block_tables' shape and device")
-        self._touch_ids(src + dst)
+            elif (out.dtype != torch.int32 or out.shape != block_tables.shape or out.stride(1) != 1
+                  or out.device != block_tables.device):
+                raise ValueError("out must be int32 of block_tables' shape, device and unit inner stride")
+        on_device = self.device.type == "cuda"
+        if not on_device:
+            self._check_move(src, dst)
         if src:
-            self._copy_pages(src, dst, move=True)
+            try:
+                a, b = array.array("i", src), array.array("i", dst)
+                self._copy_pages(a, b, move=True)
+            except (ValueError, OverflowError):
+                self._check_move(src, dst)
+                raise
+            # On a device pool its map has the marks (read with the counts), here only the old ids go.
             self._used_blocks.difference_update(src)
-        if block_tables is not None:
-            self._rename(block_tables, out, src, dst)
+            if not on_device:
+                self._touch_ids(dst)
+            if block_tables is not None:
+                self._rename(block_tables, out, a, b)
+        elif block_tables is not None and out is not block_tables:
+            out.copy_(block_tables)
         return out
+
+    def _check_move(self, src: list[int], dst: list[int]) -> None:
+        for i in src + dst:
+            if not 0 <= i < self.shape.num_blocks:
+                raise IndexError(f"physical block id out of range: {i}")
+        if len(set(src).union(dst)) != 2 * len(src):
+            raise ValueError("move_blocks takes every block id once")
 
     def free_blocks(self, block_ids: list[int]) -> None:
         """Give blocks back: they no longer count as allocated (and an 8-bit pool's stand for 0). A block
@@ -342,20 +361,20 @@ class GpuKVBlockPool:
         self._ensure_pools()
         return self._regions
 
-    def _copy_pages(self, src: list[int], dst: list[int], move: bool = False) -> None:
-        """Page dst[i] = page src[i] (ids checked) in every layer, all at once."""
+    def _copy_pages(self, src: array.array, dst: array.array, move: bool = False) -> None:
+        """Page dst[i] = page src[i] in every layer, all at once (the lists as ``move_blocks`` or
+        ``copy_blocks`` takes them)."""
         regions = self._page_regions()
         if self.device.type == "cuda":
             args: list = []
             for t in (*regions, None)[:2]:
                 args += [None, 0, 0] if t is None else [t.data_ptr(), t[0, 0].numel() * t.element_size(),
                                                         t.stride(0) * t.element_size()]
-            a, b = array.array("i", src), array.array("i", dst)
             with _hip.on_device(self.device):
                 rc = _hip.load().mx_kv_copy_pages(
-                    *args, self.shape.num_layers, self.shape.num_blocks, a.buffer_info()[0], b.buffer_info()[0],
+                    *args, self.shape.num_layers, self.shape.num_blocks, src.buffer_info()[0], dst.buffer_info()[0],
                     len(src), self._used_map.data_ptr(), int(move), _hip.stream_handle(self.device))
-            if rc != _hip.MX_ERR_UNSUPPORTED:  # a chain of copies longer than a launch takes
+            if rc != _hip.MX_ERR_UNSUPPORTED:  # else: more copies that depend on each other than a launch takes
                 _hip.check(rc, "mx_kv_copy_pages")
                 return
         last = dict(zip(dst, src))
@@ -364,19 +383,16 @@ class GpuKVBlockPool:
         for t in regions:
             t[:, to] = t[:, of]
 
-    def _rename(self, tables: torch.Tensor, out: torch.Tensor, src: list[int], dst: list[int]) -> None:
+    def _rename(self, tables: torch.Tensor, out: torch.Tensor, src: array.array, dst: array.array) -> None:
         if self.device.type != "cuda":
-            name = {s: d for s, d in zip(src, dst)}
+            name = dict(zip(src, dst))
             out.copy_(torch.tensor([[name.get(i, i) for i in row] for row in tables.tolist()],
                                    dtype=torch.int32).view(tables.shape))
             return
-        if tables.stride(1) != 1 or out.stride(1) != 1:
-            raise ValueError("block_tables and out must have unit inner stride")
-        a, b = array.array("i", src), array.array("i", dst)
         with _hip.on_device(self.device):
             _hip.check(_hip.load().mx_kv_rename_pages(
                 tables.data_ptr(), tables.stride(0), out.data_ptr(), out.stride(0), tables.shape[0], tables.shape[1],
-                a.buffer_info()[0], b.buffer_info()[0], len(src), _hip.stream_handle(self.device)),
+                src.buffer_info()[0], dst.buffer_info()[0], len(src), _hip.stream_handle(self.device)),
                 "mx_kv_rename_pages")
 
     def gather_layer(self, layer_idx: int, block_ids: list[int], seq_len: int) -> tuple[torch.Tensor, torch.Tensor]:

@@ -100,7 +100,7 @@ def test_move_blocks_renames_tables_and_frees_the_sources(kind, n):
     got = pool.move_blocks(src, dst, view)
     assert got.tolist() == want and torch.equal(view.cpu(), tables)
     _check(pool, was, {d: s for s, d in name.items()})
-    assert pool.allocated_block_count() == n + len(rest) and pool.peak_allocated_block_count() == 2 * n + len(rest)
+    assert pool.allocated_block_count() == n + len(rest) == pool.peak_allocated_block_count()
     pool.move_blocks(dst, src, got, out=got)  # back again, in place
     assert torch.equal(got.cpu()[:2], tables[:2])
 
@@ -141,3 +141,25 @@ def test_copies_in_a_captured_graph_and_on_a_side_stream():
         assert out.tolist()[1][2] == 2 and out.tolist()[1][1] == 11
         pool.copy_blocks([i], [13 + i])
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("kind", POOLS)
+def test_refusals_leave_the_pool_as_it_was(kind):
+    pool = _pool(kind, 8)
+    was = _pages(pool)
+    for src, dst in (([1], [1]), ([1, 1], [2, 3]), ([1, 2], [3, 3]), ([1, 2], [2, 3]), ([1], [])):
+        with pytest.raises(ValueError):
+            pool.move_blocks(src, dst)
+    for call in (lambda: pool.move_blocks([1], [8]), lambda: pool.move_blocks([-1], [2]), lambda: pool.copy_blocks([1], [8]),
+                 lambda: pool.free_blocks([8]), lambda: pool.move_blocks([2**31], [1])):
+        with pytest.raises(IndexError):
+            call()
+    tables = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    for bad in (tables.cpu(), tables.long(), tables.t(), tables[0]):
+        with pytest.raises(ValueError):
+            pool.move_blocks([1], [2], bad)
+    with pytest.raises(ValueError):
+        pool.move_blocks([1], [2], tables, out=tables[:1])
+    _check(pool, was, {})
+    pool.copy_blocks([], []), pool.free_blocks([])
+    assert torch.equal(pool.move_blocks([], [], tables), tables)

@@ -130,6 +130,9 @@ def test_page_entry_points_refuse_bad_arguments():
     _status(rename(rows=-1), _hip.MX_ERR_INVALID)
     _status(rename(tables=None), _hip.MX_ERR_NULL)
     _status(rename(of=(1, 1)), _hip.MX_ERR_INVALID)
+    _status(rename(of=(1, -1)), _hip.MX_ERR_INVALID)
+    for src, dst in (((0, 0), (2, 3)), ((0, 1), (2, 2)), ((0, 1), (0, 2))):
+        _status(copy(src=src, dst=dst, move=1), _hip.MX_ERR_INVALID)  # a page that occurs twice
     _status(rename(to=(3, 1)), _hip.MX_ERR_INVALID)
     _status(rename(rows=1 << 30, width=4), _hip.MX_ERR_UNSUPPORTED)
     assert lib.mx_kv_clear_pages(FAKE, 4, 64, 2, FAKE, 8, ids, 0, None) == _hip.MX_OK
@@ -205,7 +208,7 @@ def test_move_and_free_blocks_on_the_cpu_pool():
     for a, b in zip(_snapshot(pool), was):
         for now, old in zip(a, b):
             assert torch.equal(now, old[[0, 7, 8, 3, 4, 5, 6, 7, 8]])
-    assert pool.allocated_block_count() == 3 and pool.peak_allocated_block_count() == 5
+    assert pool.allocated_block_count() == pool.peak_allocated_block_count() == 3
     pool.free_blocks([1, 2, 2])
     assert pool.allocated_block_count() == 1
     assert pool.move_blocks([], [], tables).tolist() == tables.tolist()
@@ -217,6 +220,6 @@ def test_move_and_free_blocks_on_the_cpu_pool():
         pool.move_blocks([1], [2], tables.long())
     with pytest.raises(ValueError):
         pool.move_blocks([1], [2], out=tables)
-    for call in (lambda: pool.move_blocks([1], [9]), lambda: pool.copy_blocks([-1], [2]), lambda: pool.free_blocks([9])):
+    for call in (lambda: pool.move_blocks([1], [9]), lambda: pool.move_blocks([2**31], [1]), lambda: pool.copy_blocks([-1], [2]), lambda: pool.free_blocks([9])):
         with pytest.raises(IndexError):
             call()
