@@ -3,26 +3,34 @@
 // paged_attention_decode_batched (runtime/phase2/paged_attention_triton.py:745-775).
 //
 // Work. A segment is one row and one group of at most 16 query heads of a kv-head (a larger GQA group is
-// cut into equal ones; each reads the head's pages again). Its tokens are chunks of 16. The chunks of all
-// segments, row after row, form one sequence that is cut into equal ranges, one per wave, so every wave
-// streams the same bytes whatever the mix of lengths; a segment that several waves share is joined by a
-// second, small launch from their (m, l, acc), all fp32. Tables of at most kDirectChunks chunks give every
-// segment to one wave instead: one launch.
+// cut into equal ones; each reads the head's pages again). Its tokens are chunks of 16. Two forms, chosen
+// from the table's width and the number of segments (by_segment):
+//   * a workgroup per segment, whose waves take the steps in turn and join in LDS: one launch;
+//   * the chunks of all segments, row after row, as one sequence cut into equal ranges, one per wave, so
+//     that every wave streams the same bytes whatever the mix of lengths and a single row fills the chip; a
+//     segment that several waves share is joined by a second, small launch from their (m, l, acc).
+// All of them fp32.
 //
 // A wave takes 4 chunks a step, one per lane group g = lane / 16, so that what a lane scores is what it
 // weighs, and no score crosses lanes:
 //   * scores, 4 x D / 32 products v_mfma_f32_16x16x32: the A operand's row r of product j is token
 //     4 j + r % 4 of chunk r / 4, so lane group g receives tokens 4 j + i of chunk g, for head lane % 16
-//     (the B operand holds the query heads). K enters as the integers q, exact in 16 bits; the page's
-//     scale multiplies the fp32 score. The head dim is contracted in the order of the lane's 16-byte
-//     loads, the query's operand in the same order;
+//     (the B operand holds the query heads). K enters as the integers q + 1152 (fp16) or q + 128 (bf16),
+//     one permute per pair of bytes; the accumulator starts at what that adds, and the page's scale
+//     multiplies the fp32 score. The head dim is contracted in the order of the lane's 16-byte loads, the
+//     query's operand in the same order;
 //   * online softmax in fp32 on the exp2 scale; the reference maximum moves only when a score exceeds it
 //     by more than 2^8, so most steps neither rescale nor exchange maxima between lane groups;
 //   * P.V, 2 x D / 16 products over 32 tokens: lane group g supplies tokens 8 u .. 8 u + 7 of chunk g,
 //     which is what its scores gave (weights) and half of a 16-byte load of a dim's token row (V, times
-//     the page's scale: exact in 16 bits).
+//     the page's scale: exact in 16 bits, a permute and a fused multiply-add per pair).
 // Weights are rounded to the 16-bit type before the product, as the 16-bit path's are; the denominator
-// sums the rounded ones.
+// sums the rounded ones, by a product with ones.
+//
+// Bound: HBM. One layer of batch 32, U[128, 4096] tokens, Llama-3-8B heads (139 MB): 34 us, 27 at the rate
+// of a large copy; two rows of 65,521 to 131,071 tokens (403 MB) 77 us in a graph, 5.2 TB/s. Loads alone
+// took 27 of the batch's first launch's 29 us. A CU streams at most about 55 GB/s of such pages, with 64 KiB
+// or 128 KiB of loads in flight: two steps ahead instead of one measured 5 to 20 % slower.
 #include <algorithm>
 
 #include "common.h"
@@ -42,7 +50,7 @@ constexpr int kHeads = 16;         // query heads of a segment, at most
 // 37.4 us, 2048 36.5, 3072 (three per SIMD, which spills) 55.9, 4096 (two rounds) 42.5. The loads alone
 // take 27 of the launch's 29 us there, so deeper pipelines have nothing to hide.
 constexpr int kWorkers = 2048;
-constexpr int kDirectChunks = 16;  // tables of at most this many chunks: one wave per segment
+constexpr int kSegmentWaves = 8;   // waves of a workgroup that has a segment of its own, at most
 constexpr int kMaxTokens = 1 << 30;  // of a table row, so that token and chunk numbers are 32-bit
 constexpr float kLazyLog2 = 8.0f;
 
@@ -142,7 +150,7 @@ struct Cut {
     }
 };
 
-// The state of a piece: its heads' running maximum, this lane's part of the denominator, the
+// The state of a piece: its heads' running maximum and denominator (in every lane of the head), the
 // unnormalised output (acc[e][i]: dim 16 e + 4 g + i of head lane % 16).
 template <int D>
 struct Piece {
@@ -167,8 +175,8 @@ struct Regs {
 };
 
 template <int D, int BS, bool BF16>
-__device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, int h0, int nh, int c0, int nc,
-                                          int tokens, int lane, Piece<D>& st) {
+__device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, int h0, int nh, int c0, int c1,
+                                          int stride, int tokens, int lane, Piece<D>& st) {
     constexpr int NP = Regs<D, BS>::NP, KA = D / 64;
     constexpr int PT = BS < kChunk ? BS : kChunk;  // tokens of a chunk in one page
     const int g = lane >> 4, r = lane & 15;
@@ -181,39 +189,46 @@ __device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, i
     struct Ids {
         int k[NP], v[NP];
     };
-    auto load_ids = [&](int c, Ids& id) {  // c: first chunk of the step, relative to the piece
+    auto load_ids = [&](int c, Ids& id) {  // c: the step's first chunk
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             const int ck = c + (r >> 2), cv = c + g;
-            const int pk = (c0 + ck) * kChunk / BS + n, pv = (c0 + cv) * kChunk / BS + n;
-            id.k[n] = ck < nc && pk < nblk ? bt[pk] : -1;
-            id.v[n] = cv < nc && pv < nblk ? bt[pv] : -1;
+            const int pk = ck * kChunk / BS + n, pv = cv * kChunk / BS + n;
+            id.k[n] = ck < c1 && pk < nblk ? bt[pk] : -1;
+            id.v[n] = cv < c1 && pv < nblk ? bt[pv] : -1;
         }
     };
     auto in_pool = [&](int id) { return (unsigned)id < (unsigned)p.pages.num_blocks; };
 
+    // The query operand, negated where the scale is negative (its magnitude multiplies the scores), and
+    // the scores' start: K enters as q + kRawBias, so kRawBias times the query's sum comes off. In fp32 that
+    // costs a few 2^-24 of 1152 sum |q|, against weights that are rounded to 16 bits.
     half8v qf[2 * KA];
-    if (r < nh) {
-        const uint16_t* qp = p.q + (int64_t)b * p.q_sb + (int64_t)(h0 + r) * p.q_sh + 16 * g;
+    float qsum = 0.0f;
 #pragma unroll
-        for (int a = 0; a < KA; ++a)
+    for (int a = 0; a < 2 * KA; ++a) {
+        uint4 w{0, 0, 0, 0};
+        if (r < nh)
+            w = *reinterpret_cast<const uint4*>(p.q + (int64_t)b * p.q_sb + (int64_t)(h0 + r) * p.q_sh + 16 * g +
+                                                64 * (a / 2) + 8 * (a & 1));
+        const uint32_t sign = p.scale_log2e < 0.0f ? 0x80008000u : 0u;
+        w.x ^= sign, w.y ^= sign, w.z ^= sign, w.w ^= sign;
+        qf[a] = __builtin_bit_cast(half8v, w);
 #pragma unroll
-            for (int hi = 0; hi < 2; ++hi)
-                qf[2 * a + hi] = __builtin_bit_cast(half8v, *reinterpret_cast<const uint4*>(qp + 64 * a + 8 * hi));
-    } else {
-#pragma unroll
-        for (int a = 0; a < 2 * KA; ++a) qf[a] = half8v{};
+        for (int i = 0; i < 8; ++i) qsum += Elt<BF16>::widen(qf[a][i]);
     }
+    const float start = -kRawBias<BF16> * xor_sum_16_32(qsum), scale = fabsf(p.scale_log2e);
 
     st.m = kNegInf;
-    st.l = 0.0f;
+    float4v l = {0.0f, 0.0f, 0.0f, 0.0f};  // the denominator, as a product of the weights with ones
+    const half8v ones = __builtin_bit_cast(half8v, BF16 ? uint4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
+                                                        : uint4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u});
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) st.acc[e] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
 
-    Regs<D, BS> rg{};  // lanes without a page keep what is there: any bytes, masked (K) or at scale 0 (V)
-    auto load_k = [&](int c, const Ids& id) {
+    auto load_k = [&](int c, const Ids& id, Regs<D, BS>& rg) {
         // Token 4 j + r % 4 of chunk r / 4, dims 64 a + 16 g + [0, 16).
-        const int base = BS > kChunk ? (c0 + c + (r >> 2)) * kChunk % BS : 0;
+        const int base = BS > kChunk ? (c + (r >> 2)) * kChunk % BS : 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int n = 4 * j / PT, slot = base + (4 * j) % PT + (r & 3);
@@ -225,9 +240,9 @@ __device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, i
             }
         }
     };
-    auto load_v = [&](int c, const Ids& id) {
+    auto load_v = [&](int c, const Ids& id, Regs<D, BS>& rg) {
         // Token row of dim 16 e + r, chunk g; zero scale where there is no page.
-        const int base = BS > kChunk ? (c0 + c + g) * kChunk % BS : 0;
+        const int base = BS > kChunk ? (c + g) * kChunk % BS : 0;
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             rg.codes[n] = 0;
@@ -251,42 +266,54 @@ __device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, i
         }
     };
 
+    Regs<D, BS> rg{};  // lanes without a page keep what is there: any bytes, masked (K) or at scale 0 (V)
     Ids id, next;
-    load_ids(0, id);
-    load_k(0, id);
-    load_v(0, id);
-    load_ids(kStep, next);
-    for (int c = 0; c < nc; c += kStep) {
+    load_ids(c0, id);
+    load_k(c0, id, rg);
+    load_v(c0, id, rg);
+    load_ids(c0 + stride, next);
+    for (int c = c0; c < c1; c += stride) {
         // Scores of tokens 4 j + i of chunk g.
         float4v s[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            s[j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            s[j] = float4v{start, start, start, start};
 #pragma unroll
             for (int a = 0; a < KA; ++a) {
-                s[j] = Elt<BF16>::mma32(integers8<BF16>(rg.k[j][a].x, rg.k[j][a].y), qf[2 * a], s[j]);
-                s[j] = Elt<BF16>::mma32(integers8<BF16>(rg.k[j][a].z, rg.k[j][a].w), qf[2 * a + 1], s[j]);
+                s[j] = Elt<BF16>::mma32(raw8<BF16>(rg.k[j][a].x, rg.k[j][a].y), qf[2 * a], s[j]);
+                s[j] = Elt<BF16>::mma32(raw8<BF16>(rg.k[j][a].z, rg.k[j][a].w), qf[2 * a + 1], s[j]);
             }
         }
-        if (c + kStep < nc) load_k(c + kStep, next);
-        bool live[NP];
-        float vs[NP];
+        if (c + stride < c1) load_k(c + stride, next, rg);
+        bool live[NP], all = true;
+        float ks[NP];
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             live[n] = in_pool(id.v[n]);
-            if (!live[n] && r == 0 && p.err && c + g < nc && (c0 + c + g) * kChunk / BS + n < nblk) atomicOr(p.err, 4);
-            vs[n] = scale_of((int)(rg.codes[n] >> 8));
+            if (!live[n] && r == 0 && p.err && c + g < c1 && (c + g) * kChunk / BS + n < nblk) atomicOr(p.err, 4);
+            all = all && live[n];
+            ks[n] = scale_of((int)(rg.codes[n] & 0xffu)) * scale;
         }
-        const int t0 = (c0 + c + g) * kChunk;
-        float mx = kNegInf;
+        // A step whose 64 tokens all count, one page a chunk: the page's scale multiplies the maximum and
+        // goes into the exponent's fused multiply-add. Else every score is scaled, or masked, by itself.
+        const bool whole = NP == 1 && (c + kStep) * kChunk <= tokens && c + kStep <= c1 &&
+                           __builtin_amdgcn_ballot_w64(all) == ~(uint64_t)0;
+        float mx = kNegInf, mul = 1.0f;
+        if (whole) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = 4 * j / PT;
-            const float ks = scale_of((int)(rg.codes[n] & 0xffu)) * p.scale_log2e;
+            for (int j = 0; j < 4; ++j) mx = fmaxf(fmaxf(mx, fmaxf(s[j][0], s[j][1])), fmaxf(s[j][2], s[j][3]));
+            mul = ks[0];
+            mx *= mul;
+        } else {
+            const int t0 = (c + g) * kChunk;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[j][i] = live[n] && t0 + 4 * j + i < tokens ? s[j][i] * ks : kNegInf;
-                mx = fmaxf(mx, s[j][i]);
+            for (int j = 0; j < 4; ++j) {
+                const int n = 4 * j / PT;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[j][i] = live[n] && t0 + 4 * j + i < tokens ? s[j][i] * ks[n] : kNegInf;
+                    mx = fmaxf(mx, s[j][i]);
+                }
             }
         }
         if (__builtin_amdgcn_ballot_w64(mx > st.m + kLazyLog2) != 0) {
@@ -294,7 +321,7 @@ __device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, i
             const bool grow = mx > st.m + kLazyLog2;
             const float now = grow ? mx : st.m;
             const float alpha = grow ? __builtin_amdgcn_exp2f(st.m - now) : 1.0f;  // 0 from -inf
-            st.l *= alpha;
+            l *= alpha;
 #pragma unroll
             for (int e = 0; e < D / 16; ++e) st.acc[e] *= alpha;
             st.m = now;
@@ -304,23 +331,39 @@ __device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, i
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const _Float16 w = Elt<BF16>::round(__builtin_amdgcn_exp2f(s[j][i] - ref));
-                pv[j / 2][4 * (j & 1) + i] = w;
-                st.l += Elt<BF16>::widen(w);
-            }
+            for (int i = 0; i < 4; ++i)
+                pv[j / 2][4 * (j & 1) + i] =
+                    Elt<BF16>::round(__builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], mul, -ref)));
+        l = Elt<BF16>::mma32(ones, pv[0], l);
+        l = Elt<BF16>::mma32(ones, pv[1], l);
+        RawScale<BF16> vs[NP];
+        bool large = false;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            vs[n] = RawScale<BF16>((int)(rg.codes[n] >> 8));
+            large = large || vs[n].excess != 1.0f;
+        }
+        if (__builtin_amdgcn_ballot_w64(large) != 0) {  // V beyond 4064 (fp16): the rest of its scale goes to the weights
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 4 * (j & 1) + i;  // pin_f32: not computed ahead of the branch, on every step
+                    pv[j / 2][e] = Elt<BF16>::round(pin_f32(Elt<BF16>::widen(pv[j / 2][e])) * vs[4 * j / PT].excess);
+                }
+        }
 #pragma unroll
         for (int e = 0; e < D / 16; ++e)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const half8v a = values4x2<BF16>(rg.v[e][2 * u], rg.v[e][2 * u + 1], vs[8 * u / PT], vs[(8 * u + 4) / PT]);
+                const half8v a = scaled4x2<BF16>(rg.v[e][2 * u], rg.v[e][2 * u + 1], vs[8 * u / PT], vs[(8 * u + 4) / PT]);
                 st.acc[e] = Elt<BF16>::mma32(a, pv[u], st.acc[e]);
             }
-        if (c + kStep < nc) load_v(c + kStep, next);
+        if (c + stride < c1) load_v(c + stride, next, rg);
         id = next;
-        load_ids(c + 2 * kStep, next);
+        load_ids(c + 2 * stride, next);
     }
-    st.l = xor_sum_16_32(st.l);
+    st.l = l[0];
 }
 
 // A finished segment's output.
@@ -346,21 +389,58 @@ __device__ __forceinline__ void heads_of(const AttnParams& p, int vh, int& kvh, 
     nh = p.G - first < p.GS ? p.G - first : p.GS;
 }
 
+// One workgroup per segment: its waves take the steps in turn and join their pieces in LDS.
+template <int D, int BS, bool BF16>
+__global__ __launch_bounds__(kSegmentWaves * 64, 2) void kv8_attn_segment_kernel(AttnParams p) {
+    extern __shared__ float lds[];  // [waves][GS][2] (m, l), [waves][GS][D] outputs
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int waves = blockDim.x >> 6, b = blockIdx.y;
+    int kvh, h0, nh;
+    heads_of(p, blockIdx.x, kvh, h0, nh);
+    const int tokens = __builtin_amdgcn_readfirstlane(row_tokens<BS>(p, b));
+    Piece<D> st;
+    run_piece<D, BS, BF16>(p, b, kvh, h0, nh, wave * kStep, chunks_of(tokens), waves * kStep, tokens, lane, st);
+    if (waves == 1) {
+        write_out<D, BF16>(p, b, h0, nh, lane, st);
+        return;
+    }
+    float* const acc = lds + 2 * waves * p.GS;
+    const int g = lane >> 4, r = lane & 15;
+    if (r < nh) {
+        if (g == 0) *reinterpret_cast<float2*>(lds + (wave * p.GS + r) * 2) = float2{st.m, st.l};
+        float* a = acc + (wave * p.GS + r) * D + 4 * g;
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) *reinterpret_cast<float4v*>(a + 16 * e) = st.acc[e];
+    }
+    __syncthreads();
+    // 4 dims of a head a thread.
+    const float kNegInf = -__builtin_huge_valf();
+    for (int i = threadIdx.x; i < nh * (D / 4); i += blockDim.x) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4;
+        float m = kNegInf;
+        for (int w = 0; w < waves; ++w) m = fmaxf(m, lds[(w * p.GS + h) * 2]);
+        const float ref = m == kNegInf ? 0.0f : m;
+        float l = 0.0f;
+        float4v num = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < waves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(lds[(w * p.GS + h) * 2] - ref);
+            l += f * lds[(w * p.GS + h) * 2 + 1];
+            num += f * *reinterpret_cast<const float4v*>(acc + (w * p.GS + h) * D + d);
+        }
+        half4v v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = Elt<BF16>::round(l == 0.0f ? 0.0f : num[k] / l);
+        *reinterpret_cast<uint2*>(p.out + (int64_t)b * p.o_sb + (int64_t)(h0 + h) * p.o_sh + d) =
+            __builtin_bit_cast(uint2, v);
+    }
+}
+
 template <int D, int BS, bool BF16>
 __global__ __launch_bounds__(kAttnWaves * 64, 2) void kv8_attn_kernel(AttnParams p) {
     const int lane = threadIdx.x & 63;
     const int w = blockIdx.x * kAttnWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Piece<D> st;
     int kvh, h0, nh;
-    if (p.workers == 0) {
-        if (w >= p.B * p.Hv) return;
-        const int b = w / p.Hv;
-        heads_of(p, w - b * p.Hv, kvh, h0, nh);
-        const int tokens = __builtin_amdgcn_readfirstlane(row_tokens<BS>(p, b));
-        run_piece<D, BS, BF16>(p, b, kvh, h0, nh, 0, chunks_of(tokens), tokens, lane, st);
-        write_out<D, BF16>(p, b, h0, nh, lane, st);
-        return;
-    }
     // Up to 64 rows: one read of the lengths, a row a lane. More: their sum first, then 64 at a time.
     const bool one_pass = p.B <= 64;
     int at = 0, before = 0, tok = 0, incl = 0, total;  // rows [at, at + 64) in the lanes; chunks before them
@@ -390,7 +470,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, 2) void kv8_attn_kernel(AttnParams
         const int nc = n - c0 < hi - x ? n - c0 : hi - x;
         if (nc <= 0 || vh >= p.Hv) break;  // cannot happen for lengths that stay as they are
         heads_of(p, vh, kvh, h0, nh);
-        run_piece<D, BS, BF16>(p, b, kvh, h0, nh, c0, nc, tokens, lane, st);
+        run_piece<D, BS, BF16>(p, b, kvh, h0, nh, c0, c0 + nc, kStep, tokens, lane, st);
         if (nc == n) {
             write_out<D, BF16>(p, b, h0, nh, lane, st);
         } else {
@@ -481,9 +561,16 @@ __global__ __launch_bounds__(kMergeWaves * 64) void kv8_merge_kernel(AttnParams 
     *reinterpret_cast<uint2*>(o + threadIdx.x * 4) = __builtin_bit_cast(uint2, v);
 }
 
-// Waves of a launch, by the table's width: 0 where every segment goes to one wave.
-static int workers_for(int64_t max_tokens) {
-    return ceil_div(max_tokens, kChunk) <= kDirectChunks ? 0 : kWorkers;
+// Whether every segment gets a workgroup of its own, from what both forms were measured to take (us):
+// 4.7 and the longest row's bytes at 50 GB/s, which is all that one CU streams of such pages, against 9 and
+// the bytes of half-full tables at 5.4 TB/s. Of tables up to 1 MiB per segment only: with wider ones a
+// single long row among short ones would keep one CU at work for 20 us and more. Measured, one against the
+// other: 8 segments of 100 tokens 4.7 and 10.3 us, 14 of up to 1501 (bf16, D = 64) 8.7 and 10.2, 128 of up
+// to 2000 17.4 and 18.7, 256 of up to 4096 34.1 and 36.0; the other way 8 of 1024 10.6 and 8.2, 64 of up
+// to 4096 26.9 and 18.9.
+static bool by_segment(int64_t segments, int64_t max_tokens, int D) {
+    const double bytes = (double)max_tokens * D * 2;
+    return bytes <= 1 << 20 && 4.7 + bytes / 50e3 <= 9.0 + segments * bytes / 2 / 5.4e6;
 }
 
 static void head_groups(int G, int& NG, int& GS) {
@@ -502,7 +589,8 @@ extern "C" size_t mx_kv8_attn_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_blocks <= 0 || block_size <= 0 || Hq % Hkv != 0) return 0;
     int NG, GS;
     kv8::head_groups(Hq / Hkv, NG, GS);
-    return (size_t)2 * kv8::workers_for((int64_t)max_blocks * block_size) * GS * (D + 2) * sizeof(float);
+    if (kv8::by_segment((int64_t)B * Hkv * NG, (int64_t)max_blocks * block_size, D)) return 0;
+    return (size_t)2 * kv8::kWorkers * GS * (D + 2) * sizeof(float);
 }
 
 extern "C" int mx_kv8_attn_decode(const uint16_t* q, int64_t q_sb, int64_t q_sh, const uint8_t* data,
@@ -535,10 +623,11 @@ extern "C" int mx_kv8_attn_decode(const uint16_t* q, int64_t q_sb, int64_t q_sh,
     p.Hv = Hkv * p.NG;
     if (max_tokens > kv8::kMaxTokens || (int64_t)B * p.Hv * ceil_div(max_tokens, kv8::kChunk) > (int64_t)1 << 30)
         return fail(MX_ERR_UNSUPPORTED, "%s: more tokens than 32-bit numbers hold", what);
-    p.workers = kv8::workers_for(max_tokens);
+    const bool segments = kv8::by_segment((int64_t)B * p.Hv, max_tokens, D);
+    p.workers = kv8::kWorkers;
     p.scale_log2e = scale * 1.4426950408889634f;
     p.out = out, p.o_sb = o_sb, p.o_sh = o_sh, p.err = err;
-    if (p.workers > 0) {
+    if (!segments) {
         const size_t need = mx_kv8_attn_workspace_bytes(B, Hq, Hkv, D, max_blocks, block_size);
         if (!workspace || workspace_bytes < need)
             return fail(MX_ERR_WORKSPACE, "%s: workspace needs %zu bytes, got %zu", what, need, workspace_bytes);
@@ -546,20 +635,31 @@ extern "C" int mx_kv8_attn_decode(const uint16_t* q, int64_t q_sb, int64_t q_sh,
         p.part_acc = static_cast<float*>(workspace);
         p.part_ml = p.part_acc + (size_t)2 * p.workers * p.GS * D;
     }
-    const int64_t waves = p.workers > 0 ? p.workers : (int64_t)B * p.Hv;
-    const dim3 grid((unsigned)ceil_div(waves, kv8::kAttnWaves)), block(kv8::kAttnWaves * 64);
     hipStream_t st = as_stream(stream);
-#define CALL(DD, BB)                                                                                             \
-    if (flags & MX_PA_BF16) {                                                                                    \
-        hipLaunchKernelGGL((kv8::kv8_attn_kernel<DD, BB, true>), grid, block, 0, st, p);                         \
-        if (p.workers > 0)                                                                                       \
-            hipLaunchKernelGGL((kv8::kv8_merge_kernel<DD, BB, true>), dim3(Hq, B), dim3(kv8::kMergeWaves * 64), 0, st, p);  \
-    } else {                                                                                                     \
-        hipLaunchKernelGGL((kv8::kv8_attn_kernel<DD, BB, false>), grid, block, 0, st, p);                        \
-        if (p.workers > 0)                                                                                       \
-            hipLaunchKernelGGL((kv8::kv8_merge_kernel<DD, BB, false>), dim3(Hq, B), dim3(kv8::kMergeWaves * 64), 0, st, p); \
+    // Waves of a segment's workgroup: at most a step each at the table's width, within 64 KiB of LDS. A CU
+    // holds 8 of them: where there are more segments than CUs, two workgroups of 4 beat one of 8 (1024
+    // segments of up to 300 tokens 24.5 -> 18.2 us, of up to 2048 63.6 -> 59.6).
+    const int64_t piece = (int64_t)p.GS * (D + 2) * sizeof(float);
+    const int64_t most = (int64_t)B * p.Hv > 256 ? kv8::kSegmentWaves / 2 : kv8::kSegmentWaves;
+    const int waves = (int)std::min<int64_t>({most, ceil_div(max_tokens, kv8::kStep * kv8::kChunk),
+                                              65536 / piece});
+    const size_t lds = waves > 1 ? waves * piece : 0;
+#define LAUNCH(DD, BB, F)                                                                                            \
+    if (segments) {                                                                                                  \
+        hipLaunchKernelGGL((kv8::kv8_attn_segment_kernel<DD, BB, F>), dim3(p.Hv, B), dim3(waves * 64), lds, st, p);  \
+    } else {                                                                                                         \
+        hipLaunchKernelGGL((kv8::kv8_attn_kernel<DD, BB, F>), dim3(kv8::kWorkers / kv8::kAttnWaves),                 \
+                           dim3(kv8::kAttnWaves * 64), 0, st, p);                                                    \
+        hipLaunchKernelGGL((kv8::kv8_merge_kernel<DD, BB, F>), dim3(Hq, B), dim3(kv8::kMergeWaves * 64), 0, st, p);  \
+    }
+#define CALL(DD, BB)             \
+    if (flags & MX_PA_BF16) {    \
+        LAUNCH(DD, BB, true)     \
+    } else {                     \
+        LAUNCH(DD, BB, false)    \
     }
     MX_KV8_DISPATCH(D, block_size, CALL)
 #undef CALL
+#undef LAUNCH
     return check_launch(what);
 }

@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from .kv8 import BLOCK_SIZES, HEAD_DIMS, Kv8Layer, kv8_append, kv8_gather
+from .kv8 import BLOCK_SIZES, HEAD_DIMS, Kv8Layer, kv8_append, kv8_attention_decode, kv8_gather
 from .paged_attention_hip import _DTYPE_FLAGS
 from .paged_kv_kernel import GpuKVBlockPool
 
@@ -105,6 +105,13 @@ class Int8KVBlockPool(GpuKVBlockPool):
                    err=self._write_err, used_blocks=self._used_map)
         if self.sync_write_checks and not torch.cuda.is_current_stream_capturing():
             self.check_write_errors()
+
+    def attend(self, layer_idx: int, query: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+               scaling: float, num_kv_groups: int) -> torch.Tensor:
+        """One decode step's attention over a layer (``kv8_attention_decode``); a block id outside the pool
+        is reported by :meth:`check_write_errors`."""
+        return kv8_attention_decode(query, self.layer_store(layer_idx), block_tables, seq_lens, scaling,
+                                    num_kv_groups, err=self._write_err)
 
     def _gathers_on_device(self, tokens: int) -> bool:
         return True

@@ -187,17 +187,14 @@ def _decode(query: torch.Tensor, k_layer: torch.Tensor, v_layer: torch.Tensor, b
 def paged_attention_decode_batched(query: torch.Tensor, metadata: PagedDecodeBatchMetadata, num_kv_groups: int,
                                    scaling: float) -> torch.Tensor:
     """Batched decode: ``query [B, heads, 1, dim]`` -> ``[B, heads, 1, dim]`` (``:745-775``), over a 16-bit
-    pool or an ``Int8KVBlockPool`` (``kv8_attention_decode``)."""
+    pool or an ``Int8KVBlockPool`` (its ``attend``)."""
     if query.shape[0] != metadata.block_tables.shape[0]:
         raise ValueError("query batch size must match block_tables rows")
     _hip.require_device_tensor(query, "query")
     pool = metadata.pool
     pool._ensure_pools()
     if getattr(pool, "kv_bits", 16) == 8:
-        from .kv8 import kv8_attention_decode
-
-        return kv8_attention_decode(query, pool.layer_store(metadata.layer_idx), metadata.block_tables,
-                                    metadata.seq_lens, scaling, num_kv_groups, err=pool._write_err)
+        return pool.attend(metadata.layer_idx, query, metadata.block_tables, metadata.seq_lens, scaling, num_kv_groups)
     k_layer = pool.k_layer_view(metadata.layer_idx)
     v_layer = pool.v_layer_view(metadata.layer_idx)
     return _decode(query, k_layer, v_layer, metadata.block_tables, metadata.seq_lens, scaling, num_kv_groups,

@@ -293,10 +293,12 @@ def test_attention_matches_float64(hkv, bs, d, dt, group):
     b = len(lens)
     pool, cache, tables = _cached(b, lens, hkv, bs, d, dtype, g)
     q = torch.randn(b, hkv * group, 1, d, generator=g).to(dtype)
-    meta = PagedDecodeBatchMetadata(pool=pool, layer_idx=0, block_tables=tables.to(DEV), seq_lens=_int(lens).to(DEV))
-    out = paged_attention_decode_batched(q.to(DEV), meta, group, d ** -0.5)
-    _near(out, *cache.attend(q[:, :, 0], tables, lens, d ** -0.5), dtype)
-    assert (out[0] == 0).all()
+    want = cache.attend(q[:, :, 0], tables, lens, d ** -0.5)
+    for table in (tables, _widen(tables, 140_000 // bs)):  # a workgroup per segment; shared out between waves
+        meta = PagedDecodeBatchMetadata(pool=pool, layer_idx=0, block_tables=table.to(DEV), seq_lens=_int(lens).to(DEV))
+        out = paged_attention_decode_batched(q.to(DEV), meta, group, d ** -0.5)
+        _near(out, *want, dtype)
+        assert (out[0] == 0).all()
     pool.check_write_errors()
 
 
@@ -314,15 +316,61 @@ def test_attention_over_long_and_ragged_rows(hkv, bs, d, dt, group, lens):
     _near(out, *cache.attend(q[:, :, 0], tables, lens, d ** -0.5), dtype)
 
 
-def test_many_short_rows():
+def _widen(tables, blocks):
+    """The same rows in a table of ``blocks`` entries, the new ones outside the pool and never read."""
+    return torch.cat([tables, torch.full((len(tables), blocks - tables.shape[1]), -7, dtype=torch.int32)], dim=1)
+
+
+@pytest.mark.parametrize("b", [63, 64, 65, 150, 300])
+@pytest.mark.parametrize("wide", [0, 5000])
+def test_many_short_rows(b, wide):
+    """A workgroup per row (narrow table) and rows shared out between waves (wide table), with rows
+    without tokens in runs, also first and last, around the 64 rows that a wave takes at once."""
     from runtime_amd.phase2.kv8 import kv8_attention_decode
 
-    hkv, bs, d, dtype, g, b = 1, 16, 64, torch.float16, _gen(3), 150
-    lens = [(37 * i) % 90 for i in range(b)]
+    hkv, bs, d, dtype, g = 1, 16, 64, torch.float16, _gen(3)
+    lens = [0 if i < 3 or i % 64 in (62, 63, 0) or i == b - 1 else (37 * i) % 90 for i in range(b)]
     pool, cache, tables = _cached(b, lens, hkv, bs, d, dtype, g)
     q = torch.randn(b, 2, 1, d, generator=g).to(dtype)
+    want = cache.attend(q[:, :, 0], tables, lens, 0.125)
+    tables = _widen(tables, wide) if wide else tables
     out = kv8_attention_decode(q.to(DEV), pool.layer_store(0), tables.to(DEV), _int(lens).to(DEV), 0.125, 2)
-    _near(out, *cache.attend(q[:, :, 0], tables, lens, 0.125), dtype)
+    _near(out, *want, dtype)
+
+
+def test_no_row_has_tokens():
+    from runtime_amd.phase2.kv8 import kv8_attention_decode
+
+    pool = _pool(4, 2, 16, 128, torch.bfloat16)
+    q = torch.randn(70, 8, 1, 128).bfloat16().to(DEV)
+    for width in (1, 9000):
+        out = kv8_attention_decode(q, pool.layer_store(0), torch.zeros(70, width, dtype=torch.int32, device=DEV),
+                                   torch.zeros(70, dtype=torch.int32, device=DEV), 1.0, 4)
+        assert (out == 0).all()
+
+
+def test_v_of_every_size():
+    """V pages from the smallest to the largest scale side by side: in fp16 the scales above 2^5 leave a
+    factor to the weights."""
+    from runtime_amd.phase2.kv8 import kv8_attention_decode
+
+    for dtype, exps in ((torch.float16, (-24, -10, 0, 5, 6, 8, 9)), (torch.bfloat16, (-126, -20, 0, 119, 120, 121))):
+        for bs in (4, 16):
+            g, d = _gen(17), 64
+            n = 16 * len(exps)
+            pool, cache = _pool(n // bs, 1, bs, d, dtype), Kv8Cache(n // bs, 1, bs, d, dtype)
+            tables = torch.arange(n // bs)[None].int()
+            k = torch.randn(1, 1, n, d, generator=g).to(dtype)
+            ints = torch.randint(-127, 128, (1, 1, n, d), generator=g).double()
+            ints[..., 0] = 127
+            v = (ints.view(1, 1, -1, 16, d) * torch.tensor([2.0 ** e for e in exps], dtype=torch.float64)[:, None, None])
+            v = v.view(1, 1, n, d).to(dtype)
+            pool.write_tokens_batch(0, tables.to(DEV), _int([0]).to(DEV), k.to(DEV), v.to(DEV))
+            cache.write(tables, [0], k, v)
+            # Each query is a key, so that its weights lie on one page or another.
+            q = (8 * k[0, 0, 3::16][:len(exps)])[None, :, None].contiguous()
+            out = kv8_attention_decode(q.to(DEV), pool.layer_store(0), tables.to(DEV), _int([n]).to(DEV), 1.0, len(exps))
+            _near(out, *cache.attend(q[:, :, 0], tables, [n], 1.0), dtype)
 
 
 def test_large_scores_and_one_token_that_takes_all():
@@ -351,10 +399,13 @@ def test_blocks_outside_the_pool_and_poisoned_pages():
     tables[0, 2], tables[2, :2] = cache.nb, -5  # one page of row 0, all of row 2
     q = torch.randn(3, 4, 1, d, generator=g).to(dtype)
 
-    def run():
-        return kv8_attention_decode(q.to(DEV), pool.layer_store(0), tables.to(DEV), _int(lens).to(DEV), 0.125, 2,
+    def run(table=tables):
+        return kv8_attention_decode(q.to(DEV), pool.layer_store(0), table.to(DEV), _int(lens).to(DEV), 0.125, 2,
                                     err=pool._write_err)
 
+    _near(run(_widen(tables, 9000)), *cache.attend(q[:, :, 0], tables, lens, 0.125))
+    with pytest.raises(IndexError, match="attention"):
+        pool.check_write_errors()
     out = run()
     _near(out, *cache.attend(q[:, :, 0], tables, lens, 0.125))
     assert (out[2] == 0).all()
@@ -365,8 +416,9 @@ def test_blocks_outside_the_pool_and_poisoned_pages():
     bad[0, 1, 0, 3] = float("nan")
     for kv in ((bad, x), (x, bad)):  # K, then V, of head 1 in row 1's last page
         pool.write_tokens_batch(0, tables[1:2].to(DEV), _int([39]).to(DEV), kv[0].to(DEV), kv[1].to(DEV))
-        out = run()
-        assert torch.isnan(out[1, 2:]).all() and torch.isfinite(out[1, :2]).all() and torch.isfinite(out[[0, 2]]).all()
+        for out in (run(), run(_widen(tables, 9000))):
+            assert torch.isnan(out[1, 2:]).all() and torch.isfinite(out[1, :2]).all()
+            assert torch.isfinite(out[[0, 2]]).all()
         pool.write_tokens_batch(0, tables[1:2].to(DEV), _int([32]).to(DEV), x.expand(1, hkv, 8, d).to(DEV),
                                 x.expand(1, hkv, 8, d).to(DEV))
         assert torch.isfinite(run()).all()

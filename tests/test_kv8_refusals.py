@@ -91,6 +91,17 @@ def test_entry_points_refuse_what_is_theirs():
     _status(_attend(q_sh=60), _hip.MX_ERR_ALIGNMENT)
     _status(_attend(o_sh=68), _hip.MX_ERR_ALIGNMENT)
     _status(_attend(B=65536), _hip.MX_ERR_UNSUPPORTED)
+    _status(_attend(codes=ctypes.c_void_p(4097)), _hip.MX_ERR_ALIGNMENT)
+    _status(_attend(mb=1 << 27), _hip.MX_ERR_UNSUPPORTED)           # 2**31 tokens in a row
+    _status(_attend(mb=1 << 20, B=1024, hkv=4), _hip.MX_ERR_UNSUPPORTED)  # 2**32 chunks
+    # A wide table shares rows out between waves: room for their pieces, aligned, is asked for.
+    need = _hip.load().mx_kv8_attn_workspace_bytes(1, 4, 2, 64, 4096, 16)
+    assert need == 2 * 2048 * 2 * (64 + 2) * 4
+    _status(_attend(mb=4096, ws=None, wsb=0), _hip.MX_ERR_WORKSPACE)
+    _status(_attend(mb=4096, wsb=need - 1), _hip.MX_ERR_WORKSPACE)
+    _status(_attend(mb=4096, ws=ctypes.c_void_p(4096 + 128)), _hip.MX_ERR_ALIGNMENT)
+    assert _hip.load().mx_kv8_attn_workspace_bytes(1, 4, 2, 64, 4, 16) == 0
+    assert _hip.load().mx_kv8_attn_workspace_bytes(1, 5, 2, 64, 4096, 16) == 0
 
 
 def _arr(*ids):
