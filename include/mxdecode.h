@@ -629,7 +629,7 @@ int mx_kv8_attn_decode(const uint16_t* q, int64_t q_sb, int64_t q_sh, const uint
  * source is read as it was before the call, in whatever order the pairs stand.
  * Of several pairs with one dst the last counts. used (nullable, uint8
  * [num_pages]) gets 1 at every dst; with move != 0 no page may occur twice in the
- * two lists, and used gets 0 at every src. More than 448 pairs that depend on each
+ * two lists, and used's entries move along, leaving 0. More than 448 pairs that depend on each
  * other (a page that is a src and a dst) are refused (MX_ERR_UNSUPPORTED).
  * GpuKVBlockPool.copy_blocks (runtime/phase2/paged_kv_kernel.py:233-250). */
 int mx_kv_copy_pages(void* base, int64_t page_bytes, int64_t layer_stride, void* base2, int64_t page_bytes2,

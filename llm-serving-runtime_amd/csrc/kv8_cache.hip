@@ -325,7 +325,14 @@ __device__ __forceinline__ uint32_t qkv_element(const TokenParams& p, int b, int
     if (!p.part) return p.qkv[(int64_t)b * p.qkv_stride + col];
     float acc = p.bias ? widen<BF16>(p.bias[col]) : 0.0f;
     const float* q = p.part + (int64_t)b * width + col;
-    for (int s = 0; s < p.splits; ++s) acc += q[s * p.split_stride];
+    for (int s0 = 0; s0 < p.splits; s0 += 8) {  // 8 loads in flight, added in order
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = q[(s0 + u < p.splits ? s0 + u : p.splits - 1) * p.split_stride];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (s0 + u < p.splits) acc += v[u];
+    }
     return round16<BF16>(acc);
 }
 

@@ -27,7 +27,7 @@ struct CopyParams {
     Region r[2];
     int layers;
     int slices;  // workgroups per (pair, layer)
-    int move;    // sources are free afterwards: their marks are cleared
+    int move;    // sources are free afterwards: their marks go with the pages
     uint8_t* used;  // optional [pages]: 1 where a page was written
     int2 pair[kBatch];
 };
@@ -51,7 +51,7 @@ __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyParams p) {
     const int slice = blockIdx.x, layer = blockIdx.y;
     const int2 pr = p.pair[blockIdx.z];
     if (p.used && slice == 0 && layer == 0 && threadIdx.x == 0) {
-        p.used[pr.y] = 1;
+        p.used[pr.y] = p.move ? p.used[pr.x] : 1;
         if (p.move) p.used[pr.x] = 0;
     }
     copy_run(p.r[0], layer, pr.x, pr.y, slice, p.slices);

@@ -318,10 +318,10 @@ class GpuKVBlockPool:
             except (ValueError, OverflowError):
                 self._check_move(src, dst)
                 raise
-            # On a device pool its map has the marks (read with the counts), here only the old ids go.
-            self._used_blocks.difference_update(src)
-            if not on_device:
-                self._touch_ids(dst)
+            held = self._used_blocks.intersection(src)  # the device map's marks move with the pages
+            if held:
+                self._used_blocks.update([d for s, d in zip(src, dst) if s in held])
+                self._used_blocks -= held
             if block_tables is not None:
                 self._rename(block_tables, out, a, b)
         elif block_tables is not None and out is not block_tables:

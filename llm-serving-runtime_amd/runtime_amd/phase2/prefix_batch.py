@@ -21,6 +21,9 @@ scheduler):
   same group into their slots (join/finish). ``tables`` / ``lens`` are the int32 block
   tables and KV lengths the decode step reads, kept on the host and copied to
   fixed device tensors by :meth:`upload` (addresses stay valid for a captured graph);
+* :meth:`PrefixBatch.fork` and :meth:`PrefixBatch.compact` — a row continued by several (parallel
+  samples) and the live blocks brought together at the low ids, as host bookkeeping; each returns the
+  block ids that the pool has to copy or move (``GpuKVBlockPool.copy_blocks``, ``move_blocks``);
 * :meth:`PrefixBatch.unique_tokens` / :meth:`PrefixBatch.logical_tokens` — K/V tokens
   stored once vs. read per step, the byte counts the measurement is quoted on.
 """
@@ -72,12 +75,23 @@ class BlockAllocator:
     def refcount(self, i: int) -> int:
         return self._refs[i]
 
+    def compact(self) -> dict[int, int]:
+        """Rename the allocated ids so that they are the lowest ones, moving as few as can be; returns
+        {old id: new id} of those that change, whose old ids are free then."""
+        live = sum(r > 0 for r in self._refs)
+        moves = dict(zip((i for i in range(live, len(self._refs)) if self._refs[i]),
+                         (i for i in range(live) if not self._refs[i])))
+        for old, new in moves.items():
+            self._refs[new], self._refs[old] = self._refs[old], 0
+        self._free = list(range(len(self._refs) - 1, live - 1, -1))
+        return moves
+
 
 @dataclass
 class Row:
     group: int
     length: int          # tokens in the KV cache (the next token's position)
-    shared: int          # leading blocks that are the group's prefix (0 when not shared)
+    shared: int          # leading blocks that other rows hold too: the group's prefix, a fork's full blocks
     blocks: list[int]    # physical ids, prefix first
 
 
@@ -129,6 +143,42 @@ class PrefixBatch:
             old = self.rows[b]
             self.alloc.decref(old.blocks)
             self.rows[b] = self._admit(old.group, None if lengths is None else lengths[j])
+
+    def fork(self, row: int, slots: list[int]) -> tuple[list[int], list[int]]:
+        """Finish the requests in ``slots`` and continue ``row``'s request there too. The forks hold the
+        row's full blocks with it; the block that its next token goes to becomes one of their own. Returns
+        the (source, destination) ids that ``copy_blocks`` has to copy before the next step."""
+        parent = self.rows[row]
+        if row in slots or len(set(slots)) != len(slots):
+            raise ValueError("fork takes every slot once, and not the row itself")
+        if any(self.rows[b].group != parent.group for b in slots):
+            raise ValueError("a row's forks go to slots of its group")
+        full = parent.length // self.block_size
+        need = math.ceil((parent.length + self.headroom) / self.block_size)
+        copied = full < math.ceil(parent.length / self.block_size)
+        src: list[int] = []
+        dst: list[int] = []
+        for b in slots:
+            self.alloc.decref(self.rows[b].blocks)
+            held = parent.blocks[:full]
+            self.alloc.incref(held)
+            own = self.alloc.alloc(need - full)
+            self.rows[b] = Row(parent.group, parent.length, full, held + own)
+            if copied:
+                src.append(parent.blocks[full])
+                dst.append(own[0])
+        if slots:
+            parent.shared = max(parent.shared, full)
+        return src, dst
+
+    def compact(self) -> tuple[list[int], list[int]]:
+        """Bring the live blocks together at the low ids. Returns the (source, destination) ids for
+        ``move_blocks``, which also renames the device tables of :meth:`upload`."""
+        moves = self.alloc.compact()
+        for r in self.rows:
+            r.blocks = [moves.get(i, i) for i in r.blocks]
+        self.prefix_blocks = [[moves.get(i, i) for i in blocks] for blocks in self.prefix_blocks]
+        return list(moves), list(moves.values())
 
     def advance(self, steps: int = 1) -> None:
         """Host mirror of the decode step's length advance."""

@@ -163,3 +163,67 @@ def test_refusals_leave_the_pool_as_it_was(kind):
     _check(pool, was, {})
     pool.copy_blocks([], []), pool.free_blocks([])
     assert torch.equal(pool.move_blocks([], [], tables), tables)
+
+
+@pytest.mark.parametrize("kind", POOLS)
+def test_forked_and_compacted_rows_decode_as_before(kind):
+    """``PrefixBatch`` rows that share a prefix, fork and are compacted, with the pool's copies and moves and
+    attention over it: a fork decodes as its parent, and not a bit changes when blocks move."""
+    from runtime_amd.phase2.kv8_pool import Int8KVBlockPool
+    from runtime_amd.phase2.paged_attention_hip import PagedDecodeBatchMetadata, paged_attention_decode_batched
+    from runtime_amd.phase2.paged_kv_kernel import GpuKVBlockPool
+    from runtime_amd.phase2.prefix_batch import PrefixBatch
+
+    bs, hkv, d, layers = 16, 2, 64, 2
+    pb = PrefixBatch(batch=6, groups=2, prefix_tokens=32, lo=33, hi=200, block_size=bs, num_blocks=160, headroom=20, seed=2)
+    args = dict(num_blocks=160, block_size_tokens=bs, num_layers=layers, num_kv_heads=hkv, head_dim=d,
+                dtype=torch.float16, device=DEV)
+    pool = Int8KVBlockPool(**args) if kind == "int8" else GpuKVBlockPool(**args, kv_layout=kind)
+    g = torch.Generator().manual_seed(4)
+    shared = torch.randn(2, layers, 2, 1, hkv, 32, d, generator=g).half()
+    for r in pb.rows:
+        for li in range(layers):
+            kv = torch.randn(2, 1, hkv, r.length, d, generator=g).half()
+            kv[:, :, :, :32] = shared[r.group, li]
+            pool.write_tokens(li, r.blocks, 0, kv[0].to(DEV), kv[1].to(DEV))
+    tables, lens = torch.zeros(6, pb.max_blocks, dtype=torch.int32, device=DEV), torch.zeros(6, dtype=torch.int32, device=DEV)
+    q = torch.randn(6, 3 * hkv, 1, d, generator=g).half().to(DEV)
+
+    def attend(query=q):
+        return [paged_attention_decode_batched(query, PagedDecodeBatchMetadata(
+            pool=pool, layer_idx=li, block_tables=tables, seq_lens=lens, shared_blocks=True), 3, d ** -0.5)
+            for li in range(layers)]
+
+    pool.copy_blocks(*pb.fork(1, [0, 2]))
+    pb.upload(tables, lens)
+    # Forks hold the parent's tokens bit for bit. Their outputs for one query differ only by where a row is
+    # cut into pieces: each is within 6 half steps of 2**-11 of the largest |v| of the exact one.
+    same = q[1:2].expand(6, -1, -1, -1).contiguous()
+    for li, out in enumerate(attend(same)):
+        rows = [pool.gather_layer(li, r.blocks, r.length) for r in pb.rows[:3]]
+        for k, v in rows:
+            assert torch.equal(k, rows[1][0]) and torch.equal(v, rows[1][1])
+        assert (out[[0, 2]] - out[1]).abs().max() <= 12 * 2.0 ** -11 * rows[1][1].abs().max()
+        assert (out[3] - out[1]).abs().max() > 0.1
+    before = attend()
+    for li in range(layers):  # a step: each row's own token, beside the shared blocks
+        kv = torch.randn(2, 6, hkv, 1, d, generator=g).half().to(DEV)
+        pool.write_tokens_batch(li, tables, lens, kv[0], kv[1])
+    for a, b in zip(before, attend()):
+        assert torch.equal(a, b)  # what the rows held is untouched
+    pb.advance()
+    lens.add_(1)
+    before = attend()
+    assert not torch.equal(before[0][0], before[0][1])
+    pool.free_blocks([i for i in range(160) if pb.alloc.refcount(i) == 0])
+    held = pool.allocated_block_count()
+    src, dst = pb.compact()
+    assert len(src) > 4
+    pool.move_blocks(src, dst, tables, out=tables)
+    assert torch.equal(tables.cpu()[:, :2], pb.tables[:, :2])
+    for a, b in zip(before, attend()):
+        assert torch.equal(a, b)
+    assert pool.allocated_block_count() == held
+    live = {i for i in range(160) if pb.alloc.refcount(i)}
+    assert live == set(range(len(live))) and pool._used_blocks <= live
+    pool.check_write_errors()

@@ -219,7 +219,9 @@ def test_move_and_free_blocks_on_the_cpu_pool():
     for a, b in zip(_snapshot(pool), was):
         for now, old in zip(a, b):
             assert torch.equal(now, old[[0, 7, 8, 3, 4, 5, 6, 7, 8]])
-    assert pool.allocated_block_count() == pool.peak_allocated_block_count() == 3
+    assert pool._used_blocks == {1, 2, 3} and pool.peak_allocated_block_count() == 3
+    pool.move_blocks([5], [6])  # nothing was written to block 5
+    assert pool._used_blocks == {1, 2, 3}
     pool.free_blocks([1, 2, 2])
     assert pool.allocated_block_count() == 1
     assert pool.move_blocks([], [], tables).tolist() == tables.tolist()
