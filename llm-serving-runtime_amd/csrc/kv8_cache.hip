@@ -11,6 +11,8 @@
 // ranges, so nothing is ordered between waves. K is handled by (token, 8 dims) pieces, as its 16-byte
 // loads come; V by dims, each lane holding every token of its D / 64 dims, so that the token-minor
 // rows are built in registers without a transpose.
+#include <type_traits>
+
 #include "common.h"
 #include "glue_common.h"
 #include "kv8.h"
@@ -33,8 +35,15 @@ struct WriteParams {
     int32_t* err;
     uint8_t* used;  // optional [num_blocks] map: 1 where a token was written
     int pages_per_row;  // pages a row's write can touch: T tokens that begin inside a page
+    int stream;         // the states are read with the streaming policy
     int64_t units;
 };
+
+// States larger than the L2s together are gone from them when the next reader comes, and read with the
+// streaming policy they displace nothing: 134 MB of them 50 -> 37 us. Smaller ones, 8 MB that the L2s still
+// hold, take 6.6 us that way and 5.9 with the default.
+constexpr int64_t kStreamBytes = 32 << 20;
+typedef uint32_t u32x4n __attribute__((ext_vector_type(4)));
 
 // A run's codes: the one it had (0 when the write starts the page anew) and the one it gets.
 struct Codes {
@@ -156,14 +165,24 @@ __global__ __launch_bounds__(kWaves * 64) void kv8_write_kernel(WriteParams p) {
     uint4 xk[NI];
     uint32_t xv[BS];
     if (kind == 0) {
+        auto at = [&](int i) { return p.k_new + src + offset(i * TPI + lane / CH) + (lane % CH) * 8; };
+        if (p.stream) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-            xk[i] = glue::ld16(p.k_new + src + offset(i * TPI + lane / CH) + (lane % CH) * 8);
+            for (int i = 0; i < NI; ++i)
+                xk[i] = __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4n*>(at(i))));
+        } else {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) xk[i] = glue::ld16(at(i));
+        }
     } else {
+        typedef typename std::conditional<DP == 2, uint32_t, uint16_t>::type Elem;
+        auto at = [&](int s) { return reinterpret_cast<const Elem*>(p.v_new + src + offset(s) + lane * DP); };
+        if (p.stream) {
 #pragma unroll
-        for (int s = 0; s < BS; ++s) {
-            const uint16_t* q = p.v_new + src + offset(s) + lane * DP;
-            xv[s] = DP == 2 ? *reinterpret_cast<const uint32_t*>(q) : (uint32_t)*q;
+            for (int s = 0; s < BS; ++s) xv[s] = __builtin_nontemporal_load(at(s));
+        } else {
+#pragma unroll
+            for (int s = 0; s < BS; ++s) xv[s] = *at(s);
         }
     }
     const int phys = lb < p.max_blocks ? p.bt[(int64_t)b * p.bt_sb + lb] : -1;
@@ -435,13 +454,14 @@ extern "C" int mx_kv8_write(const uint16_t* k_new, const uint16_t* v_new, int64_
     if (!aligned(k_new, 16) || !aligned(v_new, 16) || new_sb % 8 || new_sh % 8 || new_st % 8)
         return fail(MX_ERR_ALIGNMENT, "%s: states must be 16-byte aligned rows", what);
     kv8::WriteParams p{k_new, v_new, new_sb, new_sh, new_st, T, block_tables, bt_sb, max_blocks, start_pos,
-                       {data, codes, Hkv, num_blocks}, err, used, 0, 0};
+                       {data, codes, Hkv, num_blocks}, err, used, 0, 0, 0};
     // Pages that T tokens beginning at any slot can touch.
     p.pages_per_row = (int)((int64_t)(T - 1 + block_size - 1) / block_size + 1);
     if ((double)B * p.pages_per_row * Hkv * 2 > 1e11) return fail(MX_ERR_UNSUPPORTED, "%s: too many tokens", what);
     p.units = (int64_t)B * p.pages_per_row * Hkv * 2;
     const int64_t groups = kv8::groups_for(p.units);
     if (groups < 0) return fail(MX_ERR_UNSUPPORTED, "%s: more tokens than one launch holds", what);
+    p.stream = (int64_t)B * T * Hkv * D * 4 > kv8::kStreamBytes;
     hipStream_t st = as_stream(stream);
 #define CALL(DD, BB)                                                                                                   \
     if (flags & MX_PA_BF16)                                                                                            \

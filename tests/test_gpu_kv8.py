@@ -76,6 +76,21 @@ def test_writes_and_rows_match_the_definition(hkv, bs, d, dt):
     assert torch.equal(k.cpu().double(), want[0]) and torch.equal(v.cpu().double(), want[1])
 
 
+@pytest.mark.parametrize("bs,d,dt,t", [(32, 128, "fp16", 8603), (32, 64, "bf16", 17001)])
+def test_a_prompt_past_32_mib_of_states(bs, d, dt, t):
+    """States that the streaming loads read (8 heads, 4 bytes a K/V element pair), from inside a page on."""
+    dtype, g, hkv, start = DTYPES[dt], _gen(t), 8, 5
+    assert 8 * t * d * 4 > 32 << 20
+    nb = -(-(start + t) // bs)
+    pool, cache = _pool(nb, hkv, bs, d, dtype), Kv8Cache(nb, hkv, bs, d, dtype)
+    tables = torch.randperm(nb, generator=g).int()[None]
+    for at, n in ((0, start), (start, t)):
+        k, v = _states(1, hkv, n, d, dtype, g), _states(1, hkv, n, d, dtype, g)
+        pool.write_tokens_batch(0, tables.to(DEV), _int([at]).to(DEV), k.to(DEV), v.to(DEV))
+        cache.write(tables, [at], k, v)
+    _same(pool, cache, tables, start + t)
+
+
 @pytest.mark.parametrize("dt", ["fp16", "bf16"])
 def test_extreme_values(dt):
     """The largest and smallest numbers of the type, zeros, halfway cases, and values that are not finite."""
