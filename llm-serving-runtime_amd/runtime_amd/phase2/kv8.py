@@ -186,7 +186,7 @@ def kv8_rope_append(qkv: torch.Tensor | None, rope: torch.Tensor, positions: tor
     _hip.require_device_tensor(q_out, "q_out")
     if q_out.dim() < 2 or q_out.dtype != layer.dtype or q_out.device != dev or q_out.shape[-1] != num_heads * d:
         raise ValueError("q_out must be [B, Hq * D] of the cache's dtype and device")
-    q2 = q_out.view(-1, num_heads * d)
+    q2 = q_out if q_out.dim() == 2 else q_out.view(-1, num_heads * d)
     b = int(q2.shape[0])
     if q2.stride(1) != 1 or (b > 1 and q2.stride(0) < num_heads * d):
         raise ValueError("q_out must have rows of their own with unit stride")
@@ -195,7 +195,7 @@ def kv8_rope_append(qkv: torch.Tensor | None, rope: torch.Tensor, positions: tor
         _hip.require_device_tensor(qkv, "qkv")
         if qkv.shape[-1] != width or qkv.dtype != layer.dtype or qkv.device != dev:
             raise ValueError("qkv must be [B, (Hq + 2 Hkv) * D] of the cache's dtype and device")
-        x = qkv.reshape(-1, width)
+        x = qkv if qkv.dim() == 2 else qkv.reshape(-1, width)
         if x.stride(1) != 1:
             x = x.contiguous()
         if x.shape[0] != b:
@@ -212,6 +212,8 @@ def kv8_rope_append(qkv: torch.Tensor | None, rope: torch.Tensor, positions: tor
             or rope.device != dev):
         raise ValueError("rope must be a contiguous fp32 [max_pos, D/2, 2] table")
     pos = _lengths(positions, b, dev)
+    if lens_out is not None and (lens_out.device != dev or abs(lens_out.data_ptr() - pos.data_ptr()) < 4 * b):
+        raise ValueError("lens_out must be on the cache's device and not the positions themselves")
     tables = _tables(block_tables, b, dev)
     with _hip.on_device(dev):
         rc = _hip.load().mx_kv8_rope_append(

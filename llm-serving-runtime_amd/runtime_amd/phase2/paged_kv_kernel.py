@@ -301,7 +301,7 @@ class GpuKVBlockPool:
                 raise ValueError("out goes with block_tables")
         else:
             if (block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.stride(1) != 1
-                    or block_tables.device.type != self.device.type):
+                    or block_tables.device != self._page_regions()[0].device):
                 raise ValueError("block_tables must be int32 [B, max_blocks] with unit inner stride on the pool's device")
             if out is None:
                 out = torch.empty(block_tables.shape, dtype=torch.int32, device=block_tables.device)
@@ -344,13 +344,13 @@ class GpuKVBlockPool:
         self._used_blocks.difference_update(ids)
         if not ids or self._used_map is None:
             return
-        codes = self._freed_codes()
+        codes, dev = self._freed_codes(), self._used_map.device
         arr = array.array("i", ids)
-        with _hip.on_device(self.device):
+        with _hip.on_device(dev):
             _hip.check(_hip.load().mx_kv_clear_pages(
                 codes.data_ptr() if codes is not None else None, codes[0, 0].numel() if codes is not None else 0,
                 codes.stride(0) if codes is not None else 0, self.shape.num_layers, self._used_map.data_ptr(),
-                self.shape.num_blocks, arr.buffer_info()[0], len(ids), _hip.stream_handle(self.device)),
+                self.shape.num_blocks, arr.buffer_info()[0], len(ids), _hip.stream_handle(dev)),
                 "mx_kv_clear_pages")
 
     def _freed_codes(self) -> torch.Tensor | None:
@@ -370,10 +370,11 @@ class GpuKVBlockPool:
             for t in (*regions, None)[:2]:
                 args += [None, 0, 0] if t is None else [t.data_ptr(), t[0, 0].numel() * t.element_size(),
                                                         t.stride(0) * t.element_size()]
-            with _hip.on_device(self.device):
+            dev = regions[0].device
+            with _hip.on_device(dev):
                 rc = _hip.load().mx_kv_copy_pages(
                     *args, self.shape.num_layers, self.shape.num_blocks, src.buffer_info()[0], dst.buffer_info()[0],
-                    len(src), self._used_map.data_ptr(), int(move), _hip.stream_handle(self.device))
+                    len(src), self._used_map.data_ptr(), int(move), _hip.stream_handle(dev))
             if rc != _hip.MX_ERR_UNSUPPORTED:  # else: more copies that depend on each other than a launch takes
                 _hip.check(rc, "mx_kv_copy_pages")
                 return
@@ -389,10 +390,10 @@ class GpuKVBlockPool:
             out.copy_(torch.tensor([[name.get(i, i) for i in row] for row in tables.tolist()],
                                    dtype=torch.int32).view(tables.shape))
             return
-        with _hip.on_device(self.device):
+        with _hip.on_device(tables.device):
             _hip.check(_hip.load().mx_kv_rename_pages(
                 tables.data_ptr(), tables.stride(0), out.data_ptr(), out.stride(0), tables.shape[0], tables.shape[1],
-                src.buffer_info()[0], dst.buffer_info()[0], len(src), _hip.stream_handle(self.device)),
+                src.buffer_info()[0], dst.buffer_info()[0], len(src), _hip.stream_handle(tables.device)),
                 "mx_kv_rename_pages")
 
     def gather_layer(self, layer_idx: int, block_ids: list[int], seq_len: int) -> tuple[torch.Tensor, torch.Tensor]:

@@ -485,6 +485,9 @@ def test_wrappers_refuse_on_the_device():
         lambda: kv8_rope_append(row, rope, n.repeat(2), qo, layer, t, 4), lambda: kv8_rope_append(row, rope, n, qo.float(), layer, t, 4),
         lambda: kv8_rope_append(row, rope, n, qo, layer, t, 4, bias=row[0]),
         lambda: kv8_rope_append(None, rope, n, qo, layer, t, 4, partials=row.float(), splits=2),
+        lambda: kv8_rope_append(row, rope, n, qo, layer, t, 4, lens_out=n), lambda: kv8_rope_append(row, rope, n, qo, layer, t, 4, lens_out=n.cpu()),
+        lambda: kv8_append(layer, t, n, x, x, err=torch.zeros(1, dtype=torch.int32)),
+        lambda: kv8_attention_decode(q, layer, t[:, :0], n, 1.0, 2), lambda: kv8_gather(layer, t[:, :0], 3),
     ]
     for i, call in enumerate(calls):
         with pytest.raises(ValueError):
@@ -579,6 +582,63 @@ def test_cache_layer_prompt_then_decode_through_the_hook():
         if t == 1:
             _near(out, *cache.attend(q[:, :, 0], table[None], [n], d ** -0.5))
     pool.check_write_errors()
+
+
+def test_rotation_in_place():
+    """q_out may be the q part of the fused rows themselves."""
+    from runtime_amd.phase2.kv8 import kv8_rope_append
+
+    for d in (64, 128):
+        hkv, hq, b, g = 2, 6, 5, _gen(d)
+        rows = torch.randn(b, (hq + 2 * hkv) * d, generator=g).half().to(DEV)
+        pos, rope = _int([3, 0, 17, 40, 16]).to(DEV), _rope(64, d)
+        tables = torch.arange(3 * b).view(b, 3).int().to(DEV)
+        pools, q = [_pool(3 * b, hkv, 16, d, torch.float16) for _ in range(2)], torch.empty(b, hq * d, dtype=torch.float16, device=DEV)
+        kv8_rope_append(rows, rope, pos, q, pools[0].layer_store(0), tables, hq)
+        kv8_rope_append(rows, rope, pos, rows[:, :hq * d], pools[1].layer_store(0), tables, hq)
+        assert torch.equal(rows[:, :hq * d], q) and torch.equal(pools[0]._data, pools[1]._data)
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+def test_hf_model_decodes_over_an_8_bit_pool(dt):
+    """The worker's paths over an 8-bit pool: prompts and ragged decode steps through the cache adapters, with
+    and without a captured graph, agree to the bit; the single-row entry point and the warm-up take it."""
+    from oracle import model as om
+    from runtime_amd.phase2.hf_decode import (DecodeRequest, DecodeState, PagedDecoder, enable_block_paged_attention,
+                                              prefill_request)
+    from runtime_amd.phase2.hip_graph_decode import CudaGraphDecodeManager
+    from runtime_amd.phase2.paged_attention_hip import paged_attention_decode, warmup_paged_attention_kernel
+
+    dtype, g = DTYPES[dt], _gen(21)
+    hf = om.random_llama(seed=3, hidden_size=256, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                         intermediate_size=512, vocab_size=512, max_position_embeddings=256)
+    om.to_device_dtype(hf, DEV, dtype).eval()
+    enable_block_paged_attention(hf)
+    prompts = [torch.randint(0, 512, (n,), generator=g) for n in (21, 16, 40)]
+    runs = []
+    for graphs in (False, True):
+        pool = _pool(24, 2, 16, 64, dtype, layers=2)
+        warmup_paged_attention_kernel(pool, num_heads=4, num_kv_groups=2, head_dim=64, block_ids=[0, 1])
+        manager = CudaGraphDecodeManager(model=hf, device=DEV, warmup_steps=1, enabled=True) if graphs else None
+        worker, states = PagedDecoder(hf, pool, max_active=4, graph_mgr=manager), []
+        for i, ids in enumerate(prompts):
+            cache, logits = prefill_request(hf, pool, list(range(8 * i, 8 * i + 8)), ids.view(1, -1).to(DEV))
+            states.append(DecodeState(DecodeRequest(str(i)), cache, int(logits.argmax()), []))
+        steps = []
+        for _ in range(6):
+            worker.decode_step(states)
+            steps.append(worker.last_logits.float().clone())
+        assert not graphs or manager.stats()["graphs"][0]["replays"] >= 4
+        runs.append((torch.stack(steps), [s.generated_token_ids for s in states], pool))
+    assert torch.equal(runs[0][0], runs[1][0]) and runs[0][1] == runs[1][1]
+    assert torch.isfinite(runs[0][0]).all() and torch.equal(runs[0][2]._data, runs[1][2]._data)
+    pool = runs[0][2]
+    q = torch.randn(1, 4, 1, 64, generator=g).to(dtype).to(DEV)
+    k, v = (x.double().cpu() for x in pool.gather_layer(1, list(range(8, 16)), 20))
+    out = paged_attention_decode(q, pool, 1, list(range(8, 16)), 20, 2, 0.125).cpu().double()
+    for h in range(4):
+        want = torch.softmax(k[0, h // 2] @ q[0, h, 0].cpu().double() * 0.125, 0) @ v[0, h // 2]
+        assert (out[0, h, 0] - want).abs().max() <= 6 * torch.finfo(dtype).eps / 2 * v[0, h // 2].abs().max() + 2.0 ** -24
 
 
 @pytest.mark.parametrize("batch", [2, 16, 40])
