@@ -606,7 +606,9 @@ int mx_kv8_rope_append(const uint16_t* qkv, int64_t qkv_stride, const float* par
  * values of pages block_tables[b] for kv-head h / (Hq / Hkv). q, out: 16-bit
  * [B, Hq, D] with strides (sb, sh, 1). Empty rows give zeros; a block outside the
  * pool is skipped and sets bit 2 of the nullable err word; a page that stands for
- * NaN makes its heads' outputs NaN. Any GQA group. workspace: at least
+ * NaN makes its heads' outputs NaN. Any GQA group. flags: MX_PA_BF16 and
+ * MX_PA_SHARED_BLOCKS (rows may share pages; the result is the same), or 0.
+ * workspace: at least
  * mx_kv8_attn_workspace_bytes, 256-byte aligned, not shared by calls that overlap
  * (its contents need not be kept or cleared). The 8-bit form of
  * mx_paged_attn_decode (runtime/phase2/paged_attention_triton.py:745-775). */

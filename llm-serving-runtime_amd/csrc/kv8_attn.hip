@@ -158,11 +158,16 @@ struct Piece {
     float4v acc[D / 16];
 };
 
-// K and V are read once, so their loads carry the streaming policy: batch 32 39.3 -> 36.5 us per call, two
-// rows of 100,000 tokens 95 -> 85.
+// Where every page stands in one row, K and V are read once and their loads carry the streaming policy:
+// batch 32 39.3 -> 36.5 us per call, two rows of 100,000 tokens 95 -> 85 (by ranges). Rows that share pages
+// (MX_PA_SHARED_BLOCKS) read them with the default one.
 typedef uint32_t u32x4n __attribute__((ext_vector_type(4)));
+template <bool STREAM>
 __device__ __forceinline__ uint4 load16(const uint8_t* p) {
-    return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4n*>(p)));
+    if constexpr (STREAM)
+        return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4n*>(p)));
+    else
+        return *reinterpret_cast<const uint4*>(p);
 }
 
 // One step's loads. NP pages stand in a chunk: 1, or 16 / BS.
@@ -174,7 +179,7 @@ struct Regs {
     uint32_t codes[NP];  // K code | V code << 8
 };
 
-template <int D, int BS, bool BF16>
+template <int D, int BS, bool BF16, bool STREAM>
 __device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, int h0, int nh, int c0, int c1,
                                           int stride, int tokens, int lane, Piece<D>& st) {
     constexpr int NP = Regs<D, BS>::NP, KA = D / 64;
@@ -236,7 +241,7 @@ __device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, i
             if (in_pool(id_)) {
                 const uint8_t* run = p.pages.data + run_offset<D, BS>(p.pages, id_, kvh, 0) + slot * 64 + 16 * g;
 #pragma unroll
-                for (int a = 0; a < KA; ++a) rg.k[j][a] = load16(run + a * (BS * 64));
+                for (int a = 0; a < KA; ++a) rg.k[j][a] = load16<STREAM>(run + a * (BS * 64));
             }
         }
     };
@@ -253,7 +258,7 @@ __device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, i
                 for (int e = 0; e < D / 16; ++e) {
                     const uint8_t* src = run + e * (16 * BS);
                     if constexpr (PT == 16) {
-                        const uint4 w = load16(src);
+                        const uint4 w = load16<STREAM>(src);
                         rg.v[e][0] = w.x, rg.v[e][1] = w.y, rg.v[e][2] = w.z, rg.v[e][3] = w.w;
                     } else if constexpr (PT == 8) {
                         const uint2 w = *reinterpret_cast<const uint2*>(src);
@@ -390,7 +395,7 @@ __device__ __forceinline__ void heads_of(const AttnParams& p, int vh, int& kvh, 
 }
 
 // One workgroup per segment: its waves take the steps in turn and join their pieces in LDS.
-template <int D, int BS, bool BF16>
+template <int D, int BS, bool BF16, bool STREAM>
 __global__ __launch_bounds__(kSegmentWaves * 64, 2) void kv8_attn_segment_kernel(AttnParams p) {
     extern __shared__ float lds[];  // [waves][GS][2] (m, l), [waves][GS][D] outputs
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -399,7 +404,7 @@ __global__ __launch_bounds__(kSegmentWaves * 64, 2) void kv8_attn_segment_kernel
     heads_of(p, blockIdx.x, kvh, h0, nh);
     const int tokens = __builtin_amdgcn_readfirstlane(row_tokens<BS>(p, b));
     Piece<D> st;
-    run_piece<D, BS, BF16>(p, b, kvh, h0, nh, wave * kStep, chunks_of(tokens), waves * kStep, tokens, lane, st);
+    run_piece<D, BS, BF16, STREAM>(p, b, kvh, h0, nh, wave * kStep, chunks_of(tokens), waves * kStep, tokens, lane, st);
     if (waves == 1) {
         write_out<D, BF16>(p, b, h0, nh, lane, st);
         return;
@@ -435,7 +440,7 @@ __global__ __launch_bounds__(kSegmentWaves * 64, 2) void kv8_attn_segment_kernel
     }
 }
 
-template <int D, int BS, bool BF16>
+template <int D, int BS, bool BF16, bool STREAM>
 __global__ __launch_bounds__(kAttnWaves * 64, 2) void kv8_attn_kernel(AttnParams p) {
     const int lane = threadIdx.x & 63;
     const int w = blockIdx.x * kAttnWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -470,7 +475,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, 2) void kv8_attn_kernel(AttnParams
         const int nc = n - c0 < hi - x ? n - c0 : hi - x;
         if (nc <= 0 || vh >= p.Hv) break;  // cannot happen for lengths that stay as they are
         heads_of(p, vh, kvh, h0, nh);
-        run_piece<D, BS, BF16>(p, b, kvh, h0, nh, c0, c0 + nc, kStep, tokens, lane, st);
+        run_piece<D, BS, BF16, STREAM>(p, b, kvh, h0, nh, c0, c0 + nc, kStep, tokens, lane, st);
         if (nc == n) {
             write_out<D, BF16>(p, b, h0, nh, lane, st);
         } else {
@@ -609,7 +614,9 @@ extern "C" int mx_kv8_attn_decode(const uint16_t* q, int64_t q_sb, int64_t q_sh,
         return fail(MX_ERR_INVALID, "%s: Hq (%d) must be a positive multiple of Hkv (%d)", what, Hq, Hkv);
     if (max_blocks < 1) return fail(MX_ERR_INVALID, "%s: max_blocks must be >= 1", what);
     if (B > 65535 || Hq > 65535) return fail(MX_ERR_UNSUPPORTED, "%s: B or Hq too large", what);
-    if (flags & ~(uint32_t)MX_PA_BF16) return fail(MX_ERR_INVALID, "%s: unknown flags 0x%x", what, flags);
+    if (flags & ~(uint32_t)(MX_PA_BF16 | MX_PA_SHARED_BLOCKS))
+        return fail(MX_ERR_INVALID, "%s: unknown flags 0x%x", what, flags);
+    const bool shared = flags & MX_PA_SHARED_BLOCKS;
     if (!aligned(q, 16) || q_sb % 8 || q_sh % 8 || !aligned(out, 16) || o_sb % 8 || o_sh % 8)
         return fail(MX_ERR_ALIGNMENT, "%s: q and out rows must be 16-byte aligned", what);
     if (!aligned(codes, 2)) return fail(MX_ERR_ALIGNMENT, "%s: codes must be 2-byte aligned", what);
@@ -644,19 +651,21 @@ extern "C" int mx_kv8_attn_decode(const uint16_t* q, int64_t q_sb, int64_t q_sh,
     const int waves = (int)std::min<int64_t>({most, ceil_div(max_tokens, kv8::kStep * kv8::kChunk),
                                               65536 / piece});
     const size_t lds = waves > 1 ? waves * piece : 0;
-#define LAUNCH(DD, BB, F)                                                                                            \
-    if (segments) {                                                                                                  \
-        hipLaunchKernelGGL((kv8::kv8_attn_segment_kernel<DD, BB, F>), dim3(p.Hv, B), dim3(waves * 64), lds, st, p);  \
-    } else {                                                                                                         \
-        hipLaunchKernelGGL((kv8::kv8_attn_kernel<DD, BB, F>), dim3(kv8::kWorkers / kv8::kAttnWaves),                 \
-                           dim3(kv8::kAttnWaves * 64), 0, st, p);                                                    \
-        hipLaunchKernelGGL((kv8::kv8_merge_kernel<DD, BB, F>), dim3(Hq, B), dim3(kv8::kMergeWaves * 64), 0, st, p);  \
+#define LAUNCH(DD, BB, F, S)                                                                                           \
+    if (segments) {                                                                                                    \
+        hipLaunchKernelGGL((kv8::kv8_attn_segment_kernel<DD, BB, F, S>), dim3(p.Hv, B), dim3(waves * 64), lds, st, p); \
+    } else {                                                                                                           \
+        hipLaunchKernelGGL((kv8::kv8_attn_kernel<DD, BB, F, S>), dim3(kv8::kWorkers / kv8::kAttnWaves),                \
+                           dim3(kv8::kAttnWaves * 64), 0, st, p);                                                      \
+        hipLaunchKernelGGL((kv8::kv8_merge_kernel<DD, BB, F>), dim3(Hq, B), dim3(kv8::kMergeWaves * 64), 0, st, p);    \
     }
-#define CALL(DD, BB)             \
-    if (flags & MX_PA_BF16) {    \
-        LAUNCH(DD, BB, true)     \
-    } else {                     \
-        LAUNCH(DD, BB, false)    \
+#define CALL(DD, BB)                                        \
+    if (flags & MX_PA_BF16) {                               \
+        if (shared) { LAUNCH(DD, BB, true, false) }         \
+        else { LAUNCH(DD, BB, true, true) }                 \
+    } else {                                                \
+        if (shared) { LAUNCH(DD, BB, false, false) }        \
+        else { LAUNCH(DD, BB, false, true) }                \
     }
     MX_KV8_DISPATCH(D, block_size, CALL)
 #undef CALL

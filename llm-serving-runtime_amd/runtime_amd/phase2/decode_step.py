@@ -382,7 +382,8 @@ class Int8DecodeModel:
                         err=buf.err, lens_out=lens_out, used_blocks=pool._used_map)
         ev = self._tick(timers, "attn")
         kv8_attention_decode(buf.q.view(bsz, s.heads, 1, s.head_dim), store, block_tables, buf.attn_lens,
-                             s.head_dim ** -0.5, s.group, out=buf.attn, err=buf.err)
+                             s.head_dim ** -0.5, s.group, out=buf.attn, err=buf.err,
+                             shared_blocks=self.shared_kv_blocks)
         self._tock(timers, "attn", ev)
 
     def uses_fused_qkv(self, bsz: int) -> bool:

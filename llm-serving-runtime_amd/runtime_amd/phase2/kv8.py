@@ -26,7 +26,7 @@ import torch
 
 from . import _hip
 from .decode_glue import _i32, _lens_ptr, _used_ptr
-from .paged_attention_hip import _DTYPE_FLAGS
+from .paged_attention_hip import _DTYPE_FLAGS, MX_PA_SHARED_BLOCKS
 
 HEAD_DIMS = (64, 128)
 BLOCK_SIZES = (4, 8, 16, 32)
@@ -236,11 +236,12 @@ def _aligned_heads(t: torch.Tensor) -> bool:
 
 def kv8_attention_decode(query: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                          scaling: float, num_kv_groups: int, out: torch.Tensor | None = None,
-                         err: torch.Tensor | None = None) -> torch.Tensor:
+                         err: torch.Tensor | None = None, shared_blocks: bool = False) -> torch.Tensor:
     """``query [B, heads, 1, dim]`` against each row's first ``seq_lens[b]`` cached tokens.
 
     Rows of length 0 give zeros. A block id outside the pool is skipped and OR-s 4 into ``err`` (an
-    int32 device word) when given. A page that a value not finite was written to makes the outputs of
+    int32 device word) when given. ``shared_blocks`` says that rows may share pages (the loads then keep
+    them in the caches; the result is the same). A page that a value not finite was written to makes the outputs of
     its heads NaN.
     """
     _hip.require_device_tensor(query, "query")
@@ -277,7 +278,7 @@ def kv8_attention_decode(query: torch.Tensor, layer: Kv8Layer, block_tables: tor
             tables.stride(0), width, lens.data_ptr(), b, hq, hkv, d,
             layer.block_size, layer.num_blocks, float(scaling), out.data_ptr(), 0 if one_row else o_sb,
             0 if one_head else o_sh, ws.data_ptr() if ws is not None else None, nbytes, _err_ptr(err, dev),
-            layer.flags, _hip.stream_handle(dev))
+            layer.flags | (MX_PA_SHARED_BLOCKS if shared_blocks else 0), _hip.stream_handle(dev))
     if rc != _hip.MX_OK:
         _hip.check(rc, "mx_kv8_attn_decode")
     return out

@@ -107,11 +107,11 @@ class Int8KVBlockPool(GpuKVBlockPool):
             self.check_write_errors()
 
     def attend(self, layer_idx: int, query: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
-               scaling: float, num_kv_groups: int) -> torch.Tensor:
+               scaling: float, num_kv_groups: int, shared_blocks: bool = False) -> torch.Tensor:
         """One decode step's attention over a layer (``kv8_attention_decode``); a block id outside the pool
         is reported by :meth:`check_write_errors`."""
         return kv8_attention_decode(query, self.layer_store(layer_idx), block_tables, seq_lens, scaling,
-                                    num_kv_groups, err=self._write_err)
+                                    num_kv_groups, err=self._write_err, shared_blocks=shared_blocks)
 
     def _gathers_on_device(self, tokens: int) -> bool:
         return True

@@ -194,7 +194,8 @@ def paged_attention_decode_batched(query: torch.Tensor, metadata: PagedDecodeBat
     pool = metadata.pool
     pool._ensure_pools()
     if getattr(pool, "kv_bits", 16) == 8:
-        return pool.attend(metadata.layer_idx, query, metadata.block_tables, metadata.seq_lens, scaling, num_kv_groups)
+        return pool.attend(metadata.layer_idx, query, metadata.block_tables, metadata.seq_lens, scaling, num_kv_groups,
+                           metadata.shared_blocks)
     k_layer = pool.k_layer_view(metadata.layer_idx)
     v_layer = pool.v_layer_view(metadata.layer_idx)
     return _decode(query, k_layer, v_layer, metadata.block_tables, metadata.seq_lens, scaling, num_kv_groups,

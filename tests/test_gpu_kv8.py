@@ -313,6 +313,8 @@ def test_attention_matches_float64(hkv, bs, d, dt, group):
         meta = PagedDecodeBatchMetadata(pool=pool, layer_idx=0, block_tables=table.to(DEV), seq_lens=_int(lens).to(DEV))
         out = paged_attention_decode_batched(q.to(DEV), meta, group, d ** -0.5)
         _near(out, *want, dtype)
+        shared = pool.attend(0, q.to(DEV), table.to(DEV), _int(lens).to(DEV), d ** -0.5, group, shared_blocks=True)
+        assert torch.equal(shared, out)
         assert (out[0] == 0).all()
     pool.check_write_errors()
 
