@@ -65,7 +65,7 @@ struct AttnParams {
     int B, G;      // rows; query heads per kv-head
     int NG, GS;    // segments per kv-head, query heads of one (the last may have fewer)
     int Hv;        // segments per row: Hkv * NG
-    int workers;   // 0: one wave per segment
+    int workers;   // waves of the launch by ranges
     float scale_log2e;
     uint16_t* out;
     int64_t o_sb, o_sh;
@@ -394,10 +394,13 @@ __device__ __forceinline__ void heads_of(const AttnParams& p, int vh, int& kvh, 
     nh = p.G - first < p.GS ? p.G - first : p.GS;
 }
 
+// LDS floats of a workgroup's (m, l) pairs, whole 16 bytes of them.
+__host__ __device__ constexpr int stats_floats(int waves, int GS) { return (2 * waves * GS + 3) / 4 * 4; }
+
 // One workgroup per segment: its waves take the steps in turn and join their pieces in LDS.
 template <int D, int BS, bool BF16, bool STREAM>
 __global__ __launch_bounds__(kSegmentWaves * 64, 2) void kv8_attn_segment_kernel(AttnParams p) {
-    extern __shared__ float lds[];  // [waves][GS][2] (m, l), [waves][GS][D] outputs
+    extern __shared__ __align__(16) float lds[];  // [waves][GS][2] (m, l), [waves][GS][D] outputs
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = blockDim.x >> 6, b = blockIdx.y;
     int kvh, h0, nh;
@@ -409,7 +412,7 @@ __global__ __launch_bounds__(kSegmentWaves * 64, 2) void kv8_attn_segment_kernel
         write_out<D, BF16>(p, b, h0, nh, lane, st);
         return;
     }
-    float* const acc = lds + 2 * waves * p.GS;
+    float* const acc = lds + stats_floats(waves, p.GS);
     const int g = lane >> 4, r = lane & 15;
     if (r < nh) {
         if (g == 0) *reinterpret_cast<float2*>(lds + (wave * p.GS + r) * 2) = float2{st.m, st.l};
@@ -649,8 +652,8 @@ extern "C" int mx_kv8_attn_decode(const uint16_t* q, int64_t q_sb, int64_t q_sh,
     const int64_t piece = (int64_t)p.GS * (D + 2) * sizeof(float);
     const int64_t most = (int64_t)B * p.Hv > 256 ? kv8::kSegmentWaves / 2 : kv8::kSegmentWaves;
     const int waves = (int)std::min<int64_t>({most, ceil_div(max_tokens, kv8::kStep * kv8::kChunk),
-                                              65536 / piece});
-    const size_t lds = waves > 1 ? waves * piece : 0;
+                                              65520 / piece});
+    const size_t lds = waves > 1 ? (kv8::stats_floats(waves, p.GS) + (size_t)waves * p.GS * D) * sizeof(float) : 0;
 #define LAUNCH(DD, BB, F, S)                                                                                           \
     if (segments) {                                                                                                    \
         hipLaunchKernelGGL((kv8::kv8_attn_segment_kernel<DD, BB, F, S>), dim3(p.Hv, B), dim3(waves * 64), lds, st, p); \

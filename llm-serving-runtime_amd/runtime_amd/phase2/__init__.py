@@ -15,11 +15,15 @@ from .paged_attention_hip import (
     set_paged_decode_context,
     warmup_paged_attention_kernel,
 )
+from .kv8 import Kv8Layer, kv8_append, kv8_attention_decode, kv8_gather, kv8_rope_append
+from .kv8_pool import Int8KVBlockPool
 from .paged_kv_kernel import GpuKVBlockPool, PoolShape
 
 __all__ = [
     "GpuKVBlockPool",
+    "Int8KVBlockPool",
     "Int8Linear",
+    "Kv8Layer",
     "PagedDecodeBatchMetadata",
     "PagedDecodeContext",
     "PoolShape",
@@ -27,6 +31,10 @@ __all__ = [
     "get_paged_decode_context",
     "hip_kernel_available",
     "int8_linear",
+    "kv8_append",
+    "kv8_attention_decode",
+    "kv8_gather",
+    "kv8_rope_append",
     "pack_weight",
     "paged_attention_decode",
     "paged_attention_decode_batched",

@@ -18,6 +18,7 @@ Modules:
                         (torch fp32 on the CPU).
 * ``kv_pool``         - the paged KV pool layout and its write/gather
                         (torch on the CPU).
+* ``kv8``             - the 8-bit KV cache (format, writes, attention) in float64, page by page.
 * ``model``           - the fp32 HF decoder (Qwen2 / Llama) holding exactly the
                         device's int8 weights: teacher-forced logits, prefill K/V,
                         continuation from given K/V, greedy decode; used by the
