@@ -17,6 +17,7 @@ namespace pages {
 
 constexpr int kBatch = 448;    // page pairs per launch: 3.5 KiB of the 4 KiB of kernel arguments
 constexpr int kThreads = 256;
+constexpr int kMaxPairs = 1 << 24;  // of one call: its lists are hashed on the host
 
 struct Region {
     char* base;
@@ -231,6 +232,7 @@ extern "C" int mx_kv_copy_pages(void* base, int64_t page_bytes, int64_t layer_st
     if (n == 0) return MX_OK;
     if (!src || !dst) return fail(MX_ERR_NULL, "%s: null pointer", what);
     if (layers < 1 || layers > 65535 || num_pages < 1) return fail(MX_ERR_INVALID, "%s: layers or pages out of range", what);
+    if (n > pages::kMaxPairs) return fail(MX_ERR_UNSUPPORTED, "%s: more than %d pairs", what, pages::kMaxPairs);
     pages::CopyParams p{};
     p.r[0] = {static_cast<char*>(base), layer_stride, page_bytes};
     p.r[1] = {static_cast<char*>(base2), layer_stride2, base2 ? page_bytes2 : 0};
@@ -283,7 +285,8 @@ extern "C" int mx_kv_rename_pages(const int32_t* tables, int64_t in_stride, int3
     if (rows < 0 || width < 0 || n < 0) return fail(MX_ERR_INVALID, "%s: sizes must be >= 0", what);
     if (rows == 0 || width == 0) return MX_OK;
     if (!tables || !out || (n > 0 && (!from || !to))) return fail(MX_ERR_NULL, "%s: null pointer", what);
-    if ((int64_t)rows * width >= ((int64_t)1 << 32)) return fail(MX_ERR_UNSUPPORTED, "%s: tables too large", what);
+    if ((int64_t)rows * width >= ((int64_t)1 << 31)) return fail(MX_ERR_UNSUPPORTED, "%s: tables too large", what);
+    if (n > pages::kMaxPairs) return fail(MX_ERR_UNSUPPORTED, "%s: more than %d pairs", what, pages::kMaxPairs);
     try {
         std::vector<int2> list(n);
         pages::IdMap old(n);

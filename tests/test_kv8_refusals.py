@@ -145,7 +145,10 @@ def test_page_entry_points_refuse_bad_arguments():
     for src, dst in (((0, 0), (2, 3)), ((0, 1), (2, 2)), ((0, 1), (0, 2))):
         _status(copy(src=src, dst=dst, move=1), _hip.MX_ERR_INVALID)  # a page that occurs twice
     _status(rename(to=(3, 1)), _hip.MX_ERR_INVALID)
-    _status(rename(rows=1 << 30, width=4), _hip.MX_ERR_UNSUPPORTED)
+    _status(rename(rows=1 << 29, width=4), _hip.MX_ERR_UNSUPPORTED)
+    many = (1 << 24) + 1  # refused before the lists are read
+    _status(lib.mx_kv_rename_pages(FAKE, 4, FAKE, 4, 2, 4, ids, ids, many, None), _hip.MX_ERR_UNSUPPORTED)
+    _status(lib.mx_kv_copy_pages(FAKE, 1024, 8192, None, 0, 0, 2, 8, ids, ids, many, None, 0, None), _hip.MX_ERR_UNSUPPORTED)
     assert lib.mx_kv_clear_pages(FAKE, 4, 64, 2, FAKE, 8, ids, 0, None) == _hip.MX_OK
     _status(lib.mx_kv_clear_pages(FAKE, 4, 64, 2, FAKE, 2, ids, 3, None), _hip.MX_ERR_INVALID)
     _status(lib.mx_kv_clear_pages(None, 4, 64, 2, None, 8, ids, 3, None), _hip.MX_ERR_NULL)
