@@ -202,7 +202,9 @@ _here = contextlib.nullcontext()
 
 def on_device(device: torch.device):
     """Context in which ``device`` is current (nothing to enter when it is already)."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    # torch.cuda.current_device() without its check that CUDA is initialised (0.1 against 0.4 us): the
+    # device is a tensor's.
+    if device.index is None or device.index == torch._C._cuda_getDevice():
         return _here
     return torch.cuda.device(device)
 

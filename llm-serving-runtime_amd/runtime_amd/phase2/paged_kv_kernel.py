@@ -164,7 +164,8 @@ class GpuKVBlockPool:
             self._k_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
             self._v_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
             self._regions = [self._k_pool, self._v_pool]
-        self._k_views, self._v_views = self._k_pool.unbind(0), self._v_pool.unbind(0)
+        self._k_views, self._v_views = (tuple(pool.select(0, i) for i in range(s.num_layers))
+                                        for pool in (self._k_pool, self._v_pool))
         if self.device.type == "cuda":
             self._used_map = torch.zeros(s.num_blocks, dtype=torch.uint8, device=self.device)
             self._write_err = torch.zeros(1, dtype=torch.int32, device=self.device)
