@@ -148,18 +148,30 @@ class PrefixBatch:
         """Finish the requests in ``slots`` and continue ``row``'s request there too. The forks hold the
         row's full blocks with it; the block that its next token goes to becomes one of their own. Returns
         the (source, destination) ids that ``copy_blocks`` has to copy before the next step."""
-        parent = self.rows[row]
+        if not all(0 <= b < self.batch for b in (row, *slots)):
+            raise ValueError(f"rows are 0 to {self.batch - 1}, got {row} and {slots}")
         if row in slots or len(set(slots)) != len(slots):
             raise ValueError("fork takes every slot once, and not the row itself")
+        parent = self.rows[row]
         if any(self.rows[b].group != parent.group for b in slots):
             raise ValueError("a row's forks go to slots of its group")
         full = parent.length // self.block_size
-        need = math.ceil((parent.length + self.headroom) / self.block_size)
+        # The usual headroom, up to the tables' width: the row may have used some of its own.
+        need = min(math.ceil((parent.length + self.headroom) / self.block_size),
+                   max(self.max_blocks, len(parent.blocks)))
         copied = full < math.ceil(parent.length / self.block_size)
+        given: dict[int, int] = {}  # block -> references that the finished requests hold
+        for b in slots:
+            for i in self.rows[b].blocks:
+                given[i] = given.get(i, 0) + 1
+        room = self.alloc.free_blocks + sum(n == self.alloc.refcount(i) for i, n in given.items())
+        if len(slots) * (need - full) > room:  # before anything changes
+            raise RuntimeError(f"out of KV blocks: need {len(slots) * (need - full)}, {room} free")
         src: list[int] = []
         dst: list[int] = []
         for b in slots:
             self.alloc.decref(self.rows[b].blocks)
+        for b in slots:
             held = parent.blocks[:full]
             self.alloc.incref(held)
             own = self.alloc.alloc(need - full)

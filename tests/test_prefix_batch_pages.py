@@ -119,3 +119,41 @@ def test_fork_refusals_and_byte_accounting():
     assert pb.unique_tokens() == 16 + 2 + 2 + 8 + 3 + 4 and pb.logical_tokens() == 18 + 18 + 11 + 12
     src, dst = pb.fork(3, [2])  # length 12: no partial block, nothing to copy
     assert (src, dst) == ([], []) and pb.rows[2].blocks[:3] == pb.rows[3].blocks[:3]
+
+
+def test_fork_names_rows_from_zero():
+    pb = PrefixBatch(batch=4, groups=1, prefix_tokens=0, lo=9, hi=9, block_size=4, num_blocks=40, headroom=4)
+    before = [list(r.blocks) for r in pb.rows]
+    for row, slots in ((-1, [3]), (3, [-1]), (0, [4]), (4, [0])):  # row -1 would be row 3 itself
+        with pytest.raises(ValueError):
+            pb.fork(row, slots)
+    assert [r.blocks for r in pb.rows] == before
+    _whole(pb, 40)
+
+
+def test_fork_of_a_row_that_used_its_headroom_fits_the_tables():
+    pb = PrefixBatch(batch=2, groups=1, prefix_tokens=0, lo=10, hi=10, block_size=4, num_blocks=16, headroom=6)
+    pb.advance(5)  # 15 of the 16 tokens that a table row has room for
+    pb.fork(0, [1])
+    assert pb.tables.shape == (2, 4) and [len(r.blocks) for r in pb.rows] == [4, 4]
+    _whole(pb, 16)
+    pb.advance()
+    assert pb.fork(1, [0]) == ([], []) and pb.rows[0].blocks == pb.rows[1].blocks  # full: nothing of its own
+    with pytest.raises(RuntimeError):
+        pb.advance()
+
+
+def test_fork_without_room_changes_nothing():
+    pb = PrefixBatch(batch=3, groups=1, prefix_tokens=0, lo=9, hi=9, block_size=4, num_blocks=10, headroom=4,
+                     lengths=[9, 1, 1])
+    assert [len(r.blocks) for r in pb.rows] == [4, 2, 2] and pb.alloc.free_blocks == 2
+    pb.fork(0, [1, 2])  # 2 of their own each, out of 2 free and 4 given back
+    assert pb.alloc.free_blocks == 2
+    _whole(pb, 10)
+    tight = PrefixBatch(batch=3, groups=1, prefix_tokens=0, lo=1, hi=9, block_size=4, num_blocks=6, headroom=4,
+                        lengths=[9, 0, 0])
+    state = [list(r.blocks) for r in tight.rows], list(tight.alloc._free)
+    with pytest.raises(RuntimeError):
+        tight.fork(0, [1, 2])
+    assert ([list(r.blocks) for r in tight.rows], list(tight.alloc._free)) == state
+    _whole(tight, 6)
