@@ -376,7 +376,8 @@ class GpuKVBlockPool:
                 rc = _hip.load().mx_kv_copy_pages(
                     *args, self.shape.num_layers, self.shape.num_blocks, src.buffer_info()[0], dst.buffer_info()[0],
                     len(src), self._used_map.data_ptr(), int(move), _hip.stream_handle(dev))
-            if rc != _hip.MX_ERR_UNSUPPORTED:  # else: more copies that depend on each other than a launch takes
+            # Left over: copies that depend on each other and are more than a launch takes. (A move's never do.)
+            if move or rc != _hip.MX_ERR_UNSUPPORTED:
                 _hip.check(rc, "mx_kv_copy_pages")
                 return
         last = dict(zip(dst, src))
