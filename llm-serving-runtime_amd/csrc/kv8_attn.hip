@@ -47,7 +47,7 @@ constexpr int kChunk = 16;         // tokens per chunk
 constexpr int kStep = 4;           // chunks per step of a wave
 constexpr int kHeads = 16;         // query heads of a segment, at most
 // Waves of a launch: 256 CUs x 8, two per SIMD. Batch 32 of U[128, 4096] tokens, per call: 1536 waves
-// 37.4 us, 2048 36.5, 3072 (three per SIMD, which spills) 55.9, 4096 (two rounds) 42.5. The loads alone
+// 37.4 us, 2048 36.5, three per SIMD (which spills) 55.9, 4096 (two rounds) 42.5. The loads alone
 // take 27 of the launch's 29 us there, so deeper pipelines have nothing to hide.
 constexpr int kWorkers = 2048;
 constexpr int kSegmentWaves = 8;   // waves of a workgroup that has a segment of its own, at most
