@@ -101,27 +101,29 @@ __device__ __forceinline__ float growth_factor(int old, int now) {
     return old == 0 || e <= 0 ? 0.0f : __uint_as_float((uint32_t)e << 23);
 }
 
-// 8 bytes -> 8 numbers q + kRawBias of the element type, exact: one byte permute per pair in fp16
-// (0x64nn is 1024 + nn), a conversion and half a permute per byte in bf16. A product with them carries
-// kRawBias times the other operand's sum, which the caller takes off in fp32.
+// 8 bytes -> the 8 integers q as numbers of the element type, exact: a byte permute and half a packed add
+// per pair in fp16, a conversion and half a permute per byte in bf16.
 template <bool BF16>
-constexpr float kRawBias = BF16 ? 128.0f : 1152.0f;
-template <bool BF16>
-__device__ __forceinline__ half8v raw8(uint32_t d0, uint32_t d1) {
-    uint32_t out[4];
+__device__ __forceinline__ half8v ints8(uint32_t d0, uint32_t d1) {
+    if constexpr (!BF16) {
+        return w8a16::dequant8(d0, d1);
+    } else {
+        uint32_t out[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t w = i < 2 ? d0 : d1;
-        if constexpr (!BF16) {
-            out[i] = __builtin_amdgcn_perm(w8a16::kMagic, w, i & 1 ? w8a16::kSelHi : w8a16::kSelLo);
-        } else {
-            const uint32_t lo = __float_as_uint((float)((w >> (16 * (i & 1))) & 0xffu));
-            const uint32_t hi = __float_as_uint((float)((w >> (16 * (i & 1) + 8)) & 0xffu));
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = (i < 2 ? d0 : d1) ^ 0x80808080u;  // q + 128 -> q in two's complement
+            const uint32_t lo = __float_as_uint((float)(int8_t)(w >> (16 * (i & 1))));
+            const uint32_t hi = __float_as_uint((float)(int8_t)(w >> (16 * (i & 1) + 8)));
             out[i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
         }
+        return __builtin_bit_cast(half8v, uint4{out[0], out[1], out[2], out[3]});
     }
-    return __builtin_bit_cast(half8v, uint4{out[0], out[1], out[2], out[3]});
 }
+
+// What a byte stands for in an operand of one permute or conversion: q + kRawBias (0x64nn is the fp16
+// number 1024 + nn).
+template <bool BF16>
+constexpr float kRawBias = BF16 ? 128.0f : 1152.0f;
 
 // A page's scale as a multiplier of such numbers: (q + kRawBias) s - kRawBias s, fused, is q s exactly
 // while kRawBias s is a finite number of the type: e <= 5 in fp16, e <= 120 in bf16. `excess` is the rest
@@ -144,7 +146,11 @@ template <bool BF16>
 __device__ __forceinline__ half8v scaled4x2(uint32_t d0, uint32_t d1, const RawScale<BF16>& a, const RawScale<BF16>& b) {
     if constexpr (!BF16) {
         const _Float16 sa = (_Float16)a.s, sb = (_Float16)b.s, ba = (_Float16)a.bias, bb = (_Float16)b.bias;
-        return __builtin_elementwise_fma(raw8<false>(d0, d1), half8v{sa, sa, sa, sa, sb, sb, sb, sb},
+        const uint4 raw{__builtin_amdgcn_perm(w8a16::kMagic, d0, w8a16::kSelLo),
+                        __builtin_amdgcn_perm(w8a16::kMagic, d0, w8a16::kSelHi),
+                        __builtin_amdgcn_perm(w8a16::kMagic, d1, w8a16::kSelLo),
+                        __builtin_amdgcn_perm(w8a16::kMagic, d1, w8a16::kSelHi)};
+        return __builtin_elementwise_fma(__builtin_bit_cast(half8v, raw), half8v{sa, sa, sa, sa, sb, sb, sb, sb},
                                          half8v{ba, ba, ba, ba, bb, bb, bb, bb});
     } else {
         // q s has at most 8 significant bits: the upper half of its fp32 pattern is the bf16 value.

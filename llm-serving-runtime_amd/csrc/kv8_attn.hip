@@ -15,8 +15,9 @@
 // weighs, and no score crosses lanes:
 //   * scores, 4 x D / 32 products v_mfma_f32_16x16x32: the A operand's row r of product j is token
 //     4 j + r % 4 of chunk r / 4, so lane group g receives tokens 4 j + i of chunk g, for head lane % 16
-//     (the B operand holds the query heads). K enters as the integers q + 1152 (fp16) or q + 128 (bf16),
-//     one permute per pair of bytes; the accumulator starts at what that adds, and the page's scale
+//     (the B operand holds the query heads). K enters as its integers q (as q + 1152, a permute less the
+//     add, fp32 would hold 1152 times the query's sum beside the score: whole units wrong for queries
+//     with a mean; the add costs nothing measurable, batch 32 33.2 us either way), and the page's scale
 //     multiplies the fp32 score. The head dim is contracted in the order of the lane's 16-byte loads, the
 //     query's operand in the same order;
 //   * online softmax in fp32 on the exp2 scale; the reference maximum moves only when a score exceeds it
@@ -205,11 +206,8 @@ __device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, i
     };
     auto in_pool = [&](int id) { return (unsigned)id < (unsigned)p.pages.num_blocks; };
 
-    // The query operand, negated where the scale is negative (its magnitude multiplies the scores), and
-    // the scores' start: K enters as q + kRawBias, so kRawBias times the query's sum comes off. In fp32 that
-    // costs a few 2^-24 of 1152 sum |q|, against weights that are rounded to 16 bits.
+    // The query operand, negated where the scale is negative (its magnitude multiplies the scores).
     half8v qf[2 * KA];
-    float qsum = 0.0f;
 #pragma unroll
     for (int a = 0; a < 2 * KA; ++a) {
         uint4 w{0, 0, 0, 0};
@@ -219,10 +217,8 @@ __device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, i
         const uint32_t sign = p.scale_log2e < 0.0f ? 0x80008000u : 0u;
         w.x ^= sign, w.y ^= sign, w.z ^= sign, w.w ^= sign;
         qf[a] = __builtin_bit_cast(half8v, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) qsum += Elt<BF16>::widen(qf[a][i]);
     }
-    const float start = -kRawBias<BF16> * xor_sum_16_32(qsum), scale = fabsf(p.scale_log2e);
+    const float scale = fabsf(p.scale_log2e);
 
     st.m = kNegInf;
     float4v l = {0.0f, 0.0f, 0.0f, 0.0f};  // the denominator, as a product of the weights with ones
@@ -282,11 +278,11 @@ __device__ __forceinline__ void run_piece(const AttnParams& p, int b, int kvh, i
         float4v s[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            s[j] = float4v{start, start, start, start};
+            s[j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int a = 0; a < KA; ++a) {
-                s[j] = Elt<BF16>::mma32(raw8<BF16>(rg.k[j][a].x, rg.k[j][a].y), qf[2 * a], s[j]);
-                s[j] = Elt<BF16>::mma32(raw8<BF16>(rg.k[j][a].z, rg.k[j][a].w), qf[2 * a + 1], s[j]);
+                s[j] = Elt<BF16>::mma32(ints8<BF16>(rg.k[j][a].x, rg.k[j][a].y), qf[2 * a], s[j]);
+                s[j] = Elt<BF16>::mma32(ints8<BF16>(rg.k[j][a].z, rg.k[j][a].w), qf[2 * a + 1], s[j]);
             }
         }
         if (c + stride < c1) load_k(c + stride, next, rg);
