@@ -76,3 +76,29 @@ def test_queries_with_a_mean(bs, d, dt, scale):
     pool, cache, tables = _filled(keys, g, bs, d, dtype)
     want = _check(pool, cache, tables, q.to(dtype), scale, dtype)
     assert (want[:, 0] - want[:, 1]).abs().max() > 0.1
+
+
+@pytest.mark.parametrize("scale", [1.0, -1.0])
+@pytest.mark.parametrize("bs,d,dt", [(16, 64, "fp16"), (16, 128, "bf16"), (4, 128, "fp16"), (32, 64, "bf16")])
+def test_large_scores(bs, d, dt, scale):
+    """Integer scores up to 10**5 that rise and fall along a row, so that the running maximum moves, with one
+    token ahead by more than 100: it takes the output alone."""
+    dtype, g = DTYPES[dt], torch.Generator().manual_seed(d)
+    q = torch.zeros(2, 3, d)
+    q[:, 0, 0], q[:, 1, 0], q[:, 2, 0] = 30.0, -30.0, 800.0
+    q[..., 1] = 1.0
+    keys = []
+    for n in LENS:
+        k = torch.zeros(n, d)
+        k[:, 0] = torch.randint(-120, 121, (n,), generator=g).float()
+        k[n // 3, 0], k[n // 2, 0] = 126.0, -126.0
+        k[:, 2:] = torch.randint(-127, 128, (n, d - 2), generator=g).float()  # the query has zeros there
+        k[:, 1] = 127.0
+        keys.append(k)
+    pool, cache, tables = _filled(keys, g, bs, d, dtype)
+    want = _check(pool, cache, tables, q.to(dtype), scale, dtype)
+    for b, n in enumerate(LENS):
+        v, _ = cache.row(tables[b], n, 0, 1)
+        for h, sign in ((0, 1), (1, -1), (2, 1)):
+            winner = v[n // 3 if sign * scale > 0 else n // 2]
+            assert (want[b, h] - winner).abs().max() <= 1e-10 * v.abs().max()
