@@ -23,7 +23,7 @@ import torch
 
 from .kv8 import BLOCK_SIZES, HEAD_DIMS, Kv8Layer, kv8_append, kv8_attention_decode, kv8_gather
 from .paged_attention_hip import _DTYPE_FLAGS
-from .paged_kv_kernel import GpuKVBlockPool
+from .paged_kv_kernel import GpuKVBlockPool, _alloc_lock
 
 ZERO_BYTE = 128  # q = 0
 
@@ -53,8 +53,12 @@ class Int8KVBlockPool(GpuKVBlockPool):
         return s.num_layers * s.num_kv_heads * 2 * (s.block_size_tokens * s.head_dim + 1)
 
     def _ensure_pools(self) -> None:
-        if self._data is not None:
-            return
+        if self._data is None:
+            with _alloc_lock:
+                if self._data is None:
+                    self._make_pools()
+
+    def _make_pools(self) -> None:
         s = self.shape
         run = s.block_size_tokens * s.head_dim
         data = torch.full((s.num_layers, s.num_blocks, s.num_kv_heads, 2, run), ZERO_BYTE, dtype=torch.uint8,
@@ -64,7 +68,7 @@ class Int8KVBlockPool(GpuKVBlockPool):
         self._write_err = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._stores = [Kv8Layer(data[i], codes[i], s.block_size_tokens, s.head_dim, self.dtype)
                         for i in range(s.num_layers)]
-        self._data, self._codes = data, codes
+        self._codes, self._data = codes, data
 
     def layer_store(self, layer_idx: int) -> Kv8Layer:
         """A layer's pages as the functions of ``kv8.py`` take them."""

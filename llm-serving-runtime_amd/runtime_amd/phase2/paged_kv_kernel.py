@@ -50,6 +50,7 @@ from __future__ import annotations
 import array
 import math
 import os
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -57,6 +58,9 @@ import torch
 from . import _hip
 
 KV_LAYOUTS = ("split", "interleaved")
+
+# Held while a pool makes its tensors: threads that use one first at the same time get the same ones.
+_alloc_lock = threading.Lock()
 
 
 @dataclass(frozen=True)
@@ -151,24 +155,30 @@ class GpuKVBlockPool:
         return self.bytes_for_blocks(self.peak_allocated_block_count())
 
     def _ensure_pools(self) -> None:
-        if self._k_pool is not None:
-            return
+        if self._k_pool is None:
+            with _alloc_lock:
+                if self._k_pool is None:
+                    self._make_pools()
+
+    def _make_pools(self) -> None:
+        """The pool's tensors; ``_k_pool``, by which other threads see that they are there, comes last."""
         s = self.shape
         if self.kv_layout == "interleaved":
             kv = torch.zeros(s.num_layers, s.num_blocks, s.num_kv_heads, 2, s.block_size_tokens, s.head_dim,
                              dtype=self.dtype, device=self.device)
-            self._k_pool, self._v_pool = kv[:, :, :, 0], kv[:, :, :, 1]
+            k_pool, v_pool = kv[:, :, :, 0], kv[:, :, :, 1]
             self._regions = [kv]
         else:
             shape = (s.num_layers, s.num_blocks, s.num_kv_heads, s.block_size_tokens, s.head_dim)
-            self._k_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
-            self._v_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
-            self._regions = [self._k_pool, self._v_pool]
+            k_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
+            v_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
+            self._regions = [k_pool, v_pool]
         self._k_views, self._v_views = (tuple(pool.select(0, i) for i in range(s.num_layers))
-                                        for pool in (self._k_pool, self._v_pool))
+                                        for pool in (k_pool, v_pool))
         if self.device.type == "cuda":
             self._used_map = torch.zeros(s.num_blocks, dtype=torch.uint8, device=self.device)
             self._write_err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._v_pool, self._k_pool = v_pool, k_pool
 
     def _touch_block(self, physical: int) -> None:
         if physical < 0 or physical >= self.shape.num_blocks:
