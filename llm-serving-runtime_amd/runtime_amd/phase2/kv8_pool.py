@@ -89,7 +89,7 @@ class Int8KVBlockPool(GpuKVBlockPool):
         bits = int(self._write_err.item())
         if bits:
             self._write_err.zero_()
-            where = "attention" if bits == 4 else "batched write"
+            where = " and ".join(name for name, hit in (("batched write", bits & ~4), ("attention", bits & 4)) if hit)
             raise IndexError(f"block table underrun or physical block id out of range during {where}")
 
     def write_tokens_batch(self, layer_idx: int, block_tables: torch.Tensor, start_positions: torch.Tensor,

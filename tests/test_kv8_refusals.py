@@ -239,3 +239,14 @@ def test_move_and_free_blocks_on_the_cpu_pool():
     for call in (lambda: pool.move_blocks([1], [9]), lambda: pool.move_blocks([2**31], [1]), lambda: pool.copy_blocks([-1], [2]), lambda: pool.free_blocks([9])):
         with pytest.raises(IndexError):
             call()
+
+
+@pytest.mark.parametrize("bits,where", [(1, "batched write"), (4, "attention"), (5, "batched write and attention")])
+def test_write_errors_name_every_kind_met(bits, where):
+    pool = Int8KVBlockPool(num_blocks=4, block_size_tokens=16, num_layers=1, num_kv_heads=2, head_dim=64,
+                           dtype=torch.float16, device="cuda")
+    pool.check_write_errors()  # nothing allocated, nothing met
+    pool._write_err = torch.tensor([bits], dtype=torch.int32)
+    with pytest.raises(IndexError, match=f"during {where}$"):
+        pool.check_write_errors()
+    pool.check_write_errors()  # reported once
