@@ -456,7 +456,7 @@ extern "C" int mx_kv8_write(const uint16_t* k_new, const uint16_t* v_new, int64_
     kv8::WriteParams p{k_new, v_new, new_sb, new_sh, new_st, T, block_tables, bt_sb, max_blocks, start_pos,
                        {data, codes, Hkv, num_blocks}, err, used, 0, 0, 0};
     // Pages that T tokens beginning at any slot can touch.
-    p.pages_per_row = (int)((int64_t)(T - 1 + block_size - 1) / block_size + 1);
+    p.pages_per_row = (int)(((int64_t)T + block_size - 2) / block_size + 1);
     if ((double)B * p.pages_per_row * Hkv * 2 > 1e11) return fail(MX_ERR_UNSUPPORTED, "%s: too many tokens", what);
     p.units = (int64_t)B * p.pages_per_row * Hkv * 2;
     const int64_t groups = kv8::groups_for(p.units);

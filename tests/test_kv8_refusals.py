@@ -241,6 +241,13 @@ def test_move_and_free_blocks_on_the_cpu_pool():
             call()
 
 
+def test_token_counts_at_the_top_of_32_bits_are_refused():
+    for t in (2**31 - 1, 2**31 - 3, 2**31 - 31):  # more pages than a launch has waves for
+        for bs in (4, 32):
+            _status(_write(T=t, bs=bs), _hip.MX_ERR_UNSUPPORTED)
+            _status(_gather(S=t, bs=bs), _hip.MX_ERR_UNSUPPORTED)
+
+
 @pytest.mark.parametrize("bits,where", [(1, "batched write"), (4, "attention"), (5, "batched write and attention")])
 def test_write_errors_name_every_kind_met(bits, where):
     pool = Int8KVBlockPool(num_blocks=4, block_size_tokens=16, num_layers=1, num_kv_heads=2, head_dim=64,
