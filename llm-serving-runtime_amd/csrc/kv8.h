@@ -217,7 +217,7 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, y));
 }
 
-// Host: whether the kernels hold these pages. Sizes are checked so that no index leaves 64 bits.
+// Host: whether the kernels hold these pages, whose byte offsets are 64-bit.
 inline int check_pages(const char* what, const void* data, const void* codes, int32_t Hkv, int32_t D, int32_t bs,
                        int32_t num_blocks) {
     if (!data || !codes) return fail(MX_ERR_NULL, "%s: null pointer", what);
@@ -225,6 +225,7 @@ inline int check_pages(const char* what, const void* data, const void* codes, in
     if (bs != 4 && bs != 8 && bs != 16 && bs != 32)
         return fail(MX_ERR_UNSUPPORTED, "%s: block_size %d unsupported (4, 8, 16 or 32)", what, bs);
     if (Hkv < 1 || num_blocks < 1) return fail(MX_ERR_INVALID, "%s: Hkv and num_blocks must be >= 1", what);
+    if ((double)num_blocks * Hkv * 2 * bs * D > 9e18) return fail(MX_ERR_UNSUPPORTED, "%s: too many pages", what);
     if (!aligned(data, 16)) return fail(MX_ERR_ALIGNMENT, "%s: pages must be 16-byte aligned", what);
     return MX_OK;
 }

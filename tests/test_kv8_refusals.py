@@ -248,6 +248,14 @@ def test_token_counts_at_the_top_of_32_bits_are_refused():
             _status(_gather(S=t, bs=bs), _hip.MX_ERR_UNSUPPORTED)
 
 
+def test_pools_whose_byte_offsets_leave_64_bits_are_refused():
+    big = dict(hkv=1 << 19, nb=2**31 - 1, bs=32, d=128)  # 2**63 bytes
+    _status(_write(**big), _hip.MX_ERR_UNSUPPORTED)
+    _status(_gather(**big), _hip.MX_ERR_UNSUPPORTED)
+    _status(_token(**big), _hip.MX_ERR_UNSUPPORTED)
+    _status(_attend(hq=1 << 19, **big), _hip.MX_ERR_UNSUPPORTED)
+
+
 @pytest.mark.parametrize("bits,where", [(1, "batched write"), (4, "attention"), (5, "batched write and attention")])
 def test_write_errors_name_every_kind_met(bits, where):
     pool = Int8KVBlockPool(num_blocks=4, block_size_tokens=16, num_layers=1, num_kv_heads=2, head_dim=64,
