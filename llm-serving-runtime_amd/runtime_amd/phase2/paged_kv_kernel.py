@@ -72,6 +72,48 @@ class PoolShape:
     head_dim: int
 
 
+# Entries of one launch over pairs that depend on each other: a pair each, and one more for a cycle.
+MAX_DEPENDENT = 448
+
+
+def dependent_batches(src, dst) -> list[tuple[list[int], list[int]]]:
+    """The copies page dst[i] = page src[i], all at once (of several with one dst the last), as lists that do the
+    same one after the other, each within ``MAX_DEPENDENT``: a page is read before it is written. A longer cycle
+    goes in shorter ones, whose shared page passes on the bytes that the next one needs."""
+    of = {d: s for s, d in zip(src, dst)}
+    of = {d: s for d, s in of.items() if s != d}
+    readers = dict.fromkeys(of, 0)
+    for s in of.values():
+        if s in readers:
+            readers[s] += 1
+    ready, pairs = [d for d, n in readers.items() if n == 0], []
+    while ready:
+        d = ready.pop()
+        s = of.pop(d)
+        pairs.append((s, d))
+        if s in of:
+            readers[s] -= 1
+            if readers[s] == 0:
+                ready.append(s)
+    batches = [pairs[i:i + MAX_DEPENDENT] for i in range(0, len(pairs), MAX_DEPENDENT)]
+    room = 0  # entries left in the last batch, which takes cycles
+    while of:  # cycles, every page read once
+        d, s = of.popitem()
+        ring = [d, s]  # ring[i] = page ring[i + 1], the last = the first
+        while of[ring[-1]] != d:
+            ring.append(of.pop(ring[-1]))
+        del of[ring[-1]]
+        while ring:
+            part = ring[:MAX_DEPENDENT - 1]
+            if len(part) + 1 > room:
+                batches.append([])
+                room = MAX_DEPENDENT
+            batches[-1] += list(zip(part[1:] + part[:1], part))
+            room -= len(part) + 1
+            ring = part[-1:] + ring[len(part):] if len(ring) > len(part) else []
+    return [([s for s, _ in b], [d for _, d in b]) for b in batches]
+
+
 def _ids(block_ids) -> list[int]:
     return list(map(int, block_ids))
 
@@ -382,14 +424,20 @@ class GpuKVBlockPool:
                 args += [None, 0, 0] if t is None else [t.data_ptr(), t[0, 0].numel() * t.element_size(),
                                                         t.stride(0) * t.element_size()]
             dev = regions[0].device
+
+            def copy(of: array.array, to: array.array) -> int:
+                return _hip.load().mx_kv_copy_pages(
+                    *args, self.shape.num_layers, self.shape.num_blocks, of.buffer_info()[0], to.buffer_info()[0],
+                    len(of), self._used_map.data_ptr(), int(move), _hip.stream_handle(dev))
+
             with _hip.on_device(dev):
-                rc = _hip.load().mx_kv_copy_pages(
-                    *args, self.shape.num_layers, self.shape.num_blocks, src.buffer_info()[0], dst.buffer_info()[0],
-                    len(src), self._used_map.data_ptr(), int(move), _hip.stream_handle(dev))
-            # Left over: copies that depend on each other and are more than a launch takes. (A move's never do.)
-            if move or rc != _hip.MX_ERR_UNSUPPORTED:
-                _hip.check(rc, "mx_kv_copy_pages")
-                return
+                rc = copy(src, dst)
+                if rc == _hip.MX_ERR_UNSUPPORTED and not move:  # more copies that depend on each other than a launch takes
+                    for of, to in dependent_batches(src, dst):
+                        _hip.check(copy(array.array("i", of), array.array("i", to)), "mx_kv_copy_pages")
+                else:
+                    _hip.check(rc, "mx_kv_copy_pages")
+            return
         last = dict(zip(dst, src))
         to = torch.tensor(list(last), device=self.device, dtype=torch.long)
         of = torch.tensor(list(last.values()), device=self.device, dtype=torch.long)

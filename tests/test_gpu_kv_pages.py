@@ -227,3 +227,28 @@ def test_forked_and_compacted_rows_decode_as_before(kind):
     live = {i for i in range(160) if pb.alloc.refcount(i)}
     assert live == set(range(len(live))) and pool._used_blocks <= live
     pool.check_write_errors()
+
+
+@pytest.mark.parametrize("kind", POOLS)
+def test_long_chains_and_cycles_in_a_captured_graph(kind):
+    """More copies that depend on each other than a launch takes, a chain of 900 pages and a cycle of 1000 with
+    a branch, captured and replayed: nothing is copied to the device or allocated."""
+    pool = _pool(kind, 2000, layers=1, hkv=1, bs=4)
+    g = torch.Generator().manual_seed(7)
+    ids = torch.randperm(2000, generator=g).tolist()
+    chain, ring = ids[:901], ids[901:1901]
+    src = [*chain[:-1], *ring, ring[500]]
+    dst = [*chain[1:], *ring[1:], ring[0], ids[1950]]
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        pool.copy_blocks(src, dst)
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        was = _pages(pool)
+        pool._used_map.zero_()
+        graph.replay()
+        _check(pool, was, dict(zip(dst, src)))
+        assert torch.equal(pool._used_map.nonzero().flatten().cpu(), torch.tensor(sorted(dst)))
+        pool.copy_blocks([3], [ids[1999]])
+        torch.cuda.synchronize()
