@@ -114,6 +114,21 @@ def dependent_batches(src, dst) -> list[tuple[list[int], list[int]]]:
     return [([s for s, _ in b], [d for _, d in b]) for b in batches]
 
 
+def _share_entries(tables: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether an entry of ``out`` is another one of its own or of ``tables`` (both of one shape and unit inner
+    stride): renaming would read what it wrote. ``out`` may be ``tables`` itself."""
+    rows, width = out.shape
+    a, b = tables.stride(0) if rows > 1 else width, out.stride(0) if rows > 1 else width
+    if rows == 0 or width == 0:
+        return False
+    if b < width:
+        return True
+    delta = (out.data_ptr() - tables.data_ptr()) // 4
+    if (delta == 0 and a == b) or delta >= (rows - 1) * a + width or -delta >= (rows - 1) * b + width:
+        return False
+    return a != b or not width <= delta % b <= b - width  # columns of their own side by side in wider rows
+
+
 def _ids(block_ids) -> list[int]:
     return list(map(int, block_ids))
 
@@ -356,11 +371,15 @@ class GpuKVBlockPool:
             if (block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.stride(1) != 1
                     or block_tables.device != self._page_regions()[0].device):
                 raise ValueError("block_tables must be int32 [B, max_blocks] with unit inner stride on the pool's device")
+            if block_tables.numel() >= 1 << 31:  # before a page moves: the renaming launch takes no more
+                raise ValueError("block_tables must have fewer than 2**31 entries")
             if out is None:
                 out = torch.empty(block_tables.shape, dtype=torch.int32, device=block_tables.device)
             elif (out.dtype != torch.int32 or out.shape != block_tables.shape or out.stride(1) != 1
                   or out.device != block_tables.device):
                 raise ValueError("out must be int32 of block_tables' shape, device and unit inner stride")
+            elif _share_entries(block_tables, out):
+                raise ValueError("out must be block_tables itself or share no entry with it, and have rows of its own")
         on_device = self.device.type == "cuda"
         if not on_device:
             self._check_move(src, dst)

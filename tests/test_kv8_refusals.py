@@ -265,3 +265,32 @@ def test_write_errors_name_every_kind_met(bits, where):
     with pytest.raises(IndexError, match=f"during {where}$"):
         pool.check_write_errors()
     pool.check_write_errors()  # reported once
+
+
+def test_move_blocks_refuses_tables_it_could_not_rename():
+    pool = _cpu_pool()
+    was = _snapshot(pool)
+    flat = torch.arange(60, dtype=torch.int32) % 9
+    tables = flat[:12].view(3, 4)
+    row = torch.zeros(1, 1 << 15, dtype=torch.int32)
+    with pytest.raises(ValueError, match=r"2\*\*31"):
+        many = row.expand(1 << 16, -1)
+        pool.move_blocks([1], [2], many, out=many)
+    for out in (flat[:4].expand(3, 4), flat[1:13].view(3, 4), flat[8:20].view(3, 4), flat[:18].view(3, 6)[:, :4],
+                flat[40:].as_strided((3, 4), (3, 1))):
+        with pytest.raises(ValueError, match="share no entry"):
+            pool.move_blocks([1], [2], tables, out=out)
+    for a, b in zip(_snapshot(pool), was):
+        for now, old in zip(a, b):
+            assert torch.equal(now, old)
+
+
+def test_move_blocks_takes_tables_beside_each_other():
+    flat = torch.arange(60, dtype=torch.int32) % 9
+    wide = flat.view(3, 20)
+    for tables, out in ((flat[:12].view(3, 4), flat[12:24].view(3, 4)), (wide[:, :4], wide[:, 4:8]), (wide[:, 9:13], wide[:, 3:7]),
+                        (wide[:, :4], wide[:, :4]), (flat[:4].expand(3, 4), flat[4:16].view(3, 4)),
+                        (wide[:1, :4], flat[4:8].view(1, 4)), (wide[:0, :4], wide[:0, :4])):
+        want = [[{1: 2}.get(i, i) for i in r] for r in tables.tolist()]
+        assert _cpu_pool().move_blocks([1], [2], tables, out=out) is out
+        assert out.tolist() == want
