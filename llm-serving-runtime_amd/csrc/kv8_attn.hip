@@ -15,23 +15,27 @@
 // weighs, and no score crosses lanes:
 //   * scores, 4 x D / 32 products v_mfma_f32_16x16x32: the A operand's row r of product j is token
 //     4 j + r % 4 of chunk r / 4, so lane group g receives tokens 4 j + i of chunk g, for head lane % 16
-//     (the B operand holds the query heads). K enters as its integers q (as q + 1152, a permute less the
-//     add, fp32 would hold 1152 times the query's sum beside the score: whole units wrong for queries
-//     with a mean; the add costs nothing measurable, batch 32 33.2 us either way), and the page's scale
-//     multiplies the fp32 score. The head dim is contracted in the order of the lane's 16-byte loads, the
-//     query's operand in the same order;
+//     (the B operand holds the query heads). K enters as its integers q, and the page's scale multiplies
+//     the fp32 score. (As q + 1152 it would take no add, but fp32 would hold 1152 times the query's sum
+//     beside the score, whole units of it lost for queries with a mean. Batch 32 with that bias and
+//     without: fp16 the same, bf16 35.1 and 36.6 us by segments, 34.3 and 33.6 by ranges.) The head dim is
+//     contracted in the order of the lane's 16-byte loads, the query's operand in the same order;
 //   * online softmax in fp32 on the exp2 scale; the reference maximum moves only when a score exceeds it
 //     by more than 2^8, so most steps neither rescale nor exchange maxima between lane groups;
 //   * P.V, 2 x D / 16 products over 32 tokens: lane group g supplies tokens 8 u .. 8 u + 7 of chunk g,
 //     which is what its scores gave (weights) and half of a 16-byte load of a dim's token row (V, times
 //     the page's scale: exact in 16 bits, a permute and a fused multiply-add per pair).
 // Weights are rounded to the 16-bit type before the product, as the 16-bit path's are; the denominator
-// sums the rounded ones, by a product with ones.
+// sums the rounded ones, by a product with ones. The smallest fp16
+// weights are off by up to 2^-25 of a wave's largest, n tokens' by n 2^-25 together: half a step of the output
+// where a wave has 2^14 tokens, a layer of 8 GB (two rows of 131,071 tokens and 8 heads: 2^10 tokens).
 //
-// Bound: HBM. One layer of batch 32, U[128, 4096] tokens, Llama-3-8B heads (139 MB): 34 us, 27 at the rate
-// of a large copy; two rows of 65,521 to 131,071 tokens (403 MB) 77 us in a graph, 5.2 TB/s. Loads alone
-// took 27 of the batch's first launch's 29 us. A CU streams at most about 55 GB/s of such pages, with 64 KiB
-// or 128 KiB of loads in flight: two steps ahead instead of one measured 5 to 20 % slower.
+// Bound: HBM. One layer of batch 32, U[128, 4096] tokens, Llama-3-8B heads (139 MB): 33 us by segments, 31.5
+// by ranges (tables of 8192 tokens), 27 at the rate of a large copy; two rows of 65,521 to 131,071 tokens
+// (403 MB) 76 us in a graph: the ranges read at 6.1 TB/s, then 8 us of merge. By ranges the loads alone took
+// 27 of the batch's first launch's 29 us. A CU streams at most about 55 GB/s of such pages, with 64 KiB or
+// 128 KiB of loads in flight: two steps ahead instead of one measured 5 to 20 % slower. In bf16, where K and
+// V cost a conversion per byte, the batch takes 36.6 us by segments and 33.6 by ranges.
 #include <algorithm>
 
 #include "common.h"
@@ -41,15 +45,16 @@
 namespace mx {
 namespace kv8 {
 
-// Waves per workgroup. They share nothing; alone, few waves spread over more CUs: one row of 100 tokens
-// 6.2 -> 5.4 us per call, 7 bf16 rows 12.1 -> 11.8, batch 32 the same (MI355X, in a graph).
+// Waves per workgroup of the form by ranges. They share nothing; alone, few waves spread over more CUs: in
+// wide tables (in a graph) one row of 100 tokens takes 10.0 us with one wave, 10.2 with two and 10.7 with
+// four, 7 bf16 rows 10.1, 10.3 and 10.6; batch 32 and two rows of 100,000 tokens the same with any.
 constexpr int kAttnWaves = 1;
 constexpr int kChunk = 16;         // tokens per chunk
 constexpr int kStep = 4;           // chunks per step of a wave
 constexpr int kHeads = 16;         // query heads of a segment, at most
-// Waves of a launch: 256 CUs x 8, two per SIMD. Batch 32 of U[128, 4096] tokens, per call: 1536 waves
-// 37.4 us, 2048 36.5, three per SIMD (which spills) 55.9, 4096 (two rounds) 42.5. The loads alone
-// take 27 of the launch's 29 us there, so deeper pipelines have nothing to hide.
+// Waves of a launch by ranges: 256 CUs x 8, two per SIMD. Per call with 1536, 2048 and 4096 (two rounds):
+// batch 32 of U[128, 4096] tokens in tables of 8192 31.4, 31.5 and 36.1 us, one row of 32,768 27.6, 27.9 and
+// 38.7, two of 65,521 to 131,071 73.5, 75.6 and 86.2. Three per SIMD spill: half as slow again.
 constexpr int kWorkers = 2048;
 constexpr int kSegmentWaves = 8;   // waves of a workgroup that has a segment of its own, at most
 constexpr int kMaxTokens = 1 << 30;  // of a table row, so that token and chunk numbers are 32-bit
@@ -160,8 +165,10 @@ struct Piece {
 };
 
 // Where every page stands in one row, K and V are read once and their loads carry the streaming policy:
-// batch 32 39.3 -> 36.5 us per call, two rows of 100,000 tokens 95 -> 85 (by ranges). Rows that share pages
-// (MX_PA_SHARED_BLOCKS) read them with the default one.
+// batch 32 34.9 -> 32.7 us per call by segments, 33.1 -> 31.5 by ranges, two rows of 100,000 tokens 85.6 ->
+// 75.6 (three layers in turn). Pages that the caches hold still from the last call read faster without it:
+// one row of 32,768 tokens 25.9 us against 27.9. Rows that share pages (MX_PA_SHARED_BLOCKS) read them with
+// the default one.
 typedef uint32_t u32x4n __attribute__((ext_vector_type(4)));
 template <bool STREAM>
 __device__ __forceinline__ uint4 load16(const uint8_t* p) {
@@ -569,9 +576,11 @@ __global__ __launch_bounds__(kMergeWaves * 64) void kv8_merge_kernel(AttnParams 
 // 4.7 and the longest row's bytes at 50 GB/s, which is all that one CU streams of such pages, against 9 and
 // the bytes of half-full tables at 5.4 TB/s. Of tables up to 1 MiB per segment only: with wider ones a
 // single long row among short ones would keep one CU at work for 20 us and more. Measured, one against the
-// other: 8 segments of 100 tokens 4.7 and 10.3 us, 14 of up to 1501 (bf16, D = 64) 8.7 and 10.2, 128 of up
-// to 2000 17.4 and 18.7, 256 of up to 4096 34.1 and 36.0; the other way 8 of 1024 10.6 and 8.2, 64 of up
-// to 4096 26.9 and 18.9.
+// other: 8 segments of 100 tokens 4.5 and 10.0 us, 14 of up to 1501 (bf16, D = 64) 7.7 and 10.1, 128 of up
+// to 2000 17.4 and 18.7; about even 256 of up to 4096 (the tables' whole width 34.1 and 36.0, U[128, 4096]
+// 32.7 and 31.5); the other way 8 of 1024 10.6 and 8.2, 64 of up to 4096 26.9 and 18.9. The rule sees the
+// tables' width, not the lengths: rows much shorter than their tables, or one long row among short ones,
+// can take the slower form.
 static bool by_segment(int64_t segments, int64_t max_tokens, int D) {
     const double bytes = (double)max_tokens * D * 2;
     return bytes <= 1 << 20 && 4.7 + bytes / 50e3 <= 9.0 + segments * bytes / 2 / 5.4e6;

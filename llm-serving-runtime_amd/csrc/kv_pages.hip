@@ -97,7 +97,7 @@ struct RenameParams {
 };
 
 // Block tables with every id of the list renamed, the others as they are. A thread finds its id by
-// bisection in the sorted list (8 steps of a register-held kernel argument through LDS).
+// bisection in the sorted list (at most 9 steps over the kernel argument's copy in LDS).
 __global__ __launch_bounds__(kThreads) void rename_kernel(RenameParams p) {
     __shared__ int2 list[kBatch];
     for (int i = threadIdx.x; i < p.n; i += kThreads) list[i] = p.pair[i];

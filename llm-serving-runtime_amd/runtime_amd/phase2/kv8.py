@@ -3,8 +3,9 @@
 The cache holds K and V of a page (a block and kv-head) as 8-bit ``q`` in [-127, 127] and one power of
 two as their scale (the format is in ``include/mxdecode.h``); :class:`~.kv8_pool.Int8KVBlockPool` owns
 its tensors and hands out a layer as :class:`Kv8Layer`. A decode step reads half the bytes of the 16-bit
-pool; a value is off by at most half a scale step when it is written, and by less than one step of the
-page's last scale however often that grows while tokens are appended.
+pool; a value is off by at most half a scale step when it is written (an fp16 magnitude above 65280, where the
+scale is at its cap of 2**9, by at most 480), and by less than one step of the page's last scale however often
+that grows while tokens are appended.
 
 * :func:`kv8_append` - new K/V states into a layer's pages (the 8-bit form of ``kv_append``);
 * :func:`kv8_rope_append` - a decode step's fused QKV rows: q rotated out, k and v into their pages
