@@ -23,7 +23,7 @@ import torch
 
 from .kv8 import BLOCK_SIZES, HEAD_DIMS, Kv8Layer, kv8_append, kv8_attention_decode, kv8_gather
 from .paged_attention_hip import _DTYPE_FLAGS
-from .paged_kv_kernel import GpuKVBlockPool, _alloc_lock
+from .paged_kv_kernel import GpuKVBlockPool, _alloc_lock, settle
 
 ZERO_BYTE = 128  # q = 0
 
@@ -68,6 +68,7 @@ class Int8KVBlockPool(GpuKVBlockPool):
         self._write_err = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._stores = [Kv8Layer(data[i], codes[i], s.block_size_tokens, s.head_dim, self.dtype)
                         for i in range(s.num_layers)]
+        settle(data.device)
         self._codes, self._data = codes, data
 
     def layer_store(self, layer_idx: int) -> Kv8Layer:

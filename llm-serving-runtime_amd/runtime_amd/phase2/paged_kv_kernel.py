@@ -72,6 +72,14 @@ class PoolShape:
     head_dim: int
 
 
+def settle(device: torch.device) -> None:
+    """Wait until a pool's tensors, filled on the current stream, hold what they begin with: its next use may be on
+    another stream. (Under capture the fills are part of the graph.)"""
+    with _hip.on_device(device):
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream().synchronize()
+
+
 # Entries of one launch over pairs that depend on each other: a pair each, and one more for a cycle.
 MAX_DEPENDENT = 448
 
@@ -235,6 +243,7 @@ class GpuKVBlockPool:
         if self.device.type == "cuda":
             self._used_map = torch.zeros(s.num_blocks, dtype=torch.uint8, device=self.device)
             self._write_err = torch.zeros(1, dtype=torch.int32, device=self.device)
+            settle(self._write_err.device)
         self._v_pool, self._k_pool = v_pool, k_pool
 
     def _touch_block(self, physical: int) -> None:
