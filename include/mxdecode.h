@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define MX_ABI_VERSION 21
+#define MX_ABI_VERSION 22
 
 typedef enum mx_status {
     MX_OK = 0,
@@ -650,6 +650,84 @@ int mx_kv_rename_pages(const int32_t* tables, int64_t in_stride, int32_t* out, i
  * blocks. */
 int mx_kv_clear_pages(uint8_t* codes, int64_t page_bytes, int64_t layer_stride, int32_t layers, uint8_t* used,
                       int32_t num_pages, const int32_t* ids, int32_t n, void* stream);
+
+/* Tokens of a tree of drafted tokens kept: of row b, token start_pos[b] + path[b, j]
+ * becomes token start_pos[b] + j for j < counts[b], in every layer, K and V; every
+ * source as it was before the call. path: int32 [B, T] (row stride path_sb) on the
+ * device, rising, below T; counts: int32 [B]. A path that does not rise or leaves
+ * [0, T) moves nothing from there on, a token outside the table or the pool is
+ * skipped, and both set bit 0 of the nullable err word. lens_out (nullable, int32
+ * [B]) gets start_pos + counts and shares no memory with start_pos or counts, which
+ * every layer reads (MX_ERR_INVALID). k, v: the first layer's views of token_bytes (a multiple of 16) per token and
+ * head, tokens of a block side by side; strides in bytes, multiples of 16. Rows own
+ * their blocks. No reference counterpart (it verifies one token at a time:
+ * runtime/phase2/worker_server.py:1010-1075). */
+int mx_kv_keep_tokens(void* k, void* v, int32_t token_bytes, int64_t layer_stride, int64_t block_stride,
+                      int64_t head_stride, int32_t layers, int32_t Hkv, int32_t block_size, int32_t num_blocks,
+                      const int32_t* block_tables, int64_t bt_sb, int32_t max_blocks, const int32_t* start_pos,
+                      const int32_t* path, int64_t path_sb, const int32_t* counts, int32_t B, int32_t T,
+                      int32_t* lens_out, int32_t* err, void* stream);
+
+/* ----------------------------------------------------------------------------
+ * Speculative decoding: several new tokens per row, of which the target keeps a
+ * path. The reference drafts and verifies one token after the other
+ * (runtime/phase2/worker_server.py:1010-1075).
+ * ------------------------------------------------------------------------- */
+
+/* Attention of T new tokens (nodes) per row over the paged cache:
+ * out[b, i, h] = sum_j p_j v_j, p = softmax of scale * q[b, h, i] . k_j over the
+ * visible tokens j of row b, those below ctx = seq_lens[b] - counts[b] and of the
+ * row's nodes (token ctx + n is node n) those with mask[b, i, n] != 0; without a
+ * mask those with n <= i. seq_lens counts the nodes; counts (int32 [B], nullable:
+ * T) is how many of the T the row has. Nodes from counts[b] on, and nodes that see
+ * nothing, get zeros. q: 16-bit [B, Hq, T, D] (strides q_sb, q_sh, q_st, 1); k, v and
+ * tables as in mx_paged_attn_decode; mask: bytes [B, T, T] (strides mask_sb, 0 for
+ * one mask, mask_st, 1), nullable; out: 16-bit [B, T, Hq, D] (strides o_sb, o_st,
+ * o_sh, 1). What invisible tokens hold, NaN included, has no effect. A block outside
+ * the pool is skipped and sets bit 2 of the nullable err word. D in {64, 128},
+ * block_size in {4, 8, 16, 32}, any GQA group, any T; scale > 0, a normal fp32
+ * number also times log2(e). Strides non-negative multiples of 8, pointers 16-byte
+ * aligned. flags: MX_PA_BF16 and MX_PA_SHARED_BLOCKS (rows may share pages; the
+ * result is the same). workspace: at least mx_tree_attn_workspace_bytes, 16-byte
+ * aligned, not shared by calls that overlap (its contents need not be kept). */
+size_t mx_tree_attn_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_blocks,
+                                    int32_t block_size);
+int mx_tree_attn(const uint16_t* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const uint16_t* k, const uint16_t* v,
+                 int64_t kv_sblk, int64_t kv_shead, const int32_t* block_tables, int64_t bt_sb, int32_t max_blocks,
+                 const int32_t* seq_lens, const uint8_t* mask, int64_t mask_sb, int64_t mask_st, const int32_t* counts,
+                 int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t block_size, int32_t num_blocks,
+                 float scale, uint16_t* out, int64_t o_sb, int64_t o_st, int64_t o_sh, void* workspace,
+                 size_t workspace_bytes, int32_t* err, uint32_t flags, void* stream);
+
+/* The path of each row's tree that the target's distributions accept, and the token
+ * that follows. logits [B, T, V] (fp16; bf16 with MX_PA_BF16, fp32 with
+ * MX_LOGITS_FP32; strides l_sb, l_st, 1) of the target at every node; tokens (int64
+ * [B, T]) the nodes' tokens; parents (int32 [B, T]) below the nodes themselves, -1 at
+ * node 0, where the walk begins; uniforms (fp32 [B, T]) in [0, 1). At a node with
+ * r = softmax(logits / temperature) (temperature <= 0: a point at the largest logit,
+ * the first on ties) the children are tried in order: token x is taken where
+ * uniforms[child] * q(x) < r(x). draft_logits (nullable, as logits): q is
+ * softmax(draft_logits / temperature) at the node, and a child not taken leaves
+ * r = max(r - q, 0) scaled to a sum of 1. Without them q is a point at x: r loses x.
+ * Where nothing would remain r stays. Where no child is taken the walk ends: the
+ * following token is the first whose running sum of r exceeds uniforms[0] times the
+ * whole. All in fp64. path_out (int32 [B, T]): the nodes taken, from node 0, then -1;
+ * counts_out (int32 [B]): how many; tokens_out (int64 [B, T]): the taken nodes'
+ * tokens without node 0's, then the following token, then -1. A token outside [0, V)
+ * is never taken. A node whose logits hold a NaN, nothing above -inf or (with a
+ * temperature) +inf has no distribution: nothing is taken there and the following
+ * token is -1. counts (int32 [B], nullable: T): nodes of each row; a row of none gets
+ * 0 and -1. T <= 1024, V <= 4194304. workspace: at least
+ * mx_verify_draft_workspace_bytes, 16-byte aligned, not shared by calls that overlap.
+ * The reference's counterpart takes the argmax of one position after the other
+ * (runtime/phase2/worker_server.py:1010-1075). */
+#define MX_LOGITS_FP32 16u
+size_t mx_verify_draft_workspace_bytes(int32_t B, int32_t T, int32_t V, int32_t draft);
+int mx_verify_draft(const void* logits, int64_t l_sb, int64_t l_st, const void* draft_logits, int64_t d_sb,
+                    int64_t d_st, const int64_t* tokens, int64_t t_sb, const int32_t* parents, int64_t p_sb,
+                    const int32_t* counts, const float* uniforms, int64_t u_sb, const float* temperatures,
+                    int64_t temp_sb, int32_t B, int32_t T, int32_t V, int64_t* tokens_out, int32_t* counts_out,
+                    int32_t* path_out, void* workspace, size_t workspace_bytes, uint32_t flags, void* stream);
 
 #ifdef __cplusplus
 }

@@ -7,6 +7,9 @@
 //
 // The copies replace GpuKVBlockPool.copy_blocks (runtime/phase2/paged_kv_kernel.py:233-250), whose
 // torch form gathers every page into a temporary and scatters it: twice the bytes.
+//
+// mx_kv_keep_tokens moves single tokens inside their rows: the accepted path of a tree of drafted tokens to the
+// places right behind the row's context. Its lists are on the device, where the verification wrote them.
 #include <algorithm>
 #include <vector>
 
@@ -218,6 +221,81 @@ static int check_region(const char* what, const Region& r, bool required) {
     return MX_OK;
 }
 
+struct KeepParams {
+    char *k, *v;
+    int64_t layer_stride, block_stride, head_stride;  // bytes
+    int token_bytes;                                  // of one token and head
+    int Hkv;
+    const int32_t* bt;
+    int64_t bt_sb;
+    int max_blocks, bs, num_blocks;
+    const int32_t* start;
+    const int32_t* path;
+    int64_t path_sb;
+    int T;
+    const int32_t* counts;
+    int32_t* lens_out;
+    int32_t* err;
+};
+
+// One workgroup per (layer, row). A thread owns 16 bytes of every token of a head's K or V, so what it moves no
+// other thread touches. Paths rise, so token j comes from place j or behind it: a batch of tokens is read before it is
+// written, and no later one comes from a place that was written before. A few dependent loads (path, table, token)
+// and stores; bound by that chain.
+__global__ __launch_bounds__(kThreads) void keep_tokens_kernel(KeepParams p) {
+    constexpr int kTogether = 8;
+    const int layer = blockIdx.x, b = blockIdx.y;
+    const int32_t* path = p.path + b * p.path_sb;
+    const int32_t* bt = p.bt + b * p.bt_sb;
+    int n = p.counts[b];
+    n = n < 0 ? 0 : n < p.T ? n : p.T;
+    const int64_t start = p.start[b];
+    if (p.lens_out && layer == 0 && threadIdx.x == 0) p.lens_out[b] = (int)start + n;
+    const int per = p.token_bytes / 16, chunks = 2 * p.Hkv * per;
+    const auto place = [&](int64_t pos) -> int64_t {  // of a token in its layer and head, or -1
+        if (pos < 0 || pos / p.bs >= p.max_blocks) return -1;
+        const int id = bt[pos / p.bs];
+        if ((unsigned)id >= (unsigned)p.num_blocks) return -1;
+        return id * p.block_stride + pos % p.bs * p.token_bytes;
+    };
+    for (int c = threadIdx.x; c < chunks; c += kThreads) {
+        const int head = c / per % p.Hkv;
+        char* base = (c < p.Hkv * per ? p.k : p.v) + layer * p.layer_stride + head * p.head_stride + c % per * 16;
+        int prev = -1;
+        for (int j0 = 0; j0 < n; j0 += kTogether) {
+            uint4 x[kTogether];
+            int64_t to[kTogether];
+            bool stop = false;
+#pragma unroll
+            for (int i = 0; i < kTogether; ++i) {
+                to[i] = -1;
+                const int j = j0 + i;
+                if (j >= n || stop) continue;
+                const int node = path[j];
+                if (node <= prev || node >= p.T) {  // not a path: nothing from here on moves
+                    stop = true;
+                    if (p.err && layer == 0) atomicOr(p.err, 1);
+                    continue;
+                }
+                prev = node;
+                if (node == j) continue;
+                const int64_t from = place(start + node);
+                to[i] = place(start + j);
+                if (from < 0 || to[i] < 0) {
+                    if (p.err && layer == 0) atomicOr(p.err, 1);
+                    to[i] = -1;
+                    continue;
+                }
+                x[i] = *reinterpret_cast<const uint4*>(base + from);
+            }
+#pragma unroll
+            for (int i = 0; i < kTogether; ++i)
+                if (to[i] >= 0) *reinterpret_cast<uint4*>(base + to[i]) = x[i];
+            if (stop) break;
+        }
+    }
+}
+
 }  // namespace pages
 }  // namespace mx
 
@@ -334,5 +412,38 @@ extern "C" int mx_kv_clear_pages(uint8_t* codes, int64_t page_bytes, int64_t lay
         std::copy(ids + i, ids + i + p.n, p.id);
         hipLaunchKernelGGL(pages::clear_kernel, dim3(p.n), dim3(pages::kThreads), 0, as_stream(stream), p);
     }
+    return check_launch(what);
+}
+
+extern "C" int mx_kv_keep_tokens(void* k, void* v, int32_t token_bytes, int64_t layer_stride, int64_t block_stride,
+                                 int64_t head_stride, int32_t layers, int32_t Hkv, int32_t block_size,
+                                 int32_t num_blocks, const int32_t* block_tables, int64_t bt_sb, int32_t max_blocks,
+                                 const int32_t* start_pos, const int32_t* path, int64_t path_sb, const int32_t* counts,
+                                 int32_t B, int32_t T, int32_t* lens_out, int32_t* err, void* stream) {
+    clear_error();
+    const char* what = "mx_kv_keep_tokens";
+    if (B < 0 || T < 0) return fail(MX_ERR_INVALID, "%s: B and T must be >= 0", what);
+    if (B == 0) return MX_OK;
+    if (!k || !v || !block_tables || !start_pos || !path || !counts) return fail(MX_ERR_NULL, "%s: null pointer", what);
+    if (layers < 1 || Hkv < 1 || block_size < 1 || num_blocks < 1 || max_blocks < 1)
+        return fail(MX_ERR_INVALID, "%s: layers, Hkv, block_size, num_blocks and max_blocks must be >= 1", what);
+    if (token_bytes < 16 || token_bytes % 16)
+        return fail(MX_ERR_UNSUPPORTED, "%s: a token of a head must be a multiple of 16 bytes (got %d)", what, token_bytes);
+    if (layer_stride % 16 || block_stride % 16 || head_stride % 16 || !aligned(k, 16) || !aligned(v, 16))
+        return fail(MX_ERR_ALIGNMENT, "%s: pointers and strides must be multiples of 16 bytes", what);
+    if (layer_stride < 0 || block_stride < 0 || head_stride < 0 || bt_sb < 0 || path_sb < 0)
+        return fail(MX_ERR_INVALID, "%s: strides must be >= 0", what);
+    if (lens_out && ((lens_out < start_pos + B && start_pos < lens_out + B) || (lens_out < counts + B && counts < lens_out + B)))
+        return fail(MX_ERR_INVALID, "%s: lens_out must not share memory with start_pos or counts", what);
+    if (B > 65535 || (int64_t)Hkv * (token_bytes / 16) > (1 << 24))
+        return fail(MX_ERR_UNSUPPORTED, "%s: more rows or heads than a launch holds", what);
+    pages::KeepParams p{};
+    p.k = static_cast<char*>(k), p.v = static_cast<char*>(v);
+    p.layer_stride = layer_stride, p.block_stride = block_stride, p.head_stride = head_stride;
+    p.token_bytes = token_bytes, p.Hkv = Hkv;
+    p.bt = block_tables, p.bt_sb = bt_sb, p.max_blocks = max_blocks, p.bs = block_size, p.num_blocks = num_blocks;
+    p.start = start_pos, p.path = path, p.path_sb = path_sb, p.T = T, p.counts = counts;
+    p.lens_out = lens_out, p.err = err;
+    hipLaunchKernelGGL(pages::keep_tokens_kernel, dim3(layers, B), dim3(pages::kThreads), 0, as_stream(stream), p);
     return check_launch(what);
 }

@@ -1,0 +1,742 @@
+// Attention of several new tokens per row over the paged cache for gfx950: the nodes of a tree of drafted
+// tokens, or a chain of tokens, attend over the row's context and their own ancestors. (The reference drafts
+// and verifies one token after the other through its decode path, runtime/phase2/worker_server.py:1010-1075.)
+//
+// out[b, i, h] = sum_j p_j v_j, p = softmax over the visible j of scale * q[b, h, i] . k_j. Token j of row b is
+// visible to node i where j < ctx (ctx = seq_lens[b] - counts[b]), or where it is node j - ctx and mask[b, i, j - ctx] is
+// set (no mask: j - ctx <= i).
+//
+// Work decomposition. The G * T query rows of a (row, kv-head) share its K and V. A segment is a (row, kv-head,
+// tile of R query rows), heads of a node next to each other; it holds ceil(visible tokens / 64) tiles. All segments form
+// one sequence of tiles that is cut into equal ranges, one per workgroup, so that the chip drains evenly whatever
+// the lengths are. A segment that one workgroup holds whole is written as output; of the others the pieces leave
+// (m, l, output / l) in fp32 in the workspace (two slots per workgroup: its first piece and its last) and a second launch joins them.
+//
+// A workgroup is RW waves over the query rows (each RT tiles of 16) times TW waves over a tile's tokens. K and V of
+// 64 tokens at a time are staged in LDS, double buffered, as rows whose 16-byte chunks are permuted by the row
+// (chunk ^ row), which spreads the reads below over all banks. Scores are computed transposed (K rows as the A operand of
+// v_mfma_f32_16x16x32, query rows as B): lane l holds the scores of tokens 4 * (l / 16) + [0, 4) of row l % 16 of two
+// 16-token tiles, which is the k order of the B operand of the second product if V^T's columns are taken in that
+// order too. ds_read_b64_tr_b16 gives them so: a group of 16 lanes reads 4 tokens x 16 dims and each lane gets one
+// dim of the 4 tokens. So probabilities never leave their lane, and V needs no transposed copy.
+//
+// The softmax is the online one in fp32 on the exp2 scale; the reference maximum moves only when it would rise by more than
+// 2^8. p enters the second product rounded to the element type, and l sums the rounded values.
+//
+// Masked places have no effect whatever they hold: scores of invisible tokens are replaced by -inf, V of tokens past the end or
+// of blocks outside the pool is staged as 0, and a drafted token whose V is not finite takes the branch `special` below.
+#include <type_traits>
+
+#include "common.h"
+#include "elt.h"
+
+namespace mx {
+namespace tree {
+
+constexpr int kTok = 64;  // tokens per tile
+constexpr int kCus = 256;
+constexpr int kXcds = 8;
+constexpr int kMinTiles = 2;       // a workgroup's range is at least this long where the whole allows
+constexpr float kLazyLog2 = 8.0f;  // rescale only when the running max rises by more than 2^8
+// The reference of the exponentials stands this much below the maximum it was taken from: p reaches 2^15 and no more, so an fp16 p
+// loses nothing of a token that counts 2^-21 of the largest, and 2^-32 at most of one that counts less. (At the maximum
+// itself 10^5 tokens of 2^-25 each, 0.4 %, would be rounded to 0.)
+constexpr float kHeadLog2 = 7.0f;
+constexpr float kLowest = -3.4028235e38f;
+
+struct Params {
+    const _Float16* q;
+    int64_t q_sb, q_sh, q_st;
+    const _Float16* k;
+    const _Float16* v;
+    int64_t kv_sblk, kv_shead;
+    const int32_t* bt;
+    int64_t bt_sb;
+    int max_blocks, bs_shift;
+    const int32_t* seq_lens;
+    const uint8_t* mask;  // null: a chain
+    int64_t mask_sb, mask_st;
+    const int32_t* counts;  // null: T
+    int B, T, Hkv, G;
+    int num_blocks;
+    float scale_log2e;
+    _Float16* out;
+    int64_t o_sb, o_st, o_sh;
+    float* part;  // [2 * workers][R][D + 4]: output / l, m, l
+    int* err;
+    int workers;
+    int nrt;  // tiles of query rows per (row, kv-head)
+    int R;    // query rows per tile
+};
+
+// What a row of the batch attends over.
+struct Row {
+    int len;    // tokens that its table holds
+    int ctx;    // token of node 0 (below 0 where the row is shorter than its nodes)
+    int count;  // nodes
+};
+
+__device__ __forceinline__ Row row_of(const Params& p, int b) {
+    Row w;
+    const int s0 = p.seq_lens[b], s = s0 > 0 ? s0 : 0, cap = p.max_blocks << p.bs_shift;
+    int c = p.counts ? p.counts[b] : p.T;
+    c = c < 0 ? 0 : c < p.T ? c : p.T;
+    w.count = c;
+    w.ctx = s - c;
+    w.len = s < cap ? s : cap;
+    return w;
+}
+
+// Tokens that a tile of query rows attends over: all of the row's (tree) or those up to its last node (chain).
+__device__ __forceinline__ int visible_end(const Params& p, const Row& w, int rt) {
+    const int first = rt * p.R / p.G;
+    if (first >= w.count) return 0;
+    if (p.mask) return w.len;
+    int last = (rt * p.R + p.R - 1) / p.G;
+    last = last < w.count ? last : w.count - 1;
+    const int64_t end = (int64_t)w.ctx + last + 1;
+    return end < 0 ? 0 : end < w.len ? (int)end : w.len;
+}
+__device__ __forceinline__ int seg_tiles(const Params& p, const Row& w, int rt) {
+    return (visible_end(p, w, rt) + kTok - 1) / kTok;
+}
+// Tiles of one kv-head of a row.
+__device__ __forceinline__ int head_tiles(const Params& p, const Row& w) {
+    int n = 0;
+    for (int rt = 0; rt < p.nrt; ++rt) n += seg_tiles(p, w, rt);
+    return n;
+}
+
+__device__ __forceinline__ int wave_scan(int v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(v, o);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+
+// Tiles of all segments (below 2^30, checked on the host).
+__device__ __forceinline__ int total_tiles(const Params& p, int lane) {
+    int sum = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        int n = 0;
+        if (b0 + lane < p.B) n = head_tiles(p, row_of(p, b0 + lane));
+        sum += __builtin_amdgcn_readlane(wave_scan(n, lane), 63) * p.Hkv;
+    }
+    return sum;
+}
+
+// Tiles before row b.
+__device__ __forceinline__ int tiles_before(const Params& p, int b, int lane) {
+    int sum = 0;
+    for (int b0 = 0; b0 < b; b0 += 64) {
+        int n = 0;
+        if (b0 + lane < b) n = head_tiles(p, row_of(p, b0 + lane));
+        sum += __builtin_amdgcn_readlane(wave_scan(n, lane), 63) * p.Hkv;
+    }
+    return sum;
+}
+
+struct Seg {
+    int b, kvh, rt, tile;
+};
+
+// The segment that holds tile x of all (x < total), and x's index in it.
+__device__ __forceinline__ Seg locate(const Params& p, int x, int lane) {
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        int n = 0;
+        if (b0 + lane < p.B) n = head_tiles(p, row_of(p, b0 + lane)) * p.Hkv;
+        const int incl = wave_scan(n, lane);
+        if (x < __builtin_amdgcn_readlane(incl, 63)) {
+            const int bl = __builtin_popcountll(__builtin_amdgcn_ballot_w64(incl <= x));
+            Seg s;
+            s.b = b0 + bl;
+            x -= __builtin_amdgcn_readlane(incl - n, bl);
+            const int per = __builtin_amdgcn_readlane(n, bl) / p.Hkv;
+            s.kvh = x / per;
+            x -= s.kvh * per;
+            const Row w = row_of(p, s.b);
+            s.rt = 0;
+            for (int m; s.rt + 1 < p.nrt && x >= (m = seg_tiles(p, w, s.rt)); ++s.rt) x -= m;
+            s.tile = x;
+            return s;
+        }
+        x -= __builtin_amdgcn_readlane(incl, 63);
+    }
+    return Seg{0, 0, 0, 0};  // unreachable for x < total
+}
+
+__device__ __forceinline__ int workers_of(const Params& p, int total) {
+    const int most = total / kMinTiles > 1 ? total / kMinTiles : 1;
+    return p.workers < most ? p.workers : most;
+}
+__device__ __forceinline__ int range_lo(int w, int total, int workers) { return (int)((int64_t)w * total / workers); }
+// The worker that holds tile x.
+__device__ __forceinline__ int worker_of(int x, int total, int workers) {
+    return (int)(((int64_t)(x + 1) * workers - 1) / total);
+}
+
+typedef __attribute__((address_space(3))) s16x4v lds_s16x4;
+__device__ __forceinline__ s16x4v read_tr(const _Float16* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+}
+
+template <bool BF16>
+__device__ __forceinline__ bool has_special(uint4 x) {  // an infinity or a NaN among 8 elements
+    constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= (w[i] & E) == E || (w[i] & (E << 16)) == (E << 16);
+    return any;
+}
+
+// D: head dim. RT: 16-row query tiles per wave. RW x TW: waves over query rows and over a tile's tokens.
+template <int D, bool BF16, int RT, int RW, int TW>
+__global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_kernel(Params p) {
+    using E = Elt<BF16>;
+    constexpr int NT = 64 * RW * TW;
+    constexpr int KC = D / 32;                // 32-dim steps of a score
+    constexpr int DT = D / 16;                // 16-dim output tiles
+    constexpr int CH = D / 8;                 // 16-byte chunks per token
+    constexpr int RPP = NT / CH;              // tokens per staging pass
+    constexpr int P = (kTok + RPP - 1) / RPP; // staging passes
+    constexpr int NTT = kTok / 16 / TW;       // 16-token tiles per wave
+    constexpr int R = 16 * RT * RW;
+    static_assert(NTT % 2 == 0 && kTok % RPP == 0, "tile split");
+    __shared__ __attribute__((aligned(16))) _Float16 ks[2][kTok * D];
+    __shared__ __attribute__((aligned(16))) _Float16 vs[2][kTok * D];
+    __shared__ int bad_step[2];  // the last step whose tile has a token of a block outside the pool
+    __shared__ int nf_step[2];   // ... a drafted token whose V is not finite
+
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rw = wave % RW, tw = wave / RW;
+    const int lane = tid & 63, g = lane >> 4, r = lane & 15;
+
+    const int total = total_tiles(p, lane);
+    const int workers = workers_of(p, total);
+    // Consecutive ranges on one XCD (workgroups go round the 8 XCDs): the tiles of query rows of a kv-head meet in its L2.
+    const int per = (workers + kXcds - 1) / kXcds;
+    const int w = (int)blockIdx.x % kXcds * per + (int)blockIdx.x / kXcds;
+    if ((int)blockIdx.x / kXcds >= per || w >= workers || total == 0) return;
+    int lo = range_lo(w, total, workers);
+    const int hi = range_lo(w + 1, total, workers);
+    if (lo >= hi) return;
+    Seg seg = locate(p, lo, lane);
+    if (tid < 2) bad_step[tid] = nf_step[tid] = 0;
+    int step = 0;  // tiles staged so far, from 1: buffer step & 1
+    const int bs = 1 << p.bs_shift;
+    const int c = tid % CH, row0 = tid / CH;  // staged chunk and first token
+    const int range0 = lo;
+
+    while (lo < hi) {
+        const Row row = row_of(p, seg.b);
+        const int end = visible_end(p, row, seg.rt);
+        const int ntiles = (end + kTok - 1) / kTok;
+        const int t0 = seg.tile, t1 = ntiles - t0 < hi - lo ? ntiles : t0 + (hi - lo);
+        const int32_t* bt = p.bt + (int64_t)seg.b * p.bt_sb;
+        const _Float16* kb = p.k + (int64_t)seg.kvh * p.kv_shead + 8 * c;
+        const _Float16* vb = p.v + (int64_t)seg.kvh * p.kv_shead + 8 * c;
+        const int last_tok = end - 1;
+
+        struct Ids {
+            int id[P];
+        };
+        struct Stage {
+            uint4 k[P], v[P];
+        };
+        auto ids_of = [&](int t) {
+            Ids s;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                int tok = t * kTok + row0 + i * RPP;
+                tok = tok < last_tok ? tok : last_tok;  // past the end: the last token's block
+                s.id[i] = bt[tok >> p.bs_shift];
+            }
+            return s;
+        };
+        auto load = [&](int t, const Ids ids) {
+            Stage s;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const int tok = t * kTok + row0 + i * RPP;
+                const int id = (unsigned)ids.id[i] < (unsigned)p.num_blocks ? ids.id[i] : 0;
+                const int64_t off = id * p.kv_sblk + (tok & (bs - 1)) * D;
+                s.k[i] = *reinterpret_cast<const uint4*>(kb + off);
+                s.v[i] = *reinterpret_cast<const uint4*>(vb + off);
+            }
+            return s;
+        };
+        // Into buffer `st & 1`; st is the staged step's number.
+        auto store = [&](int st, int t, const Ids ids, const Stage s) {
+            const int buf = st & 1;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const int rr = row0 + i * RPP, tok = t * kTok + rr;
+                const int pos = rr * D + 8 * (c ^ (rr & (CH - 1)));
+                *reinterpret_cast<uint4*>(&ks[buf][pos]) = s.k[i];
+                const bool inside = (unsigned)ids.id[i] < (unsigned)p.num_blocks;
+                const bool live = tok < end && inside;
+                *reinterpret_cast<uint4*>(&vs[buf][pos]) = live ? s.v[i] : uint4{0, 0, 0, 0};
+                if (tok < end && !inside) {
+                    bad_step[buf] = st;
+                    if (p.err && c == 0) atomicOr(p.err, 4);
+                }
+                if (t * kTok + kTok > row.ctx && live && tok >= row.ctx && has_special<BF16>(s.v[i])) nf_step[buf] = st;
+            }
+        };
+
+        // Query fragments: lane l holds dims 32 c + 8 (l / 16) + [0, 8) of row l % 16 of each of the wave's tiles.
+        half8v qf[RT][KC];
+        int node[RT];  // -1: no such row
+        int64_t odst[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int rr = seg.rt * R + (rw * RT + t) * 16 + r;
+            const int n = rr / p.G, h = seg.kvh * p.G + (rr - n * p.G);
+            node[t] = n < row.count ? n : -1;
+            odst[t] = (int64_t)seg.b * p.o_sb + (int64_t)n * p.o_st + (int64_t)h * p.o_sh;
+            const _Float16* qp = p.q + (int64_t)seg.b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)n * p.q_st + 8 * g;
+#pragma unroll
+            for (int kk = 0; kk < KC; ++kk)
+                qf[t][kk] = node[t] >= 0 ? __builtin_bit_cast(half8v, *reinterpret_cast<const uint4*>(qp + 32 * kk))
+                                         : half8v{};
+        }
+        float m[RT], l[RT];
+        float4v acc[DT][RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            m[t] = kLowest;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        // Every row of the wave sees every token below `whole`.
+        const int first_node = (seg.rt * R + rw * RT * 16) / p.G;
+        const int64_t whole64 = (int64_t)row.ctx + (p.mask ? 0 : first_node + 1);
+        const int whole = whole64 < end ? (int)whole64 : end;
+
+        auto visible = [&](int t, int tok) {  // token of tile t's row to this lane
+            const int n = tok - row.ctx;
+            if (tok >= end || node[t] < 0) return false;
+            if (n < 0) return true;
+            if (!p.mask) return n <= node[t];
+            return p.mask[(int64_t)seg.b * p.mask_sb + (int64_t)node[t] * p.mask_st + n] != 0;
+        };
+        auto compute = [&](auto masked, int st, int tile) {
+            constexpr bool MASK = decltype(masked)::value;
+            const int buf = st & 1;
+            const int tbase = tw * (kTok / TW);  // the wave's first token in the tile
+            const _Float16* kt = &ks[buf][0];
+            const _Float16* vt = &vs[buf][0];
+            float4v s[NTT][RT];
+#pragma unroll
+            for (int i = 0; i < NTT; ++i)
+#pragma unroll
+                for (int t = 0; t < RT; ++t) s[i][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int kk = 0; kk < KC; ++kk)
+#pragma unroll
+                for (int i = 0; i < NTT; ++i) {
+                    const int rr = tbase + 16 * i + r;
+                    const half8v a = __builtin_bit_cast(
+                        half8v, *reinterpret_cast<const uint4*>(kt + rr * D + 8 * ((4 * kk + g) ^ (rr & (CH - 1)))));
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) s[i][t] = E::mma32(a, qf[t][kk], s[i][t]);
+                }
+            uint32_t seen[RT];  // bit 4 i + e: token 16 i + 4 g + e is visible
+            if constexpr (MASK) {
+                const bool bad = bad_step[buf] == st;
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    seen[t] = 0;
+#pragma unroll
+                    for (int i = 0; i < NTT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int tok = tile * kTok + tbase + 16 * i + 4 * g + e;
+                            bool vis = visible(t, tok);
+                            if (bad && vis) vis = (unsigned)bt[tok >> p.bs_shift] < (unsigned)p.num_blocks;
+                            if (vis) seen[t] |= 1u << (4 * i + e);
+                            else s[i][t][e] = -__builtin_huge_valf();
+                        }
+                }
+            }
+            half8v pr[NTT / 2][RT];
+            bool rise = false;
+            float top[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                float mx = s[0][t][0];
+#pragma unroll
+                for (int i = 1; i < 4 * NTT; ++i) mx = fmaxf(mx, s[i >> 2][t][i & 3]);
+                top[t] = mx * p.scale_log2e;
+                rise |= top[t] > m[t] + (kLazyLog2 + kHeadLog2);
+            }
+            if (__builtin_amdgcn_ballot_w64(rise)) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    const float mx = fmaxf(m[t], xor_max_16_32(top[t]) - kHeadLog2);
+                    const float f = __builtin_amdgcn_exp2f(m[t] - mx);
+                    m[t] = mx;
+                    l[t] *= f;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) acc[d][t] *= f;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4 * NTT; ++i) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][t][i & 3], p.scale_log2e, -m[t]));
+                    const _Float16 h = E::round(x);
+                    pr[i >> 3][t][i & 7] = h;
+                    sum += E::widen(h);
+                }
+                l[t] += sum;
+            }
+            const bool special = MASK && nf_step[buf] == st;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int u = 0; u < NTT / 2; ++u) {
+                    // V^T: dim 16 d + r of tokens 32 u + 4 g + [0, 4) and that + 16
+                    const int ra = tbase + 32 * u + 4 * g + (r >> 2), rb = ra + 16;
+                    const int ch = 2 * d + ((r & 3) >> 1), in = 4 * (r & 1);
+                    const s16x4v x0 = read_tr(vt + ra * D + 8 * (ch ^ (ra & (CH - 1))) + in);
+                    const s16x4v x1 = read_tr(vt + rb * D + 8 * (ch ^ (rb & (CH - 1))) + in);
+                    typedef short s16x8v __attribute__((ext_vector_type(8)));
+                    s16x8v x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    if constexpr (MASK) {
+                        if (special) {
+                            // V that is not finite counts for the rows that see it and for no other: it leaves the
+                            // product (0 * inf would be NaN for everyone), and products of indicators with what is
+                            // visible say which outputs it makes infinite or NaN.
+                            constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u, ONE = BF16 ? 0x3f80u : 0x3c00u;
+                            s16x8v up{}, down{}, nan{};
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const uint32_t b = (uint16_t)x[e], a = b & 0x7fffu;
+                                if (a >= EXP) {
+                                    x[e] = 0;
+                                    if (a > EXP) nan[e] = (short)ONE;
+                                    else if (b >> 15) down[e] = (short)ONE;
+                                    else up[e] = (short)ONE;
+                                }
+                            }
+#pragma unroll
+                            for (int t = 0; t < RT; ++t) {
+                                s16x8v vis{};
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) vis[e] = seen[t] >> (8 * u + e) & 1 ? (short)ONE : (short)0;
+                                const half8v vf = __builtin_bit_cast(half8v, vis);
+                                const float4v zero{0.0f, 0.0f, 0.0f, 0.0f};
+                                const float4v cu = E::mma32(__builtin_bit_cast(half8v, up), vf, zero);
+                                const float4v cd = E::mma32(__builtin_bit_cast(half8v, down), vf, zero);
+                                const float4v cn = E::mma32(__builtin_bit_cast(half8v, nan), vf, zero);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    if (cu[i] > 0.0f) acc[d][t][i] += __builtin_huge_valf();
+                                    if (cd[i] > 0.0f) acc[d][t][i] -= __builtin_huge_valf();
+                                    if (cn[i] > 0.0f) acc[d][t][i] = __builtin_nanf("");
+                                }
+                            }
+                        }
+                    }
+                    const half8v a = __builtin_bit_cast(half8v, x);
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) acc[d][t] = E::mma32(a, pr[u][t], acc[d][t]);
+                }
+        };
+        auto tile_step = [&](int st, int tile) {
+            if (tile * kTok + kTok <= whole && bad_step[st & 1] != st) compute(std::false_type{}, st, tile);
+            else compute(std::true_type{}, st, tile);
+        };
+
+        {
+            Ids ids = ids_of(t0);
+            const Stage s = load(t0, ids);
+            ++step;
+            __syncthreads();  // the previous piece is done with LDS
+            store(step, t0, ids, s);
+        }
+        __syncthreads();
+        Ids next = ids_of(t0 + 1);
+        for (int t = t0; t + 1 < t1; ++t) {
+            const Stage s = load(t + 1, next);
+            const Ids ids = next;
+            next = ids_of(t + 2);
+            tile_step(step, t);
+            store(step + 1, t + 1, ids, s);
+            ++step;
+            __syncthreads();
+        }
+        tile_step(step, t1 - 1);
+
+        // The lanes of a row meet, then the waves over tokens (in the buffer that no step reads any more).
+#pragma unroll
+        for (int t = 0; t < RT; ++t) l[t] = node[t] < 0 ? 0.0f : xor_sum_16_32(l[t]);
+        if constexpr (TW > 1) {
+            static_assert(TW == 2 && sizeof(ks) + sizeof(vs) >= sizeof(float) * RW * 64 * RT * (DT * 4 + 2), "exchange");
+            float* xch = reinterpret_cast<float*>(&ks[0][0]) + rw * 64 * RT * DT * 4;
+            float* xml = reinterpret_cast<float*>(&vs[0][0]);
+            __syncthreads();
+            if (tw == 1) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) reinterpret_cast<float4v*>(xch)[(d * RT + t) * 64 + lane] = acc[d][t];
+                    xml[((rw * RT + t) * 64 + lane) * 2] = m[t];
+                    xml[((rw * RT + t) * 64 + lane) * 2 + 1] = l[t];
+                }
+            }
+            __syncthreads();
+            if (tw == 0) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    const float mo = xml[((rw * RT + t) * 64 + lane) * 2], lo2 = xml[((rw * RT + t) * 64 + lane) * 2 + 1];
+                    const float mx = fmaxf(m[t], mo);
+                    const float fa = __builtin_amdgcn_exp2f(m[t] - mx), fb = __builtin_amdgcn_exp2f(mo - mx);
+                    m[t] = mx;
+                    l[t] = l[t] * fa + lo2 * fb;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+                        acc[d][t] = acc[d][t] * fa + reinterpret_cast<float4v*>(xch)[(d * RT + t) * 64 + lane] * fb;
+                }
+            }
+        }
+        if (tw == 0) {
+            const bool complete = t0 == 0 && t1 == ntiles;
+            const int slot = 2 * w + (lo == range0 ? 0 : 1);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const int rr = (rw * RT + t) * 16 + r;
+                const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+                if (complete) {
+                    const int n = (seg.rt * R + rr) / p.G;
+                    if (n >= p.T) continue;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        half4v o;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[i] = l[t] == 0.0f ? (_Float16)0.0f : E::round(acc[d][t][i] * inv);
+                        *reinterpret_cast<half4v*>(p.out + odst[t] + 16 * d + 4 * g) = o;
+                    }
+                } else {
+                    float* dst = p.part + ((int64_t)slot * R + rr) * (D + 4);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+                        *reinterpret_cast<float4v*>(dst + 16 * d + 4 * g) = l[t] == 0.0f ? float4v{} : acc[d][t] * inv;
+                    if (g == 0) *reinterpret_cast<float2*>(dst + D) = float2{m[t], l[t]};
+                }
+            }
+        }
+        lo += t1 - t0;
+        // the next segment that holds a tile
+        seg.tile = 0;
+        if (lo < hi) {
+            do {
+                if (++seg.rt == p.nrt) {
+                    seg.rt = 0;
+                    if (++seg.kvh == p.Hkv) {
+                        seg.kvh = 0;
+                        ++seg.b;
+                    }
+                }
+            } while (seg_tiles(p, row_of(p, seg.b), seg.rt) == 0);
+        }
+    }
+}
+
+// Joins the pieces of the segments that more than one workgroup cut, and clears rows of segments without tokens.
+// A workgroup of 256 threads has D / 4 lanes per query row (4 dims each) and shares a row's pieces among SP groups of
+// lanes: RPG = 256 / (D / 4) / SP query rows at a time.
+template <int D, bool BF16>
+__global__ __launch_bounds__(256) void tree_merge_kernel(Params p, int sp) {
+    using E = Elt<BF16>;
+    constexpr int LN = D / 4;
+    constexpr int GR = 256 / LN;  // lane groups
+    __shared__ float4v sacc[GR][LN];
+    __shared__ float2 sml[GR];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int grp = tid / LN, x = tid % LN;
+    const int rows_per = GR / sp;
+    const int blocks = (p.R + rows_per - 1) / rows_per;
+    const int segid = blockIdx.x / blocks, rr = (blockIdx.x - segid * blocks) * rows_per + grp / sp, part = grp % sp;
+    const int rt = segid % p.nrt, kvh = segid / p.nrt % p.Hkv, b = segid / p.nrt / p.Hkv;
+    const Row row = row_of(p, b);
+    const int ntiles = seg_tiles(p, row, rt);
+    const int qrow = rt * p.R + rr, n = qrow / p.G, h = kvh * p.G + qrow - n * p.G;
+    int first = 0, pieces = 0, head = 0, total = 0, workers = 1;
+    if (ntiles > 0) {
+        total = total_tiles(p, lane);
+        workers = workers_of(p, total);
+        int x0 = tiles_before(p, b, lane) + kvh * head_tiles(p, row);
+        for (int i = 0; i < rt; ++i) x0 += seg_tiles(p, row, i);
+        first = worker_of(x0, total, workers);
+        pieces = worker_of(x0 + ntiles - 1, total, workers) - first + 1;
+        if (pieces == 1) return;  // written whole
+        head = range_lo(first, total, workers) < x0;  // the first piece is its worker's last
+    }
+    float m = kLowest, l = 0.0f;
+    float4v acc{0.0f, 0.0f, 0.0f, 0.0f};
+    const bool live = rr < p.R && n < p.T;
+    if (live) {
+        for (int k = part; k < pieces; k += sp) {
+            const int slot = 2 * (first + k) + (k == 0 ? head : 0);
+            const float* src = p.part + ((int64_t)slot * p.R + rr) * (D + 4);
+            const float4v o = *reinterpret_cast<const float4v*>(src + 4 * x);
+            const float2 ml = *reinterpret_cast<const float2*>(src + D);
+            const float mx = fmaxf(m, ml.x);
+            const float fa = __builtin_amdgcn_exp2f(m - mx), fb = __builtin_amdgcn_exp2f(ml.x - mx) * ml.y;
+            if (ml.y != 0.0f) {  // a piece of which the row sees nothing counts for nothing
+                acc = acc * fa + o * fb;
+                l = l * fa + fb;
+                m = mx;
+            }
+        }
+    }
+    if (sp > 1) {
+        sacc[grp][x] = acc;
+        if (x == 0) sml[grp] = float2{m, l};
+        __syncthreads();
+        if (part == 0) {
+            for (int i = 1; i < sp; ++i) {
+                const float2 ml = sml[grp + i];
+                if (ml.y == 0.0f) continue;
+                const float mx = fmaxf(m, ml.x);
+                const float fa = __builtin_amdgcn_exp2f(m - mx), fb = __builtin_amdgcn_exp2f(ml.x - mx);
+                acc = acc * fa + sacc[grp + i][x] * fb;
+                l = l * fa + ml.y * fb;
+                m = mx;
+            }
+        }
+    }
+    if (!live || part) return;
+    half4v o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? (_Float16)0.0f : E::round(acc[i] / l);
+    *reinterpret_cast<half4v*>(p.out + (int64_t)b * p.o_sb + (int64_t)n * p.o_st + (int64_t)h * p.o_sh + 4 * x) = o;
+}
+
+struct Plan {
+    int rt, rw, tw;  // template arguments
+    int R, nrt, workers;
+};
+
+// Query rows per workgroup: as few wasted rows as the tiles allow up to 256, so that K and V are read once.
+static Plan plan_of(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t max_tokens) {
+    Plan p{};
+    const int64_t rows = G * T;
+    if (rows <= 16) p = {1, 1, 2};
+    else if (rows <= 32) p = {2, 1, 2};
+    else if (rows <= 64) p = {2, 2, 2};
+    else if (rows <= 128) p = {2, 4, 1};
+    else p = {2, 8, 1};
+    p.R = 16 * p.rt * p.rw;
+    p.nrt = (int)ceil_div(rows, p.R);
+    const int64_t most = B * Hkv * p.nrt * ceil_div(max_tokens, kTok) / kMinTiles + 1;
+    const int64_t full = p.rw * p.tw == 8 ? kCus : 2 * kCus;
+    p.workers = (int)ceil_div(most < full ? most : full, kXcds) * kXcds;
+    return p;
+}
+
+template <int D, bool BF16>
+static void launch(const Plan& pl, const Params& p, hipStream_t st) {
+    const dim3 grid((unsigned)p.workers), block(64 * pl.rw * pl.tw);
+    if (pl.rt == 1) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 1, 1, 2>), grid, block, 0, st, p);
+    else if (pl.rw == 1) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 1, 2>), grid, block, 0, st, p);
+    else if (pl.rw == 2) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 2, 2>), grid, block, 0, st, p);
+    else if (pl.rw == 4) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 4, 1>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 8, 1>), grid, block, 0, st, p);
+    const int64_t segs = (int64_t)p.B * p.Hkv * p.nrt;
+    const int groups = 256 / (D / 4);
+    int sp = 1;
+    while (sp < groups && p.workers > 4 * sp * segs) sp *= 2;
+    const int64_t blocks = segs * ceil_div(p.R, groups / sp);
+    hipLaunchKernelGGL((tree_merge_kernel<D, BF16>), dim3((unsigned)blocks), dim3(256), 0, st, p, sp);
+}
+
+}  // namespace tree
+}  // namespace mx
+
+using namespace mx;
+
+extern "C" size_t mx_tree_attn_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D,
+                                               int32_t max_blocks, int32_t block_size) {
+    if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_blocks <= 0 || block_size <= 0 || Hq % Hkv != 0) return 0;
+    const tree::Plan pl = tree::plan_of(B, T, Hkv, Hq / Hkv, (int64_t)max_blocks * block_size);
+    return (size_t)2 * pl.workers * pl.R * (D + 4) * sizeof(float);
+}
+
+extern "C" int mx_tree_attn(const uint16_t* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const uint16_t* k,
+                            const uint16_t* v, int64_t kv_sblk, int64_t kv_shead, const int32_t* block_tables,
+                            int64_t bt_sb, int32_t max_blocks, const int32_t* seq_lens, const uint8_t* mask,
+                            int64_t mask_sb, int64_t mask_st, const int32_t* counts, int32_t B, int32_t T, int32_t Hq,
+                            int32_t Hkv, int32_t D, int32_t block_size, int32_t num_blocks, float scale, uint16_t* out,
+                            int64_t o_sb, int64_t o_st, int64_t o_sh, void* workspace, size_t workspace_bytes,
+                            int32_t* err, uint32_t flags, void* stream) {
+    clear_error();
+    const char* what = "mx_tree_attn";
+    if (B < 0 || T < 0) return fail(MX_ERR_INVALID, "%s: B and T must be >= 0", what);
+    if (B == 0 || T == 0) return MX_OK;
+    if (!q || !k || !v || !block_tables || !seq_lens || !out) return fail(MX_ERR_NULL, "%s: null pointer", what);
+    if (Hkv < 1 || Hq < 1 || Hq % Hkv != 0)
+        return fail(MX_ERR_INVALID, "%s: Hq (%d) must be a positive multiple of Hkv (%d)", what, Hq, Hkv);
+    if (D != 64 && D != 128) return fail(MX_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", what, D);
+    if (block_size != 4 && block_size != 8 && block_size != 16 && block_size != 32)
+        return fail(MX_ERR_UNSUPPORTED, "%s: block_size %d (4, 8, 16 or 32)", what, block_size);
+    if (max_blocks < 1 || num_blocks < 1) return fail(MX_ERR_INVALID, "%s: max_blocks and num_blocks must be >= 1", what);
+    if (flags & ~(uint32_t)(MX_PA_BF16 | MX_PA_SHARED_BLOCKS))
+        return fail(MX_ERR_INVALID, "%s: unknown flags 0x%x", what, flags);
+    if (!(scale >= 1.17549435e-38f) || scale * 1.4426950408889634f > 3.4e38f)
+        return fail(MX_ERR_UNSUPPORTED, "%s: scale must be positive and a normal fp32 number, also times log2(e)", what);
+    const int64_t strides[] = {q_sb, q_sh, q_st, o_sb, o_st, o_sh, kv_sblk, kv_shead};
+    for (int64_t s : strides)
+        if (s < 0 || s % 8) return fail(MX_ERR_ALIGNMENT, "%s: strides must be non-negative multiples of 8 elements", what);
+    if (mask && (mask_sb < 0 || mask_st < 0)) return fail(MX_ERR_INVALID, "%s: mask strides must be >= 0", what);
+    if (bt_sb < 0) return fail(MX_ERR_INVALID, "%s: block table stride must be >= 0", what);
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16))
+        return fail(MX_ERR_ALIGNMENT, "%s: 16-byte alignment", what);
+    const int64_t max_tokens = (int64_t)max_blocks * block_size, G = Hq / Hkv;
+    // Tokens, query rows, segments, tiles and the merge's threads are 32-bit numbers.
+    if (max_tokens > (1 << 30) || G * T > (1 << 24) || (int64_t)B * Hkv > (1 << 24))
+        return fail(MX_ERR_UNSUPPORTED, "%s: more tokens or rows than 32-bit numbers hold", what);
+    const tree::Plan pl = tree::plan_of(B, T, Hkv, G, max_tokens);
+    if ((double)B * Hkv * pl.nrt * ceil_div(max_tokens, tree::kTok) > (double)(1 << 30) ||
+        (double)B * Hkv * pl.nrt * pl.R * (D / 4) > 4.0e9)
+        return fail(MX_ERR_UNSUPPORTED, "%s: more tiles than 32-bit numbers hold", what);
+    const size_t need = mx_tree_attn_workspace_bytes(B, T, Hq, Hkv, D, max_blocks, block_size);
+    if (!workspace || workspace_bytes < need)
+        return fail(MX_ERR_WORKSPACE, "%s: workspace needs %zu bytes, got %zu", what, need, workspace ? workspace_bytes : 0);
+    if (!aligned(workspace, 16)) return fail(MX_ERR_ALIGNMENT, "%s: workspace alignment", what);
+    tree::Params p{};
+    p.q = reinterpret_cast<const _Float16*>(q), p.q_sb = q_sb, p.q_sh = q_sh, p.q_st = q_st;
+    p.k = reinterpret_cast<const _Float16*>(k), p.v = reinterpret_cast<const _Float16*>(v);
+    p.kv_sblk = kv_sblk, p.kv_shead = kv_shead;
+    p.bt = block_tables, p.bt_sb = bt_sb, p.max_blocks = max_blocks;
+    p.bs_shift = block_size == 4 ? 2 : block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
+    p.seq_lens = seq_lens;
+    p.mask = mask, p.mask_sb = mask_sb, p.mask_st = mask_st;
+    p.counts = counts;
+    p.B = B, p.T = T, p.Hkv = Hkv, p.G = (int)G;
+    p.num_blocks = num_blocks;
+    p.scale_log2e = scale * 1.4426950408889634f;
+    p.out = reinterpret_cast<_Float16*>(out), p.o_sb = o_sb, p.o_st = o_st, p.o_sh = o_sh;
+    p.part = static_cast<float*>(workspace);
+    p.err = err;
+    p.workers = pl.workers, p.nrt = pl.nrt, p.R = pl.R;
+    hipStream_t st = as_stream(stream);
+    const bool bf16 = flags & MX_PA_BF16;
+    if (D == 64) {
+        if (bf16) tree::launch<64, true>(pl, p, st);
+        else tree::launch<64, false>(pl, p, st);
+    } else {
+        if (bf16) tree::launch<128, true>(pl, p, st);
+        else tree::launch<128, false>(pl, p, st);
+    }
+    return check_launch(what);
+}

@@ -18,8 +18,11 @@ from .paged_attention_hip import (
 from .kv8 import Kv8Layer, kv8_append, kv8_attention_decode, kv8_gather, kv8_rope_append
 from .kv8_pool import Int8KVBlockPool
 from .paged_kv_kernel import GpuKVBlockPool, PoolShape
+from .speculative import DraftTree, DraftVerdict, paged_attention_tree, verify_draft
 
 __all__ = [
+    "DraftTree",
+    "DraftVerdict",
     "GpuKVBlockPool",
     "Int8KVBlockPool",
     "Int8Linear",
@@ -38,11 +41,13 @@ __all__ = [
     "pack_weight",
     "paged_attention_decode",
     "paged_attention_decode_batched",
+    "paged_attention_tree",
     "quantize_model_",
     "quantize_weight",
     "reference_sdpa_attention",
     "reset_paged_decode_batch_metadata",
     "set_paged_decode_batch_metadata",
     "set_paged_decode_context",
+    "verify_draft",
     "warmup_paged_attention_kernel",
 ]

@@ -39,6 +39,7 @@ from . import _hip
 
 if TYPE_CHECKING:
     from .paged_kv_kernel import GpuKVBlockPool
+    from .speculative import DraftTree
 
 _CHUNK_TOKENS = int(os.getenv("MX_PAGED_ATTN_CHUNK_TOKENS", "0"))
 MX_PA_SHARED_BLOCKS = 1
@@ -61,6 +62,7 @@ class PagedDecodeBatchMetadata:
     block_tables: torch.Tensor  # [B, max_blocks] int32
     seq_lens: torch.Tensor  # [B] int32, KV length to attend over (includes current token)
     shared_blocks: bool = False  # rows may alias block ids (MX_PA_SHARED_BLOCKS)
+    tree: "DraftTree | None" = None  # the new tokens are a tree's nodes, for speculative.paged_attention_tree
 
 
 PagedDecodeContext = PagedDecodeBatchMetadata

@@ -198,15 +198,16 @@ class GpuKVBlockPool:
         return self._peak_allocated_blocks
 
     def check_write_errors(self) -> None:
-        """Raise ``IndexError`` if a device KV write met a slot outside its block table or the
-        pool since the last check (the reference's ``:221-222`` check, deferred to one host
-        sync); the error word is cleared."""
+        """Raise ``IndexError`` if a device KV write (or :meth:`keep_tokens`, or tree attention) met a slot
+        outside its block table or the pool since the last check (the reference's ``:221-222`` check,
+        deferred to one host sync); the error word is cleared."""
         if self._write_err is None:
             return
         bits = int(self._write_err.item())
         if bits:
             self._write_err.zero_()
-            raise IndexError("block table underrun or physical block id out of range during batched write")
+            where = " and ".join(name for name, hit in (("batched write", bits & ~4), ("attention", bits & 4)) if hit)
+            raise IndexError(f"block table underrun or physical block id out of range during {where}")
 
     def bytes_per_block(self) -> int:
         s = self.shape
@@ -351,6 +352,74 @@ class GpuKVBlockPool:
             -1, key_states.shape[1], key_states.shape[3])
         v_layer[phys, :, offset, :] = value_states.to(self.dtype).permute(0, 2, 1, 3).reshape(
             -1, value_states.shape[1], value_states.shape[3])
+
+    def keep_tokens(self, block_tables: torch.Tensor, start_positions: torch.Tensor, path: torch.Tensor,
+                    counts: torch.Tensor, lens_out: torch.Tensor | None = None) -> None:
+        """Keep a path of drafted tokens: of every row, token ``start + path[j]`` becomes token ``start + j`` for
+        ``j < counts``, in all layers, every source as it was before the call.
+
+        ``block_tables [B, max_blocks]``, ``start_positions [B]`` (the context's length), ``path [B, T]`` rising
+        within [0, T) and ``counts [B]`` as ``speculative.verify_draft`` gives them, all on the pool's device: one
+        launch, no host sync. ``lens_out`` (int32 ``[B]``, a tensor of its own) gets ``start + counts``, the
+        rows' new lengths. A path that does not rise moves nothing from there on; that and a token outside its
+        table or the pool are reported by :meth:`check_write_errors`. Rows own the blocks behind their context.
+        A pool on the CPU checks on the host (``IndexError``).
+        """
+        if self.kv_bits != 16:
+            raise ValueError("keep_tokens moves tokens of a 16-bit pool: a token of an 8-bit page has no scale of its own")
+        b = int(block_tables.shape[0])
+        if block_tables.dim() != 2 or path.dim() != 2 or path.shape[0] != b or counts.shape != (b,) \
+                or start_positions.shape != (b,):
+            raise ValueError("keep_tokens takes block_tables [B, max_blocks], start_positions [B], path [B, T], counts [B]")
+        if any(t.dtype.is_floating_point or t.dtype == torch.bool for t in (block_tables, start_positions, path, counts)):
+            raise ValueError("block_tables, start_positions, path and counts must be whole numbers")
+        if lens_out is not None and (lens_out.dtype != torch.int32 or lens_out.shape != (b,) or not lens_out.is_contiguous()):
+            raise ValueError("lens_out must be a contiguous int32 tensor [B]")
+        if b == 0:
+            return
+        self._ensure_pools()
+        k, v = self._k_pool, self._v_pool
+        if self.device.type != "cuda":
+            self._keep_on_host(block_tables, start_positions, path, counts, lens_out)
+            return
+        device = k.device
+        if any(t.device != device for t in (block_tables, start_positions, path, counts) + (
+                () if lens_out is None else (lens_out,))):
+            raise ValueError("keep_tokens takes tensors on the pool's device")
+        tables = block_tables if block_tables.dtype == torch.int32 and block_tables.stride(1) == 1 \
+            else block_tables.to(torch.int32).contiguous()
+        path = path if path.dtype == torch.int32 and path.stride(1) == 1 else path.to(torch.int32).contiguous()
+        starts, counts = (t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+                          for t in (start_positions, counts))
+        s, size = self.shape, k.element_size()
+        with _hip.on_device(device):
+            _hip.check(_hip.load().mx_kv_keep_tokens(
+                k.data_ptr(), v.data_ptr(), s.head_dim * size, k.stride(0) * size, k.stride(1) * size, k.stride(2) * size,
+                s.num_layers, s.num_kv_heads, s.block_size_tokens, s.num_blocks, tables.data_ptr(), tables.stride(0),
+                tables.shape[1], starts.data_ptr(), path.data_ptr(), path.stride(0), counts.data_ptr(), b, path.shape[1],
+                None if lens_out is None else lens_out.data_ptr(), self._write_err.data_ptr(),
+                _hip.stream_handle(device)), "mx_kv_keep_tokens")
+
+    def _keep_on_host(self, block_tables, start_positions, path, counts, lens_out) -> None:
+        bs, width = self.block_size_tokens, int(path.shape[1])
+        src, dst, lens = [], [], []
+        for table, start, row, n in zip(block_tables.tolist(), start_positions.tolist(), path.tolist(), counts.tolist()):
+            n = min(max(n, 0), width)
+            lens.append(start + n)
+            nodes = row[:n]
+            if any(not a < b < width for a, b in zip([-1] + nodes, nodes)):
+                raise IndexError("the path of a row does not rise within its nodes")
+            for j, node in enumerate(nodes):
+                for pos, out in ((start + node, src), (start + j, dst)) if node != j else ():
+                    if pos < 0 or pos // bs >= len(table) or not 0 <= table[pos // bs] < self.shape.num_blocks:
+                        raise IndexError("block table underrun or physical block id out of range during keep_tokens")
+                    out.append((table[pos // bs], pos % bs))
+        if src:
+            (sp, so), (dp, do) = (torch.tensor(x).unbind(1) for x in (src, dst))
+            for pool in (self._k_pool, self._v_pool):
+                pool[:, dp, :, do] = pool[:, sp, :, so]
+        if lens_out is not None:
+            lens_out.copy_(torch.tensor(lens, dtype=torch.int32))
 
     def copy_blocks(self, src_block_ids: list[int], dst_block_ids: list[int]) -> None:
         """Copy full physical blocks (all layers) from src ids to dst ids (``:233-250``), every source as
