@@ -24,7 +24,8 @@
 // 2^8. p enters the second product rounded to the element type, and l sums the rounded values.
 //
 // Masked places have no effect whatever they hold: scores of invisible tokens are replaced by -inf, V of tokens past the end or
-// of blocks outside the pool is staged as 0, and a drafted token whose V is not finite takes the branch `special` below.
+// of blocks outside the pool is staged as 0, and V of a drafted token that is not finite reaches only
+// the rows that see it (nf_step below).
 #include <type_traits>
 
 #include "common.h"
@@ -177,20 +178,27 @@ __device__ __forceinline__ int worker_of(int x, int total, int workers) {
     return (int)(((int64_t)(x + 1) * workers - 1) / total);
 }
 
+typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4v lds_s16x4;
-__device__ __forceinline__ s16x4v read_tr(const _Float16* p) {
+__device__ __forceinline__ s16x4v read_tr(const char* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
 }
 
+// Elements that are not finite set to 0 in x; whether there were any.
 template <bool BF16>
-__device__ __forceinline__ bool has_special(uint4 x) {  // an infinity or a NaN among 8 elements
+__device__ __forceinline__ bool drop_special(u32x4v& x) {
     constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
     bool any = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) any |= (w[i] & E) == E || (w[i] & (E << 16)) == (E << 16);
+    for (int i = 0; i < 4; ++i) {
+        const bool lo = (x[i] & E) == E, hi = (x[i] & (E << 16)) == (E << 16);
+        x[i] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+        any |= lo || hi;
+    }
     return any;
 }
+
+#define MX_INLINE __attribute__((always_inline))
 
 // D: head dim. RT: 16-row query tiles per wave. RW x TW: waves over query rows and over a tile's tokens.
 template <int D, bool BF16, int RT, int RW, int TW>
@@ -208,7 +216,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     __shared__ __attribute__((aligned(16))) _Float16 ks[2][kTok * D];
     __shared__ __attribute__((aligned(16))) _Float16 vs[2][kTok * D];
     __shared__ int bad_step[2];  // the last step whose tile has a token of a block outside the pool
-    __shared__ int nf_step[2];   // ... a drafted token whose V is not finite
+    __shared__ int nf_step;      // ... a drafted token whose V is not finite
 
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -225,7 +233,8 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     const int hi = range_lo(w + 1, total, workers);
     if (lo >= hi) return;
     Seg seg = locate(p, lo, lane);
-    if (tid < 2) bad_step[tid] = nf_step[tid] = 0;
+    if (tid < 2) bad_step[tid] = 0;
+    if (tid == 0) nf_step = 0;
     int step = 0;  // tiles staged so far, from 1: buffer step & 1
     const int bs = 1 << p.bs_shift;
     const int c = tid % CH, row0 = tid / CH;  // staged chunk and first token
@@ -245,9 +254,9 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             int id[P];
         };
         struct Stage {
-            uint4 k[P], v[P];
+            u32x4v k[P], v[P];
         };
-        auto ids_of = [&](int t) {
+        auto ids_of = [&](int t) MX_INLINE {
             Ids s;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
@@ -257,34 +266,34 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             }
             return s;
         };
-        auto load = [&](int t, const Ids ids) {
+        auto load = [&](int t, const Ids ids) MX_INLINE {
             Stage s;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const int tok = t * kTok + row0 + i * RPP;
                 const int id = (unsigned)ids.id[i] < (unsigned)p.num_blocks ? ids.id[i] : 0;
                 const int64_t off = id * p.kv_sblk + (tok & (bs - 1)) * D;
-                s.k[i] = *reinterpret_cast<const uint4*>(kb + off);
-                s.v[i] = *reinterpret_cast<const uint4*>(vb + off);
+                s.k[i] = *reinterpret_cast<const u32x4v*>(kb + off);
+                s.v[i] = *reinterpret_cast<const u32x4v*>(vb + off);
             }
             return s;
         };
         // Into buffer `st & 1`; st is the staged step's number.
-        auto store = [&](int st, int t, const Ids ids, const Stage s) {
+        auto store = [&](int st, int t, const Ids ids, const Stage s) MX_INLINE {
             const int buf = st & 1;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const int rr = row0 + i * RPP, tok = t * kTok + rr;
                 const int pos = rr * D + 8 * (c ^ (rr & (CH - 1)));
-                *reinterpret_cast<uint4*>(&ks[buf][pos]) = s.k[i];
+                *reinterpret_cast<u32x4v*>(&ks[buf][pos]) = s.k[i];
                 const bool inside = (unsigned)ids.id[i] < (unsigned)p.num_blocks;
-                const bool live = tok < end && inside;
-                *reinterpret_cast<uint4*>(&vs[buf][pos]) = live ? s.v[i] : uint4{0, 0, 0, 0};
+                u32x4v x = tok < end && inside ? s.v[i] : u32x4v{0, 0, 0, 0};
                 if (tok < end && !inside) {
                     bad_step[buf] = st;
                     if (p.err && c == 0) atomicOr(p.err, 4);
                 }
-                if (t * kTok + kTok > row.ctx && live && tok >= row.ctx && has_special<BF16>(s.v[i])) nf_step[buf] = st;
+                if (t * kTok + kTok > row.ctx && tok >= row.ctx && drop_special<BF16>(x)) nf_step = st;
+                *reinterpret_cast<u32x4v*>(&vs[buf][pos]) = x;
             }
         };
 
@@ -301,7 +310,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             const _Float16* qp = p.q + (int64_t)seg.b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)n * p.q_st + 8 * g;
 #pragma unroll
             for (int kk = 0; kk < KC; ++kk)
-                qf[t][kk] = node[t] >= 0 ? __builtin_bit_cast(half8v, *reinterpret_cast<const uint4*>(qp + 32 * kk))
+                qf[t][kk] = node[t] >= 0 ? __builtin_bit_cast(half8v, *reinterpret_cast<const u32x4v*>(qp + 32 * kk))
                                          : half8v{};
         }
         float m[RT], l[RT];
@@ -318,19 +327,25 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
         const int64_t whole64 = (int64_t)row.ctx + (p.mask ? 0 : first_node + 1);
         const int whole = whole64 < end ? (int)whole64 : end;
 
-        auto visible = [&](int t, int tok) {  // token of tile t's row to this lane
+        auto visible = [&](int t, int tok) MX_INLINE {  // token of tile t's row to this lane
             const int n = tok - row.ctx;
             if (tok >= end || node[t] < 0) return false;
             if (n < 0) return true;
             if (!p.mask) return n <= node[t];
             return p.mask[(int64_t)seg.b * p.mask_sb + (int64_t)node[t] * p.mask_st + n] != 0;
         };
-        auto compute = [&](auto masked, int st, int tile) {
+        auto compute = [&](auto masked, int st, int tile) MX_INLINE {
             constexpr bool MASK = decltype(masked)::value;
             const int buf = st & 1;
             const int tbase = tw * (kTok / TW);  // the wave's first token in the tile
-            const _Float16* kt = &ks[buf][0];
-            const _Float16* vt = &vs[buf][0];
+            // Byte addresses in LDS: a row's chunks are permuted by an exclusive or, and so are the addresses of one lane's
+            // reads; rows 16 apart are permuted alike. (The empty asm keeps the compiler from holding all of them in registers.)
+            uint32_t ka = (uint32_t)(buf * kTok * D + (tbase + r) * D) * 2 + ((g ^ (r & (CH - 1))) << 4);
+            const int vr = tbase + 4 * g + (r >> 2);
+            uint32_t va = (uint32_t)(buf * kTok * D + vr * D) * 2 + ((((r & 3) >> 1) ^ (vr & (CH - 1))) << 4) + 8 * (r & 1);
+            asm volatile("" : "+v"(ka), "+v"(va));
+            const char* kt = reinterpret_cast<const char*>(&ks[0][0]);
+            const char* vt = reinterpret_cast<const char*>(&vs[0][0]);
             float4v s[NTT][RT];
 #pragma unroll
             for (int i = 0; i < NTT; ++i)
@@ -340,29 +355,22 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             for (int kk = 0; kk < KC; ++kk)
 #pragma unroll
                 for (int i = 0; i < NTT; ++i) {
-                    const int rr = tbase + 16 * i + r;
                     const half8v a = __builtin_bit_cast(
-                        half8v, *reinterpret_cast<const uint4*>(kt + rr * D + 8 * ((4 * kk + g) ^ (rr & (CH - 1)))));
+                        half8v, *reinterpret_cast<const u32x4v*>(kt + (ka ^ (kk << 6)) + 16 * i * D * 2));
 #pragma unroll
                     for (int t = 0; t < RT; ++t) s[i][t] = E::mma32(a, qf[t][kk], s[i][t]);
                 }
-            uint32_t seen[RT];  // bit 4 i + e: token 16 i + 4 g + e is visible
             if constexpr (MASK) {
                 const bool bad = bad_step[buf] == st;
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    seen[t] = 0;
+                for (int t = 0; t < RT; ++t)
 #pragma unroll
-                    for (int i = 0; i < NTT; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int tok = tile * kTok + tbase + 16 * i + 4 * g + e;
-                            bool vis = visible(t, tok);
-                            if (bad && vis) vis = (unsigned)bt[tok >> p.bs_shift] < (unsigned)p.num_blocks;
-                            if (vis) seen[t] |= 1u << (4 * i + e);
-                            else s[i][t][e] = -__builtin_huge_valf();
-                        }
-                }
+                    for (int i = 0; i < 4 * NTT; ++i) {
+                        const int tok = tile * kTok + tbase + 16 * (i >> 2) + 4 * g + (i & 3);
+                        bool vis = visible(t, tok);
+                        if (bad && vis) vis = (unsigned)bt[tok >> p.bs_shift] < (unsigned)p.num_blocks;
+                        if (!vis) s[i >> 2][t][i & 3] = -__builtin_huge_valf();
+                    }
             }
             half8v pr[NTT / 2][RT];
             bool rise = false;
@@ -398,83 +406,45 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
                 }
                 l[t] += sum;
             }
-            const bool special = MASK && nf_step[buf] == st;
+            typedef short s16x8v __attribute__((ext_vector_type(8)));
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int u = 0; u < NTT / 2; ++u) {
                     // V^T: dim 16 d + r of tokens 32 u + 4 g + [0, 4) and that + 16
-                    const int ra = tbase + 32 * u + 4 * g + (r >> 2), rb = ra + 16;
-                    const int ch = 2 * d + ((r & 3) >> 1), in = 4 * (r & 1);
-                    const s16x4v x0 = read_tr(vt + ra * D + 8 * (ch ^ (ra & (CH - 1))) + in);
-                    const s16x4v x1 = read_tr(vt + rb * D + 8 * (ch ^ (rb & (CH - 1))) + in);
-                    typedef short s16x8v __attribute__((ext_vector_type(8)));
-                    s16x8v x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    if constexpr (MASK) {
-                        if (special) {
-                            // V that is not finite counts for the rows that see it and for no other: it leaves the
-                            // product (0 * inf would be NaN for everyone), and products of indicators with what is
-                            // visible say which outputs it makes infinite or NaN.
-                            constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u, ONE = BF16 ? 0x3f80u : 0x3c00u;
-                            s16x8v up{}, down{}, nan{};
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const uint32_t b = (uint16_t)x[e], a = b & 0x7fffu;
-                                if (a >= EXP) {
-                                    x[e] = 0;
-                                    if (a > EXP) nan[e] = (short)ONE;
-                                    else if (b >> 15) down[e] = (short)ONE;
-                                    else up[e] = (short)ONE;
-                                }
-                            }
-#pragma unroll
-                            for (int t = 0; t < RT; ++t) {
-                                s16x8v vis{};
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) vis[e] = seen[t] >> (8 * u + e) & 1 ? (short)ONE : (short)0;
-                                const half8v vf = __builtin_bit_cast(half8v, vis);
-                                const float4v zero{0.0f, 0.0f, 0.0f, 0.0f};
-                                const float4v cu = E::mma32(__builtin_bit_cast(half8v, up), vf, zero);
-                                const float4v cd = E::mma32(__builtin_bit_cast(half8v, down), vf, zero);
-                                const float4v cn = E::mma32(__builtin_bit_cast(half8v, nan), vf, zero);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    if (cu[i] > 0.0f) acc[d][t][i] += __builtin_huge_valf();
-                                    if (cd[i] > 0.0f) acc[d][t][i] -= __builtin_huge_valf();
-                                    if (cn[i] > 0.0f) acc[d][t][i] = __builtin_nanf("");
-                                }
-                            }
-                        }
-                    }
+                    const char* src = vt + (va ^ (d << 5)) + 32 * u * D * 2;
+                    const s16x4v x0 = read_tr(src), x1 = read_tr(src + 16 * D * 2);
+                    const s16x8v x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
                     const half8v a = __builtin_bit_cast(half8v, x);
 #pragma unroll
                     for (int t = 0; t < RT; ++t) acc[d][t] = E::mma32(a, pr[u][t], acc[d][t]);
                 }
         };
-        auto tile_step = [&](int st, int tile) {
-            if (tile * kTok + kTok <= whole && bad_step[st & 1] != st) compute(std::false_type{}, st, tile);
-            else compute(std::true_type{}, st, tile);
-        };
-
         {
-            Ids ids = ids_of(t0);
+            const Ids ids = ids_of(t0);
             const Stage s = load(t0, ids);
             ++step;
             __syncthreads();  // the previous piece is done with LDS
             store(step, t0, ids, s);
         }
         __syncthreads();
+        const int step0 = step;
         Ids next = ids_of(t0 + 1);
-        for (int t = t0; t + 1 < t1; ++t) {
-            const Stage s = load(t + 1, next);
+        for (int t = t0;; ++t) {
+            const bool more = t + 1 < t1;
+            Stage s;
             const Ids ids = next;
-            next = ids_of(t + 2);
-            tile_step(step, t);
-            store(step + 1, t + 1, ids, s);
+            if (more) {
+                s = load(t + 1, next);
+                next = ids_of(t + 2);
+            }
+            if (t * kTok + kTok <= whole && bad_step[step & 1] != step) compute(std::false_type{}, step, t);
+            else compute(std::true_type{}, step, t);
+            if (!more) break;
             ++step;
+            store(step, t + 1, ids, s);
             __syncthreads();
         }
-        tile_step(step, t1 - 1);
 
         // The lanes of a row meet, then the waves over tokens (in the buffer that no step reads any more).
 #pragma unroll
@@ -506,6 +476,29 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
                     for (int d = 0; d < DT; ++d)
                         acc[d][t] = acc[d][t] * fa + reinterpret_cast<float4v*>(xch)[(d * RT + t) * 64 + lane] * fb;
                 }
+            }
+        }
+        if (tw == 0 && nf_step >= step0) {
+            // V of drafted tokens that is not finite was staged as 0 (0 * inf would be NaN for rows that do not see it): it
+            // counts for the rows that see it, whose probability of it is above 0.
+            const int from = t0 * kTok > row.ctx ? t0 * kTok : row.ctx > 0 ? row.ctx : 0;
+            const int to = t1 * kTok < end ? t1 * kTok : end;
+            for (int tok = from; tok < to; ++tok) {
+                const int id = bt[tok >> p.bs_shift];
+                if ((unsigned)id >= (unsigned)p.num_blocks) continue;
+                const _Float16* vp = p.v + (int64_t)seg.kvh * p.kv_shead + id * p.kv_sblk + (tok & (bs - 1)) * D + 4 * g;
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                    if (visible(t, tok))
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) {
+                            const half4v x = *reinterpret_cast<const half4v*>(vp + 16 * d);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float f = E::widen(x[i]);
+                                if (!(__builtin_fabsf(f) < __builtin_huge_valf())) acc[d][t][i] += f;
+                            }
+                        }
             }
         }
         if (tw == 0) {
