@@ -9,22 +9,39 @@
 // distribution whatever the draft was.
 //
 // All of it in 64 bits: an answer is a whole number, and a sum over 10^5 terms in 32 bits would put a border of the
-// running sum on the other side of a uniform number in one draw of some hundred.
+// running sum on the other side of a uniform number in one draw of some hundred. fp64 arithmetic is what bounds a pass over
+// a vocabulary (about 25 instructions per logit), so only the nodes that a path visits are read.
+//
+// A row of the batch is walked by S workgroups together, each of which owns a slice of the vocabulary. A pass over a
+// node's logits ends in one partial per slice (a sum and what it is relative to); every workgroup reads all partials
+// of its row and then decides for itself, so all take the same way and nothing else is passed on. The first nodes of every tree
+// (node 0 at least) are passed over by a launch of their own, which needs no exchange; the second launch walks.
+//
+// Partials are exchanged through 8-byte words that carry the number of the pass in their low bits, written and read
+// past the L2s (relaxed atomics of agent scope), so that a word says by itself whether it is the one waited for: no
+// fence, no counter, one round trip. Words of odd and even passes stand apart, since a workgroup is at most one pass
+// ahead of another of its row. Every wait ends: workgroups take their row and slice from a counter as they start, so all rows
+// but the last one started have all their workgroups running, finish, and make room for what the last one lacks.
 #include "common.h"
 
 namespace mx {
 namespace verify {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 16;                    // logits of a chunk per thread
-constexpr int kChunk = kThreads * kPer;     // logits per chunk
-constexpr int kMaxChunks = 1024;
+constexpr int kWaves = kThreads / 64;
+constexpr int kVec = 8;                    // neighbouring logits per thread
+constexpr int kBlock = kThreads * kVec;    // logits per step of a workgroup
+constexpr int kMaxSlices = 64;             // one lane of a wave each
 constexpr int kMaxNodes = 1024;
+constexpr int kMaxVocab = 1 << 22;
+constexpr int kMaxPolls = 1 << 23;         // seconds: a wait that long means a broken launch; the row then ends with -1
 
-struct Stat {
-    double sum;  // of exp((l - top) / temperature)
-    float top;   // largest logit; NaN: the chunk holds a NaN
-    int at;      // its first index
+// What a pass over a slice gives: sums of 2^((l - ref) c), c = log2(e) / temperature, of the logits and the draft's.
+// Greedy rows: the largest logit in ref[0] and its first index in at. ref NaN: no distribution.
+struct Part {
+    double sum[2];
+    float ref[2];
+    int at, pad;
 };
 
 struct Params {
@@ -41,8 +58,12 @@ struct Params {
     int64_t u_sb;
     const float* temps;
     int64_t temp_sb;
-    int B, T, V, chunks;
-    Stat* stats;  // [2 or 1][B][T][chunks]
+    int B, T, V;
+    int slices, len;  // of a row's vocabulary, logits per slice
+    int first;        // nodes passed over by the first launch
+    Part* parts;      // [B][first][slices]
+    uint64_t* words;  // [B][2][slices][4]
+    int* ticket;
     int64_t* tokens_out;
     int32_t* counts_out;
     int32_t* path_out;
@@ -59,10 +80,33 @@ template <int KIND>
 __device__ __forceinline__ const void* row_at(const void* base, int64_t off) {
     return static_cast<const char*>(base) + off * (KIND == 2 ? 4 : 2);
 }
+// Logits v .. v + 7 below `end` (-inf from there on); rows begin at any element.
+template <int KIND>
+__device__ __forceinline__ void load_vec(const void* row, int v, int end, float (&x)[kVec]) {
+    if (v + kVec <= end) {
+        if constexpr (KIND == 2) {
+            __builtin_memcpy(x, static_cast<const float*>(row) + v, sizeof x);
+        } else {
+            uint16_t h[kVec];
+            __builtin_memcpy(h, static_cast<const uint16_t*>(row) + v, sizeof h);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i)
+                x[i] = KIND == 0 ? (float)__builtin_bit_cast(_Float16, h[i]) : __builtin_bit_cast(float, (uint32_t)h[i] << 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) x[i] = v + i < end ? logit<KIND>(row, v + i) : -__builtin_huge_valf();
+    }
+}
 
 __device__ __forceinline__ int count_of(const Params& p, int b) {
     const int c = p.counts ? p.counts[b] : p.T;
     return c < 0 ? 0 : c < p.T ? c : p.T;
+}
+// log2(e) / temperature; 0 for a greedy row.
+__device__ __forceinline__ double rate_of(const Params& p, int b) {
+    const float t = p.temps[b * p.temp_sb];
+    return t > 0.0f ? 1.4426950408889634074 / (double)t : 0.0;
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -70,302 +114,545 @@ __device__ __forceinline__ double wave_sum(double v) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
-
-// exp((l - top) / temperature), 0 at -inf.
-__device__ __forceinline__ double weight(float l, float top, double inv) {
-    return l == -__builtin_huge_valf() ? 0.0 : exp(((double)l - (double)top) * inv);
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
 }
 
-// One workgroup per chunk of a node's logits.
-template <int KIND>
-__global__ __launch_bounds__(kThreads) void stats_kernel(Params p) {
-    __shared__ float stop[kThreads / 64];
-    __shared__ int sat[kThreads / 64];
-    __shared__ double ssum[kThreads / 64];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int chunk = blockIdx.x % p.chunks;
-    const int64_t rowid = blockIdx.x / p.chunks;
-    const bool is_draft = rowid >= (int64_t)p.B * p.T;
-    const int64_t at = rowid - (is_draft ? (int64_t)p.B * p.T : 0);
-    const int b = (int)(at / p.T), n = (int)(at - (int64_t)b * p.T);
-    if (n >= count_of(p, b)) return;
-    const void* row = is_draft ? row_at<KIND>(p.draft, b * p.d_sb + n * p.d_st) : row_at<KIND>(p.logits, b * p.l_sb + n * p.l_st);
-    const float temp = p.temps[b * p.temp_sb];
-    float x[kPer];
-    float top = -__builtin_huge_valf();
-    int first = 0x7fffffff;
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int v = chunk * kChunk + i * kThreads + tid;
-        x[i] = v < p.V ? logit<KIND>(row, v) : -__builtin_huge_valf();
-        nan |= x[i] != x[i];
-        if (x[i] > top) top = x[i], first = v;
-    }
-    for (int o = 32; o > 0; o >>= 1) {
-        const float t = __shfl_xor(top, o);
-        const int f = __shfl_xor(first, o);
-        if (t > top || (t == top && f < first)) top = t, first = f;
-    }
-    nan = __builtin_amdgcn_ballot_w64(nan) != 0;
-    if (lane == 0) stop[wave] = nan ? __builtin_nanf("") : top, sat[wave] = first;
-    __syncthreads();
-    top = stop[0], first = sat[0];
-    for (int i = 1; i < kThreads / 64; ++i) {
-        const float t = stop[i];
-        if (t != t) top = t;
-        else if (t > top || (t == top && sat[i] < first)) top = t, first = sat[i];
-    }
+// 2^t: t = n + f, |f| <= 1/2, the Taylor series of e^(f ln 2) to the 12th power (the next term is below 2e-16). t below -2000
+// counts as -2000 (the result is 0 either way), and so does NaN, which a logit of -inf gives at an infinite temperature.
+__device__ __forceinline__ double exp2_64(double t) {
+    t = fmax(t, -2000.0);
+    const double n = rint(t), f = t - n;
+    double y = 2.56784359934882051e-11;          // ln(2)^12 / 12!
+    y = __builtin_fma(y, f, 4.44553827187081178e-10);
+    y = __builtin_fma(y, f, 7.05491162080112333e-9);
+    y = __builtin_fma(y, f, 1.01780860092396999e-7);
+    y = __builtin_fma(y, f, 1.32154867901443095e-6);
+    y = __builtin_fma(y, f, 1.52527338040598403e-5);
+    y = __builtin_fma(y, f, 1.54035303933816099e-4);
+    y = __builtin_fma(y, f, 1.33335581464284434e-3);
+    y = __builtin_fma(y, f, 9.61812910762847716e-3);
+    y = __builtin_fma(y, f, 5.55041086648215800e-2);
+    y = __builtin_fma(y, f, 2.40226506959100712e-1);
+    y = __builtin_fma(y, f, 6.93147180559945309e-1);
+    y = __builtin_fma(y, f, 1.0);
+    return ldexp(y, (int)n);
+}
+__device__ __forceinline__ double weight(float l, float ref, double c) {
+    return l == -__builtin_huge_valf() ? 0.0 : exp2_64(((double)l - (double)ref) * c);
+}
+
+// A thread's running sum of 2^((l - ref) c). ref is the largest logit of the first it met; 64 bits hold the sum until
+// a logit lies 2^900 above it.
+struct Sum {
     double sum = 0.0;
-    if (temp > 0.0f && top == top && __builtin_fabsf(top) != __builtin_huge_valf()) {
-        const double inv = 1.0 / (double)temp;
+    float ref = -__builtin_huge_valf();
+    bool bad = false;
+    __device__ __forceinline__ void add(const float (&x)[kVec], double c) {
+        float top = x[0];
+        bad |= x[0] != x[0];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += weight(x[i], top, inv);
+        for (int i = 1; i < kVec; ++i) {
+            top = fmaxf(top, x[i]);
+            bad |= x[i] != x[i];
+        }
+        if (top > ref && !(((double)top - (double)ref) * c <= 900.0)) {  // (ref -inf: the difference is inf, or NaN at rate 0)
+            sum *= ref == -__builtin_huge_valf() ? 0.0 : exp2_64(((double)ref - (double)top) * c);
+            ref = top;
+        }
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) sum += weight(x[i], ref, c);
     }
-    sum = wave_sum(sum);
-    if (lane == 0) ssum[wave] = sum;
+};
+
+struct Shared {
+    double red[2][kWaves];
+    float redf[2][kWaves];
+    int redi[kWaves];
+};
+
+// A workgroup's Sums joined: every thread gets the result.
+__device__ __forceinline__ void join(Shared& sh, int which, const Sum& s, double c, double& sum, float& ref) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    float top = wave_max(s.ref);
+    const bool bad = __builtin_amdgcn_ballot_w64(s.bad) != 0;
     __syncthreads();
-    if (tid == 0) {
-        sum = 0.0;
-        for (int i = 0; i < kThreads / 64; ++i) sum += ssum[i];
-        p.stats[rowid * p.chunks + chunk] = Stat{sum, top, first};
+    if (lane == 0) sh.redf[which][wave] = bad ? __builtin_nanf("") : top;
+    __syncthreads();
+    top = sh.redf[which][0];
+    bool nan = top != top;
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) {
+        nan |= sh.redf[which][i] != sh.redf[which][i];
+        top = fmaxf(top, sh.redf[which][i]);
     }
+    double part = s.ref == -__builtin_huge_valf() ? 0.0 : s.sum * exp2_64(((double)s.ref - (double)top) * c);
+    part = wave_sum(part);
+    if (lane == 0) sh.red[which][wave] = part;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) sum += sh.red[which][i];
+    ref = nan ? __builtin_nanf("") : top;
 }
 
-// One workgroup per row of the batch.
+__device__ __forceinline__ double block_sum(Shared& sh, double v) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.red[0][threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) s += sh.red[0][i];
+    return s;
+}
+
+// A node's children that a draft without logits has drafted: their tokens stay out of the slices' sums, so that what
+// remains once some are refused is a sum and never a difference.
+struct Children {
+    int n;
+    const int* token;  // -1: outside the vocabulary
+};
+
+// One pass over slice s of a node: the softmax's sums, or a greedy row's largest logit.
 template <int KIND>
-__global__ __launch_bounds__(kThreads) void walk_kernel(Params p) {
-    __shared__ double part[kMaxChunks];   // r's weight in each chunk
-    __shared__ double scale[kMaxNodes];   // with draft logits: 1 / the mass that each child not taken left
-    __shared__ int out_of[kMaxNodes];     // without: tokens taken out of r
-    __shared__ double red[kThreads / 64];
-    __shared__ float ftop[2];
-    __shared__ int fat[2];
-    __shared__ double fz[2];
-    __shared__ int found;
-    const int b = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+__device__ __forceinline__ Part pass(const Params& p, Shared& sh, const void* lrow, const void* drow, int s, double c,
+                                     bool greedy, const Children& ch) {
+    const int tid = threadIdx.x, lo = s * p.len, end = lo + p.len < p.V ? lo + p.len : p.V;
+    Part out{};
+    if (greedy) {
+        float top = -__builtin_huge_valf();
+        int at = 0x7fffffff;
+        bool bad = false;
+        for (int v = lo + tid * kVec; v < end; v += kBlock) {
+            float x[kVec];
+            load_vec<KIND>(lrow, v, end, x);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                bad |= x[i] != x[i];
+                if (x[i] > top) top = x[i], at = v + i;
+            }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const float t = __shfl_xor(top, o);
+            const int a = __shfl_xor(at, o);
+            if (t > top || (t == top && a < at)) top = t, at = a;
+        }
+        bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+        __syncthreads();
+        if ((tid & 63) == 0) sh.redf[0][tid >> 6] = bad ? __builtin_nanf("") : top, sh.redi[tid >> 6] = at;
+        __syncthreads();
+        top = sh.redf[0][0], at = sh.redi[0];
+        bad = top != top;
+        for (int i = 1; i < kWaves; ++i) {
+            const float t = sh.redf[0][i];
+            bad |= t != t;
+            if (t > top || (t == top && sh.redi[i] < at)) top = t, at = sh.redi[i];
+        }
+        out.ref[0] = bad ? __builtin_nanf("") : top;
+        out.at = at;
+        return out;
+    }
+    Sum a, d;
+    for (int v = lo + tid * kVec; v < end; v += kBlock) {
+        float x[kVec];
+        load_vec<KIND>(lrow, v, end, x);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) a.bad |= x[i] != x[i] || x[i] == __builtin_huge_valf();
+        if (drow) {
+            float y[kVec];
+            load_vec<KIND>(drow, v, end, y);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) d.bad |= y[i] == __builtin_huge_valf();
+            d.add(y, c);
+        }
+        for (int j = 0; j < ch.n; ++j) {
+            const int t = ch.token[j] - v;
+            if ((unsigned)t < (unsigned)kVec)
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) x[i] = i == t ? -__builtin_huge_valf() : x[i];
+        }
+        a.add(x, c);
+    }
+    join(sh, 0, a, c, out.sum[0], out.ref[0]);
+    if (drow) join(sh, 1, d, c, out.sum[1], out.ref[1]);
+    return out;
+}
+
+// The children of `node` in order, their tokens (-1 outside the vocabulary): by one wave, from the tree in LDS or memory.
+template <typename P, typename T>
+__device__ __forceinline__ int children_of(P parent, T token, int node, int count, int* index, int* tok) {
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int i0 = node + 1; i0 < count; i0 += 64) {
+        const int i = i0 + lane;
+        const bool mine = i < count && parent(i) == node;
+        const uint64_t who = __builtin_amdgcn_ballot_w64(mine);
+        if (mine) {
+            const int at = n + __builtin_popcountll(who & ((1ull << lane) - 1));
+            if (index) index[at] = i;
+            tok[at] = token(i);
+        }
+        n += __builtin_popcountll(who);
+    }
+    return n;
+}
+__device__ __forceinline__ int token_in(int64_t x, int V) { return x >= 0 && x < V ? (int)x : -1; }
+
+// The nodes below `first` of every row, a workgroup per slice; clears what the walk's exchange begins with.
+template <int KIND>
+__global__ __launch_bounds__(kThreads) void first_kernel(Params p) {
+    __shared__ Shared sh;
+    __shared__ int tok[kMaxNodes];
+    __shared__ int nch;
+    const int s = blockIdx.x % p.slices, rest = blockIdx.x / p.slices;
+    const int node = rest % p.first, b = rest / p.first;
+    if (node == 0 && threadIdx.x < 8)
+        p.words[(((int64_t)b * 2 + threadIdx.x / 4) * p.slices + s) * 4 + threadIdx.x % 4] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
     const int count = count_of(p, b);
-    const int32_t* parents = p.parents + b * p.p_sb;
-    const int64_t* tokens = p.tokens + b * p.t_sb;
-    const float* uniforms = p.uniforms + b * p.u_sb;
-    const float temp = p.temps[b * p.temp_sb];
-    const bool greedy = !(temp > 0.0f);
-    const double inv = greedy ? 0.0 : 1.0 / (double)temp;
+    if (node >= count) return;
+    const double c = rate_of(p, b);
+    const bool greedy = !(p.temps[b * p.temp_sb] > 0.0f);
+    if (!p.draft && !greedy) {
+        if (threadIdx.x < 64) {
+            const int32_t* parents = p.parents + b * p.p_sb;
+            const int64_t* tokens = p.tokens + b * p.t_sb;
+            const int n = children_of([&](int i) { return parents[i]; }, [&](int i) { return token_in(tokens[i], p.V); },
+                                      node, count, nullptr, tok);
+            if (threadIdx.x == 0) nch = n;
+        }
+        __syncthreads();
+    }
+    const Children ch{!p.draft && !greedy ? nch : 0, tok};
+    const Part out = pass<KIND>(p, sh, row_at<KIND>(p.logits, b * p.l_sb + node * p.l_st),
+                                p.draft && !greedy ? row_at<KIND>(p.draft, b * p.d_sb + node * p.d_st) : nullptr, s, c,
+                                greedy, ch);
+    if (threadIdx.x == 0) p.parts[((int64_t)b * p.first + node) * p.slices + s] = out;
+}
+
+template <int KIND>
+__global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
+    __shared__ Shared sh;
+    __shared__ int parent[kMaxNodes], token[kMaxNodes];
+    __shared__ float uniform[kMaxNodes];
+    __shared__ int cidx[kMaxNodes], ctok[kMaxNodes], cfirst[kMaxNodes];  // children; the first with the same token
+    __shared__ double cw[kMaxNodes];     // without draft logits: weight, 0 once refused; with: scales of the refusals
+    __shared__ double part[kMaxSlices];  // r's weight in each slice
+    __shared__ double whole[2];
+    __shared__ float refs[2];
+    __shared__ int sbest, snch, sid, hit, tail;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float inf = __builtin_huge_valf();
+    if (tid == 0) sid = atomicAdd(p.ticket, 1);
+    __syncthreads();
+    const int b = sid / per_row, s = sid % per_row;
+    const int count = count_of(p, b);
     int64_t* tout = p.tokens_out + (int64_t)b * p.T;
     int32_t* pout = p.path_out + (int64_t)b * p.T;
-    const float inf = __builtin_huge_valf();
+    const float temp = p.temps[b * p.temp_sb];
+    const bool greedy = !(temp > 0.0f);
+    const double c = rate_of(p, b);
+    const bool drafted = p.draft && !greedy;
+    for (int i = tid; i < count; i += kThreads) {
+        const int up = p.parents[b * p.p_sb + i];
+        parent[i] = up < i ? up : -1;
+        token[i] = token_in(p.tokens[b * p.t_sb + i], p.V);
+        uniform[i] = p.uniforms[b * p.u_sb + i];
+    }
+    __syncthreads();
 
-    auto block_sum = [&](double v) {
-        v = wave_sum(v);
-        __syncthreads();
-        if (lane == 0) red[wave] = v;
-        __syncthreads();
-        double s = 0.0;
-        for (int i = 0; i < kThreads / 64; ++i) s += red[i];
-        return s;
-    };
-    // The whole of a node's distribution from its chunks: largest logit, its first index, sum of weights (0: no distribution).
-    auto gather = [&](int which, int n) {
-        const Stat* st = p.stats + (((int64_t)which * p.B + b) * p.T + n) * p.chunks;
-        __syncthreads();
+    int passes = 0;  // cooperative passes so far
+    // Every slice's words of this pass, a lane of the first wave each.
+    auto exchange = [&](const uint64_t (&mine)[4], int n, uint64_t (&all)[4]) -> bool {
+        ++passes;
+        const uint64_t tag = passes % 255 + 1;
+        uint64_t* base = p.words + ((int64_t)b * 2 + (passes & 1)) * p.slices * 4;
+        if (tid == 0)
+            for (int i = 0; i < n; ++i)
+                __hip_atomic_store(base + s * 4 + i, (mine[i] & ~0xffull) | tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        bool ok = true;
         if (wave == 0) {
-            float top = -inf;
-            int first = 0x7fffffff;
-            bool nan = false;
-            for (int c = lane; c < p.chunks; c += 64) {
-                const Stat s = st[c];
-                nan |= s.top != s.top;
-                if (s.top > top || (s.top == top && s.at < first)) top = s.top, first = s.at;
+            const int from = lane < p.slices ? lane : 0;
+            for (int i = 0; i < n; ++i) {
+                int polls = 0;
+                do {
+                    all[i] = __hip_atomic_load(base + from * 4 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    if (++polls > kMaxPolls) ok = false;
+                    else if ((all[i] & 0xff) != tag) __builtin_amdgcn_s_sleep(1);
+                } while ((all[i] & 0xff) != tag && ok);
             }
-            for (int o = 32; o > 0; o >>= 1) {
-                const float t = __shfl_xor(top, o);
-                const int f = __shfl_xor(first, o);
-                if (t > top || (t == top && f < first)) top = t, first = f;
-            }
-            nan = __builtin_amdgcn_ballot_w64(nan) != 0 || top == -inf || (!greedy && top == inf);
-            double z = 0.0;
-            for (int c = lane; c < p.chunks; c += 64) {
-                const Stat s = st[c];
-                const double w = nan || greedy || s.top == -inf ? 0.0 : s.sum * exp(((double)s.top - (double)top) * inv);
-                if (which == 0) part[c] = w;
-                z += w;
-            }
-            z = wave_sum(z);
-            if (lane == 0) ftop[which] = top, fat[which] = first, fz[which] = nan ? 0.0 : greedy ? 1.0 : z;
         }
-        __syncthreads();
+        return ok;
     };
+    auto word_of = [](double x) { return __builtin_bit_cast(uint64_t, x); };
+    // (a sum loses its low 8 bits to the tag: 2^-44 of it, and all workgroups use the same one)
+    auto sum_of = [](uint64_t w) { return __builtin_bit_cast(double, w & ~0xffull); };
+    auto ref_word = [](float x) { return (uint64_t)__builtin_bit_cast(uint32_t, x) << 32; };
+    auto ref_of = [](uint64_t w) { return __builtin_bit_cast(float, (uint32_t)(w >> 32)); };
 
     int node = 0, n = 0;
-    if (count > 0) {
-        if (tid == 0) pout[0] = 0;
-        n = 1;
-        int rejected = 0;
-        double mass = 0.0;  // sum of part
-        const void *lrow = nullptr, *drow = nullptr;
-        auto enter = [&]() {
-            gather(0, node);
-            lrow = row_at<KIND>(p.logits, b * p.l_sb + node * p.l_st);
-            if (p.draft && !greedy) {
-                gather(1, node);
-                drow = row_at<KIND>(p.draft, b * p.d_sb + node * p.d_st);
+    int refused = 0;  // with draft logits: refusals that r carries
+    bool have = false;
+    const void *lrow = nullptr, *drow = nullptr;
+
+    // Stand at `node`: its distribution's parts and its children.
+    auto enter = [&]() {
+        lrow = row_at<KIND>(p.logits, b * p.l_sb + node * p.l_st);
+        drow = drafted ? row_at<KIND>(p.draft, b * p.d_sb + node * p.d_st) : nullptr;
+        refused = 0;
+        __syncthreads();
+        if (wave == 0) {
+            const int k = children_of([&](int i) { return parent[i]; }, [&](int i) { return token[i]; }, node, count, cidx, ctok);
+            if (lane == 0) snch = k;
+        }
+        __syncthreads();
+        const int k = snch;
+        float cl = -inf;  // logits of this thread's child, loaded ahead of the pass
+        if (!drafted && !greedy && tid < k && ctok[tid] >= 0) cl = logit<KIND>(lrow, ctok[tid]);
+        Part mine{};
+        bool ok = true;
+        if (node < p.first) {
+            if (wave == 0 && lane < p.slices) mine = p.parts[((int64_t)b * p.first + node) * p.slices + lane];
+        } else {
+            const Children ch{!drafted && !greedy ? k : 0, ctok};
+            mine = pass<KIND>(p, sh, lrow, drow, s, c, greedy, ch);
+            uint64_t w[4] = {greedy ? (uint64_t)(uint32_t)mine.at << 8 : word_of(mine.sum[0]), ref_word(mine.ref[0]),
+                             word_of(mine.sum[1]), ref_word(mine.ref[1])}, all[4];
+            ok = exchange(w, drafted ? 4 : 2, all);
+            if (wave == 0) {
+                mine.at = greedy ? (int)(all[0] >> 8) : 0;
+                mine.sum[0] = sum_of(all[0]);
+                mine.ref[0] = ref_of(all[1]);
+                if (drafted) mine.sum[1] = sum_of(all[2]), mine.ref[1] = ref_of(all[3]);
             }
-            mass = fz[0];
-            rejected = 0;
-        };
-        // r's weight of token v (times `mass`, but with draft logits, once a child was refused: of sum 1)
-        auto rest = [&](int v) -> double {
-            const double w = weight(logit<KIND>(lrow, v), ftop[0], inv);
-            if (!p.draft) {
-                for (int i = 0; i < rejected; ++i)
-                    if (out_of[i] == v) return 0.0;
-                return w;
-            }
-            if (rejected == 0) return w;
-            const double q = weight(logit<KIND>(drow, v), ftop[1], inv) / fz[1];
-            double r = w / fz[0];
-            for (int i = 0; i < rejected; ++i) {
-                r -= q;
-                r = (r > 0.0 ? r : 0.0) * scale[i];
-            }
-            return r;
-        };
-        enter();
-        for (int i = 1; i < count; ++i) {
-            if (parents[i] != node || i <= node) continue;
-            const int64_t x64 = tokens[i];
-            if (x64 < 0 || x64 >= p.V || fz[0] == 0.0) continue;
-            const int x = (int)x64;
-            bool take;
-            if (greedy) {
-                take = x == fat[0];
-            } else if (!p.draft) {
-                take = (double)uniforms[i] * mass < rest(x);
-            } else {
-                if (fz[1] == 0.0) continue;
-                const double q = weight(logit<KIND>(drow, x), ftop[1], inv) / fz[1];
-                const double r = rejected ? rest(x) : weight(logit<KIND>(lrow, x), ftop[0], inv) / fz[0];
-                take = (double)uniforms[i] * q < r;
-            }
-            if (take) {
-                if (tid == 0) {
-                    pout[n] = i;
-                    tout[n - 1] = x;
+        }
+        // Children's weights count with the slices' for the largest logit. (The first 256 are at hand.)
+        float ctop = cl;
+        if (!drafted && !greedy)
+            for (int j = tid + kThreads; j < k; j += kThreads)
+                if (ctok[j] >= 0) ctop = fmaxf(ctop, logit<KIND>(lrow, ctok[j]));
+        ctop = wave_max(ctop);
+        __syncthreads();
+        if (lane == 0) sh.redf[1][wave] = ctop;
+        __syncthreads();
+        if (wave == 0) {
+            const bool live = lane < p.slices;
+            for (int i = 0; i < kWaves; ++i) ctop = fmaxf(ctop, sh.redf[1][i]);
+            for (int which = 0; which < (drafted ? 2 : 1); ++which) {
+                float ref = live ? mine.ref[which] : -inf;
+                bool bad = __builtin_amdgcn_ballot_w64(ref != ref || !ok) != 0;
+                float top = wave_max(ref);
+                if (which == 0) top = fmaxf(top, ctop);
+                bad |= top == -inf || (!greedy && top == inf);
+                int at = live && ref == top ? mine.at : 0x7fffffff;
+                if (greedy) {
+#pragma unroll
+                    for (int o = 32; o > 0; o >>= 1) {
+                        const int t = __shfl_xor(at, o);
+                        at = t < at ? t : at;
+                    }
                 }
-                ++n;
-                node = i;
-                enter();
-                continue;
-            }
-            if (greedy) continue;
-            if (!p.draft) {
-                const double keep_mass = mass;
-                __syncthreads();
-                if (tid == 0) out_of[rejected] = x;
-                ++rejected;
-                __syncthreads();
-                double s = 0.0;
-                const int c = x / kChunk;
-                for (int j = 0; j < kPer; ++j) {
-                    const int v = c * kChunk + j * kThreads + tid;
-                    if (v < p.V) s += rest(v);
-                }
-                s = block_sum(s);
-                double all = 0.0;
-                for (int j = lane; j < p.chunks; j += 64) all += j == c ? s : part[j];
-                all = wave_sum(all);
-                if (all > 0.0) {
-                    __syncthreads();
-                    if (tid == 0) part[c] = s;
-                    mass = all;
-                    __syncthreads();
-                } else {
-                    --rejected;  // nothing would remain: r stays
-                    mass = keep_mass;
-                }
-            } else {
-                __syncthreads();
-                if (tid == 0) scale[rejected] = 1.0;
-                ++rejected;
-                __syncthreads();
-                double all = 0.0;
-                for (int v = tid; v < p.V; v += kThreads) all += rest(v);
-                all = block_sum(all);
-                if (all > 0.0) {
-                    if (tid == 0) scale[rejected - 1] = 1.0 / all;
-                    __syncthreads();
-                } else {
-                    --rejected;
+                double z = 0.0;
+                if (live && !bad && !greedy && ref != -inf) z = mine.sum[which] * exp2_64(((double)ref - (double)top) * c);
+                if (which == 0 && live) part[lane] = z;
+                z = wave_sum(z);
+                if (lane == 0) {
+                    refs[which] = bad ? __builtin_nanf("") : top;
+                    whole[which] = z;
+                    if (which == 0) sbest = at;
                 }
             }
         }
-        // The token that follows.
-        int64_t next = -1;
-        if (fz[0] != 0.0) {
-            if (greedy) {
-                next = fat[0];
-            } else {
-                if (p.draft && rejected) {
-                    for (int c = 0; c < p.chunks; ++c) {
-                        double s = 0.0;
-                        for (int j = 0; j < kPer; ++j) {
-                            const int v = c * kChunk + j * kThreads + tid;
-                            if (v < p.V) s += rest(v);
-                        }
-                        s = block_sum(s);
-                        if (tid == 0) part[c] = s;
-                    }
-                }
-                __syncthreads();
-                double all = 0.0;
-                for (int c = 0; c < p.chunks; ++c) all += part[c];
-                const double goal = (double)uniforms[0] * all;
-                double before = 0.0;
-                int chunk = -1, last = -1;
-                for (int c = 0; c < p.chunks; ++c) {
-                    if (part[c] > 0.0) last = c;
-                    if (before + part[c] > goal) {
-                        chunk = c;
+        __syncthreads();
+        have = refs[0] == refs[0];
+        if (!drafted && !greedy && have) {
+            for (int j = tid; j < k; j += kThreads) {
+                const int x = ctok[j];
+                int first = j;
+                for (int i = 0; i < j; ++i)
+                    if (ctok[i] == x) {
+                        first = i;
                         break;
                     }
-                    before += part[c];
+                cfirst[j] = first;
+                cw[j] = x < 0 || first != j ? 0.0 : weight(j == tid ? cl : logit<KIND>(lrow, x), refs[0], c);
+            }
+            __syncthreads();
+        }
+    };
+    // r of token v. Without draft logits up to a factor, and so with them until a child is refused.
+    auto rest = [&](float l, float d) -> double {
+        const double w = weight(l, refs[0], c);
+        if (refused == 0) return w;
+        const double q = weight(d, refs[1], c) / whole[1];
+        double r = w / whole[0];
+        for (int i = 0; i < refused; ++i) {
+            r -= q;
+            r = (r > 0.0 ? r : 0.0) * cw[i];
+        }
+        return r;
+    };
+    // Children's weights (without draft logits): all that r still has, `but` one of them.
+    auto child_mass = [&](int k, int but) {
+        double m = 0.0;
+        for (int j = lane; j < k; j += 64) m += j == but ? 0.0 : cw[j];
+        return wave_sum(m);
+    };
+
+    if (count > 0) {
+        if (s == 0 && tid == 0) pout[0] = 0;
+        n = 1;
+        for (bool moved = true; moved;) {
+            moved = false;
+            enter();
+            const int k = snch;
+            if (!have) break;
+            double all = drafted || greedy ? 0.0 : whole[0] + child_mass(k, -1);
+            const bool qhave = drafted && refs[1] == refs[1];
+            for (int j = 0; j < k; ++j) {
+                const int x = ctok[j], i = cidx[j];
+                if (x < 0 || (drafted && !qhave)) continue;
+                bool take;
+                if (greedy) take = x == sbest;
+                else if (!drafted) take = (double)uniform[i] * all < cw[cfirst[j]];
+                else {
+                    const float l = logit<KIND>(lrow, x), d = logit<KIND>(drow, x);
+                    const double r = refused ? rest(l, d) : weight(l, refs[0], c) / whole[0];
+                    take = (double)uniform[i] * (weight(d, refs[1], c) / whole[1]) < r;
                 }
-                const bool beyond = chunk < 0;  // a uniform number of 1 or more, or none: the last token there is
-                if (beyond) chunk = last;
-                // a thread has kPer neighbouring tokens of the chunk
-                double w[kPer], mine = 0.0;
-                for (int j = 0; j < kPer; ++j) {
-                    const int v = chunk * kChunk + tid * kPer + j;
-                    w[j] = v < p.V ? rest(v) : 0.0;
-                    mine += w[j];
+                if (take) {
+                    if (s == 0 && tid == 0) {
+                        pout[n] = i;
+                        tout[n - 1] = x;
+                    }
+                    ++n;
+                    node = i;
+                    moved = true;
+                    break;
                 }
+                if (greedy) continue;
+                if (!drafted) {
+                    const int f = cfirst[j];
+                    const double left = whole[0] + child_mass(k, f);
+                    if (cw[f] > 0.0 && left > 0.0) {  // (where nothing remains r stays)
+                        all = left;
+                        __syncthreads();
+                        if (tid == 0) cw[f] = 0.0;
+                        __syncthreads();
+                    }
+                } else {
+                    // A pass for the mass that remains.
+                    __syncthreads();
+                    if (tid == 0) cw[refused] = 1.0;
+                    ++refused;
+                    __syncthreads();
+                    const int lo = s * p.len, end = lo + p.len < p.V ? lo + p.len : p.V;
+                    double m = 0.0;
+                    for (int v = lo + tid * kVec; v < end; v += kBlock) {
+                        float xl[kVec], xd[kVec];
+                        load_vec<KIND>(lrow, v, end, xl);
+                        load_vec<KIND>(drow, v, end, xd);
+#pragma unroll
+                        for (int e = 0; e < kVec; ++e) m += rest(xl[e], xd[e]);
+                    }
+                    const uint64_t w[4] = {word_of(block_sum(sh, m)), 0, 0, 0};
+                    uint64_t got[4];
+                    const bool ok = exchange(w, 1, got);
+                    if (wave == 0) {
+                        const double z = ok && lane < p.slices ? sum_of(got[0]) : 0.0;
+                        const double sum = wave_sum(z);
+                        if (sum > 0.0 && lane < p.slices) part[lane] = z * (1.0 / sum);  // of r, whose sum is 1
+                        if (lane == 0) cw[refused - 1] = sum > 0.0 ? 1.0 / sum : 0.0;
+                    }
+                    __syncthreads();
+                    if (!(cw[refused - 1] > 0.0)) --refused;  // nothing remains: r stays
+                }
+            }
+        }
+        if (s != 0) return;
+        int64_t next = -1;
+        if (have && greedy) next = sbest;
+        else if (have) {
+            const int k = snch;
+            double all = 0.0;
+            __syncthreads();
+            if (!drafted) {  // the children that were not refused, in their slices
+                for (int j = 0; j < k; ++j)
+                    if (tid == 0 && ctok[j] >= 0) part[ctok[j] / p.len] += cw[j];
+                __syncthreads();
+            }
+            for (int i = 0; i < p.slices; ++i) all += part[i];
+            const double goal = (double)uniform[0] * all;
+            double before = 0.0;
+            int slice = -1, last = 0;
+            for (int i = 0; i < p.slices; ++i) {
+                if (part[i] > 0.0) last = i;
+                if (before + part[i] > goal) {
+                    slice = i;
+                    break;
+                }
+                before += part[i];
+            }
+            const bool beyond = slice < 0;  // a uniform number that is not below 1: the last token there is
+            if (beyond) slice = last;
+            if (tid == 0) hit = 0x7fffffff, tail = -1;
+            const int lo = slice * p.len, end = lo + p.len < p.V ? lo + p.len : p.V;
+            for (int v0 = lo; v0 < end; v0 += kBlock) {
+                const int v = v0 + tid * kVec;
+                float xl[kVec], xd[kVec] = {};
+                load_vec<KIND>(lrow, v, end, xl);
+                if (refused) load_vec<KIND>(drow, v, end, xd);
+                double w[kVec], mine = 0.0;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) w[e] = rest(xl[e], xd[e]);
+                if (!drafted)
+                    for (int j = 0; j < k; ++j) {
+                        const int t = ctok[j] - v;
+                        if ((unsigned)t < (unsigned)kVec)
+#pragma unroll
+                            for (int e = 0; e < kVec; ++e) w[e] = e == t ? cw[cfirst[j]] : w[e];
+                    }
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) mine += w[e];
                 double run = mine;
+#pragma unroll
                 for (int o = 1; o < 64; o <<= 1) {
                     const double t = __shfl_up(run, o);
                     if (lane >= o) run += t;
                 }
                 __syncthreads();
-                if (lane == 63) red[wave] = run;
-                if (tid == 0) found = 0x7fffffff, fat[1] = -1;
+                if (lane == 63) sh.red[0][wave] = run;
                 __syncthreads();
-                for (int i = 0; i < wave; ++i) run += red[i];
+                double block = 0.0;
+                for (int i = 0; i < kWaves; ++i) {
+                    if (i < wave) run += sh.red[0][i];
+                    block += sh.red[0][i];
+                }
                 run = before + run - mine;
-                int hit = 0x7fffffff, tail = -1;
-                for (int j = 0; j < kPer; ++j) {
-                    run += w[j];
-                    if (w[j] > 0.0) {
-                        tail = chunk * kChunk + tid * kPer + j;
-                        if (!beyond && run > goal && hit == 0x7fffffff) hit = tail;
+                int mhit = 0x7fffffff, mtail = -1;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    run += w[e];
+                    if (w[e] > 0.0) {
+                        mtail = v + e;
+                        if (!beyond && run > goal && mhit == 0x7fffffff) mhit = v + e;
                     }
                 }
-                atomicMin(&found, hit);
-                atomicMax(&fat[1], tail);
+                if (mhit != 0x7fffffff) atomicMin(&hit, mhit);
+                if (mtail >= 0) atomicMax(&tail, mtail);
+                before += block;
                 __syncthreads();
-                next = found == 0x7fffffff ? fat[1] : found;
+                if (hit != 0x7fffffff) break;
             }
+            next = hit != 0x7fffffff ? hit : tail;
         }
         if (tid == 0) tout[n - 1] = next;
     }
+    if (s != 0) return;
     for (int i = n + tid; i < p.T; i += kThreads) {
         tout[i] = -1;
         pout[i] = -1;
@@ -373,11 +660,35 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p) {
     if (tid == 0) p.counts_out[b] = n;
 }
 
+struct Plan {
+    int slices, len, first;
+    size_t words_at, ticket_at, bytes;  // in the workspace
+};
+
+// Slices: enough workgroups to fill the chip, each with at least a step of logits. The first launch takes node 0, and as many more
+// as cost it about what an exchange takes (3 us, 4 million logits).
+static Plan plan_of(int64_t B, int64_t T, int64_t V, bool draft) {
+    Plan p{};
+    int64_t s = 1024 / B;
+    const int64_t most = ceil_div(V, kBlock);
+    s = s < 1 ? 1 : s > kMaxSlices ? kMaxSlices : s;
+    s = s < most ? s : most;
+    p.len = (int)(ceil_div(ceil_div(V, s), kVec) * kVec);
+    p.slices = (int)ceil_div(V, p.len);
+    const int64_t f = (4 << 20) / (B * V * (draft ? 2 : 1));
+    p.first = (int)(f < 1 ? 1 : f < T ? f : T);
+    p.words_at = (size_t)B * p.first * p.slices * sizeof(Part);
+    p.ticket_at = p.words_at + (size_t)B * 2 * p.slices * 4 * sizeof(uint64_t);
+    p.bytes = p.ticket_at + 16;
+    return p;
+}
+
 template <int KIND>
 static void launch(const Params& p, hipStream_t st) {
-    const int64_t rows = (int64_t)p.B * p.T * (p.draft ? 2 : 1);
-    hipLaunchKernelGGL(stats_kernel<KIND>, dim3((unsigned)(rows * p.chunks)), dim3(kThreads), 0, st, p);
-    hipLaunchKernelGGL(walk_kernel<KIND>, dim3(p.B), dim3(kThreads), 0, st, p);
+    hipLaunchKernelGGL(first_kernel<KIND>, dim3((unsigned)(p.B * p.first * p.slices)), dim3(kThreads), 0, st, p);
+    // Without an exchange to come one workgroup a row walks.
+    const int per_row = p.draft || p.first < p.T ? p.slices : 1;
+    hipLaunchKernelGGL(walk_kernel<KIND>, dim3((unsigned)(p.B * per_row)), dim3(kThreads), 0, st, p, per_row);
 }
 
 }  // namespace verify
@@ -387,7 +698,7 @@ using namespace mx;
 
 extern "C" size_t mx_verify_draft_workspace_bytes(int32_t B, int32_t T, int32_t V, int32_t draft) {
     if (B <= 0 || T <= 0 || V <= 0) return 0;
-    return (size_t)B * T * (draft ? 2 : 1) * ceil_div(V, verify::kChunk) * sizeof(verify::Stat);
+    return verify::plan_of(B, T, V, draft != 0).bytes;
 }
 
 extern "C" int mx_verify_draft(const void* logits, int64_t l_sb, int64_t l_st, const void* draft_logits, int64_t d_sb,
@@ -407,11 +718,8 @@ extern "C" int mx_verify_draft(const void* logits, int64_t l_sb, int64_t l_st, c
     if (l_sb < 0 || l_st < 0 || d_sb < 0 || d_st < 0 || t_sb < 0 || p_sb < 0 || u_sb < 0 || temp_sb < 0)
         return fail(MX_ERR_INVALID, "%s: strides must be >= 0", what);
     if (T > verify::kMaxNodes) return fail(MX_ERR_UNSUPPORTED, "%s: more than %d nodes", what, verify::kMaxNodes);
-    if (V > verify::kMaxChunks * verify::kChunk)
-        return fail(MX_ERR_UNSUPPORTED, "%s: more than %d logits", what, verify::kMaxChunks * verify::kChunk);
-    const int chunks = (int)ceil_div(V, verify::kChunk);
-    if ((double)B * T * 2 * chunks * verify::kThreads > 4.0e9)
-        return fail(MX_ERR_UNSUPPORTED, "%s: more logits than one launch holds", what);
+    if (V > verify::kMaxVocab) return fail(MX_ERR_UNSUPPORTED, "%s: more than %d logits", what, verify::kMaxVocab);
+    if (B > (1 << 20)) return fail(MX_ERR_UNSUPPORTED, "%s: more than %d rows", what, 1 << 20);
     const size_t need = mx_verify_draft_workspace_bytes(B, T, V, draft_logits != nullptr);
     if (!workspace || workspace_bytes < need)
         return fail(MX_ERR_WORKSPACE, "%s: workspace needs %zu bytes, got %zu", what, need, workspace ? workspace_bytes : 0);
@@ -421,8 +729,13 @@ extern "C" int mx_verify_draft(const void* logits, int64_t l_sb, int64_t l_st, c
     p.draft = draft_logits, p.d_sb = d_sb, p.d_st = d_st;
     p.tokens = tokens, p.t_sb = t_sb, p.parents = parents, p.p_sb = p_sb, p.counts = counts;
     p.uniforms = uniforms, p.u_sb = u_sb, p.temps = temperatures, p.temp_sb = temp_sb;
-    p.B = B, p.T = T, p.V = V, p.chunks = chunks;
-    p.stats = static_cast<verify::Stat*>(workspace);
+    p.B = B, p.T = T, p.V = V;
+    const verify::Plan pl = verify::plan_of(B, T, V, draft_logits != nullptr);
+    p.slices = pl.slices, p.len = pl.len, p.first = pl.first;
+    char* ws = static_cast<char*>(workspace);
+    p.parts = reinterpret_cast<verify::Part*>(ws);
+    p.words = reinterpret_cast<uint64_t*>(ws + pl.words_at);
+    p.ticket = reinterpret_cast<int*>(ws + pl.ticket_at);
     p.tokens_out = tokens_out, p.counts_out = counts_out, p.path_out = path_out;
     hipStream_t st = as_stream(stream);
     if (flags & MX_LOGITS_FP32) verify::launch<2>(p, st);
