@@ -33,6 +33,7 @@ constexpr int kVec = 8;                    // neighbouring logits per thread
 constexpr int kBlock = kThreads * kVec;    // logits per step of a workgroup
 constexpr int kMaxSlices = 64;             // one lane of a wave each
 constexpr int kMaxNodes = 1024;
+constexpr int kFill = 512;  // workgroups
 constexpr int kMaxVocab = 1 << 22;
 constexpr int kMaxPolls = 1 << 23;         // seconds: a wait that long means a broken launch; the row then ends with -1
 
@@ -80,24 +81,48 @@ template <int KIND>
 __device__ __forceinline__ const void* row_at(const void* base, int64_t off) {
     return static_cast<const char*>(base) + off * (KIND == 2 ? 4 : 2);
 }
-// Logits v .. v + 7 below `end` (-inf from there on); rows begin at any element.
-template <int KIND>
-__device__ __forceinline__ void load_vec(const void* row, int v, int end, float (&x)[kVec]) {
-    if (v + kVec <= end) {
-        if constexpr (KIND == 2) {
-            __builtin_memcpy(x, static_cast<const float*>(row) + v, sizeof x);
-        } else {
-            uint16_t h[kVec];
-            __builtin_memcpy(h, static_cast<const uint16_t*>(row) + v, sizeof h);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i)
-                x[i] = KIND == 0 ? (float)__builtin_bit_cast(_Float16, h[i]) : __builtin_bit_cast(float, (uint32_t)h[i] << 16);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) x[i] = v + i < end ? logit<KIND>(row, v + i) : -__builtin_huge_valf();
+// A vector of a slice [lo, end) on the way: logits v + [0, 8). The load is unconditional, so that it can stand ahead of the
+// work on the one before it: one that would pass the end is moved back, and take() drops what another thread has.
+// (Rows begin at any element: the loads may be unaligned.)
+template <int KIND, bool SMALL>
+struct Ahead {
+    typedef uint32_t raw __attribute__((ext_vector_type(KIND == 2 ? 8 : 4)));
+    raw x;
+    __device__ __forceinline__ static int at(int v, int end) {
+        const int last = SMALL ? 0 : end - kVec;
+        return v < last ? v : last;
     }
-}
+    __device__ __forceinline__ void load(const void* row, int v, int end) {
+        constexpr int S = KIND == 2 ? 4 : 2;
+        if constexpr (!SMALL) {
+            __builtin_memcpy(&x, static_cast<const char*>(row) + (int64_t)at(v, end) * S, kVec * S);
+        } else {  // a vocabulary of less than a vector
+            x = raw{};
+#pragma unroll
+            for (int e = 0; e < kVec; ++e)
+                if (e < end) {
+                    if constexpr (KIND == 2) x[e] = static_cast<const uint32_t*>(row)[e];
+                    else x[e / 2] |= (uint32_t)static_cast<const uint16_t*>(row)[e] << 16 * (e % 2);
+                }
+        }
+    }
+    // The logits as numbers, -inf where the slice has ended or another thread has the logit; returns the first's index.
+    __device__ __forceinline__ int take(int v, int end, float (&out)[kVec]) const {
+        const int from = at(v, end);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+            float f;
+            const uint32_t word = x[KIND == 2 ? e : e / 2];  // (bit_cast of a vector's element itself takes the first one)
+            if constexpr (KIND == 2) f = __builtin_bit_cast(float, word);
+            else {
+                const uint16_t h = (uint16_t)(word >> 16 * (e % 2));
+                f = KIND == 0 ? (float)__builtin_bit_cast(_Float16, h) : __builtin_bit_cast(float, (uint32_t)h << 16);
+            }
+            out[e] = from + e >= v && from + e < end ? f : -__builtin_huge_valf();
+        }
+        return from;
+    }
+};
 
 __device__ __forceinline__ int count_of(const Params& p, int b) {
     const int c = p.counts ? p.counts[b] : p.T;
@@ -144,30 +169,51 @@ __device__ __forceinline__ double weight(float l, float ref, double c) {
     return l == -__builtin_huge_valf() ? 0.0 : exp2_64(((double)l - (double)ref) * c);
 }
 
+// The same for whole slices, from a table of 2^(k / 64) in LDS: 2^t = 2^(n / 64) 2^(f / 64), |f| <= 1/2, five terms of the
+// series (the next one is below 4e-17). 15 instead of 23 fp64 instructions per logit.
+struct Exp {
+    const double* table;
+    __device__ __forceinline__ static void fill(double* table) {
+        if (threadIdx.x < 64) table[threadIdx.x] = exp2_64(threadIdx.x / 64.0);
+    }
+    __device__ __forceinline__ double operator()(float l, float ref, double c64) const {
+        const double t = fmax(((double)l - (double)ref) * c64, -128000.0);  // (l -inf: 2^-2000, which is 0)
+        const double big = t + 6755399441055744.0;                         // 1.5 * 2^52: its low bits are rint(t)
+        const double f = t - (big - 6755399441055744.0);
+        const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, big);
+        double y = 1.2417843701716923e-12;             // (ln(2) / 64)^5 / 5!
+        y = __builtin_fma(y, f, 5.732851688640402e-10);
+        y = __builtin_fma(y, f, 2.1173137155464774e-07);
+        y = __builtin_fma(y, f, 5.864904955056169e-05);
+        y = __builtin_fma(y, f, 0.010830424696249145);
+        y = __builtin_fma(y, f, 1.0);
+        return ldexp(y * table[n & 63], n >> 6);
+    }
+};
+
 // A thread's running sum of 2^((l - ref) c). ref is the largest logit of the first it met; 64 bits hold the sum until
 // a logit lies 2^900 above it.
 struct Sum {
     double sum = 0.0;
     float ref = -__builtin_huge_valf();
     bool bad = false;
-    __device__ __forceinline__ void add(const float (&x)[kVec], double c) {
+    __device__ __forceinline__ void add(const float (&x)[kVec], double c, const Exp& ex) {
         float top = x[0];
-        bad |= x[0] != x[0];
 #pragma unroll
-        for (int i = 1; i < kVec; ++i) {
-            top = fmaxf(top, x[i]);
-            bad |= x[i] != x[i];
-        }
+        for (int i = 1; i < kVec; ++i) top = fmaxf(top, x[i]);
         if (top > ref && !(((double)top - (double)ref) * c <= 900.0)) {  // (ref -inf: the difference is inf, or NaN at rate 0)
             sum *= ref == -__builtin_huge_valf() ? 0.0 : exp2_64(((double)ref - (double)top) * c);
             ref = top;
         }
+        double part = 0.0;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) sum += weight(x[i], ref, c);
+        for (int i = 0; i < kVec; ++i) part += ex(x[i], ref, c * 64.0);
+        sum += part;
     }
 };
 
 struct Shared {
+    double table[64];
     double red[2][kWaves];
     float redf[2][kWaves];
     int redi[kWaves];
@@ -217,7 +263,7 @@ struct Children {
 };
 
 // One pass over slice s of a node: the softmax's sums, or a greedy row's largest logit.
-template <int KIND>
+template <int KIND, bool SMALL>
 __device__ __forceinline__ Part pass(const Params& p, Shared& sh, const void* lrow, const void* drow, int s, double c,
                                      bool greedy, const Children& ch) {
     const int tid = threadIdx.x, lo = s * p.len, end = lo + p.len < p.V ? lo + p.len : p.V;
@@ -226,13 +272,17 @@ __device__ __forceinline__ Part pass(const Params& p, Shared& sh, const void* lr
         float top = -__builtin_huge_valf();
         int at = 0x7fffffff;
         bool bad = false;
+        Ahead<KIND, SMALL> a;
+        a.load(lrow, lo + tid * kVec, end);
+#pragma unroll 1
         for (int v = lo + tid * kVec; v < end; v += kBlock) {
             float x[kVec];
-            load_vec<KIND>(lrow, v, end, x);
+            const int from = a.take(v, end, x);
+            a.load(lrow, v + kBlock, end);
 #pragma unroll
             for (int i = 0; i < kVec; ++i) {
                 bad |= x[i] != x[i];
-                if (x[i] > top) top = x[i], at = v + i;
+                if (x[i] > top) top = x[i], at = from + i;
             }
         }
 #pragma unroll
@@ -256,26 +306,32 @@ __device__ __forceinline__ Part pass(const Params& p, Shared& sh, const void* lr
         out.at = at;
         return out;
     }
+    const Exp ex{sh.table};
     Sum a, d;
+    Ahead<KIND, SMALL> al, ad;
+    al.load(lrow, lo + tid * kVec, end);
+    if (drow) ad.load(drow, lo + tid * kVec, end);
+#pragma unroll 1
     for (int v = lo + tid * kVec; v < end; v += kBlock) {
         float x[kVec];
-        load_vec<KIND>(lrow, v, end, x);
+        const int from = al.take(v, end, x);
+        al.load(lrow, v + kBlock, end);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) a.bad |= x[i] != x[i] || x[i] == __builtin_huge_valf();
-        if (drow) {
-            float y[kVec];
-            load_vec<KIND>(drow, v, end, y);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) d.bad |= y[i] == __builtin_huge_valf();
-            d.add(y, c);
-        }
+        for (int i = 0; i < kVec; ++i) a.bad |= !(x[i] < __builtin_huge_valf());
         for (int j = 0; j < ch.n; ++j) {
-            const int t = ch.token[j] - v;
+            const int t = ch.token[j] - from;
             if ((unsigned)t < (unsigned)kVec)
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) x[i] = i == t ? -__builtin_huge_valf() : x[i];
         }
-        a.add(x, c);
+        a.add(x, c, ex);
+        if (drow) {
+            ad.take(v, end, x);
+            ad.load(drow, v + kBlock, end);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) d.bad |= !(x[i] < __builtin_huge_valf());
+            d.add(x, c, ex);
+        }
     }
     join(sh, 0, a, c, out.sum[0], out.ref[0]);
     if (drow) join(sh, 1, d, c, out.sum[1], out.ref[1]);
@@ -303,7 +359,7 @@ __device__ __forceinline__ int children_of(P parent, T token, int node, int coun
 __device__ __forceinline__ int token_in(int64_t x, int V) { return x >= 0 && x < V ? (int)x : -1; }
 
 // The nodes below `first` of every row, a workgroup per slice; clears what the walk's exchange begins with.
-template <int KIND>
+template <int KIND, bool SMALL>
 __global__ __launch_bounds__(kThreads) void first_kernel(Params p) {
     __shared__ Shared sh;
     __shared__ int tok[kMaxNodes];
@@ -313,6 +369,8 @@ __global__ __launch_bounds__(kThreads) void first_kernel(Params p) {
     if (node == 0 && threadIdx.x < 8)
         p.words[(((int64_t)b * 2 + threadIdx.x / 4) * p.slices + s) * 4 + threadIdx.x % 4] = 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
+    Exp::fill(sh.table);
+    __syncthreads();
     const int count = count_of(p, b);
     if (node >= count) return;
     const double c = rate_of(p, b);
@@ -328,13 +386,13 @@ __global__ __launch_bounds__(kThreads) void first_kernel(Params p) {
         __syncthreads();
     }
     const Children ch{!p.draft && !greedy ? nch : 0, tok};
-    const Part out = pass<KIND>(p, sh, row_at<KIND>(p.logits, b * p.l_sb + node * p.l_st),
+    const Part out = pass<KIND, SMALL>(p, sh, row_at<KIND>(p.logits, b * p.l_sb + node * p.l_st),
                                 p.draft && !greedy ? row_at<KIND>(p.draft, b * p.d_sb + node * p.d_st) : nullptr, s, c,
                                 greedy, ch);
     if (threadIdx.x == 0) p.parts[((int64_t)b * p.first + node) * p.slices + s] = out;
 }
 
-template <int KIND>
+template <int KIND, bool SMALL>
 __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
     __shared__ Shared sh;
     __shared__ int parent[kMaxNodes], token[kMaxNodes];
@@ -342,12 +400,13 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
     __shared__ int cidx[kMaxNodes], ctok[kMaxNodes], cfirst[kMaxNodes];  // children; the first with the same token
     __shared__ double cw[kMaxNodes];     // without draft logits: weight, 0 once refused; with: scales of the refusals
     __shared__ double part[kMaxSlices];  // r's weight in each slice
-    __shared__ double whole[2];
+    __shared__ double whole[2], per_whole[2];
     __shared__ float refs[2];
     __shared__ int sbest, snch, sid, hit, tail;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float inf = __builtin_huge_valf();
-    if (tid == 0) sid = atomicAdd(p.ticket, 1);
+    if (tid == 0) sid = per_row > 1 ? atomicAdd(p.ticket, 1) : (int)blockIdx.x;
+    Exp::fill(sh.table);
     __syncthreads();
     const int b = sid / per_row, s = sid % per_row;
     const int count = count_of(p, b);
@@ -357,7 +416,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
     const bool greedy = !(temp > 0.0f);
     const double c = rate_of(p, b);
     const bool drafted = p.draft && !greedy;
-    for (int i = tid; i < count; i += kThreads) {
+    for (int i = tid; i < p.T; i += kThreads) {  // (not `count`: no need to wait for it)
         const int up = p.parents[b * p.p_sb + i];
         parent[i] = up < i ? up : -1;
         token[i] = token_in(p.tokens[b * p.t_sb + i], p.V);
@@ -377,13 +436,20 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
         bool ok = true;
         if (wave == 0) {
             const int from = lane < p.slices ? lane : 0;
-            for (int i = 0; i < n; ++i) {
-                int polls = 0;
-                do {
-                    all[i] = __hip_atomic_load(base + from * 4 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    if (++polls > kMaxPolls) ok = false;
-                    else if ((all[i] & 0xff) != tag) __builtin_amdgcn_s_sleep(1);
-                } while ((all[i] & 0xff) != tag && ok);
+            for (int polls = 0;; ++polls) {
+                bool there = true;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < n) {
+                        all[i] = __hip_atomic_load(base + from * 4 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        there &= (all[i] & 0xff) == tag;
+                    }
+                if (__builtin_amdgcn_ballot_w64(!there) == 0) break;
+                if (polls > kMaxPolls) {
+                    ok = false;
+                    break;
+                }
+                __builtin_amdgcn_s_sleep(1);
             }
         }
         return ok;
@@ -419,7 +485,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
             if (wave == 0 && lane < p.slices) mine = p.parts[((int64_t)b * p.first + node) * p.slices + lane];
         } else {
             const Children ch{!drafted && !greedy ? k : 0, ctok};
-            mine = pass<KIND>(p, sh, lrow, drow, s, c, greedy, ch);
+            mine = pass<KIND, SMALL>(p, sh, lrow, drow, s, c, greedy, ch);
             uint64_t w[4] = {greedy ? (uint64_t)(uint32_t)mine.at << 8 : word_of(mine.sum[0]), ref_word(mine.ref[0]),
                              word_of(mine.sum[1]), ref_word(mine.ref[1])}, all[4];
             ok = exchange(w, drafted ? 4 : 2, all);
@@ -463,6 +529,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
                 if (lane == 0) {
                     refs[which] = bad ? __builtin_nanf("") : top;
                     whole[which] = z;
+                    per_whole[which] = 1.0 / z;
                     if (which == 0) sbest = at;
                 }
             }
@@ -485,16 +552,27 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
         }
     };
     // r of token v. Without draft logits up to a factor, and so with them until a child is refused.
-    auto rest = [&](float l, float d) -> double {
-        const double w = weight(l, refs[0], c);
-        if (refused == 0) return w;
-        const double q = weight(d, refs[1], c) / whole[1];
-        double r = w / whole[0];
-        for (int i = 0; i < refused; ++i) {
-            r -= q;
-            r = (r > 0.0 ? r : 0.0) * cw[i];
+    const Exp ex{sh.table};
+    auto rest = [&](auto& l, auto& d, auto& r) {
+        constexpr int N = sizeof(r) / sizeof(r[0]);
+#pragma unroll
+        for (int e = 0; e < N; ++e) r[e] = ex(l[e], refs[0], c * 64.0);
+        if (refused == 0) return;
+        double q[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            r[e] *= per_whole[0];
+            q[e] = ex(d[e], refs[1], c * 64.0) * per_whole[1];
         }
-        return r;
+#pragma unroll 1
+        for (int i = 0; i < refused; ++i) {
+            const double f = cw[i];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                r[e] -= q[e];
+                r[e] = (r[e] > 0.0 ? r[e] : 0.0) * f;
+            }
+        }
     };
     // Children's weights (without draft logits): all that r still has, `but` one of them.
     auto child_mass = [&](int k, int but) {
@@ -520,9 +598,11 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
                 if (greedy) take = x == sbest;
                 else if (!drafted) take = (double)uniform[i] * all < cw[cfirst[j]];
                 else {
-                    const float l = logit<KIND>(lrow, x), d = logit<KIND>(drow, x);
-                    const double r = refused ? rest(l, d) : weight(l, refs[0], c) / whole[0];
-                    take = (double)uniform[i] * (weight(d, refs[1], c) / whole[1]) < r;
+                    const float l[1] = {logit<KIND>(lrow, x)}, d[1] = {logit<KIND>(drow, x)};
+                    double r[1];
+                    rest(l, d, r);
+                    if (!refused) r[0] *= per_whole[0];
+                    take = (double)uniform[i] * (ex(d[0], refs[1], c * 64.0) * per_whole[1]) < r[0];
                 }
                 if (take) {
                     if (s == 0 && tid == 0) {
@@ -552,12 +632,20 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
                     __syncthreads();
                     const int lo = s * p.len, end = lo + p.len < p.V ? lo + p.len : p.V;
                     double m = 0.0;
+                    Ahead<KIND, SMALL> al, ad;
+                    al.load(lrow, lo + tid * kVec, end);
+                    ad.load(drow, lo + tid * kVec, end);
+#pragma unroll 1
                     for (int v = lo + tid * kVec; v < end; v += kBlock) {
                         float xl[kVec], xd[kVec];
-                        load_vec<KIND>(lrow, v, end, xl);
-                        load_vec<KIND>(drow, v, end, xd);
+                        double r[kVec];
+                        al.take(v, end, xl);
+                        ad.take(v, end, xd);
+                        al.load(lrow, v + kBlock, end);
+                        ad.load(drow, v + kBlock, end);
+                        rest(xl, xd, r);
 #pragma unroll
-                        for (int e = 0; e < kVec; ++e) m += rest(xl[e], xd[e]);
+                        for (int e = 0; e < kVec; ++e) m += r[e];
                     }
                     const uint64_t w[4] = {word_of(block_sum(sh, m)), 0, 0, 0};
                     uint64_t got[4];
@@ -601,14 +689,18 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
             if (beyond) slice = last;
             if (tid == 0) hit = 0x7fffffff, tail = -1;
             const int lo = slice * p.len, end = lo + p.len < p.V ? lo + p.len : p.V;
+            Ahead<KIND, SMALL> al, ad;
+            al.load(lrow, lo + tid * kVec, end);
+            if (refused) ad.load(drow, lo + tid * kVec, end);
+#pragma unroll 1
             for (int v0 = lo; v0 < end; v0 += kBlock) {
-                const int v = v0 + tid * kVec;
                 float xl[kVec], xd[kVec] = {};
-                load_vec<KIND>(lrow, v, end, xl);
-                if (refused) load_vec<KIND>(drow, v, end, xd);
+                const int v = al.take(v0 + tid * kVec, end, xl);
+                if (refused) ad.take(v0 + tid * kVec, end, xd);
+                al.load(lrow, v0 + kBlock + tid * kVec, end);
+                if (refused) ad.load(drow, v0 + kBlock + tid * kVec, end);
                 double w[kVec], mine = 0.0;
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) w[e] = rest(xl[e], xd[e]);
+                rest(xl, xd, w);
                 if (!drafted)
                     for (int j = 0; j < k; ++j) {
                         const int t = ctok[j] - v;
@@ -669,7 +761,7 @@ struct Plan {
 // as cost it about what an exchange takes (3 us, 4 million logits).
 static Plan plan_of(int64_t B, int64_t T, int64_t V, bool draft) {
     Plan p{};
-    int64_t s = 1024 / B;
+    int64_t s = kFill / B;
     const int64_t most = ceil_div(V, kBlock);
     s = s < 1 ? 1 : s > kMaxSlices ? kMaxSlices : s;
     s = s < most ? s : most;
@@ -683,12 +775,17 @@ static Plan plan_of(int64_t B, int64_t T, int64_t V, bool draft) {
     return p;
 }
 
-template <int KIND>
+template <int KIND, bool SMALL>
 static void launch(const Params& p, hipStream_t st) {
-    hipLaunchKernelGGL(first_kernel<KIND>, dim3((unsigned)(p.B * p.first * p.slices)), dim3(kThreads), 0, st, p);
+    hipLaunchKernelGGL((first_kernel<KIND, SMALL>), dim3((unsigned)(p.B * p.first * p.slices)), dim3(kThreads), 0, st, p);
     // Without an exchange to come one workgroup a row walks.
     const int per_row = p.draft || p.first < p.T ? p.slices : 1;
-    hipLaunchKernelGGL(walk_kernel<KIND>, dim3((unsigned)(p.B * per_row)), dim3(kThreads), 0, st, p, per_row);
+    hipLaunchKernelGGL((walk_kernel<KIND, SMALL>), dim3((unsigned)(p.B * per_row)), dim3(kThreads), 0, st, p, per_row);
+}
+template <int KIND>
+static void launch_any(const Params& p, hipStream_t st) {
+    if (p.V < kVec) launch<KIND, true>(p, st);
+    else launch<KIND, false>(p, st);
 }
 
 }  // namespace verify
@@ -738,8 +835,8 @@ extern "C" int mx_verify_draft(const void* logits, int64_t l_sb, int64_t l_st, c
     p.ticket = reinterpret_cast<int*>(ws + pl.ticket_at);
     p.tokens_out = tokens_out, p.counts_out = counts_out, p.path_out = path_out;
     hipStream_t st = as_stream(stream);
-    if (flags & MX_LOGITS_FP32) verify::launch<2>(p, st);
-    else if (flags & MX_PA_BF16) verify::launch<1>(p, st);
-    else verify::launch<0>(p, st);
+    if (flags & MX_LOGITS_FP32) verify::launch_any<2>(p, st);
+    else if (flags & MX_PA_BF16) verify::launch_any<1>(p, st);
+    else verify::launch_any<0>(p, st);
     return check_launch(what);
 }
