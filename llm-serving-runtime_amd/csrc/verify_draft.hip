@@ -111,15 +111,14 @@ struct Ahead {
         const int from = at(v, end);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-            float f;
             const uint32_t word = x[KIND == 2 ? e : e / 2];  // (bit_cast of a vector's element itself takes the first one)
-            if constexpr (KIND == 2) f = __builtin_bit_cast(float, word);
-            else {
-                const uint16_t h = (uint16_t)(word >> 16 * (e % 2));
-                f = KIND == 0 ? (float)__builtin_bit_cast(_Float16, h) : __builtin_bit_cast(float, (uint32_t)h << 16);
-            }
-            out[e] = from + e >= v && from + e < end ? f : -__builtin_huge_valf();
+            if constexpr (KIND == 2) out[e] = __builtin_bit_cast(float, word);
+            else if constexpr (KIND == 1) out[e] = __builtin_bit_cast(float, e % 2 ? word & 0xffff0000u : word << 16);
+            else out[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(word >> 16 * (e % 2)));
         }
+        if (__builtin_amdgcn_ballot_w64(v + kVec > end))
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) out[e] = from + e >= v && from + e < end ? out[e] : -__builtin_huge_valf();
         return from;
     }
 };
@@ -169,25 +168,26 @@ __device__ __forceinline__ double weight(float l, float ref, double c) {
     return l == -__builtin_huge_valf() ? 0.0 : exp2_64(((double)l - (double)ref) * c);
 }
 
-// The same for whole slices, from a table of 2^(k / 64) in LDS: 2^t = 2^(n / 64) 2^(f / 64), |f| <= 1/2, five terms of the
-// series (the next one is below 4e-17). 15 instead of 23 fp64 instructions per logit.
+// The same for whole slices, from a table of 2^(k / 128) in LDS: 2^t = 2^(n / 128) 2^(f / 128), |f| <= 1/2, four terms of the
+// series (the next one is below 2e-15). All instructions cost alike here, fp64 or not: about 19 a logit.
+constexpr int kTable = 128;  // 2^7
 struct Exp {
     const double* table;
     __device__ __forceinline__ static void fill(double* table) {
-        if (threadIdx.x < 64) table[threadIdx.x] = exp2_64(threadIdx.x / 64.0);
+        if (threadIdx.x < kTable) table[threadIdx.x] = exp2_64((double)threadIdx.x / kTable);
     }
-    __device__ __forceinline__ double operator()(float l, float ref, double c64) const {
-        const double t = fmax(((double)l - (double)ref) * c64, -128000.0);  // (l -inf: 2^-2000, which is 0)
-        const double big = t + 6755399441055744.0;                         // 1.5 * 2^52: its low bits are rint(t)
+    // of (l - ref) c, given c * kTable
+    __device__ __forceinline__ double operator()(float l, float ref, double ct) const {
+        const double t = fmax(((double)l - (double)ref) * ct, -2000.0 * kTable);  // (l -inf: 2^-2000, which is 0)
+        const double big = t + 6755399441055744.0;          // 1.5 * 2^52: its low bits are rint(t)
         const double f = t - (big - 6755399441055744.0);
         const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, big);
-        double y = 1.2417843701716923e-12;             // (ln(2) / 64)^5 / 5!
-        y = __builtin_fma(y, f, 5.732851688640402e-10);
-        y = __builtin_fma(y, f, 2.1173137155464774e-07);
-        y = __builtin_fma(y, f, 5.864904955056169e-05);
-        y = __builtin_fma(y, f, 0.010830424696249145);
+        double y = 3.583032305400251e-11;               // (ln(2) / 128)^4 / 4!
+        y = __builtin_fma(y, f, 2.6466421444330967e-08);
+        y = __builtin_fma(y, f, 1.4662262387640423e-05);
+        y = __builtin_fma(y, f, 0.0054152123481245725);
         y = __builtin_fma(y, f, 1.0);
-        return ldexp(y * table[n & 63], n >> 6);
+        return ldexp(y * table[n & (kTable - 1)], n >> 7);
     }
 };
 
@@ -196,24 +196,28 @@ struct Exp {
 struct Sum {
     double sum = 0.0;
     float ref = -__builtin_huge_valf();
-    bool bad = false;
+    bool bad = false;  // a NaN (an infinity shows in ref, or below)
     __device__ __forceinline__ void add(const float (&x)[kVec], double c, const Exp& ex) {
-        float top = x[0];
+        float top = fmaxf(x[0], x[1]);
 #pragma unroll
-        for (int i = 1; i < kVec; ++i) top = fmaxf(top, x[i]);
+        for (int i = 2; i < kVec; ++i) top = fmaxf(top, x[i]);
+        bad |= top == __builtin_huge_valf();
+#pragma unroll
+        for (int i = 0; i < kVec; i += 2) bad |= __builtin_isunordered(x[i], x[i + 1]);
         if (top > ref && !(((double)top - (double)ref) * c <= 900.0)) {  // (ref -inf: the difference is inf, or NaN at rate 0)
             sum *= ref == -__builtin_huge_valf() ? 0.0 : exp2_64(((double)ref - (double)top) * c);
             ref = top;
         }
+        const double ct = c * kTable;
         double part = 0.0;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) part += ex(x[i], ref, c * 64.0);
+        for (int i = 0; i < kVec; ++i) part += ex(x[i], ref, ct);
         sum += part;
     }
 };
 
 struct Shared {
-    double table[64];
+    double table[kTable];
     double red[2][kWaves];
     float redf[2][kWaves];
     int redi[kWaves];
@@ -316,8 +320,6 @@ __device__ __forceinline__ Part pass(const Params& p, Shared& sh, const void* lr
         float x[kVec];
         const int from = al.take(v, end, x);
         al.load(lrow, v + kBlock, end);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) a.bad |= !(x[i] < __builtin_huge_valf());
         for (int j = 0; j < ch.n; ++j) {
             const int t = ch.token[j] - from;
             if ((unsigned)t < (unsigned)kVec)
@@ -328,8 +330,6 @@ __device__ __forceinline__ Part pass(const Params& p, Shared& sh, const void* lr
         if (drow) {
             ad.take(v, end, x);
             ad.load(drow, v + kBlock, end);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) d.bad |= !(x[i] < __builtin_huge_valf());
             d.add(x, c, ex);
         }
     }
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
     __shared__ double part[kMaxSlices];  // r's weight in each slice
     __shared__ double whole[2], per_whole[2];
     __shared__ float refs[2];
-    __shared__ int sbest, snch, sid, hit, tail;
+    __shared__ int sbest, snch, sid, stail[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float inf = __builtin_huge_valf();
     if (tid == 0) sid = per_row > 1 ? atomicAdd(p.ticket, 1) : (int)blockIdx.x;
@@ -497,10 +497,14 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
             }
         }
         // Children's weights count with the slices' for the largest logit. (The first 256 are at hand.)
-        float ctop = cl;
+        // (One that is NaN counts as infinite: either way there is no distribution.)
+        float ctop = cl == cl ? cl : inf;
         if (!drafted && !greedy)
             for (int j = tid + kThreads; j < k; j += kThreads)
-                if (ctok[j] >= 0) ctop = fmaxf(ctop, logit<KIND>(lrow, ctok[j]));
+                if (ctok[j] >= 0) {
+                    const float l = logit<KIND>(lrow, ctok[j]);
+                    ctop = fmaxf(ctop, l == l ? l : inf);
+                }
         ctop = wave_max(ctop);
         __syncthreads();
         if (lane == 0) sh.redf[1][wave] = ctop;
@@ -556,13 +560,13 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
     auto rest = [&](auto& l, auto& d, auto& r) {
         constexpr int N = sizeof(r) / sizeof(r[0]);
 #pragma unroll
-        for (int e = 0; e < N; ++e) r[e] = ex(l[e], refs[0], c * 64.0);
+        for (int e = 0; e < N; ++e) r[e] = ex(l[e], refs[0], c * kTable);
         if (refused == 0) return;
         double q[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             r[e] *= per_whole[0];
-            q[e] = ex(d[e], refs[1], c * 64.0) * per_whole[1];
+            q[e] = ex(d[e], refs[1], c * kTable) * per_whole[1];
         }
 #pragma unroll 1
         for (int i = 0; i < refused; ++i) {
@@ -602,7 +606,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
                     double r[1];
                     rest(l, d, r);
                     if (!refused) r[0] *= per_whole[0];
-                    take = (double)uniform[i] * (ex(d[0], refs[1], c * 64.0) * per_whole[1]) < r[0];
+                    take = (double)uniform[i] * (ex(d[0], refs[1], c * kTable) * per_whole[1]) < r[0];
                 }
                 if (take) {
                     if (s == 0 && tid == 0) {
@@ -666,28 +670,30 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
         if (have && greedy) next = sbest;
         else if (have) {
             const int k = snch;
-            double all = 0.0;
+            double all;
+            int hit_at, tail_at;
             __syncthreads();
             if (!drafted) {  // the children that were not refused, in their slices
                 for (int j = 0; j < k; ++j)
                     if (tid == 0 && ctok[j] >= 0) part[ctok[j] / p.len] += cw[j];
                 __syncthreads();
             }
-            for (int i = 0; i < p.slices; ++i) all += part[i];
-            const double goal = (double)uniform[0] * all;
-            double before = 0.0;
-            int slice = -1, last = 0;
-            for (int i = 0; i < p.slices; ++i) {
-                if (part[i] > 0.0) last = i;
-                if (before + part[i] > goal) {
-                    slice = i;
-                    break;
-                }
-                before += part[i];
+            // Every wave finds the slice, a lane for each: the first whose running sum exceeds the goal.
+            const double mine_part = lane < p.slices ? part[lane] : 0.0;
+            double upto = mine_part;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const double t = __shfl_up(upto, o);
+                if (lane >= o) upto += t;
             }
-            const bool beyond = slice < 0;  // a uniform number that is not below 1: the last token there is
-            if (beyond) slice = last;
-            if (tid == 0) hit = 0x7fffffff, tail = -1;
+            all = __shfl(upto, 63);
+            const double goal = (double)uniform[0] * all;
+            const uint64_t above = __builtin_amdgcn_ballot_w64(upto > goal && mine_part > 0.0);
+            const uint64_t some = __builtin_amdgcn_ballot_w64(mine_part > 0.0);
+            const bool beyond = above == 0;  // a uniform number that is not below 1: the last token there is
+            const int slice = beyond ? (some ? 63 - __builtin_clzll(some) : 0) : __builtin_ctzll(above);
+            double before = __shfl(upto - mine_part, slice);
+            hit_at = tail_at = -1;
             const int lo = slice * p.len, end = lo + p.len < p.V ? lo + p.len : p.V;
             Ahead<KIND, SMALL> al, ad;
             al.load(lrow, lo + tid * kVec, end);
@@ -697,8 +703,10 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
                 float xl[kVec], xd[kVec] = {};
                 const int v = al.take(v0 + tid * kVec, end, xl);
                 if (refused) ad.take(v0 + tid * kVec, end, xd);
-                al.load(lrow, v0 + kBlock + tid * kVec, end);
-                if (refused) ad.load(drow, v0 + kBlock + tid * kVec, end);
+                if (v0 + kBlock < end) {
+                    al.load(lrow, v0 + kBlock + tid * kVec, end);
+                    if (refused) ad.load(drow, v0 + kBlock + tid * kVec, end);
+                }
                 double w[kVec], mine = 0.0;
                 rest(xl, xd, w);
                 if (!drafted)
@@ -725,22 +733,32 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
                     block += sh.red[0][i];
                 }
                 run = before + run - mine;
-                int mhit = 0x7fffffff, mtail = -1;
+                int mhit = -1, mtail = -1;
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
                     run += w[e];
                     if (w[e] > 0.0) {
                         mtail = v + e;
-                        if (!beyond && run > goal && mhit == 0x7fffffff) mhit = v + e;
+                        if (!beyond && run > goal && mhit < 0) mhit = v + e;
                     }
                 }
-                if (mhit != 0x7fffffff) atomicMin(&hit, mhit);
-                if (mtail >= 0) atomicMax(&tail, mtail);
+                // Threads are in the tokens' order: the first one with a hit, the last one with any weight.
+                const uint64_t hits = __builtin_amdgcn_ballot_w64(mhit >= 0), tails = __builtin_amdgcn_ballot_w64(mtail >= 0);
+                const int whit = hits ? __builtin_amdgcn_readlane(mhit, __builtin_ctzll(hits)) : -1;
+                const int wtail = tails ? __builtin_amdgcn_readlane(mtail, 63 - __builtin_clzll(tails)) : -1;
+                if (lane == 0) sh.redi[wave] = whit, stail[wave] = wtail;
                 before += block;
                 __syncthreads();
-                if (hit != 0x7fffffff) break;
+#pragma unroll
+                for (int i = kWaves - 1; i >= 0; --i) {
+                    if (sh.redi[i] >= 0) hit_at = sh.redi[i];
+                }
+#pragma unroll
+                for (int i = 0; i < kWaves; ++i)
+                    if (stail[i] >= 0) tail_at = stail[i];
+                if (hit_at >= 0) break;
             }
-            next = hit != 0x7fffffff ? hit : tail;
+            next = hit_at >= 0 ? hit_at : tail_at;
         }
         if (tid == 0) tout[n - 1] = next;
     }
