@@ -178,6 +178,13 @@ __device__ __forceinline__ int worker_of(int x, int total, int workers) {
     return (int)(((int64_t)(x + 1) * workers - 1) / total);
 }
 
+// 16 bytes per lane from memory to LDS, lane l's at `to` + 16 l (`to` the same in all lanes). As a builtin the load would be waited
+// for ahead of every later read of LDS, whatever that reads; so the caller waits (vmcnt) before the barrier that hands the
+// tile over. Nothing is written to a register.
+__device__ __forceinline__ void load_to_lds(const void* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "m0", "memory");
+}
+
 typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4v lds_s16x4;
 __device__ __forceinline__ s16x4v read_tr(const char* p) {
@@ -208,11 +215,11 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     constexpr int KC = D / 32;                // 32-dim steps of a score
     constexpr int DT = D / 16;                // 16-dim output tiles
     constexpr int CH = D / 8;                 // 16-byte chunks per token
-    constexpr int RPP = NT / CH;              // tokens per staging pass
-    constexpr int P = (kTok + RPP - 1) / RPP; // staging passes
+    constexpr int RPL = 64 / CH;              // tokens per load instruction of a wave (1 KiB)
+    constexpr int P = kTok / RPL / (RW * TW); // load instructions per wave and tile, of K and of V each
     constexpr int NTT = kTok / 16 / TW;       // 16-token tiles per wave
     constexpr int R = 16 * RT * RW;
-    static_assert(NTT % 2 == 0 && kTok % RPP == 0, "tile split");
+    static_assert(NTT % 2 == 0 && P * RPL * RW * TW == kTok, "tile split");
     __shared__ __attribute__((aligned(16))) _Float16 ks[2][kTok * D];
     __shared__ __attribute__((aligned(16))) _Float16 vs[2][kTok * D];
     __shared__ int bad_step[2];  // the last step whose tile has a token of a block outside the pool
@@ -237,8 +244,9 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     if (tid == 0) nf_step = 0;
     int step = 0;  // tiles staged so far, from 1: buffer step & 1
     const int bs = 1 << p.bs_shift;
-    const int c = tid % CH, row0 = tid / CH;  // staged chunk and first token
     const int range0 = lo;
+    const uint32_t ks_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&ks[0][0];
+    const uint32_t vs_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&vs[0][0];
 
     while (lo < hi) {
         const Row row = row_of(p, seg.b);
@@ -246,55 +254,72 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
         const int ntiles = (end + kTok - 1) / kTok;
         const int t0 = seg.tile, t1 = ntiles - t0 < hi - lo ? ntiles : t0 + (hi - lo);
         const int32_t* bt = p.bt + (int64_t)seg.b * p.bt_sb;
-        const _Float16* kb = p.k + (int64_t)seg.kvh * p.kv_shead + 8 * c;
-        const _Float16* vb = p.v + (int64_t)seg.kvh * p.kv_shead + 8 * c;
+        const _Float16* kb = p.k + (int64_t)seg.kvh * p.kv_shead;
+        const _Float16* vb = p.v + (int64_t)seg.kvh * p.kv_shead;
         const int last_tok = end - 1;
+        const int safe = row.ctx < end ? row.ctx > 0 ? row.ctx : 0 : end;  // tokens below it are context, and there
 
+        // Loads go from memory to LDS without a register: a lane's 16 bytes land at 16 times the lane behind the instruction's
+        // place, so the permutation of a token's chunks is in the addresses that the lanes read from.
         struct Ids {
             int id[P];
-        };
-        struct Stage {
-            u32x4v k[P], v[P];
         };
         auto ids_of = [&](int t) MX_INLINE {
             Ids s;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                int tok = t * kTok + row0 + i * RPP;
-                tok = tok < last_tok ? tok : last_tok;  // past the end: the last token's block
+                int tok = t * kTok + (wave * P + i) * RPL + lane / CH;
+                tok = tok < last_tok ? tok : last_tok;  // past the end: the last token again
                 s.id[i] = bt[tok >> p.bs_shift];
             }
             return s;
         };
-        auto load = [&](int t, const Ids ids) MX_INLINE {
-            Stage s;
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const int tok = t * kTok + row0 + i * RPP;
-                const int id = (unsigned)ids.id[i] < (unsigned)p.num_blocks ? ids.id[i] : 0;
-                const int64_t off = id * p.kv_sblk + (tok & (bs - 1)) * D;
-                s.k[i] = *reinterpret_cast<const u32x4v*>(kb + off);
-                s.v[i] = *reinterpret_cast<const u32x4v*>(vb + off);
-            }
-            return s;
-        };
-        // Into buffer `st & 1`; st is the staged step's number.
-        auto store = [&](int st, int t, const Ids ids, const Stage s) MX_INLINE {
+        // Tile t into buffer `st & 1`; st is the staged step's number.
+        auto issue = [&](int st, int t, Ids ids) MX_INLINE {
             const int buf = st & 1;
+            bool bad = false;
+            // All ids are waited for here: one by one, the waits would count the tile's own loads in between.
+#pragma unroll
+            for (int i = 0; i < P; ++i) asm volatile("" : "+v"(ids.id[i]));
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                const int rr = row0 + i * RPP, tok = t * kTok + rr;
-                const int pos = rr * D + 8 * (c ^ (rr & (CH - 1)));
-                *reinterpret_cast<u32x4v*>(&ks[buf][pos]) = s.k[i];
+                const int rr = (wave * P + i) * RPL + lane / CH;
+                int tok = t * kTok + rr;
+                tok = tok < last_tok ? tok : last_tok;
                 const bool inside = (unsigned)ids.id[i] < (unsigned)p.num_blocks;
-                u32x4v x = tok < end && inside ? s.v[i] : u32x4v{0, 0, 0, 0};
-                if (tok < end && !inside) {
-                    bad_step[buf] = st;
-                    if (p.err && c == 0) atomicOr(p.err, 4);
-                }
-                if (t * kTok + kTok > row.ctx && tok >= row.ctx && drop_special<BF16>(x)) nf_step = st;
-                *reinterpret_cast<u32x4v*>(&vs[buf][pos]) = x;
+                bad |= !inside;
+                const int64_t off = (inside ? ids.id[i] : 0) * p.kv_sblk + (tok & (bs - 1)) * D + 8 * (lane % CH ^ (rr & (CH - 1)));
+                const uint32_t at = (uint32_t)(buf * kTok * D + (wave * P + i) * 512) * 2;
+                load_to_lds(kb + off, ks_at + at);
+                load_to_lds(vb + off, vs_at + at);
             }
+            if (bad) {
+                bad_step[buf] = st;
+                if (p.err) atomicOr(p.err, 4);
+            }
+        };
+        // The compiler does not track those loads.
+        auto arrived = [&]() MX_INLINE {
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+        };
+        // V of a tile with drafted tokens, an end or a bad block: 0 where there is no token, and where a drafted token's is not
+        // finite (see nf_step).
+        auto clean = [&](int st, int t) MX_INLINE {
+            const int buf = st & 1;
+            const bool bad = bad_step[buf] == st;
+            for (int i = tid; i < kTok * CH; i += NT) {
+                const int tok = t * kTok + i / CH;
+                u32x4v* at = reinterpret_cast<u32x4v*>(&vs[buf][0]) + i;
+                u32x4v x = *at;
+                if (tok >= end || (bad && (unsigned)bt[tok >> p.bs_shift] >= (unsigned)p.num_blocks)) x = u32x4v{0, 0, 0, 0};
+                else if (tok < row.ctx || !drop_special<BF16>(x)) continue;
+                else nf_step = st;
+                *at = x;
+            }
+            __syncthreads();
         };
 
         // Query fragments: lane l holds dims 32 c + 8 (l / 16) + [0, 8) of row l % 16 of each of the wave's tiles.
@@ -420,30 +445,25 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
                     for (int t = 0; t < RT; ++t) acc[d][t] = E::mma32(a, pr[u][t], acc[d][t]);
                 }
         };
-        {
-            const Ids ids = ids_of(t0);
-            const Stage s = load(t0, ids);
-            ++step;
-            __syncthreads();  // the previous piece is done with LDS
-            store(step, t0, ids, s);
-        }
-        __syncthreads();
+        ++step;
+        __syncthreads();  // the previous piece is done with LDS
+        issue(step, t0, ids_of(t0));
+        arrived();
         const int step0 = step;
         Ids next = ids_of(t0 + 1);
         for (int t = t0;; ++t) {
             const bool more = t + 1 < t1;
-            Stage s;
-            const Ids ids = next;
             if (more) {
-                s = load(t + 1, next);
+                issue(step + 1, t + 1, next);
                 next = ids_of(t + 2);
             }
-            if (t * kTok + kTok <= whole && bad_step[step & 1] != step) compute(std::false_type{}, step, t);
+            const bool bad = bad_step[step & 1] == step;
+            if (t * kTok + kTok > safe || bad) clean(step, t);
+            if (t * kTok + kTok <= whole && !bad) compute(std::false_type{}, step, t);
             else compute(std::true_type{}, step, t);
             if (!more) break;
+            arrived();
             ++step;
-            store(step, t + 1, ids, s);
-            __syncthreads();
         }
 
         // The lanes of a row meet, then the waves over tokens (in the buffer that no step reads any more).
