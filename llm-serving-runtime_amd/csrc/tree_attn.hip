@@ -248,6 +248,10 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     const uint32_t ks_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&ks[0][0];
     const uint32_t vs_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&vs[0][0];
 
+    half8v ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = E::round(1.0f);
+
     while (lo < hi) {
         const Row row = row_of(p, seg.b);
         const int end = visible_end(p, row, seg.rt);
@@ -338,12 +342,12 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
                 qf[t][kk] = node[t] >= 0 ? __builtin_bit_cast(half8v, *reinterpret_cast<const u32x4v*>(qp + 32 * kk))
                                          : half8v{};
         }
-        float m[RT], l[RT];
-        float4v acc[DT][RT];
+        float m[RT];
+        float4v l[RT], acc[DT][RT];  // (l's four are the same)
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            m[t] = kLowest;
-            l[t] = 0.0f;
+            m[t] = 0.0f;
+            l[t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int d = 0; d < DT; ++d) acc[d][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -359,8 +363,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             if (!p.mask) return n <= node[t];
             return p.mask[(int64_t)seg.b * p.mask_sb + (int64_t)node[t] * p.mask_st + n] != 0;
         };
-        auto compute = [&](auto masked, int st, int tile) MX_INLINE {
-            constexpr bool MASK = decltype(masked)::value;
+        auto compute = [&](bool masked, int st, int tile) MX_INLINE {
             const int buf = st & 1;
             const int tbase = tw * (kTok / TW);  // the wave's first token in the tile
             // Byte addresses in LDS: a row's chunks are permuted by an exclusive or, and so are the addresses of one lane's
@@ -373,19 +376,16 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             const char* vt = reinterpret_cast<const char*>(&vs[0][0]);
             float4v s[NTT][RT];
 #pragma unroll
-            for (int i = 0; i < NTT; ++i)
-#pragma unroll
-                for (int t = 0; t < RT; ++t) s[i][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
             for (int kk = 0; kk < KC; ++kk)
 #pragma unroll
                 for (int i = 0; i < NTT; ++i) {
                     const half8v a = __builtin_bit_cast(
                         half8v, *reinterpret_cast<const u32x4v*>(kt + (ka ^ (kk << 6)) + 16 * i * D * 2));
 #pragma unroll
-                    for (int t = 0; t < RT; ++t) s[i][t] = E::mma32(a, qf[t][kk], s[i][t]);
+                    for (int t = 0; t < RT; ++t)
+                        s[i][t] = E::mma32(a, qf[t][kk], kk ? s[i][t] : float4v{0.0f, 0.0f, 0.0f, 0.0f});
                 }
-            if constexpr (MASK) {
+            if (masked) {
                 const bool bad = bad_step[buf] == st;
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
@@ -397,40 +397,44 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
                         if (!vis) s[i >> 2][t][i & 3] = -__builtin_huge_valf();
                     }
             }
-            half8v pr[NTT / 2][RT];
-            bool rise = false;
+            // What a score's exponential is taken of, score * scale - m; the maximum of these says whether m has to move. (It
+            // begins where the row's first visible scores are, wherever that is.)
+            bool move = false;
             float top[RT];
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                float mx = s[0][t][0];
 #pragma unroll
-                for (int i = 1; i < 4 * NTT; ++i) mx = fmaxf(mx, s[i >> 2][t][i & 3]);
-                top[t] = mx * p.scale_log2e;
-                rise |= top[t] > m[t] + (kLazyLog2 + kHeadLog2);
+                for (int i = 0; i < 4 * NTT; ++i) s[i >> 2][t][i & 3] = __builtin_fmaf(s[i >> 2][t][i & 3], p.scale_log2e, -m[t]);
+                top[t] = fmaxf(s[0][t][0], s[0][t][1]);
+#pragma unroll
+                for (int i = 2; i < 4 * NTT; i += 2) top[t] = fmaxf(fmaxf(top[t], s[i >> 2][t][i & 3]), s[i >> 2][t][(i & 3) + 1]);
+                move |= top[t] > (l[t][0] == 0.0f ? -__builtin_huge_valf() : kLazyLog2 + kHeadLog2);
             }
-            if (__builtin_amdgcn_ballot_w64(rise)) {
+            if (__builtin_amdgcn_ballot_w64(move)) {
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
-                    const float mx = fmaxf(m[t], xor_max_16_32(top[t]) - kHeadLog2);
-                    const float f = __builtin_amdgcn_exp2f(m[t] - mx);
-                    m[t] = mx;
+                    const bool fresh = l[t][0] == 0.0f;
+                    const float up = xor_max_16_32(top[t]) - kHeadLog2;
+                    const float by = (fresh || up > 0.0f) && up > -__builtin_huge_valf() ? up : 0.0f;
+                    const float f = fresh ? 1.0f : __builtin_amdgcn_exp2f(-by);
+                    m[t] += by;
                     l[t] *= f;
 #pragma unroll
                     for (int d = 0; d < DT; ++d) acc[d][t] *= f;
+#pragma unroll
+                    for (int i = 0; i < 4 * NTT; ++i) s[i >> 2][t][i & 3] -= by;
                 }
             }
+            // l sums the rounded probabilities: a product with ones, which adds up a row's four lanes as well.
+            half8v pr[NTT / 2][RT];
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                float sum = 0.0f;
+            for (int t = 0; t < RT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4 * NTT; ++i) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][t][i & 3], p.scale_log2e, -m[t]));
-                    const _Float16 h = E::round(x);
-                    pr[i >> 3][t][i & 7] = h;
-                    sum += E::widen(h);
-                }
-                l[t] += sum;
-            }
+                for (int i = 0; i < 4 * NTT; ++i) pr[i >> 3][t][i & 7] = E::round(__builtin_amdgcn_exp2f(s[i >> 2][t][i & 3]));
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int u = 0; u < NTT / 2; ++u) l[t] = E::mma32(ones, pr[u][t], l[t]);
             typedef short s16x8v __attribute__((ext_vector_type(8)));
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -459,16 +463,16 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             }
             const bool bad = bad_step[step & 1] == step;
             if (t * kTok + kTok > safe || bad) clean(step, t);
-            if (t * kTok + kTok <= whole && !bad) compute(std::false_type{}, step, t);
-            else compute(std::true_type{}, step, t);
+            compute(t * kTok + kTok > whole || bad, step, t);
             if (!more) break;
             arrived();
             ++step;
         }
 
-        // The lanes of a row meet, then the waves over tokens (in the buffer that no step reads any more).
+        float ls[RT];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) l[t] = node[t] < 0 ? 0.0f : xor_sum_16_32(l[t]);
+        for (int t = 0; t < RT; ++t) ls[t] = node[t] < 0 ? 0.0f : l[t][0];
+        // The waves over tokens meet in LDS.
         if constexpr (TW > 1) {
             static_assert(TW == 2 && sizeof(ks) + sizeof(vs) >= sizeof(float) * RW * 64 * RT * (DT * 4 + 2), "exchange");
             float* xch = reinterpret_cast<float*>(&ks[0][0]) + rw * 64 * RT * DT * 4;
@@ -480,7 +484,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
 #pragma unroll
                     for (int d = 0; d < DT; ++d) reinterpret_cast<float4v*>(xch)[(d * RT + t) * 64 + lane] = acc[d][t];
                     xml[((rw * RT + t) * 64 + lane) * 2] = m[t];
-                    xml[((rw * RT + t) * 64 + lane) * 2 + 1] = l[t];
+                    xml[((rw * RT + t) * 64 + lane) * 2 + 1] = ls[t];
                 }
             }
             __syncthreads();
@@ -491,7 +495,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
                     const float mx = fmaxf(m[t], mo);
                     const float fa = __builtin_amdgcn_exp2f(m[t] - mx), fb = __builtin_amdgcn_exp2f(mo - mx);
                     m[t] = mx;
-                    l[t] = l[t] * fa + lo2 * fb;
+                    ls[t] = ls[t] * fa + lo2 * fb;
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
                         acc[d][t] = acc[d][t] * fa + reinterpret_cast<float4v*>(xch)[(d * RT + t) * 64 + lane] * fb;
@@ -527,7 +531,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
                 const int rr = (rw * RT + t) * 16 + r;
-                const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+                const float inv = ls[t] == 0.0f ? 0.0f : 1.0f / ls[t];
                 if (complete) {
                     const int n = (seg.rt * R + rr) / p.G;
                     if (n >= p.T) continue;
@@ -535,15 +539,15 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
                     for (int d = 0; d < DT; ++d) {
                         half4v o;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[i] = l[t] == 0.0f ? (_Float16)0.0f : E::round(acc[d][t][i] * inv);
+                        for (int i = 0; i < 4; ++i) o[i] = ls[t] == 0.0f ? (_Float16)0.0f : E::round(acc[d][t][i] * inv);
                         *reinterpret_cast<half4v*>(p.out + odst[t] + 16 * d + 4 * g) = o;
                     }
                 } else {
                     float* dst = p.part + ((int64_t)slot * R + rr) * (D + 4);
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
-                        *reinterpret_cast<float4v*>(dst + 16 * d + 4 * g) = l[t] == 0.0f ? float4v{} : acc[d][t] * inv;
-                    if (g == 0) *reinterpret_cast<float2*>(dst + D) = float2{m[t], l[t]};
+                        *reinterpret_cast<float4v*>(dst + 16 * d + 4 * g) = ls[t] == 0.0f ? float4v{} : acc[d][t] * inv;
+                    if (g == 0) *reinterpret_cast<float2*>(dst + D) = float2{m[t], ls[t]};
                 }
             }
         }
