@@ -222,6 +222,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     static_assert(NTT % 2 == 0 && P * RPL * RW * TW == kTok, "tile split");
     __shared__ __attribute__((aligned(16))) _Float16 ks[2][kTok * D];
     __shared__ __attribute__((aligned(16))) _Float16 vs[2][kTok * D];
+    __shared__ uint64_t words[R];  // of a masked tile: bit j of word n: token j is visible to the n-th node of the query rows
     __shared__ int bad_step[2];  // the last step whose tile has a token of a block outside the pool
     __shared__ int nf_step;      // ... a drafted token whose V is not finite
 
@@ -309,11 +310,41 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             __builtin_amdgcn_sched_barrier(0);
             __syncthreads();
         };
-        // V of a tile with drafted tokens, an end or a bad block: 0 where there is no token, and where a drafted token's is not
-        // finite (see nf_step).
+        const int first_node = seg.rt * R / p.G;
+        const int last_row_node = (seg.rt * R + R - 1) / p.G;
+        const int nodes = (last_row_node < row.count ? last_row_node + 1 : row.count) - first_node;
+        // Every row of the workgroup sees every token below this.
+        const int64_t open64 = (int64_t)row.ctx + (p.mask ? 0 : first_node + 1);
+        const int open = open64 < end ? (int)open64 : end;
+        // A tile with drafted tokens, an end or a bad block. V: 0 where there is no token, and where a drafted token's is not
+        // finite (see nf_step). And who sees what, a bit a token: a wave takes a node at a time, a lane a token, so the bytes of
+        // a mask row come in one load (as loads of each lane's own bytes two such tiles at a row's end took 20 us).
         auto clean = [&](int st, int t) MX_INLINE {
             const int buf = st & 1;
             const bool bad = bad_step[buf] == st;
+            if (t * kTok + kTok > open || bad) {
+                const int tok = t * kTok + lane, n = tok - row.ctx;
+                bool there = tok < end;
+                if (bad && there) there = (unsigned)bt[tok >> p.bs_shift] < (unsigned)p.num_blocks;
+                const bool drafted = there && n >= 0;
+                constexpr int U = 8;
+                for (int i0 = wave; i0 < nodes; i0 += U * RW * TW) {
+                    uint8_t see[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int i = i0 + u * RW * TW;
+                        see[u] = 1;
+                        if (p.mask && drafted && i < nodes)
+                            see[u] = p.mask[(int64_t)seg.b * p.mask_sb + (int64_t)(first_node + i) * p.mask_st + n];
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int i = i0 + u * RW * TW;
+                        const uint64_t word = __builtin_amdgcn_ballot_w64(there && see[u] != 0 && (p.mask || n <= first_node + i));
+                        if (lane == 0 && i < nodes) words[i] = word;
+                    }
+                }
+            }
             for (int i = tid; i < kTok * CH; i += NT) {
                 const int tok = t * kTok + i / CH;
                 u32x4v* at = reinterpret_cast<u32x4v*>(&vs[buf][0]) + i;
@@ -352,8 +383,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             for (int d = 0; d < DT; ++d) acc[d][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
         }
         // Every row of the wave sees every token below `whole`.
-        const int first_node = (seg.rt * R + rw * RT * 16) / p.G;
-        const int64_t whole64 = (int64_t)row.ctx + (p.mask ? 0 : first_node + 1);
+        const int64_t whole64 = (int64_t)row.ctx + (p.mask ? 0 : (seg.rt * R + rw * RT * 16) / p.G + 1);
         const int whole = whole64 < end ? (int)whole64 : end;
 
         auto visible = [&](int t, int tok) MX_INLINE {  // token of tile t's row to this lane
@@ -386,16 +416,14 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
                         s[i][t] = E::mma32(a, qf[t][kk], kk ? s[i][t] : float4v{0.0f, 0.0f, 0.0f, 0.0f});
                 }
             if (masked) {
-                const bool bad = bad_step[buf] == st;
 #pragma unroll
-                for (int t = 0; t < RT; ++t)
+                for (int t = 0; t < RT; ++t) {
+                    uint64_t seen = node[t] >= 0 ? words[node[t] - first_node] : 0;
+                    seen >>= tbase + 4 * g;
 #pragma unroll
-                    for (int i = 0; i < 4 * NTT; ++i) {
-                        const int tok = tile * kTok + tbase + 16 * (i >> 2) + 4 * g + (i & 3);
-                        bool vis = visible(t, tok);
-                        if (bad && vis) vis = (unsigned)bt[tok >> p.bs_shift] < (unsigned)p.num_blocks;
-                        if (!vis) s[i >> 2][t][i & 3] = -__builtin_huge_valf();
-                    }
+                    for (int i = 0; i < 4 * NTT; ++i)
+                        if (!(seen >> (16 * (i >> 2) + (i & 3)) & 1)) s[i >> 2][t][i & 3] = -__builtin_huge_valf();
+                }
             }
             // What a score's exponential is taken of, score * scale - m; the maximum of these says whether m has to move. (It
             // begins where the row's first visible scores are, wherever that is.)
