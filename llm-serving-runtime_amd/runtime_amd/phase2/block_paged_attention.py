@@ -4,7 +4,8 @@ Same contract as the reference hook (``runtime/phase2/block_paged_attention.py:2
 registered as ``ALL_ATTENTION_FUNCTIONS["block_paged"]`` with
 ``config._attn_implementation = "block_paged"`` (``runtime/phase2/worker_server.py:274-281``).
 When decode metadata is set, ``q_len == 1`` and the query is on a device, the
-fused HIP kernel runs and ``[B, 1, Hq, D]`` is returned (``:37-48``); otherwise
+fused HIP kernel runs and ``[B, 1, Hq, D]`` is returned (``:37-48``); with a draft
+tree in the metadata its nodes attend over the paged cache (``paged_attention_tree``); otherwise
 attention on the gathered K/V (prefill, ``:50-60``): one HIP launch for a causal prompt
 on the device (``_prefill_kernel_takes``), else the eager chain.
 
@@ -27,6 +28,7 @@ from torch.utils._python_dispatch import _get_current_dispatch_mode
 
 from . import _hip
 from .paged_attention_hip import _DTYPE_FLAGS, get_paged_decode_batch_metadata, paged_attention_decode_batched
+from .speculative import paged_attention_tree
 
 
 def repeat_kv(hidden_states: torch.Tensor, n_rep: int) -> torch.Tensor:
@@ -112,6 +114,8 @@ def block_paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor
                                   attention_mask: torch.Tensor | None, scaling: float, dropout: float = 0.0, **kwargs):
     num_kv_groups = getattr(module, "num_key_value_groups", 1)
     meta = get_paged_decode_batch_metadata()
+    if meta is not None and meta.tree is not None and query.is_cuda:
+        return paged_attention_tree(query, meta, num_kv_groups, scaling), None
     if meta is not None and query.shape[-2] == 1 and query.is_cuda:
         attn_output = paged_attention_decode_batched(query=query, metadata=meta, num_kv_groups=num_kv_groups,
                                                      scaling=scaling)

@@ -13,6 +13,10 @@ The slice of ``TransformersBackend`` that drives the hot path
 * :func:`greedy_decode` — prefill every row, bind the rows into one batch
   cache (``BlockPagedBatchCache.from_caches``, ``:605-611``), then ``steps``
   decode steps;
+* :func:`paged_draft_step` / :func:`speculative_decode` — a forward of a tree of drafted tokens over the
+  batch cache, and the loop that drafts, verifies and keeps (the worker's speculative loop, ``:1010-1075``,
+  which verifies one row's drafted tokens one after the other); :func:`prompt_lookup` drafts from the row's
+  own tokens;
 * :class:`PagedDecoder` — the worker's persistent-slot sequence around the same
   forward (``_bind_states_to_persistent`` -> ``dense_active_cache`` -> model ->
   ``write_back_dense`` -> ``extract_cache``, ``:366-389,619-641,733-794``), with an
@@ -42,6 +46,7 @@ from .block_paged_attention import register_block_paged_attention
 from .paged_attention_hip import set_paged_decode_batch_metadata
 from .paged_kv_cache import BlockPagedBatchCache, BlockPagedCache
 from .paged_kv_kernel import GpuKVBlockPool
+from .speculative import DraftTree, verify_draft
 
 
 def enable_block_paged_attention(model) -> None:
@@ -116,6 +121,107 @@ def greedy_decode(model, pool: GpuKVBlockPool, prompts: list[torch.Tensor], bloc
     if keep_logits:
         return out_tokens, torch.stack(kept, dim=1)
     return out_tokens
+
+
+# ---------------------------------------------------------------------------------------------
+# Speculative decoding.
+# ---------------------------------------------------------------------------------------------
+
+
+@torch.no_grad()
+def paged_draft_step(model, cache: BlockPagedBatchCache, tokens: torch.Tensor, tree: DraftTree) -> torch.Tensor:
+    """One forward of the drafted ``tokens [B, T]`` (node 0 each row's last certain token) at their tree's
+    positions; returns logits ``[B, T, V]``. ``cache.keep_drafted`` says afterwards which nodes stay."""
+    if tokens.dim() != 2 or tokens.shape[0] != cache.block_tables.shape[0]:
+        raise ValueError("paged_draft_step takes tokens of shape [B, T] matching the cache rows")
+    tree.check_batch(int(tokens.shape[0]), int(tokens.shape[1]), tokens.device)
+    cache.draft_tree = tree
+    try:
+        out = model(input_ids=tokens, position_ids=tree.position_ids(cache.seq_lens), past_key_values=cache,
+                    use_cache=True)
+    finally:
+        set_paged_decode_batch_metadata(None)
+    return out.logits
+
+
+def prompt_lookup(rows: list[list[int]], size: int, ngram: int = 2) -> list[list[int]]:
+    """Chains of ``size`` tokens drafted from the rows themselves: each row's last token, then what followed the
+    latest earlier place of its last ``ngram`` tokens (fewer where there is none; else the last token again)."""
+    out = []
+    for row in rows:
+        found: list[int] = []
+        for n in range(min(ngram, len(row) - 1), 0, -1):
+            tail = row[-n:]
+            at = next((i for i in range(len(row) - n - 1, -1, -1) if row[i:i + n] == tail), None)
+            if at is not None:
+                found = row[at + n:at + n + size - 1]
+                break
+        out.append(row[-1:] + found + row[-1:] * (size - 1 - len(found)))
+    return out
+
+
+@torch.no_grad()
+def speculative_decode(model, pool: GpuKVBlockPool, prompts: list[torch.Tensor], block_ids_rows: list[list[int]],
+                       steps: int, tree: DraftTree | int, propose=None, temperature: float = 0.0,
+                       generator: torch.Generator | None = None) -> tuple[list[list[int]], int]:
+    """Prefill each prompt, then draft, verify and keep until every row has ``steps`` tokens after its first.
+
+    ``tree`` is the shape of the drafts (a number: chains of that many nodes). ``propose(rows)`` gets every
+    row's tokens so far (prompt and output) and returns the nodes' tokens ``[B, T]``, node 0 the row's last
+    token, as a list or tensor, or a pair of them and the draft model's logits ``[B, T, V]``; without it
+    :func:`prompt_lookup` drafts. Returns the rows' ``steps + 1`` new tokens and the forwards that took. At
+    ``temperature`` 0 they are the tokens of :func:`greedy_decode`; above it samples of the model, with uniform
+    numbers from ``generator``. A row needs blocks for its prompt, its tokens and two drafts (a row that is
+    done is drafted behind its last one until all are).
+    """
+    if len(prompts) != len(block_ids_rows) or not prompts:
+        raise ValueError("one block-id row per prompt is required")
+    if pool.kv_bits != 16:
+        raise ValueError("speculative decoding takes a 16-bit pool")
+    if steps < 0:
+        raise ValueError("steps must be >= 0")
+    device = pool.k_layer_view(0).device
+    if isinstance(tree, int):
+        tree = DraftTree.chain(tree, device)
+    size, batch = tree.size, len(prompts)
+    caches, first = [], []
+    for ids, blocks in zip(prompts, block_ids_rows):
+        need = -(-(int(ids.numel()) + steps + 2 * size) // pool.block_size_tokens)
+        if len(blocks) < need:
+            raise ValueError(f"a row of {ids.numel()} prompt tokens, {steps} steps and two drafts of {size} needs {need} "
+                             f"blocks, got {len(blocks)}")
+        cache, logits = prefill_request(model, pool, blocks, ids.view(1, -1).to(device))
+        caches.append(cache)
+        first.append(logits)
+    pool.check_write_errors()
+    cache = BlockPagedBatchCache.from_caches(caches, pool)
+    # The first token comes from the prefill's logits: a tree of one node.
+    alone = DraftTree.chain(1, device)
+    logits = torch.cat(first, dim=0).unsqueeze(1)
+    verdict = verify_draft(logits, torch.zeros(batch, 1, dtype=torch.int64, device=device), alone,
+                           torch.rand(batch, 1, device=device, generator=generator), temperature)
+    rows = [ids.tolist() + new for ids, new in zip(prompts, verdict.tokens.tolist())]
+    lengths = [len(row) for row in rows]
+    forwards = 0
+    while min(len(row) - n for row, n in zip(rows, lengths)) < steps:
+        drafted = prompt_lookup(rows, size) if propose is None else propose(rows)
+        drafted, draft_logits = drafted if isinstance(drafted, tuple) else (drafted, None)
+        tokens = torch.as_tensor(drafted, dtype=torch.int64).to(device)
+        # A row that is done stays where it is: its nodes are drafted in the same place again and none is kept.
+        done = [len(row) - n >= steps for row, n in zip(rows, lengths)]
+        logits = paged_draft_step(model, cache, tokens, tree)
+        forwards += 1
+        verdict = verify_draft(logits, tokens, tree, torch.rand(batch, size, device=device, generator=generator),
+                               temperature, draft_logits=draft_logits)
+        counts = verdict.counts
+        if any(done):
+            counts = counts * torch.tensor([not d for d in done], dtype=torch.int32, device=device)
+        cache.keep_drafted(verdict.path, counts)
+        for row, new, n in zip(rows, verdict.tokens.tolist(), counts.tolist()):
+            row += new[:n]
+    cache.draft_tree = None
+    pool.check_write_errors()
+    return [row[n - 1:n + steps] for row, n in zip(rows, lengths)], forwards
 
 
 # ---------------------------------------------------------------------------------------------

@@ -30,17 +30,27 @@ Differences that keep the decode step free of host round trips:
   otherwise rebinds fresh tensors, as the reference's eager path does
   (``:146-157``).
 
+Drafted tokens (``speculative.DraftTree``): while a batch cache's ``draft_tree`` is set, a forward of the
+tree's nodes writes their K/V behind each row's context, publishes the tree with the metadata (the attention
+hook then runs ``paged_attention_tree`` over the pool) and counts the nodes in the lengths;
+``BlockPagedBatchCache.keep_drafted`` moves the accepted path behind the context and sets the lengths to it.
+
 transformers 5.15 makes ``get_max_length`` abstract; it returns the same value
 as ``get_max_cache_shape`` (the capacity of the row's blocks).
 """
 
 from __future__ import annotations
 
+from typing import TYPE_CHECKING
+
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
 from .paged_attention_hip import PagedDecodeBatchMetadata, set_paged_decode_batch_metadata
 from .paged_kv_kernel import GpuKVBlockPool
+
+if TYPE_CHECKING:
+    from .speculative import DraftTree
 
 
 def _decoder_layer_count(config) -> int:
@@ -184,21 +194,27 @@ class BlockPagedBatchLayer(CacheLayerMixin):
             self.lazy_initialization(key_states, value_states)
         parent = self._parent
         kv_len = int(key_states.shape[-2])
+        tree = parent.draft_tree
+        if tree is not None and kv_len != tree.size:
+            raise ValueError(f"a forward of {kv_len} tokens while a draft of {tree.size} nodes is set")
+        added = kv_len if tree is None or tree.counts is None else tree.counts
+        if tree is not None and self.layer_idx == 0:
+            parent.draft_start = self._row_seq_lens.clone()
         parent.pool.write_tokens_batch(self.layer_idx, parent.block_tables, self._row_seq_lens, key_states,
                                        value_states)
         if getattr(parent, "_graph_safe", False):
-            self._row_seq_lens.add_(kv_len)
+            self._row_seq_lens.add_(added)
             if self.layer_idx == 0:
                 parent.seq_lens.copy_(self._row_seq_lens)
         else:
-            self._row_seq_lens = self._row_seq_lens + kv_len
+            self._row_seq_lens = self._row_seq_lens + added
             if self.layer_idx == 0:
                 parent.seq_lens = self._row_seq_lens.clone()
 
-        if kv_len == 1:
+        if kv_len == 1 or tree is not None:
             set_paged_decode_batch_metadata(PagedDecodeBatchMetadata(
                 pool=self.pool, layer_idx=self.layer_idx, block_tables=parent.block_tables,
-                seq_lens=parent.seq_lens))
+                seq_lens=parent.seq_lens, tree=tree))
             return key_states, value_states
 
         set_paged_decode_batch_metadata(None)
@@ -273,7 +289,13 @@ class BlockPagedBatchCache(Cache):
     ``allocate_slot``/``bind_cache`` and returned by ``release_slot``;
     ``dense_active_cache`` / ``write_back_dense`` run one decode over a subset
     of slots and copy lengths and tables back.
+
+    ``draft_tree`` (None: plain decoding) is the tree whose nodes the next forward takes;
+    ``draft_start [B]`` are the lengths of the contexts that its nodes were written behind.
     """
+
+    draft_tree: "DraftTree | None" = None
+    draft_start: torch.Tensor | None = None
 
     def __init__(self, config, pool: GpuKVBlockPool, *, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                  block_ids_rows: list[list[int]]) -> None:
@@ -385,6 +407,22 @@ class BlockPagedBatchCache(Cache):
         for i, slot in enumerate(slots):
             if self.block_ids_rows[slot] != dense.block_ids_rows[i]:
                 self.sync_block_ids_row(slot, list(dense.block_ids_rows[i]))
+
+    def keep_drafted(self, path: torch.Tensor, counts: torch.Tensor) -> None:
+        """After a forward of ``draft_tree``'s nodes: keep the nodes ``path[b, :counts[b]]`` of each row
+        (``speculative.verify_draft``'s), drop the others and set the lengths to what is kept."""
+        if self.draft_tree is None or self.draft_start is None:
+            raise RuntimeError("keep_drafted follows a forward of a draft tree's nodes")
+        lens = torch.empty_like(self.draft_start)
+        self.pool.keep_tokens(self.block_tables, self.draft_start, path, counts, lens_out=lens)
+        in_place = getattr(self, "_graph_safe", False)
+        for target in (self, *self.layers):
+            name = "seq_lens" if target is self else "_row_seq_lens"
+            if in_place:
+                getattr(target, name).copy_(lens)
+            else:
+                setattr(target, name, lens.clone())
+        self.draft_start = None
 
     def extract_cache(self, index: int, seq_len: int | None = None) -> BlockPagedCache:
         """A batch-1 cache over slot ``index``. ``seq_len``, when the caller knows it (a decode
