@@ -64,11 +64,20 @@ struct Params {
     _Float16* out;
     int64_t o_sb, o_st, o_sh;
     float* part;  // [2 * workers][R][D + 4]: output / l, m, l
+    int2* pieces;  // [segments]: 2 * the worker of a segment's first piece (+ 1: its last one), and how many pieces
     int* err;
     int workers;
     int nrt;  // tiles of query rows per (row, kv-head)
     int R;    // query rows per tile
 };
+
+// A pointer to memory on the device (and not, as far as the compiler can tell of one read from memory, to LDS).
+template <typename T>
+using global = __attribute__((address_space(1))) T;
+template <typename T>
+__device__ __forceinline__ global<T>* as_global(T* p) {
+    return (global<T>*)p;
+}
 
 // What a row of the batch attends over.
 struct Row {
@@ -79,8 +88,8 @@ struct Row {
 
 __device__ __forceinline__ Row row_of(const Params& p, int b) {
     Row w;
-    const int s0 = p.seq_lens[b], s = s0 > 0 ? s0 : 0, cap = p.max_blocks << p.bs_shift;
-    int c = p.counts ? p.counts[b] : p.T;
+    const int s0 = as_global(p.seq_lens)[b], s = s0 > 0 ? s0 : 0, cap = p.max_blocks << p.bs_shift;
+    int c = p.counts ? as_global(p.counts)[b] : p.T;
     c = c < 0 ? 0 : c < p.T ? c : p.T;
     w.count = c;
     w.ctx = s - c;
@@ -117,75 +126,110 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
     return v;
 }
 
-// Tiles of all segments (below 2^30, checked on the host).
-__device__ __forceinline__ int total_tiles(const Params& p, int lane) {
-    int sum = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        int n = 0;
-        if (b0 + lane < p.B) n = head_tiles(p, row_of(p, b0 + lane));
-        sum += __builtin_amdgcn_readlane(wave_scan(n, lane), 63) * p.Hkv;
-    }
-    return sum;
-}
-
-// Tiles before row b.
-__device__ __forceinline__ int tiles_before(const Params& p, int b, int lane) {
-    int sum = 0;
-    for (int b0 = 0; b0 < b; b0 += 64) {
-        int n = 0;
-        if (b0 + lane < b) n = head_tiles(p, row_of(p, b0 + lane));
-        sum += __builtin_amdgcn_readlane(wave_scan(n, lane), 63) * p.Hkv;
-    }
-    return sum;
-}
-
 struct Seg {
     int b, kvh, rt, tile;
 };
 
-// The segment that holds tile x of all (x < total), and x's index in it.
-__device__ __forceinline__ Seg locate(const Params& p, int x, int lane) {
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        int n = 0;
-        if (b0 + lane < p.B) n = head_tiles(p, row_of(p, b0 + lane)) * p.Hkv;
-        const int incl = wave_scan(n, lane);
-        if (x < __builtin_amdgcn_readlane(incl, 63)) {
-            const int bl = __builtin_popcountll(__builtin_amdgcn_ballot_w64(incl <= x));
-            Seg s;
-            s.b = b0 + bl;
-            x -= __builtin_amdgcn_readlane(incl - n, bl);
-            const int per = __builtin_amdgcn_readlane(n, bl) / p.Hkv;
-            s.kvh = x / per;
-            x -= s.kvh * per;
-            const Row w = row_of(p, s.b);
-            s.rt = 0;
-            for (int m; s.rt + 1 < p.nrt && x >= (m = seg_tiles(p, w, s.rt)); ++s.rt) x -= m;
-            s.tile = x;
-            return s;
+// The rows of a batch as a wave holds them: up to 64 in its lanes, read once; of more, each when it is asked for.
+struct Rows {
+    Row mine;   // row `lane` (B <= 64)
+    int tiles;  // of it
+    int incl;   // of it and those before it
+    int total;  // of all (below 2^30, checked on the host)
+    __device__ __forceinline__ void read(const Params& p, int lane) {
+        mine = Row{0, 0, 0};
+        total = 0;
+        for (int b0 = 0; b0 < p.B; b0 += 64) {
+            if (b0 + lane < p.B) mine = row_of(p, b0 + lane);
+            tiles = b0 + lane < p.B ? head_tiles(p, mine) * p.Hkv : 0;
+            incl = wave_scan(tiles, lane);
+            total += __builtin_amdgcn_readlane(incl, 63);
         }
-        x -= __builtin_amdgcn_readlane(incl, 63);
     }
-    return Seg{0, 0, 0, 0};  // unreachable for x < total
-}
+    __device__ __forceinline__ Row at(const Params& p, int b) const {
+        if (p.B > 64) return row_of(p, b);
+        return Row{__builtin_amdgcn_readlane(mine.len, b), __builtin_amdgcn_readlane(mine.ctx, b),
+                   __builtin_amdgcn_readlane(mine.count, b)};
+    }
+    // The segment that holds tile x of all (x < total), and x's index in it.
+    __device__ __forceinline__ Seg locate(const Params& p, int x, int lane) const {
+        int n = tiles, up = incl;
+        for (int b0 = 0; b0 < p.B; b0 += 64) {
+            if (p.B > 64) {
+                n = b0 + lane < p.B ? head_tiles(p, row_of(p, b0 + lane)) * p.Hkv : 0;
+                up = wave_scan(n, lane);
+            }
+            const int sum = __builtin_amdgcn_readlane(up, 63);
+            if (x < sum) {
+                const int bl = __builtin_popcountll(__builtin_amdgcn_ballot_w64(up <= x));
+                Seg s;
+                s.b = b0 + bl;
+                const int here = __builtin_amdgcn_readlane(n, bl);
+                x -= __builtin_amdgcn_readlane(up, bl) - here;
+                const int per = (unsigned)here / (unsigned)p.Hkv;
+                s.kvh = (unsigned)x / (unsigned)per;
+                x -= s.kvh * per;
+                s.rt = 0;
+                if (p.nrt > 1) {
+                    const Row w = at(p, s.b);
+                    for (int m; s.rt + 1 < p.nrt && x >= (m = seg_tiles(p, w, s.rt)); ++s.rt) x -= m;
+                }
+                s.tile = x;
+                return s;
+            }
+            x -= sum;
+        }
+        return Seg{0, 0, 0, 0};  // unreachable for x < total
+    }
+};
 
 __device__ __forceinline__ int workers_of(const Params& p, int total) {
     const int most = total / kMinTiles > 1 ? total / kMinTiles : 1;
     return p.workers < most ? p.workers : most;
 }
-__device__ __forceinline__ int range_lo(int w, int total, int workers) { return (int)((int64_t)w * total / workers); }
+// a / b, in 32 bits where they do (64-bit division is a long sequence, and every workgroup begins with two).
+__device__ __forceinline__ int quotient(uint64_t a, int b) {
+    return a >> 32 ? (int)(a / (uint32_t)b) : (int)((uint32_t)a / (uint32_t)b);
+}
+__device__ __forceinline__ int range_lo(int w, int total, int workers) { return quotient((uint64_t)w * total, workers); }
 // The worker that holds tile x.
 __device__ __forceinline__ int worker_of(int x, int total, int workers) {
-    return (int)(((int64_t)(x + 1) * workers - 1) / total);
+    return quotient((uint64_t)(x + 1) * workers - 1, total);
 }
 
-// 16 bytes per lane from memory to LDS, lane l's at `to` + 16 l (`to` the same in all lanes). As a builtin the load would be waited
-// for ahead of every later read of LDS, whatever that reads; so the caller waits (vmcnt) before the barrier that hands the
-// tile over. Nothing is written to a register.
-__device__ __forceinline__ void load_to_lds(const void* from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "m0", "memory");
+// N times 16 bytes per lane from memory to LDS: load i's of lane l, at from[i], to `to` + 1024 i + 16 l (`to` the same in all
+// lanes). As a builtin the loads would be waited for ahead of every later read of LDS, whatever that reads; so the caller
+// waits (vmcnt) before the barrier that hands the tile over. Nothing is written to a register. An instruction's offset counts
+// on both sides, so M0, which holds the place in LDS, is set once, and left as it was.
+template <int N>
+__device__ __forceinline__ void load_to_lds(const char* const (&from)[N], uint32_t to) {
+    static_assert(N == 1 || N == 2 || N == 4, "offsets are below 4096");
+    uint32_t was;
+    const int at = __builtin_amdgcn_readfirstlane((int)to);
+    if constexpr (N == 1)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
+                     "s_mov_b32 m0, %0"
+                     : "=&s"(was)
+                     : "s"(at), "v"(from[0])
+                     : "memory");
+    else if constexpr (N == 2)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
+                     "global_load_lds_dwordx4 %3, off offset:1024\n\ts_mov_b32 m0, %0"
+                     : "=&s"(was)
+                     : "s"(at), "v"(from[0]), "v"(from[1] - 1024)
+                     : "memory");
+    else
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
+                     "global_load_lds_dwordx4 %3, off offset:1024\n\tglobal_load_lds_dwordx4 %4, off offset:2048\n\t"
+                     "global_load_lds_dwordx4 %5, off offset:3072\n\ts_mov_b32 m0, %0"
+                     : "=&s"(was)
+                     : "s"(at), "v"(from[0]), "v"(from[1] - 1024), "v"(from[2] - 2048), "v"(from[3] - 3072)
+                     : "memory");
 }
 
 typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+typedef float f32x2v __attribute__((ext_vector_type(2)));
+typedef int i32x2v __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4v lds_s16x4;
 __device__ __forceinline__ s16x4v read_tr(const char* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
@@ -207,6 +251,23 @@ __device__ __forceinline__ bool drop_special(u32x4v& x) {
 
 #define MX_INLINE __attribute__((always_inline))
 
+// The kernel's arguments read again from where the launch left them. What the loop over tiles does not use would otherwise stay
+// in scalar registers across it (or, as there are not enough of them, in lanes of vector registers, at a v_readlane each).
+__device__ __forceinline__ Params reload() {
+    uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    args = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)args) |
+           (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(args >> 32)) << 32;
+    const auto* from = (const __attribute__((address_space(4))) uint64_t*)args;
+    static_assert(sizeof(Params) % 8 == 0, "read in words");
+    uint64_t words[sizeof(Params) / 8];
+#pragma unroll
+    for (size_t i = 0; i < sizeof(Params) / 8; ++i) words[i] = from[i];
+    Params p;
+    __builtin_memcpy(&p, words, sizeof p);
+    return p;
+}
+
 // D: head dim. RT: 16-row query tiles per wave. RW x TW: waves over query rows and over a tile's tokens.
 template <int D, bool BF16, int RT, int RW, int TW>
 __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_kernel(Params p) {
@@ -223,6 +284,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     __shared__ __attribute__((aligned(16))) _Float16 ks[2][kTok * D];
     __shared__ __attribute__((aligned(16))) _Float16 vs[2][kTok * D];
     __shared__ uint64_t words[R];  // of a masked tile: bit j of word n: token j is visible to the n-th node of the query rows
+    __shared__ float2 xml[TW > 1 ? RW * RT * 64 : 1];
     __shared__ int bad_step[2];  // the last step whose tile has a token of a block outside the pool
     __shared__ int nf_step;      // ... a drafted token whose V is not finite
 
@@ -231,21 +293,20 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     const int rw = wave % RW, tw = wave / RW;
     const int lane = tid & 63, g = lane >> 4, r = lane & 15;
 
-    const int total = total_tiles(p, lane);
+    Rows rows;
+    rows.read(p, lane);
+    const int total = rows.total;
     const int workers = workers_of(p, total);
     // Consecutive ranges on one XCD (workgroups go round the 8 XCDs): the tiles of query rows of a kv-head meet in its L2.
     const int per = (workers + kXcds - 1) / kXcds;
     const int w = (int)blockIdx.x % kXcds * per + (int)blockIdx.x / kXcds;
     if ((int)blockIdx.x / kXcds >= per || w >= workers || total == 0) return;
-    int lo = range_lo(w, total, workers);
-    const int hi = range_lo(w + 1, total, workers);
+    const int lo = range_lo(w, total, workers), hi = range_lo(w + 1, total, workers);
     if (lo >= hi) return;
-    Seg seg = locate(p, lo, lane);
     if (tid < 2) bad_step[tid] = 0;
     if (tid == 0) nf_step = 0;
-    int step = 0;  // tiles staged so far, from 1: buffer step & 1
+    int step = 1;  // number of the tile at work, buffer step & 1
     const int bs = 1 << p.bs_shift;
-    const int range0 = lo;
     const uint32_t ks_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&ks[0][0];
     const uint32_t vs_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&vs[0][0];
 
@@ -253,50 +314,81 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = E::round(1.0f);
 
-    while (lo < hi) {
-        const Row row = row_of(p, seg.b);
-        const int end = visible_end(p, row, seg.rt);
-        const int ntiles = (end + kTok - 1) / kTok;
-        const int t0 = seg.tile, t1 = ntiles - t0 < hi - lo ? ntiles : t0 + (hi - lo);
-        const int32_t* bt = p.bt + (int64_t)seg.b * p.bt_sb;
-        const _Float16* kb = p.k + (int64_t)seg.kvh * p.kv_shead;
-        const _Float16* vb = p.v + (int64_t)seg.kvh * p.kv_shead;
-        const int last_tok = end - 1;
-        const int safe = row.ctx < end ? row.ctx > 0 ? row.ctx : 0 : end;  // tokens below it are context, and there
+    // A tile and what it belongs to.
+    struct Tile {
+        Seg seg;
+        Row row;
+        int end, ntiles;  // of the segment: tokens that it attends over, tiles
+        int64_t head;     // elements before its kv-head in a block
+        const global<const int32_t>* bt;
+    };
+    auto enter = [&](const Params& p, Tile& x) MX_INLINE {
+        x.row = rows.at(p, x.seg.b);
+        x.end = visible_end(p, x.row, x.seg.rt);
+        x.ntiles = (x.end + kTok - 1) / kTok;
+        x.head = (int64_t)x.seg.kvh * p.kv_shead;
+        x.bt = as_global(p.bt) + (int64_t)x.seg.b * p.bt_sb;
+    };
+    auto advance = [&](Tile& x) MX_INLINE {  // to the next one; there is one
+        if (++x.seg.tile < x.ntiles) return;
+        x.seg.tile = 0;
+        const Params p = reload();
+        do {
+            if (++x.seg.rt == p.nrt) {
+                x.seg.rt = 0;
+                if (++x.seg.kvh == p.Hkv) {
+                    x.seg.kvh = 0;
+                    ++x.seg.b;
+                }
+            }
+            enter(p, x);
+        } while (x.ntiles == 0);
+    };
 
         // Loads go from memory to LDS without a register: a lane's 16 bytes land at 16 times the lane behind the instruction's
         // place, so the permutation of a token's chunks is in the addresses that the lanes read from.
         struct Ids {
             int id[P];
         };
-        auto ids_of = [&](int t) MX_INLINE {
+        auto ids_of = [&](const Tile& x) MX_INLINE {
             Ids s;
+            const int last_tok = x.end - 1;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                int tok = t * kTok + (wave * P + i) * RPL + lane / CH;
+                int tok = x.seg.tile * kTok + (wave * P + i) * RPL + lane / CH;
                 tok = tok < last_tok ? tok : last_tok;  // past the end: the last token again
-                s.id[i] = bt[tok >> p.bs_shift];
+                s.id[i] = x.bt[tok >> p.bs_shift];
             }
             return s;
         };
-        // Tile t into buffer `st & 1`; st is the staged step's number.
-        auto issue = [&](int st, int t, Ids ids) MX_INLINE {
+        // Tile x, number st, into buffer `st & 1`.
+        auto issue = [&](int st, const Tile& x, Ids ids) MX_INLINE {
             const int buf = st & 1;
+            const _Float16 *kb = p.k + x.head, *vb = p.v + x.head;
+            const int last_tok = x.end - 1;
             bool bad = false;
             // All ids are waited for here: one by one, the waits would count the tile's own loads in between.
 #pragma unroll
             for (int i = 0; i < P; ++i) asm volatile("" : "+v"(ids.id[i]));
+            constexpr int N = P < 4 ? P : 4;
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const int rr = (wave * P + i) * RPL + lane / CH;
-                int tok = t * kTok + rr;
-                tok = tok < last_tok ? tok : last_tok;
-                const bool inside = (unsigned)ids.id[i] < (unsigned)p.num_blocks;
-                bad |= !inside;
-                const int64_t off = (inside ? ids.id[i] : 0) * p.kv_sblk + (tok & (bs - 1)) * D + 8 * (lane % CH ^ (rr & (CH - 1)));
-                const uint32_t at = (uint32_t)(buf * kTok * D + (wave * P + i) * 512) * 2;
-                load_to_lds(kb + off, ks_at + at);
-                load_to_lds(vb + off, vs_at + at);
+            for (int i0 = 0; i0 < P; i0 += N) {
+                const char *kf[N], *vf[N];
+#pragma unroll
+                for (int i = i0; i < i0 + N; ++i) {
+                    const int rr = (wave * P + i) * RPL + lane / CH;
+                    int tok = x.seg.tile * kTok + rr;
+                    tok = tok < last_tok ? tok : last_tok;
+                    const bool inside = (unsigned)ids.id[i] < (unsigned)p.num_blocks;
+                    bad |= !inside;
+                    const int64_t off =
+                        (inside ? ids.id[i] : 0) * p.kv_sblk + (tok & (bs - 1)) * D + 8 * (lane % CH ^ (rr & (CH - 1)));
+                    kf[i - i0] = reinterpret_cast<const char*>(kb + off);
+                    vf[i - i0] = reinterpret_cast<const char*>(vb + off);
+                }
+                const uint32_t at = (uint32_t)(buf * kTok * D + (wave * P + i0) * 512) * 2;
+                load_to_lds<N>(kf, ks_at + at);
+                load_to_lds<N>(vf, vs_at + at);
             }
             if (bad) {
                 bad_step[buf] = st;
@@ -310,16 +402,38 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             __builtin_amdgcn_sched_barrier(0);
             __syncthreads();
         };
-        const int first_node = seg.rt * R / p.G;
-        const int last_row_node = (seg.rt * R + R - 1) / p.G;
-        const int nodes = (last_row_node < row.count ? last_row_node + 1 : row.count) - first_node;
-        // Every row of the workgroup sees every token below this.
-        const int64_t open64 = (int64_t)row.ctx + (p.mask ? 0 : first_node + 1);
-        const int open = open64 < end ? (int)open64 : end;
+    Tile ahead;  // the next one to load, with its block ids
+    ahead.seg = rows.locate(p, lo, lane);
+    enter(p, ahead);
+    __syncthreads();  // bad_step
+    Ids ids = ids_of(ahead);
+    issue(step, ahead, ids);
+    Tile cur = ahead;
+    if (lo + 1 < hi) {
+        advance(ahead);
+        ids = ids_of(ahead);
+    }
+    arrived();
+
+    // A piece after the other: the tiles of one segment in this range. The first tile of the next one is on its way already.
+    for (int at = lo; at < hi;) {
+        const Seg seg = cur.seg;
+        const Row row = cur.row;
+        const int end = cur.end, ntiles = cur.ntiles, t0 = seg.tile;
+        const int t1 = ntiles - t0 < hi - at ? ntiles : t0 + (hi - at);
+        const int step0 = step;
+        const int safe = row.ctx < end ? row.ctx > 0 ? row.ctx : 0 : end;  // tokens below it are context, and there
         // A tile with drafted tokens, an end or a bad block. V: 0 where there is no token, and where a drafted token's is not
         // finite (see nf_step). And who sees what, a bit a token: a wave takes a node at a time, a lane a token, so the bytes of
         // a mask row come in one load (as loads of each lane's own bytes two such tiles at a row's end took 20 us).
         auto clean = [&](int st, int t) MX_INLINE {
+            const Params p = reload();
+            const auto* bt = as_global(p.bt) + (int64_t)seg.b * p.bt_sb;
+            const int first_node = seg.rt * R / p.G, last_row_node = (seg.rt * R + R - 1) / p.G;
+            const int nodes = (last_row_node < row.count ? last_row_node + 1 : row.count) - first_node;
+            // Every row of the workgroup sees every token below this.
+            const int64_t open64 = (int64_t)row.ctx + (p.mask ? 0 : first_node + 1);
+            const int open = open64 < end ? (int)open64 : end;
             const int buf = st & 1;
             const bool bad = bad_step[buf] == st;
             if (t * kTok + kTok > open || bad) {
@@ -335,7 +449,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
                         const int i = i0 + u * RW * TW;
                         see[u] = 1;
                         if (p.mask && drafted && i < nodes)
-                            see[u] = p.mask[(int64_t)seg.b * p.mask_sb + (int64_t)(first_node + i) * p.mask_st + n];
+                            see[u] = as_global(p.mask)[(int64_t)seg.b * p.mask_sb + (int64_t)(first_node + i) * p.mask_st + n];
                     }
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
@@ -357,20 +471,20 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             __syncthreads();
         };
 
+        const Params here = reload();
+        const int first_node = seg.rt * R / here.G;
         // Query fragments: lane l holds dims 32 c + 8 (l / 16) + [0, 8) of row l % 16 of each of the wave's tiles.
         half8v qf[RT][KC];
         int node[RT];  // -1: no such row
-        int64_t odst[RT];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             const int rr = seg.rt * R + (rw * RT + t) * 16 + r;
-            const int n = rr / p.G, h = seg.kvh * p.G + (rr - n * p.G);
+            const int n = rr / here.G, h = seg.kvh * here.G + (rr - n * here.G);
             node[t] = n < row.count ? n : -1;
-            odst[t] = (int64_t)seg.b * p.o_sb + (int64_t)n * p.o_st + (int64_t)h * p.o_sh;
-            const _Float16* qp = p.q + (int64_t)seg.b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)n * p.q_st + 8 * g;
+            const auto* qp = as_global(here.q) + (int64_t)seg.b * here.q_sb + (int64_t)h * here.q_sh + (int64_t)n * here.q_st + 8 * g;
 #pragma unroll
             for (int kk = 0; kk < KC; ++kk)
-                qf[t][kk] = node[t] >= 0 ? __builtin_bit_cast(half8v, *reinterpret_cast<const u32x4v*>(qp + 32 * kk))
+                qf[t][kk] = node[t] >= 0 ? __builtin_bit_cast(half8v, *(const global<u32x4v>*)(qp + 32 * kk))
                                          : half8v{};
         }
         float m[RT];
@@ -383,16 +497,9 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             for (int d = 0; d < DT; ++d) acc[d][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
         }
         // Every row of the wave sees every token below `whole`.
-        const int64_t whole64 = (int64_t)row.ctx + (p.mask ? 0 : (seg.rt * R + rw * RT * 16) / p.G + 1);
+        const int64_t whole64 = (int64_t)row.ctx + (here.mask ? 0 : (seg.rt * R + rw * RT * 16) / here.G + 1);
         const int whole = whole64 < end ? (int)whole64 : end;
 
-        auto visible = [&](int t, int tok) MX_INLINE {  // token of tile t's row to this lane
-            const int n = tok - row.ctx;
-            if (tok >= end || node[t] < 0) return false;
-            if (n < 0) return true;
-            if (!p.mask) return n <= node[t];
-            return p.mask[(int64_t)seg.b * p.mask_sb + (int64_t)node[t] * p.mask_st + n] != 0;
-        };
         auto compute = [&](bool masked, int st, int tile) MX_INLINE {
             const int buf = st & 1;
             const int tbase = tw * (kTok / TW);  // the wave's first token in the tile
@@ -477,22 +584,19 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
                     for (int t = 0; t < RT; ++t) acc[d][t] = E::mma32(a, pr[u][t], acc[d][t]);
                 }
         };
-        ++step;
-        __syncthreads();  // the previous piece is done with LDS
-        issue(step, t0, ids_of(t0));
-        arrived();
-        const int step0 = step;
-        Ids next = ids_of(t0 + 1);
         for (int t = t0;; ++t) {
-            const bool more = t + 1 < t1;
+            const bool more = at + (t + 1 - t0) < hi;  // tiles of this range, of this piece or a later one
             if (more) {
-                issue(step + 1, t + 1, next);
-                next = ids_of(t + 2);
+                issue(step + 1, ahead, ids);
+                if (at + (t + 2 - t0) < hi) {
+                    advance(ahead);
+                    ids = ids_of(ahead);
+                }
             }
             const bool bad = bad_step[step & 1] == step;
             if (t * kTok + kTok > safe || bad) clean(step, t);
             compute(t * kTok + kTok > whole || bad, step, t);
-            if (!more) break;
+            if (t + 1 == t1) break;
             arrived();
             ++step;
         }
@@ -500,51 +604,58 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
         float ls[RT];
 #pragma unroll
         for (int t = 0; t < RT; ++t) ls[t] = node[t] < 0 ? 0.0f : l[t][0];
-        // The waves over tokens meet in LDS.
+        // The waves over tokens meet in the buffers of the last tile (the others may be loading).
         if constexpr (TW > 1) {
-            static_assert(TW == 2 && sizeof(ks) + sizeof(vs) >= sizeof(float) * RW * 64 * RT * (DT * 4 + 2), "exchange");
-            float* xch = reinterpret_cast<float*>(&ks[0][0]) + rw * 64 * RT * DT * 4;
-            float* xml = reinterpret_cast<float*>(&vs[0][0]);
+            static_assert(TW == 2 && RW <= 2 && sizeof(ks[0]) >= sizeof(float4v) * 64 * RT * DT, "exchange");
+            float4v* xch = reinterpret_cast<float4v*>(rw == 0 ? &ks[step & 1][0] : &vs[step & 1][0]) + lane;
             __syncthreads();
             if (tw == 1) {
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) reinterpret_cast<float4v*>(xch)[(d * RT + t) * 64 + lane] = acc[d][t];
-                    xml[((rw * RT + t) * 64 + lane) * 2] = m[t];
-                    xml[((rw * RT + t) * 64 + lane) * 2 + 1] = ls[t];
+                    for (int d = 0; d < DT; ++d) xch[(d * RT + t) * 64] = acc[d][t];
+                    xml[(rw * RT + t) * 64 + lane] = float2{m[t], ls[t]};
                 }
             }
             __syncthreads();
             if (tw == 0) {
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
-                    const float mo = xml[((rw * RT + t) * 64 + lane) * 2], lo2 = xml[((rw * RT + t) * 64 + lane) * 2 + 1];
-                    const float mx = fmaxf(m[t], mo);
-                    const float fa = __builtin_amdgcn_exp2f(m[t] - mx), fb = __builtin_amdgcn_exp2f(mo - mx);
-                    m[t] = mx;
-                    ls[t] = ls[t] * fa + lo2 * fb;
+                    const float2 other = xml[(rw * RT + t) * 64 + lane];
+                    // A wave that has seen nothing has no reference.
+                    const float ma = ls[t] == 0.0f ? kLowest : m[t], mb = other.y == 0.0f ? kLowest : other.x;
+                    m[t] = fmaxf(ma, mb);
+                    const float fa = __builtin_amdgcn_exp2f(ma - m[t]), fb = __builtin_amdgcn_exp2f(mb - m[t]);
+                    ls[t] = ls[t] * fa + other.y * fb;
 #pragma unroll
-                    for (int d = 0; d < DT; ++d)
-                        acc[d][t] = acc[d][t] * fa + reinterpret_cast<float4v*>(xch)[(d * RT + t) * 64 + lane] * fb;
+                    for (int d = 0; d < DT; ++d) acc[d][t] = acc[d][t] * fa + xch[(d * RT + t) * 64] * fb;
                 }
             }
         }
+        const Params p = reload();
         if (tw == 0 && nf_step >= step0) {
             // V of drafted tokens that is not finite was staged as 0 (0 * inf would be NaN for rows that do not see it): it
             // counts for the rows that see it, whose probability of it is above 0.
+            const auto* bt = as_global(p.bt) + (int64_t)seg.b * p.bt_sb;
+            auto visible = [&](int t, int tok) MX_INLINE {  // token of tile t's row to this lane
+                const int n = tok - row.ctx;
+                if (tok >= end || node[t] < 0) return false;
+                if (n < 0) return true;
+                if (!p.mask) return n <= node[t];
+                return as_global(p.mask)[(int64_t)seg.b * p.mask_sb + (int64_t)node[t] * p.mask_st + n] != 0;
+            };
             const int from = t0 * kTok > row.ctx ? t0 * kTok : row.ctx > 0 ? row.ctx : 0;
             const int to = t1 * kTok < end ? t1 * kTok : end;
             for (int tok = from; tok < to; ++tok) {
                 const int id = bt[tok >> p.bs_shift];
                 if ((unsigned)id >= (unsigned)p.num_blocks) continue;
-                const _Float16* vp = p.v + (int64_t)seg.kvh * p.kv_shead + id * p.kv_sblk + (tok & (bs - 1)) * D + 4 * g;
+                const auto* vp = as_global(p.v) + (int64_t)seg.kvh * p.kv_shead + id * p.kv_sblk + (tok & (bs - 1)) * D + 4 * g;
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
                     if (visible(t, tok))
 #pragma unroll
                         for (int d = 0; d < DT; ++d) {
-                            const half4v x = *reinterpret_cast<const half4v*>(vp + 16 * d);
+                            const half4v x = *(const global<half4v>*)(vp + 16 * d);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const float f = E::widen(x[i]);
@@ -555,43 +666,41 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
         }
         if (tw == 0) {
             const bool complete = t0 == 0 && t1 == ntiles;
-            const int slot = 2 * w + (lo == range0 ? 0 : 1);
+            const int slot = 2 * w + (at == lo ? 0 : 1);
+            if (t0 == 0 && tid == 0) {
+                const int pieces = worker_of(at + ntiles - 1, total, workers) - w + 1;
+                *(global<i32x2v>*)(as_global(p.pieces) + (seg.b * p.Hkv + seg.kvh) * p.nrt + seg.rt) = i32x2v{slot, pieces};
+            }
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
                 const int rr = (rw * RT + t) * 16 + r;
                 const float inv = ls[t] == 0.0f ? 0.0f : 1.0f / ls[t];
                 if (complete) {
-                    const int n = (seg.rt * R + rr) / p.G;
+                    const int n = (seg.rt * R + rr) / p.G, h = seg.kvh * p.G + (seg.rt * R + rr - n * p.G);
                     if (n >= p.T) continue;
+                    auto* dst = as_global(p.out) + (int64_t)seg.b * p.o_sb + (int64_t)n * p.o_st + (int64_t)h * p.o_sh + 4 * g;
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
                         half4v o;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) o[i] = ls[t] == 0.0f ? (_Float16)0.0f : E::round(acc[d][t][i] * inv);
-                        *reinterpret_cast<half4v*>(p.out + odst[t] + 16 * d + 4 * g) = o;
+                        *(global<half4v>*)(dst + 16 * d) = o;
                     }
                 } else {
-                    float* dst = p.part + ((int64_t)slot * R + rr) * (D + 4);
+                    auto* dst = as_global(p.part) + ((int64_t)slot * R + rr) * (D + 4);
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
-                        *reinterpret_cast<float4v*>(dst + 16 * d + 4 * g) = ls[t] == 0.0f ? float4v{} : acc[d][t] * inv;
-                    if (g == 0) *reinterpret_cast<float2*>(dst + D) = float2{m[t], ls[t]};
+                        *(global<float4v>*)(dst + 16 * d + 4 * g) = ls[t] == 0.0f ? float4v{} : acc[d][t] * inv;
+                    if (g == 0) *(global<f32x2v>*)(dst + D) = f32x2v{m[t], ls[t]};
                 }
             }
         }
-        lo += t1 - t0;
-        // the next segment that holds a tile
-        seg.tile = 0;
-        if (lo < hi) {
-            do {
-                if (++seg.rt == p.nrt) {
-                    seg.rt = 0;
-                    if (++seg.kvh == p.Hkv) {
-                        seg.kvh = 0;
-                        ++seg.b;
-                    }
-                }
-            } while (seg_tiles(p, row_of(p, seg.b), seg.rt) == 0);
+        at += t1 - t0;
+        if (at < hi) {
+            cur.seg.tile = t1 - 1;
+            advance(cur);
+            arrived();
+            ++step;
         }
     }
 }
@@ -606,39 +715,40 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(Params p, int sp) {
     constexpr int GR = 256 / LN;  // lane groups
     __shared__ float4v sacc[GR][LN];
     __shared__ float2 sml[GR];
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x;
     const int grp = tid / LN, x = tid % LN;
     const int rows_per = GR / sp;
     const int blocks = (p.R + rows_per - 1) / rows_per;
     const int segid = blockIdx.x / blocks, rr = (blockIdx.x - segid * blocks) * rows_per + grp / sp, part = grp % sp;
     const int rt = segid % p.nrt, kvh = segid / p.nrt % p.Hkv, b = segid / p.nrt / p.Hkv;
-    const Row row = row_of(p, b);
-    const int ntiles = seg_tiles(p, row, rt);
     const int qrow = rt * p.R + rr, n = qrow / p.G, h = kvh * p.G + qrow - n * p.G;
-    int first = 0, pieces = 0, head = 0, total = 0, workers = 1;
-    if (ntiles > 0) {
-        total = total_tiles(p, lane);
-        workers = workers_of(p, total);
-        int x0 = tiles_before(p, b, lane) + kvh * head_tiles(p, row);
-        for (int i = 0; i < rt; ++i) x0 += seg_tiles(p, row, i);
-        first = worker_of(x0, total, workers);
-        pieces = worker_of(x0 + ntiles - 1, total, workers) - first + 1;
-        if (pieces == 1) return;  // written whole
-        head = range_lo(first, total, workers) < x0;  // the first piece is its worker's last
-    }
+    const int2 info = p.pieces[segid];  // nothing sensible where the segment has no tile
+    const bool any = seg_tiles(p, row_of(p, b), rt) > 0;
+    if (any && info.y == 1) return;  // written whole
+    const int first = info.x >> 1, head = info.x & 1, pieces = any ? info.y : 0;
     float m = kLowest, l = 0.0f;
     float4v acc{0.0f, 0.0f, 0.0f, 0.0f};
     const bool live = rr < p.R && n < p.T;
     if (live) {
-        for (int k = part; k < pieces; k += sp) {
-            const int slot = 2 * (first + k) + (k == 0 ? head : 0);
-            const float* src = p.part + ((int64_t)slot * p.R + rr) * (D + 4);
-            const float4v o = *reinterpret_cast<const float4v*>(src + 4 * x);
-            const float2 ml = *reinterpret_cast<const float2*>(src + D);
-            const float mx = fmaxf(m, ml.x);
-            const float fa = __builtin_amdgcn_exp2f(m - mx), fb = __builtin_amdgcn_exp2f(ml.x - mx) * ml.y;
-            if (ml.y != 0.0f) {  // a piece of which the row sees nothing counts for nothing
-                acc = acc * fa + o * fb;
+        constexpr int U = 4;  // pieces in flight
+        for (int k0 = part; k0 < pieces; k0 += U * sp) {
+            float4v o[U];
+            float2 ml[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = k0 + u * sp < pieces ? k0 + u * sp : k0;
+                const int slot = 2 * (first + k) + (k == 0 ? head : 0);
+                const float* src = p.part + ((int64_t)slot * p.R + rr) * (D + 4);
+                o[u] = *reinterpret_cast<const float4v*>(src + 4 * x);
+                ml[u] = *reinterpret_cast<const float2*>(src + D);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                // (a piece of which the row sees nothing counts for nothing)
+                if (k0 + u * sp >= pieces || ml[u].y == 0.0f) continue;
+                const float mx = fmaxf(m, ml[u].x);
+                const float fa = __builtin_amdgcn_exp2f(m - mx), fb = __builtin_amdgcn_exp2f(ml[u].x - mx) * ml[u].y;
+                acc = acc * fa + o[u] * fb;
                 l = l * fa + fb;
                 m = mx;
             }
@@ -689,6 +799,8 @@ static Plan plan_of(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t max_to
     return p;
 }
 
+static size_t part_bytes(const Plan& p, int D) { return (size_t)2 * p.workers * p.R * (D + 4) * sizeof(float); }
+
 template <int D, bool BF16>
 static void launch(const Plan& pl, const Params& p, hipStream_t st) {
     const dim3 grid((unsigned)p.workers), block(64 * pl.rw * pl.tw);
@@ -714,7 +826,7 @@ extern "C" size_t mx_tree_attn_workspace_bytes(int32_t B, int32_t T, int32_t Hq,
                                                int32_t max_blocks, int32_t block_size) {
     if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_blocks <= 0 || block_size <= 0 || Hq % Hkv != 0) return 0;
     const tree::Plan pl = tree::plan_of(B, T, Hkv, Hq / Hkv, (int64_t)max_blocks * block_size);
-    return (size_t)2 * pl.workers * pl.R * (D + 4) * sizeof(float);
+    return tree::part_bytes(pl, D) + (size_t)B * Hkv * pl.nrt * sizeof(int2);
 }
 
 extern "C" int mx_tree_attn(const uint16_t* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const uint16_t* k,
@@ -772,6 +884,7 @@ extern "C" int mx_tree_attn(const uint16_t* q, int64_t q_sb, int64_t q_sh, int64
     p.scale_log2e = scale * 1.4426950408889634f;
     p.out = reinterpret_cast<_Float16*>(out), p.o_sb = o_sb, p.o_st = o_st, p.o_sh = o_sh;
     p.part = static_cast<float*>(workspace);
+    p.pieces = reinterpret_cast<int2*>(static_cast<char*>(workspace) + tree::part_bytes(pl, D));
     p.err = err;
     p.workers = pl.workers, p.nrt = pl.nrt, p.R = pl.R;
     hipStream_t st = as_stream(stream);

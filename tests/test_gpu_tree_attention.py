@@ -201,6 +201,19 @@ def test_large_scores_and_a_single_winner():
     c.check(c.run())
 
 
+@pytest.mark.parametrize("lens", [[3], [20, 40], [65, 90], [300]])
+@pytest.mark.parametrize("t,sign", [(1, -1), (3, -1), (3, 1)])
+def test_scores_far_from_zero(lens, t, sign):
+    """All scores near +-2000 (the running reference has to go there, also below 0), in rows that leave some of a
+    workgroup's waves without a token."""
+    c = Case(21, lens=[n + t for n in lens], t=t, d=128, group=2)
+    c.k *= 0.1
+    c.q *= 0.1
+    c.k[..., 0] = 150.0
+    c.q[..., 0] = 150.0 * sign
+    c.check(c.run())
+
+
 def test_a_flat_tail_under_a_large_token_keeps_its_weight():
     """4000 tokens whose probabilities are 2^-24 of the largest's: their sum counts."""
     c = Case(12, lens=[4001], t=1, d=64, hkv=1, group=1)
