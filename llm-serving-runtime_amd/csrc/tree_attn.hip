@@ -44,6 +44,7 @@ constexpr float kLazyLog2 = 8.0f;  // rescale only when the running max rises by
 // itself 10^5 tokens of 2^-25 each, 0.4 %, would be rounded to 0.)
 constexpr float kHeadLog2 = 7.0f;
 constexpr float kLowest = -3.4028235e38f;
+constexpr int kMfma = 0x8, kDsRead = 0x100;  // kinds of instructions, for the compiler's scheduler
 
 struct Params {
     const _Float16* q;
@@ -268,19 +269,393 @@ __device__ __forceinline__ Params reload() {
     return p;
 }
 
+typedef short s16x8v __attribute__((ext_vector_type(8)));
+
+// A tile and its segment, the same in all lanes.
+struct Tile {
+    Seg seg;
+    int end, ntiles;  // of the segment: tokens that it attends over, tiles
+
+    __device__ __forceinline__ void enter(const Params& p, const Rows& rows) {
+        end = visible_end(p, rows.at(p, seg.b), seg.rt);
+        ntiles = (end + kTok - 1) / kTok;
+    }
+    // To the next segment that holds a tile; there is one.
+    __device__ __forceinline__ void next_segment(const Rows& rows) {
+        const Params p = reload();
+        seg.tile = 0;
+        do {
+            if (++seg.rt == p.nrt) {
+                seg.rt = 0;
+                if (++seg.kvh == p.Hkv) {
+                    seg.kvh = 0;
+                    ++seg.b;
+                }
+            }
+            enter(p, rows);
+        } while (ntiles == 0);
+    }
+    // Every node of the segment sees every token below this (if its block is one of the pool).
+    __device__ __forceinline__ int open(const Params& p, const Row& row) const {
+        const int64_t n = (int64_t)row.ctx + (p.mask ? 0 : seg.rt * p.R / p.G + 1);
+        return n < end ? n > 0 ? (int)n : 0 : end;
+    }
+};
+
+// Tiles on their way from the pool to LDS, WAVES waves sharing them. The loads go without a register: a lane's 16 bytes land at 16
+// times the lane behind the instruction's place, so the permutation of a token's chunks is in the addresses that the lanes
+// read from. Block ids are held 64 at a time, one a lane (an instruction's 1 KiB holds tokens of two blocks at most), and read
+// ahead of the tile that needs them: ids read a tile at a time, by scalar loads, took 1300 of a tile's 5600 cycles.
+template <int D, int WAVES>
+struct Loader {
+    static constexpr int CH = D / 8;                // 16-byte chunks per token
+    static constexpr int RPL = 64 / CH;             // tokens per load instruction of a wave
+    static constexpr int P = kTok / RPL / WAVES;    // load instructions per wave and tile, of K and of V each
+    static constexpr int IPL = RPL / 4;             // blocks per instruction, at most
+    static_assert(P * RPL * WAVES == kTok, "tile split");
+    Tile x;           // the next one to load
+    int64_t head;     // elements before its kv-head in a block
+    int ids, coming;  // the 64 block ids around it, and those to take their place
+    bool change;
+
+    __device__ __forceinline__ void look_up(const Params& p, int lane) {
+        head = (int64_t)x.seg.kvh * p.kv_shead;
+        const int i = (x.seg.tile * kTok >> p.bs_shift & ~63) + lane, last = (x.end - 1) >> p.bs_shift;
+        coming = as_global(p.bt)[(int64_t)x.seg.b * p.bt_sb + (i < last ? i : last)];  // past the end: the last one again
+        change = true;
+    }
+    __device__ __forceinline__ void advance(const Rows& rows, int bs_shift, int lane) {
+        if (++x.seg.tile >= x.ntiles) x.next_segment(rows);
+        if ((x.seg.tile * kTok >> bs_shift & 63) == 0) look_up(reload(), lane);
+    }
+    // The tile to ks_at and vs_at; returns whether a block lies outside the pool (its tokens read block 0).
+    __device__ __forceinline__ bool issue(const Params& p, uint32_t ks_at, uint32_t vs_at, int wave, int lane) {
+        if (change) {
+            ids = coming;
+            asm volatile("" : "+v"(ids));  // waited for in this branch
+            change = false;
+        }
+        const int last = x.end - 1, bs = 1 << p.bs_shift;
+        const _Float16 *kb = p.k + head, *vb = p.v + head;
+        bool bad = false;
+        constexpr int N = P < 4 ? P : 4;
+#pragma unroll
+        for (int i0 = 0; i0 < P; i0 += N) {
+            const char *kf[N], *vf[N];
+#pragma unroll
+            for (int i = i0; i < i0 + N; ++i) {
+                int64_t blk[IPL];
+#pragma unroll
+                for (int j = 0; j < IPL; ++j) {
+                    const int tok = x.seg.tile * kTok + (wave * P + i) * RPL + 4 * j;
+                    const int id = __builtin_amdgcn_readlane(ids, tok >> p.bs_shift & 63);
+                    const bool inside = (unsigned)id < (unsigned)p.num_blocks;
+                    bad |= !inside;
+                    blk[j] = (inside ? id : 0) * p.kv_sblk;
+                }
+                const int rr = (wave * P + i) * RPL + lane / CH;
+                int tok = x.seg.tile * kTok + rr;
+                tok = tok < last ? tok : last;
+                const int at = (tok & (bs - 1)) * D + 8 * (lane % CH ^ (rr & (CH - 1)));
+                const int64_t off = (IPL == 2 && (lane / CH & 4) ? blk[IPL - 1] : blk[0]) + at;
+                kf[i - i0] = reinterpret_cast<const char*>(kb + off);
+                vf[i - i0] = reinterpret_cast<const char*>(vb + off);
+            }
+            const uint32_t at = (uint32_t)(wave * P + i0) * 1024;
+            load_to_lds<N>(kf, ks_at + at);
+            load_to_lds<N>(vf, vs_at + at);
+        }
+        if (bad && p.err) atomicOr(p.err, 4);
+        return bad;
+    }
+};
+
+// The query rows of a wave (RT tiles of 16) and what they have gathered, over NTT 16-token tiles at a time.
+template <int D, bool BF16, int RT, int NTT>
+struct Queries {
+    using E = Elt<BF16>;
+    static constexpr int KC = D / 32;  // 32-dim steps of a score
+    static constexpr int DT = D / 16;  // 16-dim output tiles
+    static constexpr int CH = D / 8;   // 16-byte chunks per token
+    half8v q[RT][KC];                  // lane l: dims 32 c + 8 (l / 16) + [0, 8) of row l % 16 of each tile
+    // (vectors: of arrays here the compiler keeps some in memory)
+    int node __attribute__((ext_vector_type(RT)));  // -1: no such row
+    float m __attribute__((ext_vector_type(RT)));
+    float4v l[RT], acc[DT][RT];        // (l's four are the same)
+
+    // Rows row0 .. of the segment.
+    __device__ __forceinline__ void load(const Params& p, const Seg& seg, int count, int row0, int lane) {
+        const int g = lane >> 4, r = lane & 15;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int rr = row0 + t * 16 + r;
+            const int n = rr / p.G, h = seg.kvh * p.G + (rr - n * p.G);
+            node[t] = n < count ? n : -1;
+            const auto* qp = as_global(p.q) + (int64_t)seg.b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)n * p.q_st + 8 * g;
+#pragma unroll
+            for (int kk = 0; kk < KC; ++kk)
+                q[t][kk] = node[t] >= 0 ? __builtin_bit_cast(half8v, *(const global<u32x4v>*)(qp + 32 * kk)) : half8v{};
+            m[t] = 0.0f;
+            l[t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    // Scores of the tokens from `first` of the tile whose K begins at byte `at` of k. A row's chunks are permuted by an exclusive
+    // or, and so are the addresses of one lane's reads; rows 16 apart are permuted alike. (The empty asm keeps the
+    // compiler from holding all addresses in registers.)
+    __device__ __forceinline__ void scores(const char* k, uint32_t at, int first, int lane, float4v (&s)[NTT][RT]) const {
+        const int g = lane >> 4, r = lane & 15;
+        uint32_t ka = at + (uint32_t)(first + r) * D * 2 + ((g ^ (r & (CH - 1))) << 4);
+        asm volatile("" : "+v"(ka));
+#pragma unroll
+        for (int kk = 0; kk < KC; ++kk)
+#pragma unroll
+            for (int i = 0; i < NTT; ++i) {
+                const half8v a = __builtin_bit_cast(half8v, *reinterpret_cast<const u32x4v*>(k + (ka ^ (kk << 6)) + 16 * i * D * 2));
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                    s[i][t] = E::mma32(a, q[t][kk], kk ? s[i][t] : float4v{0.0f, 0.0f, 0.0f, 0.0f});
+            }
+        // Reads a step ahead of the products that use them: left to itself the compiler waits for each pair of reads.
+        __builtin_amdgcn_sched_group_barrier(kDsRead, NTT, 0);
+#pragma unroll
+        for (int kk = 0; kk + 1 < KC; ++kk) {
+            __builtin_amdgcn_sched_group_barrier(kDsRead, NTT, 0);
+            __builtin_amdgcn_sched_group_barrier(kMfma, NTT * RT, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, NTT * RT, 0);
+    }
+    // -inf where words (of nodes from `node0` on) say that a token is not visible.
+    __device__ __forceinline__ void hide(const uint64_t* words, int node0, int first, int lane, float4v (&s)[NTT][RT]) const {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            uint64_t seen = node[t] >= 0 ? words[node[t] - node0] : 0;
+            seen >>= first + 4 * (lane >> 4);
+#pragma unroll
+            for (int i = 0; i < 4 * NTT; ++i)
+                if (!(seen >> (16 * (i >> 2) + (i & 3)) & 1)) s[i >> 2][t][i & 3] = -__builtin_huge_valf();
+        }
+    }
+    // Scores to probabilities: m moved where it has to be, what was gathered with it.
+    __device__ __forceinline__ void softmax(float scale_log2e, float4v (&s)[NTT][RT], half8v (&pr)[NTT / 2][RT]) {
+        // What a score's exponential is taken of, score * scale - m; the maximum of these says whether m has to move. (It
+        // begins where the row's first visible scores are, wherever that is.)
+        bool move = false;
+        float top[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4 * NTT; ++i) s[i >> 2][t][i & 3] = __builtin_fmaf(s[i >> 2][t][i & 3], scale_log2e, -m[t]);
+            top[t] = fmaxf(s[0][t][0], s[0][t][1]);
+#pragma unroll
+            for (int i = 2; i < 4 * NTT; i += 2) top[t] = fmaxf(fmaxf(top[t], s[i >> 2][t][i & 3]), s[i >> 2][t][(i & 3) + 1]);
+            move |= top[t] > (l[t][0] == 0.0f ? -__builtin_huge_valf() : kLazyLog2 + kHeadLog2);
+        }
+        if (__builtin_amdgcn_ballot_w64(move)) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const bool fresh = l[t][0] == 0.0f;
+                const float up = xor_max_16_32(top[t]) - kHeadLog2;
+                const float by = (fresh || up > 0.0f) && up > -__builtin_huge_valf() ? up : 0.0f;
+                const float f = fresh ? 1.0f : __builtin_amdgcn_exp2f(-by);
+                m[t] += by;
+                l[t] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d][t] *= f;
+#pragma unroll
+                for (int i = 0; i < 4 * NTT; ++i) s[i >> 2][t][i & 3] -= by;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4 * NTT; ++i) pr[i >> 3][t][i & 7] = E::round(__builtin_amdgcn_exp2f(s[i >> 2][t][i & 3]));
+    }
+    // P.V of the same tokens, V beginning at byte `at` of v; l sums the rounded probabilities by a product with ones, which
+    // adds up a row's four lanes as well.
+    __device__ __forceinline__ void gather(const char* v, uint32_t at, int first, int lane, const half8v (&pr)[NTT / 2][RT]) {
+        const int g = lane >> 4, r = lane & 15, vr = first + 4 * g + (r >> 2);
+        uint32_t va = at + (uint32_t)vr * D * 2 + ((((r & 3) >> 1) ^ (vr & (CH - 1))) << 4) + 8 * (r & 1);
+        asm volatile("" : "+v"(va));
+        half8v ones;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ones[i] = E::round(1.0f);
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int u = 0; u < NTT / 2; ++u) l[t] = E::mma32(ones, pr[u][t], l[t]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int u = 0; u < NTT / 2; ++u) {
+                // V^T: dim 16 d + r of tokens 32 u + 4 g + [0, 4) and that + 16
+                const char* src = v + (va ^ (d << 5)) + 32 * u * D * 2;
+                const s16x4v x0 = read_tr(src), x1 = read_tr(src + 16 * D * 2);
+                const half8v a = __builtin_bit_cast(half8v, (s16x8v)__builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int t = 0; t < RT; ++t) acc[d][t] = E::mma32(a, pr[u][t], acc[d][t]);
+            }
+        // Reads two dim tiles ahead.
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * NTT, 0);
+        __builtin_amdgcn_sched_group_barrier(kMfma, RT * NTT / 2, 0);
+#pragma unroll
+        for (int d = 0; d + 2 < DT; ++d) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, RT * NTT / 2, 0);
+            __builtin_amdgcn_sched_group_barrier(kDsRead, NTT, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, RT * NTT, 0);
+    }
+    // V of drafted tokens that is not finite was staged as 0 where a node does not see every token of the tile (0 * inf would be
+    // NaN for it): it counts for the rows that see it, whose probability of it is above 0. Tiles [from, to) of x's segment.
+    __device__ __forceinline__ void add_special(const Params& p, const Tile& x, const Row& row, int from, int to, int lane) {
+        const int open = x.open(p, row) / kTok;
+        int tok = (from > open ? from : open) * kTok;
+        tok = tok > row.ctx ? tok : row.ctx;
+        for (; tok < to * kTok && tok < x.end; ++tok) {
+            const int id = as_global(p.bt)[(int64_t)x.seg.b * p.bt_sb + (tok >> p.bs_shift)], n = tok - row.ctx;
+            if ((unsigned)id >= (unsigned)p.num_blocks) continue;
+            const auto* vp = as_global(p.v) + (int64_t)x.seg.kvh * p.kv_shead + id * p.kv_sblk +
+                             (tok & ((1 << p.bs_shift) - 1)) * D + 4 * (lane >> 4);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const bool see = node[t] >= 0 && (p.mask ? as_global(p.mask)[(int64_t)x.seg.b * p.mask_sb +
+                                                                             (int64_t)node[t] * p.mask_st + n] != 0
+                                                         : n <= node[t]);
+                if (see)
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        const half4v v = *(const global<half4v>*)(vp + 16 * d);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float f = E::widen(v[i]);
+                            if (!(__builtin_fabsf(f) < __builtin_huge_valf())) acc[d][t][i] += f;
+                        }
+                    }
+            }
+        }
+    }
+    // Rows row0 .. of the segment (the sums ls): as output where the piece is the whole segment, else to rows part0 .. of the
+    // partials.
+    __device__ __forceinline__ void store(const Params& p, const Seg& seg, bool complete, int row0, int64_t part0, const float (&ls)[RT],
+                                          int lane) const {
+        const int g = lane >> 4, r = lane & 15;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const float inv = ls[t] == 0.0f ? 0.0f : 1.0f / ls[t];
+            if (complete) {
+                const int rr = row0 + t * 16 + r, n = rr / p.G, h = seg.kvh * p.G + (rr - n * p.G);
+                if (n >= p.T) continue;
+                auto* dst = as_global(p.out) + (int64_t)seg.b * p.o_sb + (int64_t)n * p.o_st + (int64_t)h * p.o_sh + 4 * g;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    half4v o;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = ls[t] == 0.0f ? (_Float16)0.0f : E::round(acc[d][t][i] * inv);
+                    *(global<half4v>*)(dst + 16 * d) = o;
+                }
+            } else {
+                auto* dst = as_global(p.part) + (part0 + t * 16 + r) * (D + 4);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    *(global<float4v>*)(dst + 16 * d + 4 * g) = ls[t] == 0.0f ? float4v{} : acc[d][t] * inv;
+                if (g == 0) *(global<f32x2v>*)(dst + D) = f32x2v{m[t], ls[t]};
+            }
+        }
+    }
+};
+
+// A tile that some node does not see whole, by tid of NT threads in whole waves. V (at vt): 0 where there is no token, and
+// where a drafted token's is not finite; returns whether there was one. And who sees what, a bit a token: a wave takes a
+// node at a time, a lane a token, so the bytes of a mask row come in one load (as loads of each lane's own bytes two such
+// tiles at a row's end took 20 us).
+template <int D, bool BF16, int NT>
+__device__ __forceinline__ bool clean_tile(const Tile& x, const Rows& rows, bool bad, uint64_t* words, _Float16* vt, int tid) {
+    constexpr int CH = D / 8, WAVES = NT / 64;
+    const Params p = reload();
+    const Row row = rows.at(p, x.seg.b);
+    const auto* bt = as_global(p.bt) + (int64_t)x.seg.b * p.bt_sb;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), t0 = x.seg.tile * kTok;
+    const int first_node = x.seg.rt * p.R / p.G, last_node = (x.seg.rt * p.R + p.R - 1) / p.G;
+    const int nodes = (last_node < row.count ? last_node + 1 : row.count) - first_node;
+    const int tok = t0 + lane, n = tok - row.ctx;
+    bool there = tok < x.end;
+    if (bad && there) there = (unsigned)bt[tok >> p.bs_shift] < (unsigned)p.num_blocks;
+    const bool drafted = there && n >= 0;
+    constexpr int U = 8;
+    for (int i0 = wave; i0 < nodes; i0 += U * WAVES) {
+        uint8_t see[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * WAVES;
+            see[u] = 1;
+            if (p.mask && drafted && i < nodes)
+                see[u] = as_global(p.mask)[(int64_t)x.seg.b * p.mask_sb + (int64_t)(first_node + i) * p.mask_st + n];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * WAVES;
+            const uint64_t word = __builtin_amdgcn_ballot_w64(there && see[u] != 0 && (p.mask || n <= first_node + i));
+            if (lane == 0 && i < nodes) words[i] = word;
+        }
+    }
+    bool special = false;
+    const int drop = t0 + kTok > x.open(p, row) ? row.ctx : x.end;  // from this token on
+    for (int i = tid; i < kTok * CH; i += NT) {
+        const int tok = t0 + i / CH;
+        u32x4v* at = reinterpret_cast<u32x4v*>(vt) + i;
+        u32x4v v = *at;
+        if (tok >= x.end || (bad && (unsigned)bt[tok >> p.bs_shift] >= (unsigned)p.num_blocks)) v = u32x4v{0, 0, 0, 0};
+        else if (tok < drop || !drop_special<BF16>(v)) continue;
+        else special = true;
+        *at = v;
+    }
+    return special;
+}
+
+__device__ __forceinline__ void wait_for_loads() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The tiles of a workgroup.
+struct Range {
+    int w, lo, hi, total, workers;
+    // Consecutive ranges on one XCD (workgroups go round the 8 XCDs): the tiles of query rows of a kv-head meet in its L2.
+    __device__ __forceinline__ Range(const Params& p, int total) : total(total), workers(workers_of(p, total)) {
+        const int per = (workers + kXcds - 1) / kXcds;
+        w = (int)blockIdx.x % kXcds * per + (int)blockIdx.x / kXcds;
+        lo = hi = 0;
+        if ((int)blockIdx.x / kXcds >= per || w >= workers) return;
+        lo = range_lo(w, total, workers), hi = range_lo(w + 1, total, workers);
+    }
+};
+
+// Tiles [t0, t1) of x's segment, which begin `first` tiles into the range, as wave rw over query rows has them (with the sums ls);
+// and, with the first of them, how many pieces the segment has, for the launch that joins them.
+template <int D, bool BF16, int RT, int NTT>
+__device__ __forceinline__ void store_piece(const Params& p, const Queries<D, BF16, RT, NTT>& rs, const Tile& x, int t0, int t1,
+                                            const Range& range, int first, int rw, int tid, const float (&ls)[RT]) {
+    const int slot = 2 * range.w + (first == 0 ? 0 : 1);
+    rs.store(p, x.seg, t0 == 0 && t1 == x.ntiles, x.seg.rt * p.R + rw * RT * 16, (int64_t)slot * p.R + rw * RT * 16, ls, tid & 63);
+    if (t0 == 0 && tid == 0) {
+        const int pieces = worker_of(range.lo + first + x.ntiles - 1, range.total, range.workers) - range.w + 1;
+        *(global<i32x2v>*)(as_global(p.pieces) + ((int64_t)x.seg.b * p.Hkv + x.seg.kvh) * p.nrt + x.seg.rt) = i32x2v{slot, pieces};
+    }
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+
 // D: head dim. RT: 16-row query tiles per wave. RW x TW: waves over query rows and over a tile's tokens.
 template <int D, bool BF16, int RT, int RW, int TW>
 __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_kernel(Params p) {
-    using E = Elt<BF16>;
     constexpr int NT = 64 * RW * TW;
-    constexpr int KC = D / 32;                // 32-dim steps of a score
-    constexpr int DT = D / 16;                // 16-dim output tiles
-    constexpr int CH = D / 8;                 // 16-byte chunks per token
-    constexpr int RPL = 64 / CH;              // tokens per load instruction of a wave (1 KiB)
-    constexpr int P = kTok / RPL / (RW * TW); // load instructions per wave and tile, of K and of V each
-    constexpr int NTT = kTok / 16 / TW;       // 16-token tiles per wave
-    constexpr int R = 16 * RT * RW;
-    static_assert(NTT % 2 == 0 && P * RPL * RW * TW == kTok, "tile split");
+    constexpr int NTT = kTok / 16 / TW;  // 16-token tiles per wave
+    constexpr int R = 16 * RT * RW, TB = kTok * D * 2;
+    static_assert(NTT % 2 == 0, "tile split");
     __shared__ __attribute__((aligned(16))) _Float16 ks[2][kTok * D];
     __shared__ __attribute__((aligned(16))) _Float16 vs[2][kTok * D];
     __shared__ uint64_t words[R];  // of a masked tile: bit j of word n: token j is visible to the n-th node of the query rows
@@ -291,330 +666,81 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rw = wave % RW, tw = wave / RW;
-    const int lane = tid & 63, g = lane >> 4, r = lane & 15;
+    const int lane = tid & 63;
 
     Rows rows;
     rows.read(p, lane);
-    const int total = rows.total;
-    const int workers = workers_of(p, total);
-    // Consecutive ranges on one XCD (workgroups go round the 8 XCDs): the tiles of query rows of a kv-head meet in its L2.
-    const int per = (workers + kXcds - 1) / kXcds;
-    const int w = (int)blockIdx.x % kXcds * per + (int)blockIdx.x / kXcds;
-    if ((int)blockIdx.x / kXcds >= per || w >= workers || total == 0) return;
-    const int lo = range_lo(w, total, workers), hi = range_lo(w + 1, total, workers);
-    if (lo >= hi) return;
+    const Range range(p, rows.total);
+    if (range.lo >= range.hi) return;
     if (tid < 2) bad_step[tid] = 0;
     if (tid == 0) nf_step = 0;
-    int step = 1;  // number of the tile at work, buffer step & 1
-    const int bs = 1 << p.bs_shift;
-    const uint32_t ks_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&ks[0][0];
-    const uint32_t vs_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&vs[0][0];
+    int step = 1, left = range.hi - range.lo;  // number of the tile at work (buffer step & 1), tiles from it on
+    const uint32_t ks_at = lds_address(&ks[0][0]), vs_at = lds_address(&vs[0][0]);
 
-    half8v ones;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ones[i] = E::round(1.0f);
-
-    // A tile and what it belongs to.
-    struct Tile {
-        Seg seg;
-        Row row;
-        int end, ntiles;  // of the segment: tokens that it attends over, tiles
-        int64_t head;     // elements before its kv-head in a block
-        const global<const int32_t>* bt;
-    };
-    auto enter = [&](const Params& p, Tile& x) MX_INLINE {
-        x.row = rows.at(p, x.seg.b);
-        x.end = visible_end(p, x.row, x.seg.rt);
-        x.ntiles = (x.end + kTok - 1) / kTok;
-        x.head = (int64_t)x.seg.kvh * p.kv_shead;
-        x.bt = as_global(p.bt) + (int64_t)x.seg.b * p.bt_sb;
-    };
-    auto advance = [&](Tile& x) MX_INLINE {  // to the next one; there is one
-        if (++x.seg.tile < x.ntiles) return;
-        x.seg.tile = 0;
-        const Params p = reload();
-        do {
-            if (++x.seg.rt == p.nrt) {
-                x.seg.rt = 0;
-                if (++x.seg.kvh == p.Hkv) {
-                    x.seg.kvh = 0;
-                    ++x.seg.b;
-                }
-            }
-            enter(p, x);
-        } while (x.ntiles == 0);
-    };
-
-        // Loads go from memory to LDS without a register: a lane's 16 bytes land at 16 times the lane behind the instruction's
-        // place, so the permutation of a token's chunks is in the addresses that the lanes read from.
-        struct Ids {
-            int id[P];
-        };
-        auto ids_of = [&](const Tile& x) MX_INLINE {
-            Ids s;
-            const int last_tok = x.end - 1;
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                int tok = x.seg.tile * kTok + (wave * P + i) * RPL + lane / CH;
-                tok = tok < last_tok ? tok : last_tok;  // past the end: the last token again
-                s.id[i] = x.bt[tok >> p.bs_shift];
-            }
-            return s;
-        };
-        // Tile x, number st, into buffer `st & 1`.
-        auto issue = [&](int st, const Tile& x, Ids ids) MX_INLINE {
-            const int buf = st & 1;
-            const _Float16 *kb = p.k + x.head, *vb = p.v + x.head;
-            const int last_tok = x.end - 1;
-            bool bad = false;
-            // All ids are waited for here: one by one, the waits would count the tile's own loads in between.
-#pragma unroll
-            for (int i = 0; i < P; ++i) asm volatile("" : "+v"(ids.id[i]));
-            constexpr int N = P < 4 ? P : 4;
-#pragma unroll
-            for (int i0 = 0; i0 < P; i0 += N) {
-                const char *kf[N], *vf[N];
-#pragma unroll
-                for (int i = i0; i < i0 + N; ++i) {
-                    const int rr = (wave * P + i) * RPL + lane / CH;
-                    int tok = x.seg.tile * kTok + rr;
-                    tok = tok < last_tok ? tok : last_tok;
-                    const bool inside = (unsigned)ids.id[i] < (unsigned)p.num_blocks;
-                    bad |= !inside;
-                    const int64_t off =
-                        (inside ? ids.id[i] : 0) * p.kv_sblk + (tok & (bs - 1)) * D + 8 * (lane % CH ^ (rr & (CH - 1)));
-                    kf[i - i0] = reinterpret_cast<const char*>(kb + off);
-                    vf[i - i0] = reinterpret_cast<const char*>(vb + off);
-                }
-                const uint32_t at = (uint32_t)(buf * kTok * D + (wave * P + i0) * 512) * 2;
-                load_to_lds<N>(kf, ks_at + at);
-                load_to_lds<N>(vf, vs_at + at);
-            }
-            if (bad) {
-                bad_step[buf] = st;
-                if (p.err) atomicOr(p.err, 4);
-            }
-        };
-        // The compiler does not track those loads.
-        auto arrived = [&]() MX_INLINE {
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-            __builtin_amdgcn_sched_barrier(0);
-            __syncthreads();
-        };
-    Tile ahead;  // the next one to load, with its block ids
-    ahead.seg = rows.locate(p, lo, lane);
-    enter(p, ahead);
+    Loader<D, RW * TW> ahead;
+    ahead.x.seg = rows.locate(p, range.lo, lane);
+    ahead.x.enter(p, rows);
+    ahead.look_up(p, lane);
+    Tile cur = ahead.x;
     __syncthreads();  // bad_step
-    Ids ids = ids_of(ahead);
-    issue(step, ahead, ids);
-    Tile cur = ahead;
-    if (lo + 1 < hi) {
-        advance(ahead);
-        ids = ids_of(ahead);
-    }
+    auto issue = [&](int st, int more) MX_INLINE {  // tile number st, `more` behind it
+        if (ahead.issue(p, ks_at + (st & 1) * TB, vs_at + (st & 1) * TB, wave, lane)) bad_step[st & 1] = st;
+        if (more) ahead.advance(rows, p.bs_shift, lane);
+    };
+    // The compiler does not track those loads.
+    auto arrived = [&]() MX_INLINE {
+        wait_for_loads();
+        __syncthreads();
+    };
+    issue(step, left - 1);
     arrived();
 
     // A piece after the other: the tiles of one segment in this range. The first tile of the next one is on its way already.
-    for (int at = lo; at < hi;) {
-        const Seg seg = cur.seg;
-        const Row row = cur.row;
-        const int end = cur.end, ntiles = cur.ntiles, t0 = seg.tile;
-        const int t1 = ntiles - t0 < hi - at ? ntiles : t0 + (hi - at);
-        const int step0 = step;
-        const int safe = row.ctx < end ? row.ctx > 0 ? row.ctx : 0 : end;  // tokens below it are context, and there
-        // A tile with drafted tokens, an end or a bad block. V: 0 where there is no token, and where a drafted token's is not
-        // finite (see nf_step). And who sees what, a bit a token: a wave takes a node at a time, a lane a token, so the bytes of
-        // a mask row come in one load (as loads of each lane's own bytes two such tiles at a row's end took 20 us).
-        auto clean = [&](int st, int t) MX_INLINE {
+    for (;;) {
+        const int t0 = cur.seg.tile, t1 = cur.ntiles - t0 < left ? cur.ntiles : t0 + left, step0 = step;
+        Queries<D, BF16, RT, NTT> rs;
+        int open;
+        {
             const Params p = reload();
-            const auto* bt = as_global(p.bt) + (int64_t)seg.b * p.bt_sb;
-            const int first_node = seg.rt * R / p.G, last_row_node = (seg.rt * R + R - 1) / p.G;
-            const int nodes = (last_row_node < row.count ? last_row_node + 1 : row.count) - first_node;
-            // Every row of the workgroup sees every token below this.
-            const int64_t open64 = (int64_t)row.ctx + (p.mask ? 0 : first_node + 1);
-            const int open = open64 < end ? (int)open64 : end;
-            const int buf = st & 1;
-            const bool bad = bad_step[buf] == st;
-            if (t * kTok + kTok > open || bad) {
-                const int tok = t * kTok + lane, n = tok - row.ctx;
-                bool there = tok < end;
-                if (bad && there) there = (unsigned)bt[tok >> p.bs_shift] < (unsigned)p.num_blocks;
-                const bool drafted = there && n >= 0;
-                constexpr int U = 8;
-                for (int i0 = wave; i0 < nodes; i0 += U * RW * TW) {
-                    uint8_t see[U];
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const int i = i0 + u * RW * TW;
-                        see[u] = 1;
-                        if (p.mask && drafted && i < nodes)
-                            see[u] = as_global(p.mask)[(int64_t)seg.b * p.mask_sb + (int64_t)(first_node + i) * p.mask_st + n];
-                    }
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const int i = i0 + u * RW * TW;
-                        const uint64_t word = __builtin_amdgcn_ballot_w64(there && see[u] != 0 && (p.mask || n <= first_node + i));
-                        if (lane == 0 && i < nodes) words[i] = word;
-                    }
-                }
-            }
-            for (int i = tid; i < kTok * CH; i += NT) {
-                const int tok = t * kTok + i / CH;
-                u32x4v* at = reinterpret_cast<u32x4v*>(&vs[buf][0]) + i;
-                u32x4v x = *at;
-                if (tok >= end || (bad && (unsigned)bt[tok >> p.bs_shift] >= (unsigned)p.num_blocks)) x = u32x4v{0, 0, 0, 0};
-                else if (tok < row.ctx || !drop_special<BF16>(x)) continue;
-                else nf_step = st;
-                *at = x;
-            }
-            __syncthreads();
-        };
-
-        const Params here = reload();
-        const int first_node = seg.rt * R / here.G;
-        // Query fragments: lane l holds dims 32 c + 8 (l / 16) + [0, 8) of row l % 16 of each of the wave's tiles.
-        half8v qf[RT][KC];
-        int node[RT];  // -1: no such row
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const int rr = seg.rt * R + (rw * RT + t) * 16 + r;
-            const int n = rr / here.G, h = seg.kvh * here.G + (rr - n * here.G);
-            node[t] = n < row.count ? n : -1;
-            const auto* qp = as_global(here.q) + (int64_t)seg.b * here.q_sb + (int64_t)h * here.q_sh + (int64_t)n * here.q_st + 8 * g;
-#pragma unroll
-            for (int kk = 0; kk < KC; ++kk)
-                qf[t][kk] = node[t] >= 0 ? __builtin_bit_cast(half8v, *(const global<u32x4v>*)(qp + 32 * kk))
-                                         : half8v{};
+            const Row row = rows.at(p, cur.seg.b);
+            open = cur.open(p, row);
+            rs.load(p, cur.seg, row.count, cur.seg.rt * R + rw * RT * 16, lane);
+            // Waited for here: in the loop the wait would be there every time, and for the loads of the next tile.
+            wait_for_loads();
         }
-        float m[RT];
-        float4v l[RT], acc[DT][RT];  // (l's four are the same)
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            m[t] = 0.0f;
-            l[t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int d = 0; d < DT; ++d) acc[d][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        // Every row of the wave sees every token below `whole`.
-        const int64_t whole64 = (int64_t)row.ctx + (here.mask ? 0 : (seg.rt * R + rw * RT * 16) / here.G + 1);
-        const int whole = whole64 < end ? (int)whole64 : end;
-
-        auto compute = [&](bool masked, int st, int tile) MX_INLINE {
-            const int buf = st & 1;
-            const int tbase = tw * (kTok / TW);  // the wave's first token in the tile
-            // Byte addresses in LDS: a row's chunks are permuted by an exclusive or, and so are the addresses of one lane's
-            // reads; rows 16 apart are permuted alike. (The empty asm keeps the compiler from holding all of them in registers.)
-            uint32_t ka = (uint32_t)(buf * kTok * D + (tbase + r) * D) * 2 + ((g ^ (r & (CH - 1))) << 4);
-            const int vr = tbase + 4 * g + (r >> 2);
-            uint32_t va = (uint32_t)(buf * kTok * D + vr * D) * 2 + ((((r & 3) >> 1) ^ (vr & (CH - 1))) << 4) + 8 * (r & 1);
-            asm volatile("" : "+v"(ka), "+v"(va));
-            const char* kt = reinterpret_cast<const char*>(&ks[0][0]);
-            const char* vt = reinterpret_cast<const char*>(&vs[0][0]);
-            float4v s[NTT][RT];
-#pragma unroll
-            for (int kk = 0; kk < KC; ++kk)
-#pragma unroll
-                for (int i = 0; i < NTT; ++i) {
-                    const half8v a = __builtin_bit_cast(
-                        half8v, *reinterpret_cast<const u32x4v*>(kt + (ka ^ (kk << 6)) + 16 * i * D * 2));
-#pragma unroll
-                    for (int t = 0; t < RT; ++t)
-                        s[i][t] = E::mma32(a, qf[t][kk], kk ? s[i][t] : float4v{0.0f, 0.0f, 0.0f, 0.0f});
-                }
+        for (;;) {
+            if (left > 1) issue(step + 1, left - 2);
+            const int buf = step & 1;
+            const bool bad = bad_step[buf] == step, masked = cur.seg.tile * kTok + kTok > open || bad;
             if (masked) {
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    uint64_t seen = node[t] >= 0 ? words[node[t] - first_node] : 0;
-                    seen >>= tbase + 4 * g;
-#pragma unroll
-                    for (int i = 0; i < 4 * NTT; ++i)
-                        if (!(seen >> (16 * (i >> 2) + (i & 3)) & 1)) s[i >> 2][t][i & 3] = -__builtin_huge_valf();
-                }
+                if (clean_tile<D, BF16, NT>(cur, rows, bad, words, &vs[buf][0], tid)) nf_step = step;
+                __syncthreads();
             }
-            // What a score's exponential is taken of, score * scale - m; the maximum of these says whether m has to move. (It
-            // begins where the row's first visible scores are, wherever that is.)
-            bool move = false;
-            float top[RT];
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-#pragma unroll
-                for (int i = 0; i < 4 * NTT; ++i) s[i >> 2][t][i & 3] = __builtin_fmaf(s[i >> 2][t][i & 3], p.scale_log2e, -m[t]);
-                top[t] = fmaxf(s[0][t][0], s[0][t][1]);
-#pragma unroll
-                for (int i = 2; i < 4 * NTT; i += 2) top[t] = fmaxf(fmaxf(top[t], s[i >> 2][t][i & 3]), s[i >> 2][t][(i & 3) + 1]);
-                move |= top[t] > (l[t][0] == 0.0f ? -__builtin_huge_valf() : kLazyLog2 + kHeadLog2);
-            }
-            if (__builtin_amdgcn_ballot_w64(move)) {
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    const bool fresh = l[t][0] == 0.0f;
-                    const float up = xor_max_16_32(top[t]) - kHeadLog2;
-                    const float by = (fresh || up > 0.0f) && up > -__builtin_huge_valf() ? up : 0.0f;
-                    const float f = fresh ? 1.0f : __builtin_amdgcn_exp2f(-by);
-                    m[t] += by;
-                    l[t] *= f;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[d][t] *= f;
-#pragma unroll
-                    for (int i = 0; i < 4 * NTT; ++i) s[i >> 2][t][i & 3] -= by;
-                }
-            }
-            // l sums the rounded probabilities: a product with ones, which adds up a row's four lanes as well.
+            float4v s[NTT][RT];
             half8v pr[NTT / 2][RT];
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4 * NTT; ++i) pr[i >> 3][t][i & 7] = E::round(__builtin_amdgcn_exp2f(s[i >> 2][t][i & 3]));
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int u = 0; u < NTT / 2; ++u) l[t] = E::mma32(ones, pr[u][t], l[t]);
-            typedef short s16x8v __attribute__((ext_vector_type(8)));
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int u = 0; u < NTT / 2; ++u) {
-                    // V^T: dim 16 d + r of tokens 32 u + 4 g + [0, 4) and that + 16
-                    const char* src = vt + (va ^ (d << 5)) + 32 * u * D * 2;
-                    const s16x4v x0 = read_tr(src), x1 = read_tr(src + 16 * D * 2);
-                    const s16x8v x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    const half8v a = __builtin_bit_cast(half8v, x);
-#pragma unroll
-                    for (int t = 0; t < RT; ++t) acc[d][t] = E::mma32(a, pr[u][t], acc[d][t]);
-                }
-        };
-        for (int t = t0;; ++t) {
-            const bool more = at + (t + 1 - t0) < hi;  // tiles of this range, of this piece or a later one
-            if (more) {
-                issue(step + 1, ahead, ids);
-                if (at + (t + 2 - t0) < hi) {
-                    advance(ahead);
-                    ids = ids_of(ahead);
-                }
-            }
-            const bool bad = bad_step[step & 1] == step;
-            if (t * kTok + kTok > safe || bad) clean(step, t);
-            compute(t * kTok + kTok > whole || bad, step, t);
-            if (t + 1 == t1) break;
+            rs.scores(reinterpret_cast<const char*>(&ks[0][0]), buf * TB, tw * (kTok / TW), lane, s);
+            if (masked) rs.hide(words, cur.seg.rt * R / reload().G, tw * (kTok / TW), lane, s);
+            rs.softmax(p.scale_log2e, s, pr);
+            rs.gather(reinterpret_cast<const char*>(&vs[0][0]), buf * TB, tw * (kTok / TW), lane, pr);
+            if (cur.seg.tile + 1 == t1) break;
             arrived();
-            ++step;
+            ++cur.seg.tile, ++step, --left;
         }
 
         float ls[RT];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) ls[t] = node[t] < 0 ? 0.0f : l[t][0];
+        for (int t = 0; t < RT; ++t) ls[t] = rs.node[t] < 0 ? 0.0f : rs.l[t][0];
         // The waves over tokens meet in the buffers of the last tile (the others may be loading).
         if constexpr (TW > 1) {
-            static_assert(TW == 2 && RW <= 2 && sizeof(ks[0]) >= sizeof(float4v) * 64 * RT * DT, "exchange");
+            static_assert(TW == 2 && RW <= 2 && sizeof(ks[0]) >= sizeof(float4v) * 64 * RT * (D / 16), "exchange");
             float4v* xch = reinterpret_cast<float4v*>(rw == 0 ? &ks[step & 1][0] : &vs[step & 1][0]) + lane;
             __syncthreads();
             if (tw == 1) {
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) xch[(d * RT + t) * 64] = acc[d][t];
-                    xml[(rw * RT + t) * 64 + lane] = float2{m[t], ls[t]};
+                    for (int d = 0; d < D / 16; ++d) xch[(d * RT + t) * 64] = rs.acc[d][t];
+                    xml[(rw * RT + t) * 64 + lane] = float2{rs.m[t], ls[t]};
                 }
             }
             __syncthreads();
@@ -623,85 +749,24 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
                 for (int t = 0; t < RT; ++t) {
                     const float2 other = xml[(rw * RT + t) * 64 + lane];
                     // A wave that has seen nothing has no reference.
-                    const float ma = ls[t] == 0.0f ? kLowest : m[t], mb = other.y == 0.0f ? kLowest : other.x;
-                    m[t] = fmaxf(ma, mb);
-                    const float fa = __builtin_amdgcn_exp2f(ma - m[t]), fb = __builtin_amdgcn_exp2f(mb - m[t]);
+                    const float ma = ls[t] == 0.0f ? kLowest : rs.m[t], mb = other.y == 0.0f ? kLowest : other.x;
+                    rs.m[t] = fmaxf(ma, mb);
+                    const float fa = __builtin_amdgcn_exp2f(ma - rs.m[t]), fb = __builtin_amdgcn_exp2f(mb - rs.m[t]);
                     ls[t] = ls[t] * fa + other.y * fb;
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[d][t] = acc[d][t] * fa + xch[(d * RT + t) * 64] * fb;
+                    for (int d = 0; d < D / 16; ++d) rs.acc[d][t] = rs.acc[d][t] * fa + xch[(d * RT + t) * 64] * fb;
                 }
-            }
-        }
-        const Params p = reload();
-        if (tw == 0 && nf_step >= step0) {
-            // V of drafted tokens that is not finite was staged as 0 (0 * inf would be NaN for rows that do not see it): it
-            // counts for the rows that see it, whose probability of it is above 0.
-            const auto* bt = as_global(p.bt) + (int64_t)seg.b * p.bt_sb;
-            auto visible = [&](int t, int tok) MX_INLINE {  // token of tile t's row to this lane
-                const int n = tok - row.ctx;
-                if (tok >= end || node[t] < 0) return false;
-                if (n < 0) return true;
-                if (!p.mask) return n <= node[t];
-                return as_global(p.mask)[(int64_t)seg.b * p.mask_sb + (int64_t)node[t] * p.mask_st + n] != 0;
-            };
-            const int from = t0 * kTok > row.ctx ? t0 * kTok : row.ctx > 0 ? row.ctx : 0;
-            const int to = t1 * kTok < end ? t1 * kTok : end;
-            for (int tok = from; tok < to; ++tok) {
-                const int id = bt[tok >> p.bs_shift];
-                if ((unsigned)id >= (unsigned)p.num_blocks) continue;
-                const auto* vp = as_global(p.v) + (int64_t)seg.kvh * p.kv_shead + id * p.kv_sblk + (tok & (bs - 1)) * D + 4 * g;
-#pragma unroll
-                for (int t = 0; t < RT; ++t)
-                    if (visible(t, tok))
-#pragma unroll
-                        for (int d = 0; d < DT; ++d) {
-                            const half4v x = *(const global<half4v>*)(vp + 16 * d);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float f = E::widen(x[i]);
-                                if (!(__builtin_fabsf(f) < __builtin_huge_valf())) acc[d][t][i] += f;
-                            }
-                        }
             }
         }
         if (tw == 0) {
-            const bool complete = t0 == 0 && t1 == ntiles;
-            const int slot = 2 * w + (at == lo ? 0 : 1);
-            if (t0 == 0 && tid == 0) {
-                const int pieces = worker_of(at + ntiles - 1, total, workers) - w + 1;
-                *(global<i32x2v>*)(as_global(p.pieces) + (seg.b * p.Hkv + seg.kvh) * p.nrt + seg.rt) = i32x2v{slot, pieces};
-            }
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                const int rr = (rw * RT + t) * 16 + r;
-                const float inv = ls[t] == 0.0f ? 0.0f : 1.0f / ls[t];
-                if (complete) {
-                    const int n = (seg.rt * R + rr) / p.G, h = seg.kvh * p.G + (seg.rt * R + rr - n * p.G);
-                    if (n >= p.T) continue;
-                    auto* dst = as_global(p.out) + (int64_t)seg.b * p.o_sb + (int64_t)n * p.o_st + (int64_t)h * p.o_sh + 4 * g;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        half4v o;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[i] = ls[t] == 0.0f ? (_Float16)0.0f : E::round(acc[d][t][i] * inv);
-                        *(global<half4v>*)(dst + 16 * d) = o;
-                    }
-                } else {
-                    auto* dst = as_global(p.part) + ((int64_t)slot * R + rr) * (D + 4);
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-                        *(global<float4v>*)(dst + 16 * d + 4 * g) = ls[t] == 0.0f ? float4v{} : acc[d][t] * inv;
-                    if (g == 0) *(global<f32x2v>*)(dst + D) = f32x2v{m[t], ls[t]};
-                }
-            }
+            const Params p = reload();
+            if (nf_step >= step0) rs.add_special(p, cur, rows.at(p, cur.seg.b), t0, t1, lane);
+            store_piece<D, BF16, RT, NTT>(p, rs, cur, t0, t1, range, step0 - 1, rw, tid, ls);
         }
-        at += t1 - t0;
-        if (at < hi) {
-            cur.seg.tile = t1 - 1;
-            advance(cur);
-            arrived();
-            ++step;
-        }
+        if (left == 1) break;
+        cur.next_segment(rows);
+        arrived();
+        ++step, --left;
     }
 }
 
