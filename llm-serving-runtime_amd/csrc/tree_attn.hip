@@ -37,7 +37,6 @@ namespace tree {
 constexpr int kTok = 64;  // tokens per tile
 constexpr int kCus = 256;
 constexpr int kXcds = 8;
-constexpr int kMinTiles = 2;       // a workgroup's range is at least this long where the whole allows
 constexpr float kLazyLog2 = 8.0f;  // rescale only when the running max rises by more than 2^8
 // The reference of the exponentials stands this much below the maximum it was taken from: p reaches 2^15 and no more, so an fp16 p
 // loses nothing of a token that counts 2^-21 of the largest, and 2^-32 at most of one that counts less. (At the maximum
@@ -184,10 +183,7 @@ struct Rows {
     }
 };
 
-__device__ __forceinline__ int workers_of(const Params& p, int total) {
-    const int most = total / kMinTiles > 1 ? total / kMinTiles : 1;
-    return p.workers < most ? p.workers : most;
-}
+__device__ __forceinline__ int workers_of(const Params& p, int total) { return p.workers < total ? p.workers : total; }
 // a / b, in 32 bits where they do (64-bit division is a long sequence, and every workgroup begins with two).
 __device__ __forceinline__ int quotient(uint64_t a, int b) {
     return a >> 32 ? (int)(a / (uint32_t)b) : (int)((uint32_t)a / (uint32_t)b);
@@ -668,6 +664,9 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     const int rw = wave % RW, tw = wave / RW;
     const int lane = tid & 63;
 
+    // Waves 4 .. 7 share the four SIMDs with waves 0 .. 3: they issue their loads behind the scores, when the others have the
+    // matrix cores, and not ahead of them (8 rows of 64 nodes: 73 against 75 us).
+    const bool late = RW * TW == 8 && wave >= 4;
     Rows rows;
     rows.read(p, lane);
     const Range range(p, rows.total);
@@ -709,7 +708,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             wait_for_loads();
         }
         for (;;) {
-            if (left > 1) issue(step + 1, left - 2);
+            if (left > 1 && !late) issue(step + 1, left - 2);
             const int buf = step & 1;
             const bool bad = bad_step[buf] == step, masked = cur.seg.tile * kTok + kTok > open || bad;
             if (masked) {
@@ -719,6 +718,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             float4v s[NTT][RT];
             half8v pr[NTT / 2][RT];
             rs.scores(reinterpret_cast<const char*>(&ks[0][0]), buf * TB, tw * (kTok / TW), lane, s);
+            if (left > 1 && late) issue(step + 1, left - 2);
             if (masked) rs.hide(words, cur.seg.rt * R / reload().G, tw * (kTok / TW), lane, s);
             rs.softmax(p.scale_log2e, s, pr);
             rs.gather(reinterpret_cast<const char*>(&vs[0][0]), buf * TB, tw * (kTok / TW), lane, pr);
@@ -858,7 +858,7 @@ static Plan plan_of(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t max_to
     else p = {2, 8, 1};
     p.R = 16 * p.rt * p.rw;
     p.nrt = (int)ceil_div(rows, p.R);
-    const int64_t most = B * Hkv * p.nrt * ceil_div(max_tokens, kTok) / kMinTiles + 1;
+    const int64_t most = B * Hkv * p.nrt * ceil_div(max_tokens, kTok);
     const int64_t full = p.rw * p.tw == 8 ? kCus : 2 * kCus;
     p.workers = (int)ceil_div(most < full ? most : full, kXcds) * kXcds;
     return p;

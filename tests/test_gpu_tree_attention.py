@@ -177,6 +177,18 @@ def test_what_masked_places_hold_has_no_effect(dtype, t, group):
     c.check(c.run(_tree(parents)), see)
 
 
+@pytest.mark.parametrize("d,group,t", [(64, 4, 200), (128, 1, 300)])
+def test_infinities_in_a_chain_of_several_tiles_of_query_rows(d, group, t):
+    """Nodes of a later tile of query rows see a token whole that hides from the first ones'."""
+    c = Case(23, [t + 30, t + 101], t, group=group, d=d)
+    for row, ctx in enumerate((30, 101)):
+        for node, sign in ((5, 1), (t // 2, 1), (t - 1, 1)):
+            b, o = c.slot(row, ctx + node)
+            c.v[b, 0, o, 3 + node % 5] = sign * float("inf")
+            c.v[b, 1, o, 60] = float("nan")
+    c.check(c.run())
+
+
 def test_both_infinities_in_one_sum_give_nan():
     c = Case(10, lens=[40], t=6, d=64)
     for node, x in ((1, float("inf")), (2, -float("inf"))):
