@@ -35,6 +35,7 @@ namespace mx {
 namespace tree {
 
 constexpr int kTok = 64;  // tokens per tile
+constexpr int kPieceTiles = 1;  // a segment counts for its tiles and this: its query rows, its output
 constexpr int kCus = 256;
 constexpr int kXcds = 8;
 constexpr float kLazyLog2 = 8.0f;  // rescale only when the running max rises by more than 2^8
@@ -110,10 +111,15 @@ __device__ __forceinline__ int visible_end(const Params& p, const Row& w, int rt
 __device__ __forceinline__ int seg_tiles(const Params& p, const Row& w, int rt) {
     return (visible_end(p, w, rt) + kTok - 1) / kTok;
 }
-// Tiles of one kv-head of a row.
-__device__ __forceinline__ int head_tiles(const Params& p, const Row& w) {
+// What a segment counts for when the whole is cut into ranges.
+__device__ __forceinline__ int seg_units(const Params& p, const Row& w, int rt) {
+    const int n = seg_tiles(p, w, rt);
+    return n == 0 ? 0 : n + kPieceTiles;
+}
+// ... and one kv-head of a row.
+__device__ __forceinline__ int head_units(const Params& p, const Row& w) {
     int n = 0;
-    for (int rt = 0; rt < p.nrt; ++rt) n += seg_tiles(p, w, rt);
+    for (int rt = 0; rt < p.nrt; ++rt) n += seg_units(p, w, rt);
     return n;
 }
 
@@ -133,7 +139,7 @@ struct Seg {
 // The rows of a batch as a wave holds them: up to 64 in its lanes, read once; of more, each when it is asked for.
 struct Rows {
     Row mine;   // row `lane` (B <= 64)
-    int tiles;  // of it
+    int units;  // of it
     int incl;   // of it and those before it
     int total;  // of all (below 2^30, checked on the host)
     __device__ __forceinline__ void read(const Params& p, int lane) {
@@ -141,8 +147,8 @@ struct Rows {
         total = 0;
         for (int b0 = 0; b0 < p.B; b0 += 64) {
             if (b0 + lane < p.B) mine = row_of(p, b0 + lane);
-            tiles = b0 + lane < p.B ? head_tiles(p, mine) * p.Hkv : 0;
-            incl = wave_scan(tiles, lane);
+            units = b0 + lane < p.B ? head_units(p, mine) * p.Hkv : 0;
+            incl = wave_scan(units, lane);
             total += __builtin_amdgcn_readlane(incl, 63);
         }
     }
@@ -151,12 +157,12 @@ struct Rows {
         return Row{__builtin_amdgcn_readlane(mine.len, b), __builtin_amdgcn_readlane(mine.ctx, b),
                    __builtin_amdgcn_readlane(mine.count, b)};
     }
-    // The segment that holds tile x of all (x < total), and x's index in it.
+    // The segment that holds unit x of all (x < total), and x's index in it: a tile, or behind the last one.
     __device__ __forceinline__ Seg locate(const Params& p, int x, int lane) const {
-        int n = tiles, up = incl;
+        int n = units, up = incl;
         for (int b0 = 0; b0 < p.B; b0 += 64) {
             if (p.B > 64) {
-                n = b0 + lane < p.B ? head_tiles(p, row_of(p, b0 + lane)) * p.Hkv : 0;
+                n = b0 + lane < p.B ? head_units(p, row_of(p, b0 + lane)) * p.Hkv : 0;
                 up = wave_scan(n, lane);
             }
             const int sum = __builtin_amdgcn_readlane(up, 63);
@@ -172,7 +178,7 @@ struct Rows {
                 s.rt = 0;
                 if (p.nrt > 1) {
                     const Row w = at(p, s.b);
-                    for (int m; s.rt + 1 < p.nrt && x >= (m = seg_tiles(p, w, s.rt)); ++s.rt) x -= m;
+                    for (int m; s.rt + 1 < p.nrt && x >= (m = seg_units(p, w, s.rt)); ++s.rt) x -= m;
                 }
                 s.tile = x;
                 return s;
@@ -189,7 +195,7 @@ __device__ __forceinline__ int quotient(uint64_t a, int b) {
     return a >> 32 ? (int)(a / (uint32_t)b) : (int)((uint32_t)a / (uint32_t)b);
 }
 __device__ __forceinline__ int range_lo(int w, int total, int workers) { return quotient((uint64_t)w * total, workers); }
-// The worker that holds tile x.
+// The worker that holds unit x.
 __device__ __forceinline__ int worker_of(int x, int total, int workers) {
     return quotient((uint64_t)(x + 1) * workers - 1, total);
 }
@@ -313,6 +319,7 @@ struct Loader {
     int64_t head;     // elements before its kv-head in a block
     int ids, coming;  // the 64 block ids around it, and those to take their place
     bool change;
+    int left;         // units of the range from this tile on
 
     __device__ __forceinline__ void look_up(const Params& p, int lane) {
         head = (int64_t)x.seg.kvh * p.kv_shead;
@@ -321,7 +328,13 @@ struct Loader {
         change = true;
     }
     __device__ __forceinline__ void advance(const Rows& rows, int bs_shift, int lane) {
-        if (++x.seg.tile >= x.ntiles) x.next_segment(rows);
+        --left;
+        if (++x.seg.tile >= x.ntiles) {
+            left -= kPieceTiles;
+            if (left <= 0) return;
+            x.next_segment(rows);
+        }
+        if (left <= 0) return;
         if ((x.seg.tile * kTok >> bs_shift & 63) == 0) look_up(reload(), lane);
     }
     // The tile to ks_at and vs_at; returns whether a block lies outside the pool (its tokens read block 0).
@@ -615,7 +628,7 @@ __device__ __forceinline__ void wait_for_loads() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// The tiles of a workgroup.
+// The units of a workgroup.
 struct Range {
     int w, lo, hi, total, workers;
     // Consecutive ranges on one XCD (workgroups go round the 8 XCDs): the tiles of query rows of a kv-head meet in its L2.
@@ -628,7 +641,7 @@ struct Range {
     }
 };
 
-// Tiles [t0, t1) of x's segment, which begin `first` tiles into the range, as wave rw over query rows has them (with the sums ls);
+// Tiles [t0, t1) of x's segment, which begin `first` units into the range, as wave rw over query rows has them (with the sums ls);
 // and, with the first of them, how many pieces the segment has, for the launch that joins them.
 template <int D, bool BF16, int RT, int NTT>
 __device__ __forceinline__ void store_piece(const Params& p, const Queries<D, BF16, RT, NTT>& rs, const Tile& x, int t0, int t1,
@@ -673,30 +686,38 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     if (range.lo >= range.hi) return;
     if (tid < 2) bad_step[tid] = 0;
     if (tid == 0) nf_step = 0;
-    int step = 1, left = range.hi - range.lo;  // number of the tile at work (buffer step & 1), tiles from it on
+    int step = 1;  // number of the tile at work, buffer step & 1
     const uint32_t ks_at = lds_address(&ks[0][0]), vs_at = lds_address(&vs[0][0]);
 
     Loader<D, RW * TW> ahead;
     ahead.x.seg = rows.locate(p, range.lo, lane);
     ahead.x.enter(p, rows);
+    ahead.left = range.hi - range.lo;
+    if (ahead.x.seg.tile >= ahead.x.ntiles) {
+        ahead.left -= ahead.x.ntiles + kPieceTiles - ahead.x.seg.tile;
+        if (ahead.left <= 0) return;
+        ahead.x.next_segment(rows);
+    }
     ahead.look_up(p, lane);
     Tile cur = ahead.x;
+    int left = ahead.left;  // units from the tile at work on
     __syncthreads();  // bad_step
-    auto issue = [&](int st, int more) MX_INLINE {  // tile number st, `more` behind it
+    auto issue = [&](int st) MX_INLINE {  // tile number st
         if (ahead.issue(p, ks_at + (st & 1) * TB, vs_at + (st & 1) * TB, wave, lane)) bad_step[st & 1] = st;
-        if (more) ahead.advance(rows, p.bs_shift, lane);
+        ahead.advance(rows, p.bs_shift, lane);
     };
     // The compiler does not track those loads.
     auto arrived = [&]() MX_INLINE {
         wait_for_loads();
         __syncthreads();
     };
-    issue(step, left - 1);
+    issue(step);
     arrived();
 
     // A piece after the other: the tiles of one segment in this range. The first tile of the next one is on its way already.
     for (;;) {
         const int t0 = cur.seg.tile, t1 = cur.ntiles - t0 < left ? cur.ntiles : t0 + left, step0 = step;
+        const int first = range.hi - range.lo - left;
         Queries<D, BF16, RT, NTT> rs;
         int open;
         {
@@ -708,7 +729,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             wait_for_loads();
         }
         for (;;) {
-            if (left > 1 && !late) issue(step + 1, left - 2);
+            if (ahead.left > 0 && !late) issue(step + 1);
             const int buf = step & 1;
             const bool bad = bad_step[buf] == step, masked = cur.seg.tile * kTok + kTok > open || bad;
             if (masked) {
@@ -718,13 +739,13 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
             float4v s[NTT][RT];
             half8v pr[NTT / 2][RT];
             rs.scores(reinterpret_cast<const char*>(&ks[0][0]), buf * TB, tw * (kTok / TW), lane, s);
-            if (left > 1 && late) issue(step + 1, left - 2);
+            if (ahead.left > 0 && late) issue(step + 1);
             if (masked) rs.hide(words, cur.seg.rt * R / reload().G, tw * (kTok / TW), lane, s);
             rs.softmax(p.scale_log2e, s, pr);
             rs.gather(reinterpret_cast<const char*>(&vs[0][0]), buf * TB, tw * (kTok / TW), lane, pr);
             if (cur.seg.tile + 1 == t1) break;
             arrived();
-            ++cur.seg.tile, ++step, --left;
+            ++cur.seg.tile, ++step;
         }
 
         float ls[RT];
@@ -761,12 +782,13 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
         if (tw == 0) {
             const Params p = reload();
             if (nf_step >= step0) rs.add_special(p, cur, rows.at(p, cur.seg.b), t0, t1, lane);
-            store_piece<D, BF16, RT, NTT>(p, rs, cur, t0, t1, range, step0 - 1, rw, tid, ls);
+            store_piece<D, BF16, RT, NTT>(p, rs, cur, t0, t1, range, first, rw, tid, ls);
         }
-        if (left == 1) break;
+        left -= t1 - t0 + kPieceTiles;
+        if (left <= 0) break;
         cur.next_segment(rows);
         arrived();
-        ++step, --left;
+        ++step;
     }
 }
 
@@ -858,7 +880,7 @@ static Plan plan_of(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t max_to
     else p = {2, 8, 1};
     p.R = 16 * p.rt * p.rw;
     p.nrt = (int)ceil_div(rows, p.R);
-    const int64_t most = B * Hkv * p.nrt * ceil_div(max_tokens, kTok);
+    const int64_t most = B * Hkv * p.nrt * (ceil_div(max_tokens, kTok) + kPieceTiles);
     const int64_t full = p.rw * p.tw == 8 ? kCus : 2 * kCus;
     p.workers = (int)ceil_div(most < full ? most : full, kXcds) * kXcds;
     return p;
@@ -928,7 +950,7 @@ extern "C" int mx_tree_attn(const uint16_t* q, int64_t q_sb, int64_t q_sh, int64
     if (max_tokens > (1 << 30) || G * T > (1 << 24) || (int64_t)B * Hkv > (1 << 24))
         return fail(MX_ERR_UNSUPPORTED, "%s: more tokens or rows than 32-bit numbers hold", what);
     const tree::Plan pl = tree::plan_of(B, T, Hkv, G, max_tokens);
-    if ((double)B * Hkv * pl.nrt * ceil_div(max_tokens, tree::kTok) > (double)(1 << 30) ||
+    if ((double)B * Hkv * pl.nrt * (ceil_div(max_tokens, tree::kTok) + tree::kPieceTiles) > (double)(1 << 30) ||
         (double)B * Hkv * pl.nrt * pl.R * (D / 4) > 4.0e9)
         return fail(MX_ERR_UNSUPPORTED, "%s: more tiles than 32-bit numbers hold", what);
     const size_t need = mx_tree_attn_workspace_bytes(B, T, Hq, Hkv, D, max_blocks, block_size);
