@@ -35,7 +35,11 @@ namespace mx {
 namespace tree {
 
 constexpr int kTok = 64;  // tokens per tile
-constexpr int kPieceTiles = 1;  // a segment counts for its tiles and this: its query rows, its output
+// A segment counts for its tiles and this many more: its query rows, its masked tiles, its output (13,000 cycles next to a tile's
+// 5,000, and the memory rests). 32 rows of U[128, 4096] tokens with 16 nodes each take 80 us where it counts for nothing (the
+// ranges over the shortest rows hold six segments and end last), 70, 66, 64, 59, 56, 56, 58 with 1, 2, 3, 4, 6, 8, 10; 8 rows of
+// 64 nodes 74, 72, 71, 69, 69, 67, 70, 71.
+constexpr int kPieceTiles = 6;
 constexpr int kCus = 256;
 constexpr int kXcds = 8;
 constexpr float kLazyLog2 = 8.0f;  // rescale only when the running max rises by more than 2^8
