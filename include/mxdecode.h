@@ -687,9 +687,10 @@ int mx_kv_keep_tokens(void* k, void* v, int32_t token_bytes, int64_t layer_strid
  * the pool is skipped and sets bit 2 of the nullable err word. D in {64, 128},
  * block_size in {4, 8, 16, 32}, any GQA group, any T; scale > 0, a normal fp32
  * number also times log2(e). Strides non-negative multiples of 8, pointers 16-byte
- * aligned. flags: MX_PA_BF16 and MX_PA_SHARED_BLOCKS (rows may share pages; the
- * result is the same). workspace: at least mx_tree_attn_workspace_bytes, 16-byte
- * aligned, not shared by calls that overlap (its contents need not be kept). */
+ * aligned. flags: MX_PA_BF16 and MX_PA_SHARED_BLOCKS (rows share pages, which then
+ * are read through the caches; the result is the same). workspace: at least
+ * mx_tree_attn_workspace_bytes, 16-byte aligned, not shared by calls that overlap
+ * (its contents need not be kept). */
 size_t mx_tree_attn_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_blocks,
                                     int32_t block_size);
 int mx_tree_attn(const uint16_t* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const uint16_t* k, const uint16_t* v,

@@ -207,32 +207,40 @@ __device__ __forceinline__ int worker_of(int x, int total, int workers) {
 // N times 16 bytes per lane from memory to LDS: load i's of lane l, at from[i], to `to` + 1024 i + 16 l (`to` the same in all
 // lanes). As a builtin the loads would be waited for ahead of every later read of LDS, whatever that reads; so the caller
 // waits (vmcnt) before the barrier that hands the tile over. Nothing is written to a register. An instruction's offset counts
-// on both sides, so M0, which holds the place in LDS, is set once, and left as it was.
-template <int N>
+// on both sides, so M0, which holds the place in LDS, is set once, and left as it was. STREAM: past the caches.
+#define MX_LOADS_TO_LDS(NT)                                                                                               \
+    if constexpr (N == 1)                                                                                                 \
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off" NT "\n\t"       \
+                     "s_mov_b32 m0, %0"                                                                                   \
+                     : "=&s"(was)                                                                                         \
+                     : "s"(at), "v"(from[0])                                                                              \
+                     : "memory");                                                                                         \
+    else if constexpr (N == 2)                                                                                            \
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off" NT "\n\t"       \
+                     "global_load_lds_dwordx4 %3, off offset:1024" NT "\n\ts_mov_b32 m0, %0"                              \
+                     : "=&s"(was)                                                                                         \
+                     : "s"(at), "v"(from[0]), "v"(from[1] - 1024)                                                         \
+                     : "memory");                                                                                         \
+    else                                                                                                                  \
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off" NT "\n\t"       \
+                     "global_load_lds_dwordx4 %3, off offset:1024" NT                                                     \
+                     "\n\tglobal_load_lds_dwordx4 %4, off offset:2048" NT                                                 \
+                     "\n\tglobal_load_lds_dwordx4 %5, off offset:3072" NT "\n\ts_mov_b32 m0, %0"                          \
+                     : "=&s"(was)                                                                                         \
+                     : "s"(at), "v"(from[0]), "v"(from[1] - 1024), "v"(from[2] - 2048), "v"(from[3] - 3072)               \
+                     : "memory")
+template <int N, bool STREAM>
 __device__ __forceinline__ void load_to_lds(const char* const (&from)[N], uint32_t to) {
     static_assert(N == 1 || N == 2 || N == 4, "offsets are below 4096");
     uint32_t was;
     const int at = __builtin_amdgcn_readfirstlane((int)to);
-    if constexpr (N == 1)
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
-                     "s_mov_b32 m0, %0"
-                     : "=&s"(was)
-                     : "s"(at), "v"(from[0])
-                     : "memory");
-    else if constexpr (N == 2)
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
-                     "global_load_lds_dwordx4 %3, off offset:1024\n\ts_mov_b32 m0, %0"
-                     : "=&s"(was)
-                     : "s"(at), "v"(from[0]), "v"(from[1] - 1024)
-                     : "memory");
-    else
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
-                     "global_load_lds_dwordx4 %3, off offset:1024\n\tglobal_load_lds_dwordx4 %4, off offset:2048\n\t"
-                     "global_load_lds_dwordx4 %5, off offset:3072\n\ts_mov_b32 m0, %0"
-                     : "=&s"(was)
-                     : "s"(at), "v"(from[0]), "v"(from[1] - 1024), "v"(from[2] - 2048), "v"(from[3] - 3072)
-                     : "memory");
+    if constexpr (STREAM) {
+        MX_LOADS_TO_LDS(" nt");
+    } else {
+        MX_LOADS_TO_LDS("");
+    }
 }
+#undef MX_LOADS_TO_LDS
 
 typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
 typedef float f32x2v __attribute__((ext_vector_type(2)));
@@ -312,7 +320,7 @@ struct Tile {
 // times the lane behind the instruction's place, so the permutation of a token's chunks is in the addresses that the lanes
 // read from. Block ids are held 64 at a time, one a lane (an instruction's 1 KiB holds tokens of two blocks at most), and read
 // ahead of the tile that needs them: ids read a tile at a time, by scalar loads, took 1300 of a tile's 5600 cycles.
-template <int D, int WAVES>
+template <int D, int WAVES, bool STREAM>
 struct Loader {
     static constexpr int CH = D / 8;                // 16-byte chunks per token
     static constexpr int RPL = 64 / CH;             // tokens per load instruction of a wave
@@ -375,8 +383,8 @@ struct Loader {
                 vf[i - i0] = reinterpret_cast<const char*>(vb + off);
             }
             const uint32_t at = (uint32_t)(wave * P + i0) * 1024;
-            load_to_lds<N>(kf, ks_at + at);
-            load_to_lds<N>(vf, vs_at + at);
+            load_to_lds<N, STREAM>(kf, ks_at + at);
+            load_to_lds<N, STREAM>(vf, vs_at + at);
         }
         if (bad && p.err) atomicOr(p.err, 4);
         return bad;
@@ -662,8 +670,9 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
 
-// D: head dim. RT: 16-row query tiles per wave. RW x TW: waves over query rows and over a tile's tokens.
-template <int D, bool BF16, int RT, int RW, int TW>
+// D: head dim. RT: 16-row query tiles per wave. RW x TW: waves over query rows and over a tile's tokens. STREAM: K and V are read
+// past the caches.
+template <int D, bool BF16, int RT, int RW, int TW, bool STREAM>
 __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_kernel(Params p) {
     constexpr int NT = 64 * RW * TW;
     constexpr int NTT = kTok / 16 / TW;  // 16-token tiles per wave
@@ -693,7 +702,7 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     int step = 1;  // number of the tile at work, buffer step & 1
     const uint32_t ks_at = lds_address(&ks[0][0]), vs_at = lds_address(&vs[0][0]);
 
-    Loader<D, RW * TW> ahead;
+    Loader<D, RW * TW, STREAM> ahead;
     ahead.x.seg = rows.locate(p, range.lo, lane);
     ahead.x.enter(p, rows);
     ahead.left = range.hi - range.lo;
@@ -892,14 +901,20 @@ static Plan plan_of(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t max_to
 
 static size_t part_bytes(const Plan& p, int D) { return (size_t)2 * p.workers * p.R * (D + 4) * sizeof(float); }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool STREAM>
 static void launch(const Plan& pl, const Params& p, hipStream_t st) {
     const dim3 grid((unsigned)p.workers), block(64 * pl.rw * pl.tw);
-    if (pl.rt == 1) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 1, 1, 2>), grid, block, 0, st, p);
-    else if (pl.rw == 1) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 1, 2>), grid, block, 0, st, p);
-    else if (pl.rw == 2) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 2, 2>), grid, block, 0, st, p);
-    else if (pl.rw == 4) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 4, 1>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 8, 1>), grid, block, 0, st, p);
+    if (pl.rt == 1) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 1, 1, 2, STREAM>), grid, block, 0, st, p);
+    else if (pl.rw == 1) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 1, 2, STREAM>), grid, block, 0, st, p);
+    else if (pl.rw == 2) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 2, 2, STREAM>), grid, block, 0, st, p);
+    else if (pl.rw == 4) hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 4, 1, STREAM>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((tree_attn_kernel<D, BF16, 2, 8, 1, STREAM>), grid, block, 0, st, p);
+}
+
+template <int D, bool BF16>
+static void launch(const Plan& pl, const Params& p, bool stream, hipStream_t st) {
+    if (stream) launch<D, BF16, true>(pl, p, st);
+    else launch<D, BF16, false>(pl, p, st);
     const int64_t segs = (int64_t)p.B * p.Hkv * p.nrt;
     const int groups = 256 / (D / 4);
     int sp = 1;
@@ -978,14 +993,18 @@ extern "C" int mx_tree_attn(const uint16_t* q, int64_t q_sb, int64_t q_sh, int64
     p.pieces = reinterpret_cast<int2*>(static_cast<char*>(workspace) + tree::part_bytes(pl, D));
     p.err = err;
     p.workers = pl.workers, p.nrt = pl.nrt, p.R = pl.R;
+    // Read once, K and V only push out of the caches what is read again, and each other: 32 rows of U[128, 4096] tokens 73 us a call
+    // through the caches, 64 past them, one row of 131,071 tokens 119 and 110. Blocks that rows share are read again, and so are
+    // those of several tiles of query rows.
+    const bool past = pl.nrt == 1 && !(flags & MX_PA_SHARED_BLOCKS);
     hipStream_t st = as_stream(stream);
     const bool bf16 = flags & MX_PA_BF16;
     if (D == 64) {
-        if (bf16) tree::launch<64, true>(pl, p, st);
-        else tree::launch<64, false>(pl, p, st);
+        if (bf16) tree::launch<64, true>(pl, p, past, st);
+        else tree::launch<64, false>(pl, p, past, st);
     } else {
-        if (bf16) tree::launch<128, true>(pl, p, st);
-        else tree::launch<128, false>(pl, p, st);
+        if (bf16) tree::launch<128, true>(pl, p, past, st);
+        else tree::launch<128, false>(pl, p, past, st);
     }
     return check_launch(what);
 }
