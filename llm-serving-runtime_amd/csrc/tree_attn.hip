@@ -6,6 +6,12 @@
 // visible to node i where j < ctx (ctx = seq_lens[b] - counts[b]), or where it is node j - ctx and mask[b, i, j - ctx] is
 // set (no mask: j - ctx <= i).
 //
+// Bound: few query rows read K and V from HBM (4 D bytes a token and head); 256 query rows need as long for the products,
+// and there the softmax, the addresses and the exchange through LDS come on top, since the waves of a SIMD hide little of each other's.
+// Measured, both launches: 32 rows of U[128, 4096] tokens with 16 nodes (G 4, D 128, 279 MB) 65 us, 4.3 TB/s; one row of 131,071
+// tokens with 25 nodes (537 MB) 111 us, 4.8 TB/s; 8 rows of U[4096, 8192] tokens with 64 nodes 78 us, 670 TFLOP/s; two
+// chunks of 509 tokens over U[2048, 4096] 88 us, 690 TFLOP/s; one row of 705 tokens with 5 nodes 16 us.
+//
 // Work decomposition. The G * T query rows of a (row, kv-head) share its K and V. A segment is a (row, kv-head,
 // tile of R query rows), heads of a node next to each other; it holds ceil(visible tokens / 64) tiles. All segments form
 // one sequence of tiles that is cut into equal ranges, one per workgroup, so that the chip drains evenly whatever
@@ -805,7 +811,9 @@ __global__ __launch_bounds__(64 * RW * TW, RW * TW == 2 ? 1 : 2) void tree_attn_
     }
 }
 
-// Joins the pieces of the segments that more than one workgroup cut, and clears rows of segments without tokens.
+// Joins the pieces of the segments that more than one workgroup cut, and clears rows of segments without tokens. Bound by the
+// pieces' bytes, 4 (D + 4) a query row and piece: 383 pieces of 256 rows of a chunk (52 MB) 12 us, 4.3 TB/s; a few pieces 4 us, of
+// which a launch and two dependent loads are most.
 // A workgroup of 256 threads has D / 4 lanes per query row (4 dims each) and shares a row's pieces among SP groups of
 // lanes: RPG = 256 / (D / 4) / SP query rows at a time.
 template <int D, bool BF16>
@@ -882,7 +890,12 @@ struct Plan {
     int R, nrt, workers;
 };
 
-// Query rows per workgroup: as few wasted rows as the tiles allow up to 256, so that K and V are read once.
+// Query rows per workgroup: as few wasted rows as the tiles allow up to 256, so that K and V are read once. The next larger shape
+// takes, on 32 rows of U[128, 4096] tokens, 54 us for 16 query rows (this one 50), 59 for 32 (55) and 66 for 64 (58), and 159
+// for 100 query rows over 131,071 tokens (102); workgroups of 128 query rows for 256 of them, which read K and V twice, 79 on 8
+// rows of U[4096, 8192] tokens (72), 88 on a chunk (76).
+// Workgroups: what the CUs hold at once, two by the LDS or one of eight waves. Half as many take 71 and 125 us on the 32 rows with 16 nodes
+// and on the long row (58, 102), twice as many 70 and 117, and 81 on the 8 rows with 64 nodes (69): more pieces to begin and to join.
 static Plan plan_of(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t max_tokens) {
     Plan p{};
     const int64_t rows = G * T;
@@ -917,6 +930,8 @@ static void launch(const Plan& pl, const Params& p, bool stream, hipStream_t st)
     else launch<D, BF16, false>(pl, p, st);
     const int64_t segs = (int64_t)p.B * p.Hkv * p.nrt;
     const int groups = 256 / (D / 4);
+    // A row's pieces are shared among groups of lanes where there are more than four to a segment: 64 pieces take 9 us so, 19 one
+    // after the other. With few the blocks that hold more rows each end as early (7 us either way at two pieces).
     int sp = 1;
     while (sp < groups && p.workers > 4 * sp * segs) sp *= 2;
     const int64_t blocks = segs * ceil_div(p.R, groups / sp);

@@ -33,7 +33,9 @@ constexpr int kVec = 8;                    // neighbouring logits per thread
 constexpr int kBlock = kThreads * kVec;    // logits per step of a workgroup
 constexpr int kMaxSlices = 64;             // one lane of a wave each
 constexpr int kMaxNodes = 1024;
-constexpr int kFill = 512;  // workgroups
+// Workgroups, two a CU: 256 take 66 us for 32 rows of 16 nodes (128,256 logits), 1024 take 73, these 57; one row of 5 nodes
+// (151,936) takes 19 us with 64 slices, 21 with 32.
+constexpr int kFill = 512;
 constexpr int kMaxVocab = 1 << 22;
 constexpr int kMaxPolls = 1 << 23;         // seconds: a wait that long means a broken launch; the row then ends with -1
 
@@ -776,7 +778,10 @@ struct Plan {
 };
 
 // Slices: enough workgroups to fill the chip, each with at least a step of logits. The first launch takes node 0, and as many more
-// as cost it about what an exchange takes (3 us, 4 million logits).
+// as cost it about what the walk's passes over those that its path visits would (a pass and its exchange 10 us, twice that with
+// draft logits): 4 million logits, 12 with draft logits. Both launches together: one row of 5 nodes 27 us with node 0 alone, 19
+// with all; 32 rows of 16 nodes 57, 55, 59, 58, 65 us with 4, 8, 12, 16, 24 million, 8 rows of 16 nodes 41, 46, 49, -, 52; 8
+// chains of 7 with draft logits 60 us with node 0 alone, 58, 50, 41, 41, 41 with those numbers, 4 chains of 24 87, 73, 59, -, 77.
 static Plan plan_of(int64_t B, int64_t T, int64_t V, bool draft) {
     Plan p{};
     int64_t s = kFill / B;
@@ -785,7 +790,7 @@ static Plan plan_of(int64_t B, int64_t T, int64_t V, bool draft) {
     s = s < most ? s : most;
     p.len = (int)(ceil_div(ceil_div(V, s), kVec) * kVec);
     p.slices = (int)ceil_div(V, p.len);
-    const int64_t f = (4 << 20) / (B * V * (draft ? 2 : 1));
+    const int64_t f = draft ? (12 << 20) / (B * V * 2) : (4 << 20) / (B * V);
     p.first = (int)(f < 1 ? 1 : f < T ? f : T);
     p.words_at = (size_t)B * p.first * p.slices * sizeof(Part);
     p.ticket_at = p.words_at + (size_t)B * 2 * p.slices * 4 * sizeof(uint64_t);
