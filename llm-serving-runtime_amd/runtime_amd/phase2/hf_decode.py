@@ -172,7 +172,8 @@ def speculative_decode(model, pool: GpuKVBlockPool, prompts: list[torch.Tensor],
     :func:`prompt_lookup` drafts. Returns the rows' ``steps + 1`` new tokens and the forwards that took. At
     ``temperature`` 0 they are the tokens of :func:`greedy_decode`; above it samples of the model, with uniform
     numbers from ``generator``. A row needs blocks for its prompt, its tokens and two drafts (a row that is
-    done is drafted behind its last one until all are).
+    done is drafted behind its last one until all are). Drafted tokens outside the vocabulary and logits that
+    hold no distribution (a NaN) raise ``ValueError``.
     """
     if len(prompts) != len(block_ids_rows) or not prompts:
         raise ValueError("one block-id row per prompt is required")
@@ -203,10 +204,19 @@ def speculative_decode(model, pool: GpuKVBlockPool, prompts: list[torch.Tensor],
     rows = [ids.tolist() + new for ids, new in zip(prompts, verdict.tokens.tolist())]
     lengths = [len(row) for row in rows]
     forwards = 0
+    vocab = model.get_input_embeddings().num_embeddings
+
+    def check_tokens() -> None:
+        if any(row[-1] < 0 for row in rows):
+            raise ValueError("the model's logits hold no distribution")
+
+    check_tokens()
     while min(len(row) - n for row, n in zip(rows, lengths)) < steps:
         drafted = prompt_lookup(rows, size) if propose is None else propose(rows)
         drafted, draft_logits = drafted if isinstance(drafted, tuple) else (drafted, None)
         tokens = torch.as_tensor(drafted, dtype=torch.int64).to(device)
+        if tokens.numel() and not 0 <= int(tokens.min()) <= int(tokens.max()) < vocab:
+            raise ValueError(f"drafted tokens must be in [0, {vocab})")
         # A row that is done stays where it is: its nodes are drafted in the same place again and none is kept.
         done = [len(row) - n >= steps for row, n in zip(rows, lengths)]
         logits = paged_draft_step(model, cache, tokens, tree)
@@ -219,6 +229,7 @@ def speculative_decode(model, pool: GpuKVBlockPool, prompts: list[torch.Tensor],
         cache.keep_drafted(verdict.path, counts)
         for row, new, n in zip(rows, verdict.tokens.tolist(), counts.tolist()):
             row += new[:n]
+        check_tokens()
     cache.draft_tree = None
     pool.check_write_errors()
     return [row[n - 1:n + steps] for row, n in zip(rows, lengths)], forwards

@@ -144,3 +144,21 @@ def test_refusals(setup):
         paged_draft_step(model, cache, torch.zeros(2, 3, dtype=torch.int64, device=DEV), DraftTree.chain(4, DEV))
     with pytest.raises(RuntimeError, match="follows"):
         cache.keep_drafted(torch.zeros(2, 3, dtype=torch.int32, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV))
+
+
+def test_tokens_outside_the_vocabulary_and_logits_without_a_distribution(setup):
+    """Neither reaches the embedding."""
+    from runtime_amd.phase2.hf_decode import speculative_decode
+
+    model, make_pool, prompts, blocks, _ = setup
+    for bad in (-1, 1024):
+        with pytest.raises(ValueError, match="drafted tokens"):
+            speculative_decode(model, make_pool(), prompts, blocks, 4, 2, lambda rows: [[r[-1], bad] for r in rows])
+    kept = model.lm_head.weight.data
+    try:
+        model.lm_head.weight.data = torch.full_like(kept, float("nan"))
+        for temperature in (0.0, 1.0):
+            with pytest.raises(ValueError, match="distribution"):
+                speculative_decode(model, make_pool(), prompts, blocks, 4, 2, temperature=temperature)
+    finally:
+        model.lm_head.weight.data = kept
