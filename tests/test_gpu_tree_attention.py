@@ -256,6 +256,26 @@ def test_many_short_rows():
     c.check(c.run())
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_random_shapes(seed):
+    """Row counts, nodes, heads, lengths (0 and below the nodes too), masks, pages and types drawn together."""
+    rng = np.random.default_rng(1000 + seed)
+    t = int(rng.choice([1, 2, 3, 5, 9, 17, 33, 70]))
+    hkv, group = int(rng.integers(1, 4)), int(rng.choice([1, 2, 3, 4, 7, 8]))
+    rows = int(rng.integers(1, max(2, min(70, 2400 // (t * hkv * group)))))
+    lens = [int(rng.choice([0, t, int(rng.integers(0, 80)), int(rng.integers(t, t + 700))])) for _ in range(rows)]
+    c = Case(seed, lens, t, hkv=hkv, group=group, d=int(rng.choice([64, 128])), bs=int(rng.choice([4, 8, 16, 32])),
+             dtype=torch.bfloat16 if rng.random() < 0.4 else torch.float16)
+    counts = [int(rng.integers(-1, t + 2)) for _ in range(rows)] if rng.random() < 0.5 else None
+    see = None
+    tree = _modules()[2].chain(t, DEV, counts=None if counts is None else torch.tensor(counts))
+    if rng.random() < 0.7:
+        parents = [_random_parents(t, rng, 5) for _ in range(rows)]
+        see = np.stack([oracle.visible(p) for p in parents])
+        tree = _tree(parents, counts)
+    c.check(c.run(tree, shared=bool(rng.random() < 0.3)), see, counts)
+
+
 def test_strides_layouts_and_shared_blocks():
     c = Case(15, lens=[90, 33], t=9, d=128, layout="split")
     want = c.run()
