@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define MX_ABI_VERSION 22
+#define MX_ABI_VERSION 23
 
 typedef enum mx_status {
     MX_OK = 0,
@@ -419,6 +419,16 @@ int mx_kv_append(const uint16_t* k_new, const uint16_t* v_new, int64_t new_sb, i
                  int32_t max_blocks, const int32_t* start_pos, uint16_t* k_pool, uint16_t* v_pool, int64_t kv_sblk,
                  int64_t kv_shead, int32_t block_size, int32_t num_pool_blocks, int32_t* err, uint8_t* used_blocks,
                  void* stream);
+
+/* mx_kv_append of the first counts[b] (int32 [B] on the device; below 0: none, above
+ * T: all) of each row's T tokens. The others have no slot: nothing of them is
+ * written, marked or reported. No reference counterpart (its batched writes have
+ * as many tokens in every row). */
+int mx_kv_append_counts(const uint16_t* k_new, const uint16_t* v_new, int64_t new_sb, int64_t new_sh, int64_t new_st,
+                        int32_t B, int32_t T, int32_t Hkv, int32_t D, const int32_t* block_tables, int64_t bt_sb,
+                        int32_t max_blocks, const int32_t* start_pos, const int32_t* counts, uint16_t* k_pool,
+                        uint16_t* v_pool, int64_t kv_sblk, int64_t kv_shead, int32_t block_size,
+                        int32_t num_pool_blocks, int32_t* err, uint8_t* used_blocks, void* stream);
 
 /* The first S tokens of B rows of the pool, contiguous: k_out and v_out
  * [B, Hkv, S, D] (16-bit elements) from per-layer views of the layout

@@ -76,6 +76,7 @@ struct AppendParams {
     int bs, num_pool_blocks;
     int32_t* err;
     uint8_t* used;  // optional [num_pool_blocks] map: 1 where a token was written
+    const int32_t* counts;  // optional: tokens of each row (NULL: T)
 };
 
 // One thread per 8-element chunk of one (row, token, kv-head); K and V share the slot.
@@ -89,6 +90,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendParams p, int
     r /= p.Hkv;
     const int t = (int)(r % p.T);
     const int b = (int)(r / p.T);
+    if (p.counts && t >= p.counts[b]) return;
     const int64_t dst = slot_offset(p.bt, p.bt_sb, p.max_blocks, b, p.start[b] + t, p.bs, p.num_pool_blocks, p.sblk,
                                     p.shead, h, p.D);
     if (dst < 0) {
@@ -597,6 +599,24 @@ __global__ __launch_bounds__(kArgThreads) void argmax_kernel(const uint16_t* __r
 
 inline bool a16(const void* p) { return aligned(p, 16); }
 
+static int append_common(const char* what, const AppendParams& p, int32_t B, void* stream) {
+    if (B < 0 || p.T < 0) return fail(MX_ERR_INVALID, "%s: B and T must be >= 0 (B=%d T=%d)", what, B, p.T);
+    if (B == 0 || p.T == 0) return MX_OK;
+    if (!p.k_new || !p.v_new || !p.bt || !p.start || !p.k_pool || !p.v_pool)
+        return fail(MX_ERR_NULL, "%s: null pointer", what);
+    if (p.Hkv <= 0 || p.D <= 0 || p.D % 8 || p.bs <= 0 || p.max_blocks <= 0 || p.num_pool_blocks <= 0)
+        return fail(MX_ERR_INVALID, "%s: need Hkv, max_blocks, block_size, pool > 0 and D %% 8 == 0 "
+                                    "(Hkv=%d D=%d bs=%d max_blocks=%d pool=%d)", what, p.Hkv, p.D, p.bs, p.max_blocks,
+                    p.num_pool_blocks);
+    if (p.sb % 8 || p.sh % 8 || p.st % 8 || p.sblk % 8 || p.shead % 8 || !a16(p.k_new) || !a16(p.v_new) ||
+        !a16(p.k_pool) || !a16(p.v_pool))
+        return fail(MX_ERR_ALIGNMENT, "%s: states and pool need 16-byte aligned rows", what);
+    const int64_t total = (int64_t)B * p.T * p.Hkv * (p.D / 8);
+    hipLaunchKernelGGL(kv_append_kernel, dim3((unsigned)ceil_div(total, kThreads)), dim3(kThreads), 0, as_stream(stream), p,
+                       total);
+    return check_launch(what);
+}
+
 }  // namespace glue
 }  // namespace mx
 
@@ -608,24 +628,24 @@ extern "C" int mx_kv_append(const uint16_t* k_new, const uint16_t* v_new, int64_
                             uint16_t* v_pool, int64_t kv_sblk, int64_t kv_shead, int32_t block_size,
                             int32_t num_pool_blocks, int32_t* err, uint8_t* used_blocks, void* stream) {
     clear_error();
-    if (B < 0 || T < 0) return fail(MX_ERR_INVALID, "mx_kv_append: B and T must be >= 0 (B=%d T=%d)", B, T);
-    if (B == 0 || T == 0) return MX_OK;
-    if (!k_new || !v_new || !block_tables || !start_pos || !k_pool || !v_pool)
-        return fail(MX_ERR_NULL, "mx_kv_append: null pointer");
-    if (Hkv <= 0 || D <= 0 || D % 8 || block_size <= 0 || max_blocks <= 0 || num_pool_blocks <= 0)
-        return fail(MX_ERR_INVALID, "mx_kv_append: need Hkv, max_blocks, block_size, pool > 0 and D %% 8 == 0 "
-                                    "(Hkv=%d D=%d bs=%d max_blocks=%d pool=%d)", Hkv, D, block_size, max_blocks,
-                    num_pool_blocks);
-    if (new_sb % 8 || new_sh % 8 || new_st % 8 || kv_sblk % 8 || kv_shead % 8 || !glue::a16(k_new) ||
-        !glue::a16(v_new) || !glue::a16(k_pool) || !glue::a16(v_pool))
-        return fail(MX_ERR_ALIGNMENT, "mx_kv_append: states and pool need 16-byte aligned rows");
-    glue::AppendParams p{k_new, v_new, new_sb, new_sh, new_st, T, Hkv, D, block_tables, bt_sb, max_blocks,
-                         start_pos, k_pool, v_pool, kv_sblk, kv_shead, block_size, num_pool_blocks, err,
-                         used_blocks};
-    const int64_t total = (int64_t)B * T * Hkv * (D / 8);
-    hipLaunchKernelGGL(glue::kv_append_kernel, dim3((unsigned)ceil_div(total, glue::kThreads)), dim3(glue::kThreads),
-                       0, as_stream(stream), p, total);
-    return check_launch("mx_kv_append");
+    const glue::AppendParams p{k_new, v_new, new_sb, new_sh, new_st, T, Hkv, D, block_tables, bt_sb, max_blocks,
+                               start_pos, k_pool, v_pool, kv_sblk, kv_shead, block_size, num_pool_blocks, err,
+                               used_blocks, nullptr};
+    return glue::append_common("mx_kv_append", p, B, stream);
+}
+
+extern "C" int mx_kv_append_counts(const uint16_t* k_new, const uint16_t* v_new, int64_t new_sb, int64_t new_sh,
+                                   int64_t new_st, int32_t B, int32_t T, int32_t Hkv, int32_t D,
+                                   const int32_t* block_tables, int64_t bt_sb, int32_t max_blocks,
+                                   const int32_t* start_pos, const int32_t* counts, uint16_t* k_pool, uint16_t* v_pool,
+                                   int64_t kv_sblk, int64_t kv_shead, int32_t block_size, int32_t num_pool_blocks,
+                                   int32_t* err, uint8_t* used_blocks, void* stream) {
+    clear_error();
+    if (B > 0 && T > 0 && !counts) return fail(MX_ERR_NULL, "mx_kv_append_counts: null pointer");
+    const glue::AppendParams p{k_new, v_new, new_sb, new_sh, new_st, T, Hkv, D, block_tables, bt_sb, max_blocks,
+                               start_pos, k_pool, v_pool, kv_sblk, kv_shead, block_size, num_pool_blocks, err,
+                               used_blocks, counts};
+    return glue::append_common("mx_kv_append_counts", p, B, stream);
 }
 
 extern "C" int mx_kv_gather(const uint16_t* k_pool, const uint16_t* v_pool, int64_t kv_sblk, int64_t kv_shead,

@@ -15,7 +15,7 @@ import threading
 import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "libmxdecode.so")
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 MX_OK = 0
 MX_ERR_INVALID = -1
@@ -73,6 +73,11 @@ SIGNATURES = {
     "mx_kv_append": (
         ctypes.c_int,
         [_p, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _p, _i64, _i32, _p, _p, _p, _i64, _i64, _i32, _i32, _p,
+         _p, _p],
+    ),
+    "mx_kv_append_counts": (
+        ctypes.c_int,
+        [_p, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _p, _i64, _i32, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _p,
          _p, _p],
     ),
     "mx_kv_gather": (

@@ -122,13 +122,14 @@ def rope_table(max_pos: int, head_dim: int, theta: float, device: torch.device |
 
 def kv_append(k_layer: torch.Tensor, v_layer: torch.Tensor, block_tables: torch.Tensor, start_pos: torch.Tensor,
               key_states: torch.Tensor, value_states: torch.Tensor, err: torch.Tensor | None = None,
-              used_blocks: torch.Tensor | None = None) -> None:
+              used_blocks: torch.Tensor | None = None, counts: torch.Tensor | None = None) -> None:
     """Write ``key/value_states [B, Hkv, T, D]`` at positions ``start_pos[b] + t`` of each row.
 
     ``k_layer``/``v_layer`` are per-layer pool views ``[num_blocks, Hkv, bs, D]``.
     Slots outside the table or the pool are skipped and flagged in ``err``
     (an int32 device word, OR-ed with 1) when given. ``used_blocks`` (uint8
-    ``[num_blocks]``, optional) gets 1 at every block a token was written to.
+    ``[num_blocks]``, optional) gets 1 at every block a token was written to. ``counts`` (int32
+    ``[B]`` on the device, optional): tokens of each row; those from there on are not written.
     """
     _hip.require_device_tensor(key_states, "key_states")
     dev = k_layer.device
@@ -154,11 +155,17 @@ def kv_append(k_layer: torch.Tensor, v_layer: torch.Tensor, block_tables: torch.
     starts = _i32(start_pos if start_pos.dim() == 1 else start_pos.reshape(-1), dev)
     used = _used_ptr(used_blocks, nb, dev)
     lib = _hip.load()
-    _hip.check(lib.mx_kv_append(
-        key_states.data_ptr(), value_states.data_ptr(), strides[0], strides[1], strides[2], b, t, hkv, d,
-        tables.data_ptr(), tables.stride(0), tables.shape[1], starts.data_ptr(), k_layer.data_ptr(),
-        v_layer.data_ptr(), pool_strides[0], pool_strides[1], bs, nb,
-        err.data_ptr() if err is not None else None, used, _hip.stream_handle(dev)), "mx_kv_append")
+    args = (key_states.data_ptr(), value_states.data_ptr(), strides[0], strides[1], strides[2], b, t, hkv, d,
+            tables.data_ptr(), tables.stride(0), tables.shape[1], starts.data_ptr())
+    pool = (k_layer.data_ptr(), v_layer.data_ptr(), pool_strides[0], pool_strides[1], bs, nb,
+            err.data_ptr() if err is not None else None, used, _hip.stream_handle(dev))
+    if counts is None:
+        _hip.check(lib.mx_kv_append(*args, *pool), "mx_kv_append")
+        return
+    counts = _i32(counts, dev)
+    if counts.shape != (b,):
+        raise ValueError("counts must be [B]")
+    _hip.check(lib.mx_kv_append_counts(*args, counts.data_ptr(), *pool), "mx_kv_append_counts")
 
 
 def kv_gather(k_layer: torch.Tensor, v_layer: torch.Tensor, block_tables: torch.Tensor, tokens: int,

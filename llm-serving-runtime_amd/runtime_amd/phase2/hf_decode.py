@@ -131,7 +131,11 @@ def greedy_decode(model, pool: GpuKVBlockPool, prompts: list[torch.Tensor], bloc
 @torch.no_grad()
 def paged_draft_step(model, cache: BlockPagedBatchCache, tokens: torch.Tensor, tree: DraftTree) -> torch.Tensor:
     """One forward of the drafted ``tokens [B, T]`` (node 0 each row's last certain token) at their tree's
-    positions; returns logits ``[B, T, V]``. ``cache.keep_drafted`` says afterwards which nodes stay."""
+    positions; returns logits ``[B, T, V]``. ``cache.keep_drafted`` says afterwards which nodes stay.
+
+    Every row needs blocks of its own for its context and its nodes. A node that finds none has no K and V: it is
+    reported by ``cache.pool.check_write_errors()``, and other rows' blocks are left as they are.
+    """
     if tokens.dim() != 2 or tokens.shape[0] != cache.block_tables.shape[0]:
         raise ValueError("paged_draft_step takes tokens of shape [B, T] matching the cache rows")
     tree.check_batch(int(tokens.shape[0]), int(tokens.shape[1]), tokens.device)

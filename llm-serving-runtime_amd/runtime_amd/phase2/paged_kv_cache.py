@@ -32,7 +32,9 @@ Differences that keep the decode step free of host round trips:
 
 Drafted tokens (``speculative.DraftTree``): while a batch cache's ``draft_tree`` is set, a forward of the
 tree's nodes writes their K/V behind each row's context, publishes the tree with the metadata (the attention
-hook then runs ``paged_attention_tree`` over the pool) and counts the nodes in the lengths;
+hook then runs ``paged_attention_tree`` over the pool) and counts the nodes in the lengths. Only a row's own
+nodes (``DraftTree.counts``) are written, and only into the row's own blocks: a node that finds none is dropped
+and reported by the pool's ``check_write_errors``.
 ``BlockPagedBatchCache.keep_drafted`` moves the accepted path behind the context and sets the lengths to it.
 
 transformers 5.15 makes ``get_max_length`` abstract; it returns the same value
@@ -198,10 +200,15 @@ class BlockPagedBatchLayer(CacheLayerMixin):
         if tree is not None and kv_len != tree.size:
             raise ValueError(f"a forward of {kv_len} tokens while a draft of {tree.size} nodes is set")
         added = kv_len if tree is None or tree.counts is None else tree.counts
-        if tree is not None and self.layer_idx == 0:
-            parent.draft_start = self._row_seq_lens.clone()
-        parent.pool.write_tokens_batch(self.layer_idx, parent.block_tables, self._row_seq_lens, key_states,
-                                       value_states)
+        tables = parent.block_tables
+        if tree is not None:
+            if self.layer_idx == 0:
+                parent.draft_start, parent._draft_tables = self._row_seq_lens.clone(), parent._owned_tables()
+            tables = parent._draft_tables
+            parent.pool.write_tokens_batch(self.layer_idx, tables, self._row_seq_lens, key_states, value_states,
+                                           counts=tree.counts)
+        else:
+            parent.pool.write_tokens_batch(self.layer_idx, tables, self._row_seq_lens, key_states, value_states)
         if getattr(parent, "_graph_safe", False):
             self._row_seq_lens.add_(added)
             if self.layer_idx == 0:
@@ -213,8 +220,7 @@ class BlockPagedBatchLayer(CacheLayerMixin):
 
         if kv_len == 1 or tree is not None:
             set_paged_decode_batch_metadata(PagedDecodeBatchMetadata(
-                pool=self.pool, layer_idx=self.layer_idx, block_tables=parent.block_tables,
-                seq_lens=parent.seq_lens, tree=tree))
+                pool=self.pool, layer_idx=self.layer_idx, block_tables=tables, seq_lens=parent.seq_lens, tree=tree))
             return key_states, value_states
 
         set_paged_decode_batch_metadata(None)
@@ -296,6 +302,9 @@ class BlockPagedBatchCache(Cache):
 
     draft_tree: "DraftTree | None" = None
     draft_start: torch.Tensor | None = None
+    _draft_tables: torch.Tensor | None = None  # the draft's block tables, of the rows' own blocks
+    _owned: torch.Tensor | None = None         # int32 [B, 1]: blocks of each row, from the first draft on
+    _owned_rows: list[int] | None = None       # what _owned holds
 
     def __init__(self, config, pool: GpuKVBlockPool, *, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                  block_ids_rows: list[list[int]]) -> None:
@@ -358,6 +367,7 @@ class BlockPagedBatchCache(Cache):
         self.block_ids_rows[slot] = []
         self.seq_lens[slot] = 0
         self.block_tables[slot].zero_()
+        self._set_owned(slot)
         self._free_slots.append(slot)
 
     def _set_row_length(self, slot: int, seq_len: int) -> None:
@@ -408,13 +418,31 @@ class BlockPagedBatchCache(Cache):
             if self.block_ids_rows[slot] != dense.block_ids_rows[i]:
                 self.sync_block_ids_row(slot, list(dense.block_ids_rows[i]))
 
+    def _set_owned(self, index: int) -> None:
+        if self._owned is not None:
+            self._owned_rows[index] = len(self.block_ids_rows[index])
+            self._owned[index] = self._owned_rows[index]
+
+    def _owned_tables(self) -> torch.Tensor:
+        """``block_tables`` with -1 behind each row's blocks. The tables' padding names block 0, which may be another
+        row's: a draft that reaches past its row's blocks must not write or read it, and -1 is skipped and reported."""
+        owned = [len(row) for row in self.block_ids_rows]
+        if owned != self._owned_rows:
+            if self.block_tables.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a draft over these rows must run once before it is captured")
+            blocks = torch.tensor(owned, dtype=torch.int32).unsqueeze(1).to(self.block_tables.device)
+            self._owned = blocks if self._owned is None else self._owned.copy_(blocks)
+            self._owned_rows = owned
+        place = torch.arange(self.block_tables.shape[1], dtype=torch.int32, device=self.block_tables.device)
+        return torch.where(place < self._owned, self.block_tables, -1)
+
     def keep_drafted(self, path: torch.Tensor, counts: torch.Tensor) -> None:
         """After a forward of ``draft_tree``'s nodes: keep the nodes ``path[b, :counts[b]]`` of each row
         (``speculative.verify_draft``'s), drop the others and set the lengths to what is kept."""
         if self.draft_tree is None or self.draft_start is None:
             raise RuntimeError("keep_drafted follows a forward of a draft tree's nodes")
         lens = torch.empty_like(self.draft_start)
-        self.pool.keep_tokens(self.block_tables, self.draft_start, path, counts, lens_out=lens)
+        self.pool.keep_tokens(self._draft_tables, self.draft_start, path, counts, lens_out=lens)
         in_place = getattr(self, "_graph_safe", False)
         for target in (self, *self.layers):
             name = "seq_lens" if target is self else "_row_seq_lens"
@@ -422,7 +450,7 @@ class BlockPagedBatchCache(Cache):
                 getattr(target, name).copy_(lens)
             else:
                 setattr(target, name, lens.clone())
-        self.draft_start = None
+        self.draft_start = self._draft_tables = None
 
     def extract_cache(self, index: int, seq_len: int | None = None) -> BlockPagedCache:
         """A batch-1 cache over slot ``index``. ``seq_len``, when the caller knows it (a decode
@@ -451,3 +479,4 @@ class BlockPagedBatchCache(Cache):
         if len(block_ids) > int(self.block_tables.shape[1]):
             self.ensure_max_blocks(len(block_ids))
         self.block_tables[index] = _table_row(block_ids, int(self.block_tables.shape[1]), self.block_tables.device)
+        self._set_owned(index)

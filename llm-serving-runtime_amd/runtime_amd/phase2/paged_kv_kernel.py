@@ -300,7 +300,8 @@ class GpuKVBlockPool:
         self.write_tokens_batch(layer_idx, table, starts, key_states, value_states)
 
     def write_tokens_batch(self, layer_idx: int, block_tables: torch.Tensor, start_positions: torch.Tensor,
-                           key_states: torch.Tensor, value_states: torch.Tensor) -> None:
+                           key_states: torch.Tensor, value_states: torch.Tensor,
+                           counts: torch.Tensor | None = None) -> None:
         """KV write: tables ``[B, max_blocks]``, starts ``[B]``, states ``[B, Hkv, kv_len, D]``.
 
         Same semantics as the reference (``:176-227``). On a device pool it is
@@ -310,6 +311,8 @@ class GpuKVBlockPool:
         ``IndexError`` (``:221-222``); written blocks are marked in a device map
         for the usage accounting. A pool on the CPU (host-side tests of the
         cache bookkeeping) checks on the host and takes an indexed torch store.
+
+        ``counts [B]`` (optional): tokens of each row; those from there on are neither written nor looked up.
         """
         if key_states.shape != value_states.shape:
             raise ValueError("key_states and value_states must match shape")
@@ -317,6 +320,8 @@ class GpuKVBlockPool:
         kv_len = int(key_states.shape[-2])
         if block_tables.shape[0] != batch_size or start_positions.shape[0] != batch_size:
             raise ValueError("batch dimension mismatch in write_tokens_batch")
+        if counts is not None and counts.shape != (batch_size,):
+            raise ValueError("counts must be [B]")
         if kv_len == 0 or batch_size == 0:
             return
         self._ensure_pools()
@@ -331,7 +336,7 @@ class GpuKVBlockPool:
             if key_states.dtype != self.dtype or value_states.dtype != self.dtype:
                 key_states, value_states = key_states.to(self.dtype), value_states.to(self.dtype)
             kv_append(k_layer, v_layer, block_tables, start_positions, key_states, value_states, err=self._write_err,
-                      used_blocks=self._used_map)
+                      used_blocks=self._used_map, counts=counts)
             if self.sync_write_checks and not torch.cuda.is_current_stream_capturing():
                 self.check_write_errors()
             return
@@ -339,9 +344,18 @@ class GpuKVBlockPool:
         pos = start_positions.to(device=device, dtype=torch.int64).view(-1, 1) + torch.arange(
             kv_len, device=device, dtype=torch.int64).view(1, -1)  # [B, T]
         logical = torch.div(pos, bs, rounding_mode="floor")
+        live = None
+        if counts is not None:
+            live = torch.arange(kv_len, device=device).view(1, -1) < counts.to(device).view(-1, 1)
+            if not bool(live.any()):
+                return
+            logical, pos = logical.masked_fill(~live, 0), pos.masked_fill(~live, 0)
         if int(logical.max().item()) >= tables.shape[1] or int(pos.min().item()) < 0:
             raise IndexError("block table underrun during batched write")
         physical = torch.gather(tables, 1, logical)  # [B, T]
+        if live is not None:  # the rows' tokens, side by side
+            physical, pos = physical[live].view(1, -1), pos[live].view(1, -1)
+            key_states, value_states = (x.permute(1, 0, 2, 3)[:, live].unsqueeze(0) for x in (key_states, value_states))
         if int(physical.min().item()) < 0 or int(physical.max().item()) >= self.shape.num_blocks:
             raise IndexError("physical block id out of range during batched write")
         self._touch_blocks(physical)
