@@ -199,12 +199,14 @@ class BlockPagedBatchLayer(CacheLayerMixin):
         tree = parent.draft_tree
         if tree is not None and kv_len != tree.size:
             raise ValueError(f"a forward of {kv_len} tokens while a draft of {tree.size} nodes is set")
-        added = kv_len if tree is None or tree.counts is None else tree.counts
+        added: int | torch.Tensor = kv_len
         tables = parent.block_tables
         if tree is not None:
             if self.layer_idx == 0:
                 parent.draft_start, parent._draft_tables = self._row_seq_lens.clone(), parent._owned_tables()
-            tables = parent._draft_tables
+                # (the kernels take counts outside 0..T for the nearer one)
+                parent._draft_added = kv_len if tree.counts is None else tree.counts.clamp(0, kv_len)
+            tables, added = parent._draft_tables, parent._draft_added
             parent.pool.write_tokens_batch(self.layer_idx, tables, self._row_seq_lens, key_states, value_states,
                                            counts=tree.counts)
         else:
@@ -303,6 +305,7 @@ class BlockPagedBatchCache(Cache):
     draft_tree: "DraftTree | None" = None
     draft_start: torch.Tensor | None = None
     _draft_tables: torch.Tensor | None = None  # the draft's block tables, of the rows' own blocks
+    _draft_added: int | torch.Tensor = 0       # nodes of each row: what its length grows by
     _owned: torch.Tensor | None = None         # int32 [B, 1]: blocks of each row, from the first draft on
     _owned_rows: list[int] | None = None       # what _owned holds
 

@@ -48,7 +48,7 @@ class DraftTree:
     parents: torch.Tensor            # int32 [1 or B, T]; -1: no parent
     depth: torch.Tensor              # int64 [1 or B, T]; ancestors of each node
     mask: torch.Tensor | None        # bool [1 or B, T, T]: node i sees node j; None: a chain
-    counts: torch.Tensor | None = None  # int32 [B]: nodes of each row; None: all T
+    counts: torch.Tensor | None = None  # int32 [B]: nodes of each row (below 0: none, above T: T); None: all T
 
     @property
     def size(self) -> int:

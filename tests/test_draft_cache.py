@@ -150,3 +150,17 @@ def test_append_with_counts_refuses_bad_arguments_before_it_launches():
         assert call(**spoil) == _hip.MX_ERR_INVALID, spoil
     assert call(k=at + 2) == call(st=60) == _hip.MX_ERR_ALIGNMENT
     assert call(B=0, counts=None) == call(T=0) == _hip.MX_OK
+
+
+@pytest.mark.parametrize("graph_safe", [False, True])
+def test_counts_outside_the_tree_count_as_none_and_all(graph_safe):
+    """As in the kernels: the length of a row grows by the nodes that it has."""
+    rows, lens, counts = [[1, 2], [3, 4], [5, 6], [7, 8]], [2, 5, 3, 0], [0, -1, 3, 9]
+    pool, cache = _setup(rows, lens)
+    cache._graph_safe = graph_safe
+    before, states = _pages(pool), _states(4, 2)
+    _forward(cache, states, DraftTree.chain(2, "cpu", counts=torch.tensor(counts)))
+    assert torch.equal(_pages(pool), _expected(before, rows, lens, [0, 0, 2, 2], states))
+    assert cache.seq_lens.tolist() == [2, 5, 5, 2]
+    assert all(layer._row_seq_lens.tolist() == [2, 5, 5, 2] for layer in cache.layers)
+    assert get_paged_decode_batch_metadata().seq_lens.tolist() == [2, 5, 5, 2]

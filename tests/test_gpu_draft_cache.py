@@ -187,3 +187,16 @@ def test_batched_writes_with_counts(dtype):
     assert pool.allocated_block_count() == 5
     with pytest.raises(ValueError, match="counts"):
         pool.write_tokens_batch(0, tables, starts, k, v, counts=counts[:2])
+
+
+def test_attention_of_counts_outside_the_tree():
+    """A count above T is T, below 0 none: the outputs are those of the clipped counts, bit for bit."""
+    rows, lens = [[1, 2], [3, 4], [5, 6]], [2, 5, 3]
+    q = torch.randn(3, 4, 2, D, generator=torch.Generator().manual_seed(3)).half().to(DEV)
+    outs = []
+    for counts in ([5, -1, 1], [2, 0, 1]):
+        pool, cache = _setup(rows, lens)
+        _forward(cache, _states(3, 2), DraftTree.chain(2, DEV, counts=torch.tensor(counts)))
+        assert cache.seq_lens.tolist() == [4, 5, 4]
+        outs.append(paged_attention_tree(q, get_paged_decode_batch_metadata(), 2, 0.125))
+    assert torch.equal(*outs) and not outs[0][1].any() and not outs[0][2, 1].any() and outs[0][0].any()
