@@ -176,8 +176,9 @@ def speculative_decode(model, pool: GpuKVBlockPool, prompts: list[torch.Tensor],
     :func:`prompt_lookup` drafts. Returns the rows' ``steps + 1`` new tokens and the forwards that took. At
     ``temperature`` 0 they are the tokens of :func:`greedy_decode`; above it samples of the model, with uniform
     numbers from ``generator``. A row needs blocks for its prompt, its tokens and two drafts (a row that is
-    done is drafted behind its last one until all are). Drafted tokens outside the vocabulary and logits that
-    hold no distribution (a NaN) raise ``ValueError``.
+    done is drafted behind its last one until all are). Trees that leave a row without a node (``counts`` below 1:
+    the row could not go on), drafted tokens outside the vocabulary and logits that hold no distribution (a NaN)
+    raise ``ValueError``.
     """
     if len(prompts) != len(block_ids_rows) or not prompts:
         raise ValueError("one block-id row per prompt is required")
@@ -189,6 +190,9 @@ def speculative_decode(model, pool: GpuKVBlockPool, prompts: list[torch.Tensor],
     if isinstance(tree, int):
         tree = DraftTree.chain(tree, device)
     size, batch = tree.size, len(prompts)
+    tree.check_batch(batch, size, device)
+    if tree.counts is not None and int(tree.counts.min()) < 1:
+        raise ValueError("every row's tree needs a node: counts must be at least 1")
     caches, first = [], []
     for ids, blocks in zip(prompts, block_ids_rows):
         need = -(-(int(ids.numel()) + steps + 2 * size) // pool.block_size_tokens)

@@ -164,3 +164,17 @@ def test_counts_outside_the_tree_count_as_none_and_all(graph_safe):
     assert cache.seq_lens.tolist() == [2, 5, 5, 2]
     assert all(layer._row_seq_lens.tolist() == [2, 5, 5, 2] for layer in cache.layers)
     assert get_paged_decode_batch_metadata().seq_lens.tolist() == [2, 5, 5, 2]
+
+
+@pytest.mark.parametrize("counts", [[0, 3], [2, -1]])
+def test_speculative_decode_refuses_rows_without_a_node(counts):
+    """Such a row keeps nothing and would be drafted for ever. Refused ahead of the prefill: no model is asked."""
+    from runtime_amd.phase2.hf_decode import speculative_decode
+
+    pool = GpuKVBlockPool(num_blocks=8, block_size_tokens=4, num_layers=1, num_kv_heads=1, head_dim=8, dtype=torch.float32,
+                          device="cpu")
+    prompts = [torch.tensor([1, 2])] * 2
+    with pytest.raises(ValueError, match="at least 1"):
+        speculative_decode(None, pool, prompts, [[0, 1, 2], [3, 4, 5]], 2, DraftTree.chain(3, "cpu", counts=torch.tensor(counts)))
+    with pytest.raises(ValueError, match="does not fit"):
+        speculative_decode(None, pool, prompts, [[0, 1, 2], [3, 4, 5]], 2, DraftTree.from_parents([[-1, 0, 0]] * 3, "cpu"))

@@ -200,3 +200,13 @@ def test_attention_of_counts_outside_the_tree():
         assert cache.seq_lens.tolist() == [4, 5, 4]
         outs.append(paged_attention_tree(q, get_paged_decode_batch_metadata(), 2, 0.125))
     assert torch.equal(*outs) and not outs[0][1].any() and not outs[0][2, 1].any() and outs[0][0].any()
+
+
+@pytest.mark.parametrize("counts", [[0, 3], [2, -1]])
+def test_speculative_decode_refuses_rows_without_a_node(counts):
+    from runtime_amd.phase2.hf_decode import speculative_decode
+
+    pool, _ = _setup([[0]], [0])
+    with pytest.raises(ValueError, match="at least 1"):
+        speculative_decode(None, pool, [torch.tensor([1, 2])] * 2, [[0, 1, 2], [3, 4, 5]], 2,
+                           DraftTree.chain(3, DEV, counts=torch.tensor(counts)))
