@@ -114,7 +114,7 @@ def block_paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor
                                   attention_mask: torch.Tensor | None, scaling: float, dropout: float = 0.0, **kwargs):
     num_kv_groups = getattr(module, "num_key_value_groups", 1)
     meta = get_paged_decode_batch_metadata()
-    if meta is not None and meta.tree is not None and query.is_cuda:
+    if meta is not None and meta.tree is not None:  # (a host query is refused: the key and value are the nodes' alone)
         return paged_attention_tree(query, meta, num_kv_groups, scaling), None
     if meta is not None and query.shape[-2] == 1 and query.is_cuda:
         attn_output = paged_attention_decode_batched(query=query, metadata=meta, num_kv_groups=num_kv_groups,

@@ -134,8 +134,11 @@ def paged_draft_step(model, cache: BlockPagedBatchCache, tokens: torch.Tensor, t
     positions; returns logits ``[B, T, V]``. ``cache.keep_drafted`` says afterwards which nodes stay.
 
     Every row needs blocks of its own for its context and its nodes. A node that finds none has no K and V: it is
-    reported by ``cache.pool.check_write_errors()``, and other rows' blocks are left as they are.
+    reported by ``cache.pool.check_write_errors()``, and other rows' blocks are left as they are. A pool on the host
+    and an 8-bit pool are refused (``ValueError``): tree attention reads neither.
     """
+    if cache.pool.kv_bits != 16 or cache.pool.device.type != "cuda":
+        raise ValueError("paged_draft_step takes a cache over a 16-bit pool on a ROCm device")
     if tokens.dim() != 2 or tokens.shape[0] != cache.block_tables.shape[0]:
         raise ValueError("paged_draft_step takes tokens of shape [B, T] matching the cache rows")
     tree.check_batch(int(tokens.shape[0]), int(tokens.shape[1]), tokens.device)

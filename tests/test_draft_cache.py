@@ -178,3 +178,31 @@ def test_speculative_decode_refuses_rows_without_a_node(counts):
         speculative_decode(None, pool, prompts, [[0, 1, 2], [3, 4, 5]], 2, DraftTree.chain(3, "cpu", counts=torch.tensor(counts)))
     with pytest.raises(ValueError, match="does not fit"):
         speculative_decode(None, pool, prompts, [[0, 1, 2], [3, 4, 5]], 2, DraftTree.from_parents([[-1, 0, 0]] * 3, "cpu"))
+
+
+def test_host_drafts_are_refused():
+    """On the host nothing attends over the pool: the nodes would see each other alone."""
+    from oracle import model as om
+    from runtime_amd.phase2.block_paged_attention import block_paged_attention_forward
+    from runtime_amd.phase2.hf_decode import enable_block_paged_attention, paged_draft_step
+
+    model = om.random_llama(seed=0, hidden_size=64, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                            intermediate_size=64, vocab_size=64, max_position_embeddings=64, head_dim=16)
+    enable_block_paged_attention(model)
+    pool = GpuKVBlockPool(num_blocks=8, block_size_tokens=4, num_layers=2, num_kv_heads=2, head_dim=16,
+                          dtype=torch.float32, device="cpu")
+    cache = BlockPagedBatchCache(model.config, pool, block_tables=torch.tensor([[1, 2]]), seq_lens=torch.tensor([3]),
+                                 block_ids_rows=[[1, 2]])
+    tokens, tree = torch.tensor([[5, 6]]), DraftTree.chain(2, "cpu")
+    with pytest.raises(ValueError, match="16-bit pool on a ROCm device"):
+        paged_draft_step(model, cache, tokens, tree)
+    assert cache.seq_lens.tolist() == [3] and cache.draft_tree is None
+    # ... and in the hook, for a model that is called by hand
+    cache.draft_tree = tree
+    with torch.no_grad(), pytest.raises(ValueError, match="device tensor"):
+        model(input_ids=tokens, position_ids=tree.position_ids(cache.seq_lens), past_key_values=cache, use_cache=True)
+    meta = get_paged_decode_batch_metadata()
+    assert meta.tree is tree
+    q = torch.zeros(1, 4, 2, 16)
+    with pytest.raises(ValueError, match="device tensor"):
+        block_paged_attention_forward(torch.nn.Module(), q, q[:, :2], q[:, :2], None, 0.25)

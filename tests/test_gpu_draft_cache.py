@@ -210,3 +210,16 @@ def test_speculative_decode_refuses_rows_without_a_node(counts):
     with pytest.raises(ValueError, match="at least 1"):
         speculative_decode(None, pool, [torch.tensor([1, 2])] * 2, [[0, 1, 2], [3, 4, 5]], 2,
                            DraftTree.chain(3, DEV, counts=torch.tensor(counts)))
+
+
+def test_drafts_over_an_8_bit_pool_are_refused_before_they_write():
+    from runtime_amd.phase2.hf_decode import paged_draft_step
+    from runtime_amd.phase2.kv8_pool import Int8KVBlockPool
+
+    pool = Int8KVBlockPool(num_blocks=4, block_size_tokens=16, num_layers=2, num_kv_heads=2, head_dim=64,
+                           dtype=torch.float16, device=DEV)
+    cache = BlockPagedBatchCache(_Cfg(), pool, block_tables=torch.tensor([[1, 2]]), seq_lens=torch.tensor([3]),
+                                 block_ids_rows=[[1, 2]])
+    with pytest.raises(ValueError, match="16-bit"):
+        paged_draft_step(None, cache, torch.zeros(1, 2, dtype=torch.int64, device=DEV), DraftTree.chain(2, DEV))
+    assert cache.seq_lens.tolist() == [3] and cache.draft_tree is None
