@@ -131,7 +131,8 @@ def greedy_decode(model, pool: GpuKVBlockPool, prompts: list[torch.Tensor], bloc
 @torch.no_grad()
 def paged_draft_step(model, cache: BlockPagedBatchCache, tokens: torch.Tensor, tree: DraftTree) -> torch.Tensor:
     """One forward of the drafted ``tokens [B, T]`` (node 0 each row's last certain token) at their tree's
-    positions; returns logits ``[B, T, V]``. ``cache.keep_drafted`` says afterwards which nodes stay.
+    positions; returns logits ``[B, T, V]``. ``cache.keep_drafted`` says afterwards which nodes stay; without it all
+    do, as a chunk of a prompt that was drafted as a chain. A forward that raises leaves the lengths as they were.
 
     Every row needs blocks of its own for its context and its nodes. A node that finds none has no K and V: it is
     reported by ``cache.pool.check_write_errors()``, and other rows' blocks are left as they are. A pool on the host
@@ -142,11 +143,15 @@ def paged_draft_step(model, cache: BlockPagedBatchCache, tokens: torch.Tensor, t
     if tokens.dim() != 2 or tokens.shape[0] != cache.block_tables.shape[0]:
         raise ValueError("paged_draft_step takes tokens of shape [B, T] matching the cache rows")
     tree.check_batch(int(tokens.shape[0]), int(tokens.shape[1]), tokens.device)
-    cache.draft_tree = tree
+    cache.draft_tree, cache.draft_start = tree, None
     try:
         out = model(input_ids=tokens, position_ids=tree.position_ids(cache.seq_lens), past_key_values=cache,
                     use_cache=True)
+    except BaseException:
+        cache.drop_drafted()
+        raise
     finally:
+        cache.draft_tree = None
         set_paged_decode_batch_metadata(None)
     return out.logits
 
@@ -241,7 +246,6 @@ def speculative_decode(model, pool: GpuKVBlockPool, prompts: list[torch.Tensor],
         for row, new, n in zip(rows, verdict.tokens.tolist(), counts.tolist()):
             row += new[:n]
         check_tokens()
-    cache.draft_tree = None
     pool.check_write_errors()
     return [row[n - 1:n + steps] for row, n in zip(rows, lengths)], forwards
 

@@ -210,6 +210,8 @@ class BlockPagedBatchLayer(CacheLayerMixin):
             parent.pool.write_tokens_batch(self.layer_idx, tables, self._row_seq_lens, key_states, value_states,
                                            counts=tree.counts)
         else:
+            if self.layer_idx == 0:
+                parent.draft_start = None  # tokens behind a draft: all of it stays
             parent.pool.write_tokens_batch(self.layer_idx, tables, self._row_seq_lens, key_states, value_states)
         if getattr(parent, "_graph_safe", False):
             self._row_seq_lens.add_(added)
@@ -298,8 +300,10 @@ class BlockPagedBatchCache(Cache):
     ``dense_active_cache`` / ``write_back_dense`` run one decode over a subset
     of slots and copy lengths and tables back.
 
-    ``draft_tree`` (None: plain decoding) is the tree whose nodes the next forward takes;
-    ``draft_start [B]`` are the lengths of the contexts that its nodes were written behind.
+    ``draft_tree`` (None: plain decoding) is the tree whose nodes the next forwards take;
+    ``hf_decode.paged_draft_step`` sets it for its forward, a caller who sets it takes it back before the next plain
+    forward. ``draft_start [B]`` are the lengths of the contexts that the last draft's nodes were written behind, until
+    ``keep_drafted``, ``drop_drafted`` or a plain forward.
     """
 
     draft_tree: "DraftTree | None" = None
@@ -442,10 +446,18 @@ class BlockPagedBatchCache(Cache):
     def keep_drafted(self, path: torch.Tensor, counts: torch.Tensor) -> None:
         """After a forward of ``draft_tree``'s nodes: keep the nodes ``path[b, :counts[b]]`` of each row
         (``speculative.verify_draft``'s), drop the others and set the lengths to what is kept."""
-        if self.draft_tree is None or self.draft_start is None:
+        if self.draft_start is None:
             raise RuntimeError("keep_drafted follows a forward of a draft tree's nodes")
         lens = torch.empty_like(self.draft_start)
         self.pool.keep_tokens(self._draft_tables, self.draft_start, path, counts, lens_out=lens)
+        self._end_draft(lens)
+
+    def drop_drafted(self) -> None:
+        """Back to the lengths ahead of a draft's forward, one that raised midway included."""
+        if self.draft_start is not None:
+            self._end_draft(self.draft_start)
+
+    def _end_draft(self, lens: torch.Tensor) -> None:
         in_place = getattr(self, "_graph_safe", False)
         for target in (self, *self.layers):
             name = "seq_lens" if target is self else "_row_seq_lens"

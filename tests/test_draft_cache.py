@@ -206,3 +206,39 @@ def test_host_drafts_are_refused():
     q = torch.zeros(1, 4, 2, 16)
     with pytest.raises(ValueError, match="device tensor"):
         block_paged_attention_forward(torch.nn.Module(), q, q[:, :2], q[:, :2], None, 0.25)
+
+
+def test_a_plain_forward_follows_a_draft():
+    """After a draft that was kept in part, and after one that was kept whole without a word; what is not kept any more
+    cannot be kept later."""
+    rows = [[1, 2, 3], [4, 5, 6]]
+    pool, cache = _setup(rows, [2, 5])
+    tree = DraftTree.from_parents([-1, 0, 0], "cpu")
+    _forward(cache, _states(2, 3), tree)
+    cache.draft_tree = None  # as paged_draft_step leaves it
+    cache.keep_drafted(torch.tensor([[0, 2, -1], [0, -1, -1]]), torch.tensor([2, 1]))
+    assert cache.seq_lens.tolist() == [4, 6]
+    for layer, (k, v) in zip(cache.layers, _states(2, 1)):
+        layer.update(k, v)
+    assert cache.seq_lens.tolist() == [5, 7] and get_paged_decode_batch_metadata().tree is None
+    _forward(cache, _states(2, 2), DraftTree.chain(2, "cpu"))
+    cache.draft_tree = None
+    for layer, (k, v) in zip(cache.layers, _states(2, 1)):
+        layer.update(k, v)
+    assert cache.seq_lens.tolist() == [8, 10]
+    with pytest.raises(RuntimeError, match="follows"):
+        cache.keep_drafted(torch.tensor([[0, 1]] * 2), torch.tensor([1, 1]))
+
+
+@pytest.mark.parametrize("graph_safe", [False, True])
+def test_a_draft_can_be_dropped_midway(graph_safe):
+    pool, cache = _setup([[1, 2], [3, 4]], [2, 5])
+    cache._graph_safe = graph_safe
+    cache.draft_tree = DraftTree.chain(3, "cpu")
+    cache.layers[0].update(*_states(2, 3)[0])
+    assert cache.seq_lens.tolist() == [5, 8]
+    cache.drop_drafted()
+    cache.drop_drafted()
+    assert cache.seq_lens.tolist() == [2, 5] and all(x._row_seq_lens.tolist() == [2, 5] for x in cache.layers)
+    with pytest.raises(RuntimeError, match="follows"):
+        cache.keep_drafted(torch.tensor([[0, 1, 2]] * 2), torch.tensor([1, 1]))

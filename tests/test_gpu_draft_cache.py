@@ -223,3 +223,90 @@ def test_drafts_over_an_8_bit_pool_are_refused_before_they_write():
     with pytest.raises(ValueError, match="16-bit"):
         paged_draft_step(None, cache, torch.zeros(1, 2, dtype=torch.int64, device=DEV), DraftTree.chain(2, DEV))
     assert cache.seq_lens.tolist() == [3] and cache.draft_tree is None
+
+
+@pytest.fixture(scope="module")
+def model():
+    import copy
+
+    from oracle import model as om
+    from runtime_amd.phase2.hf_decode import enable_block_paged_attention
+
+    model = om.random_llama(seed=0, hidden_size=256, num_hidden_layers=2, num_attention_heads=8, num_key_value_heads=2,
+                            intermediate_size=512, vocab_size=1024, max_position_embeddings=512, head_dim=64)
+    om.margin_controlled_(model, seed=0)
+    model = om.to_device_dtype(copy.deepcopy(model), torch.device(DEV), torch.float16).eval()
+    enable_block_paged_attention(model)
+    return model
+
+
+def _prompts(model):
+    """Two rows in a batch cache and what greedy decoding makes of them."""
+    from runtime_amd.phase2.hf_decode import greedy_decode, prefill_request
+
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, 1024, (n,), generator=g) for n in (5, 18)]
+    rows = [[9, 2, 30], [4, 7, 1]]
+
+    def pool():
+        return GpuKVBlockPool(num_blocks=32, block_size_tokens=16, num_layers=2, num_kv_heads=2, head_dim=64,
+                              dtype=torch.float16, device=DEV)
+
+    want = greedy_decode(model, pool(), prompts, rows, 12).tolist()
+    mine = pool()
+    caches = [prefill_request(model, mine, r, p.view(1, -1).to(DEV))[0] for p, r in zip(prompts, rows)]
+    return BlockPagedBatchCache.from_caches(caches, mine), want
+
+
+def test_decode_steps_between_drafts(model):
+    """Greedy tokens of drafts, kept in part, and of plain steps on the same cache in turn; a draft kept whole as well."""
+    from runtime_amd.phase2.hf_decode import paged_decode_step, paged_draft_step
+
+    cache, want = _prompts(model)
+    tree = DraftTree.from_parents([-1, 0, 0, 2], DEV)
+    at = 0  # tokens of `want` in the cache
+    for turn in range(3):
+        # the second branch is the answer, the first one is not; of the answer's two nodes one is kept
+        tokens = torch.tensor([[w[at], (w[at + 1] + 1) % 1024, w[at + 1], w[at + 2]] for w in want], device=DEV)
+        logits = paged_draft_step(model, cache, tokens, tree)
+        assert cache.draft_tree is None
+        best = logits.argmax(dim=-1).tolist()
+        assert all([b[0], b[2], b[3]] == w[at + 1:at + 4] for b, w in zip(best, want))
+        cache.keep_drafted(torch.tensor([[0, 2, -1, -1]] * 2, dtype=torch.int32, device=DEV),
+                           torch.tensor([2, 2], dtype=torch.int32, device=DEV))
+        at += 2
+        logits = paged_decode_step(model, cache, torch.tensor([[w[at]] for w in want], device=DEV))
+        at += 1
+        assert logits.argmax(dim=-1).tolist() == [w[at] for w in want]
+    # a chain that stays whole
+    logits = paged_draft_step(model, cache, torch.tensor([w[at:at + 2] for w in want], device=DEV), DraftTree.chain(2, DEV))
+    assert logits.argmax(dim=-1).tolist() == [w[at + 1:at + 3] for w in want]
+    at += 2
+    logits = paged_decode_step(model, cache, torch.tensor([[w[at]] for w in want], device=DEV))
+    assert logits.argmax(dim=-1).tolist() == [w[at + 1] for w in want]
+    with pytest.raises(RuntimeError, match="follows"):
+        cache.keep_drafted(torch.tensor([[0, 1]] * 2, dtype=torch.int32, device=DEV),
+                           torch.tensor([1, 1], dtype=torch.int32, device=DEV))
+
+
+def test_a_forward_that_raises_leaves_the_lengths(model):
+    from runtime_amd.phase2.hf_decode import paged_decode_step, paged_draft_step
+
+    cache, want = _prompts(model)
+    lens = cache.seq_lens.tolist()
+    tokens = torch.tensor([w[:2] for w in want], device=DEV)
+    layer = model.model.layers[1]
+
+    def stop(*args):
+        raise KeyError("stopped behind the first layer")
+
+    hook = layer.register_forward_pre_hook(stop)
+    try:
+        with pytest.raises(KeyError):
+            paged_draft_step(model, cache, tokens, DraftTree.chain(2, DEV))
+    finally:
+        hook.remove()
+    assert get_paged_decode_batch_metadata() is None and cache.draft_tree is None
+    assert cache.seq_lens.tolist() == lens and all(x._row_seq_lens.tolist() == lens for x in cache.layers)
+    logits = paged_decode_step(model, cache, tokens[:, :1])
+    assert logits.argmax(dim=-1).tolist() == [w[1] for w in want]
