@@ -28,6 +28,7 @@ from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _hip
 from .kv8 import _lengths, _tables
@@ -150,9 +151,12 @@ def paged_attention_tree(query: torch.Tensor, metadata: PagedDecodeBatchMetadata
     context's length plus ``T``, or plus the row's ``tree.counts``). Without a tree the T tokens are a chain.
     Nodes past a row's count, and nodes that see nothing, give zeros. fp16 or bf16 query and 16-bit pool of
     one dtype, head_dim in {64, 128}, block size in {4, 8, 16, 32}, any GQA group. A block id outside the
-    pool is skipped and reported by ``pool.check_write_errors()``.
+    pool is skipped and reported by ``pool.check_write_errors()``. There is no gradient: a query that asks for one
+    (call it under ``torch.no_grad()``) or is being traced raises ``RuntimeError``.
     """
     _hip.require_device_tensor(query, "query")
+    if query.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0 or torch.jit.is_tracing():
+        raise RuntimeError("tree attention has no gradient and cannot be traced: the result would be a constant")
     if query.dim() != 4:
         raise ValueError("query must be [B, heads, T, dim]")
     bsz, hq, nodes, d = query.shape

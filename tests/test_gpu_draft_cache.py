@@ -310,3 +310,29 @@ def test_a_forward_that_raises_leaves_the_lengths(model):
     assert cache.seq_lens.tolist() == lens and all(x._row_seq_lens.tolist() == lens for x in cache.layers)
     logits = paged_decode_step(model, cache, tokens[:, :1])
     assert logits.argmax(dim=-1).tolist() == [w[1] for w in want]
+
+
+def test_a_gradient_is_refused_and_not_lost():
+    """Where the query asks for one; under no_grad, or for a leaf that asks for none, the call is as ever."""
+    import torch.autograd.forward_ad as fwad
+
+    _, cache = _setup([[1, 2]], [3])
+    _forward(cache, _states(1, 2), DraftTree.chain(2, DEV))
+    meta = get_paged_decode_batch_metadata()
+    q = torch.randn(1, 4, 2, D, generator=torch.Generator().manual_seed(3)).half().to(DEV)
+    want = paged_attention_tree(q, meta, 2, 0.125)
+    leaf = q.clone().requires_grad_()
+    for query in (leaf, leaf * 1):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            paged_attention_tree(query, meta, 2, 0.125)
+        with torch.no_grad():
+            assert torch.equal(paged_attention_tree(query, meta, 2, 0.125), want)
+        with torch.inference_mode():
+            assert torch.equal(paged_attention_tree(query, meta, 2, 0.125), want)
+    with fwad.dual_level(), pytest.raises(RuntimeError, match="no gradient"):
+        paged_attention_tree(fwad.make_dual(q, torch.ones_like(q)), meta, 2, 0.125)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda x: paged_attention_tree(x, meta, 2, 0.125), q, check_trace=False)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: paged_attention_tree(x, meta, 2, 0.125))(q.unsqueeze(0))
+    assert torch.equal(paged_attention_tree(q, meta, 2, 0.125), want)
