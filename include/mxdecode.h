@@ -730,9 +730,13 @@ int mx_tree_attn(const uint16_t* q, int64_t q_sb, int64_t q_sh, int64_t q_st, co
  * token is -1. counts (int32 [B], nullable: T): nodes of each row; a row of none gets
  * 0 and -1. T <= 1024, V <= 4194304. workspace: at least
  * mx_verify_draft_workspace_bytes, 16-byte aligned, not shared by calls that overlap.
+ * A row is walked by several workgroups, whose waits for each other are bounded:
+ * one that runs out ends the row as a node without a distribution does (with
+ * MX_VERIFY_NO_WAIT, for tests of that end, after one look).
  * The reference's counterpart takes the argmax of one position after the other
  * (runtime/phase2/worker_server.py:1010-1075). */
 #define MX_LOGITS_FP32 16u
+#define MX_VERIFY_NO_WAIT 32u
 size_t mx_verify_draft_workspace_bytes(int32_t B, int32_t T, int32_t V, int32_t draft);
 int mx_verify_draft(const void* logits, int64_t l_sb, int64_t l_st, const void* draft_logits, int64_t d_sb,
                     int64_t d_st, const int64_t* tokens, int64_t t_sb, const int32_t* parents, int64_t p_sb,

@@ -38,6 +38,7 @@ constexpr int kMaxNodes = 1024;
 constexpr int kFill = 512;
 constexpr int kMaxVocab = 1 << 22;
 constexpr int kMaxPolls = 1 << 23;         // seconds: a wait that long means a broken launch; the row then ends with -1
+                                           // (MX_VERIFY_NO_WAIT: after one look, which shows that end)
 
 // What a pass over a slice gives: sums of 2^((l - ref) c), c = log2(e) / temperature, of the logits and the draft's.
 // Greedy rows: the largest logit in ref[0] and its first index in at. ref NaN: no distribution.
@@ -64,6 +65,7 @@ struct Params {
     int B, T, V;
     int slices, len;  // of a row's vocabulary, logits per slice
     int first;        // nodes passed over by the first launch
+    int max_polls;    // of a wait
     Part* parts;      // [B][first][slices]
     uint64_t* words;  // [B][2][slices][4]
     int* ticket;
@@ -447,7 +449,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
                         there &= (all[i] & 0xff) == tag;
                     }
                 if (__builtin_amdgcn_ballot_w64(!there) == 0) break;
-                if (polls > kMaxPolls) {
+                if (polls >= p.max_polls) {
                     ok = false;
                     break;
                 }
@@ -660,10 +662,15 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
                         const double z = ok && lane < p.slices ? sum_of(got[0]) : 0.0;
                         const double sum = wave_sum(z);
                         if (sum > 0.0 && lane < p.slices) part[lane] = z * (1.0 / sum);  // of r, whose sum is 1
-                        if (lane == 0) cw[refused - 1] = sum > 0.0 ? 1.0 / sum : 0.0;
+                        if (lane == 0) cw[refused - 1] = !ok ? __builtin_nan("") : sum > 0.0 ? 1.0 / sum : 0.0;
                     }
                     __syncthreads();
-                    if (!(cw[refused - 1] > 0.0)) --refused;  // nothing remains: r stays
+                    const double f = cw[refused - 1];
+                    if (f != f) {  // the wait gave up
+                        have = false;
+                        break;
+                    }
+                    if (!(f > 0.0)) --refused;  // nothing remains: r stays
                 }
             }
         }
@@ -833,7 +840,8 @@ extern "C" int mx_verify_draft(const void* logits, int64_t l_sb, int64_t l_st, c
     if (B == 0 || T == 0) return MX_OK;
     if (!logits || !tokens || !parents || !uniforms || !temperatures || !tokens_out || !counts_out || !path_out)
         return fail(MX_ERR_NULL, "%s: null pointer", what);
-    if (flags & ~(uint32_t)(MX_PA_BF16 | MX_LOGITS_FP32) || flags == (MX_PA_BF16 | MX_LOGITS_FP32))
+    if (flags & ~(uint32_t)(MX_PA_BF16 | MX_LOGITS_FP32 | MX_VERIFY_NO_WAIT) ||
+        (flags & (MX_PA_BF16 | MX_LOGITS_FP32)) == (MX_PA_BF16 | MX_LOGITS_FP32))
         return fail(MX_ERR_INVALID, "%s: unknown flags 0x%x", what, flags);
     if (l_sb < 0 || l_st < 0 || d_sb < 0 || d_st < 0 || t_sb < 0 || p_sb < 0 || u_sb < 0 || temp_sb < 0)
         return fail(MX_ERR_INVALID, "%s: strides must be >= 0", what);
@@ -852,6 +860,7 @@ extern "C" int mx_verify_draft(const void* logits, int64_t l_sb, int64_t l_st, c
     p.B = B, p.T = T, p.V = V;
     const verify::Plan pl = verify::plan_of(B, T, V, draft_logits != nullptr);
     p.slices = pl.slices, p.len = pl.len, p.first = pl.first;
+    p.max_polls = flags & MX_VERIFY_NO_WAIT ? 0 : verify::kMaxPolls;
     char* ws = static_cast<char*>(workspace);
     p.parts = reinterpret_cast<verify::Part*>(ws);
     p.words = reinterpret_cast<uint64_t*>(ws + pl.words_at);
