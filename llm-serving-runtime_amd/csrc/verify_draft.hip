@@ -20,7 +20,8 @@
 // Partials are exchanged through 8-byte words that carry the number of the pass in their low bits, written and read
 // past the L2s (relaxed atomics of agent scope), so that a word says by itself whether it is the one waited for: no
 // fence, no counter, one round trip. Words of odd and even passes stand apart, since a workgroup is at most one pass
-// ahead of another of its row. Every wait ends: workgroups take their row and slice from a counter as they start, so all rows
+// ahead of another of its row, and so do those of passes over a node and of refusals, each numbered by itself: what a word
+// held before is then always two passes older, and a number taken modulo 255 tells the two apart. Every wait ends: workgroups take their row and slice from a counter as they start, so all rows
 // but the last one started have all their workgroups running, finish, and make room for what the last one lacks.
 #include "common.h"
 
@@ -31,6 +32,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kVec = 8;                    // neighbouring logits per thread
 constexpr int kBlock = kThreads * kVec;    // logits per step of a workgroup
+constexpr int kWords = 5;                  // exchanged per slice: four of a pass over a node, one of a refusal
 constexpr int kMaxSlices = 64;             // one lane of a wave each
 constexpr int kMaxNodes = 1024;
 // Workgroups, two a CU: 256 take 66 us for 32 rows of 16 nodes (128,256 logits), 1024 take 73, these 57; one row of 5 nodes
@@ -67,7 +69,7 @@ struct Params {
     int first;        // nodes passed over by the first launch
     int max_polls;    // of a wait
     Part* parts;      // [B][first][slices]
-    uint64_t* words;  // [B][2][slices][4]
+    uint64_t* words;  // [B][2][slices][kWords]
     int* ticket;
     int64_t* tokens_out;
     int32_t* counts_out;
@@ -370,8 +372,8 @@ __global__ __launch_bounds__(kThreads) void first_kernel(Params p) {
     __shared__ int nch;
     const int s = blockIdx.x % p.slices, rest = blockIdx.x / p.slices;
     const int node = rest % p.first, b = rest / p.first;
-    if (node == 0 && threadIdx.x < 8)
-        p.words[(((int64_t)b * 2 + threadIdx.x / 4) * p.slices + s) * 4 + threadIdx.x % 4] = 0;
+    if (node == 0 && threadIdx.x < 2 * kWords)
+        p.words[(((int64_t)b * 2 + threadIdx.x / kWords) * p.slices + s) * kWords + threadIdx.x % kWords] = 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
     Exp::fill(sh.table);
     __syncthreads();
@@ -428,15 +430,14 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
     }
     __syncthreads();
 
-    int passes = 0;  // cooperative passes so far
-    // Every slice's words of this pass, a lane of the first wave each.
-    auto exchange = [&](const uint64_t (&mine)[4], int n, uint64_t (&all)[4]) -> bool {
-        ++passes;
-        const uint64_t tag = passes % 255 + 1;
-        uint64_t* base = p.words + ((int64_t)b * 2 + (passes & 1)) * p.slices * 4;
+    int node_passes = 0, refusal_passes = 0;  // cooperative passes so far
+    // Every slice's words of pass number `pass` of its kind, n of them from `first` on; a lane of the first wave each.
+    auto exchange = [&](int pass, int first, const uint64_t (&mine)[4], int n, uint64_t (&all)[4]) -> bool {
+        const uint64_t tag = pass % 255 + 1;
+        uint64_t* base = p.words + ((int64_t)b * 2 + (pass & 1)) * p.slices * kWords + first;
         if (tid == 0)
             for (int i = 0; i < n; ++i)
-                __hip_atomic_store(base + s * 4 + i, (mine[i] & ~0xffull) | tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(base + s * kWords + i, (mine[i] & ~0xffull) | tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         bool ok = true;
         if (wave == 0) {
             const int from = lane < p.slices ? lane : 0;
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (i < n) {
-                        all[i] = __hip_atomic_load(base + from * 4 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        all[i] = __hip_atomic_load(base + from * kWords + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                         there &= (all[i] & 0xff) == tag;
                     }
                 if (__builtin_amdgcn_ballot_w64(!there) == 0) break;
@@ -492,7 +493,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
             mine = pass<KIND, SMALL>(p, sh, lrow, drow, s, c, greedy, ch);
             uint64_t w[4] = {greedy ? (uint64_t)(uint32_t)mine.at << 8 : word_of(mine.sum[0]), ref_word(mine.ref[0]),
                              word_of(mine.sum[1]), ref_word(mine.ref[1])}, all[4];
-            ok = exchange(w, drafted ? 4 : 2, all);
+            ok = exchange(++node_passes, 0, w, drafted ? 4 : 2, all);
             if (wave == 0) {
                 mine.at = greedy ? (int)(all[0] >> 8) : 0;
                 mine.sum[0] = sum_of(all[0]);
@@ -657,7 +658,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(Params p, int per_row) {
                     }
                     const uint64_t w[4] = {word_of(block_sum(sh, m)), 0, 0, 0};
                     uint64_t got[4];
-                    const bool ok = exchange(w, 1, got);
+                    const bool ok = exchange(++refusal_passes, 4, w, 1, got);
                     if (wave == 0) {
                         const double z = ok && lane < p.slices ? sum_of(got[0]) : 0.0;
                         const double sum = wave_sum(z);
@@ -800,7 +801,7 @@ static Plan plan_of(int64_t B, int64_t T, int64_t V, bool draft) {
     const int64_t f = draft ? (12 << 20) / (B * V * 2) : (4 << 20) / (B * V);
     p.first = (int)(f < 1 ? 1 : f < T ? f : T);
     p.words_at = (size_t)B * p.first * p.slices * sizeof(Part);
-    p.ticket_at = p.words_at + (size_t)B * 2 * p.slices * 4 * sizeof(uint64_t);
+    p.ticket_at = p.words_at + (size_t)B * 2 * p.slices * kWords * sizeof(uint64_t);
     p.bytes = p.ticket_at + 16;
     return p;
 }

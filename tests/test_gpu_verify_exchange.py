@@ -70,3 +70,64 @@ def test_a_pass_whose_wait_runs_out_ends_the_row(temperature):
         assert 1 <= n <= t and path == list(range(n)) + [-1] * (t - n)
         assert row == [5] * t if n == t and row[-1] == 5 else row == [5] * (n - 1) + [-1] * (t - n + 1)
     assert bool((cut[1] < t).any())
+
+
+def _oracle(logits, tokens, parents, u, temps, draft=None):
+    """What the 64-bit oracle makes of each row, as verify_draft's tokens and nodes."""
+    from oracle import speculative as oracle
+
+    t = tokens.shape[1]
+    rows, nodes = [], []
+    for b in range(tokens.shape[0]):
+        kept, following = oracle.verify_row(logits[b].double().numpy(), tokens[b].tolist(), parents, t, u[b].tolist(),
+                                            float(temps[b]), None if draft is None else draft[b].double().numpy())
+        out = [int(tokens[b, i]) for i in kept[1:]] + [following]
+        rows.append(out + [-1] * (t - len(out)))
+        nodes.append(kept + [-1] * (t - len(kept)))
+    return rows, nodes
+
+
+def test_more_refusals_at_a_node_than_a_word_has_numbers():
+    """Passes over two nodes with 510 refusals between them: the number that marks a word comes round, so a word that a
+    refusal leaves alone would pass for one of the second node's."""
+    v, a, n = 20011, 400, 511
+    t = a + n + 8
+    assert _hip.verify_draft_workspace_bytes(1, a, v, 1) == _hip.verify_draft_workspace_bytes(1, t, v, 1)
+    g = torch.Generator().manual_seed(5)
+    parents = [-1] * (a + 1) + [a] * n + list(range(a + n, t - 1))
+    parents[a] = 0
+    logits, tokens = 3 * torch.randn(1, t, v, generator=g), torch.randint(0, v, (1, t), generator=g)
+    draft = logits + torch.randn(1, t, v, generator=g)
+    u = torch.rand(1, t, generator=g)
+    # Node a: the target is even over the upper half of the vocabulary, the draft over the lower one, whose tokens are refused.
+    logits[0, a], draft[0, a] = -10.0, -10.0
+    logits[0, a, v // 2:], draft[0, a, :v // 2] = 0.0, 0.0
+    tokens[0, a + 1:a + n] = torch.arange(n - 1)
+    tokens[0, a + n] = v // 2 + 77
+    u[0, a:a + n] = 0.9
+    u[0, a] = u[0, a + n] = 0.0
+    for i in range(a + n, t - 1):  # ... and its last child is kept, and some behind it
+        tokens[0, i + 1] = int(draft[0, i].argmax())
+    temps = torch.ones(1)
+    want = _oracle(logits, tokens, parents, u, temps, draft)
+    assert want[1][0][:3] == [0, a, a + n]
+    got = _call(logits, tokens, parents, u, temps, draft)
+    assert (got[0].tolist(), got[2].tolist()) == want
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.9])
+def test_more_passes_than_a_word_has_numbers(temperature):
+    """A chain of 1000 nodes, all kept: 209 nodes in the first launch, the others a pass of the row's workgroups each."""
+    v, t = 20011, 1000
+    assert _hip.verify_draft_workspace_bytes(1, 250, v, 0) == _hip.verify_draft_workspace_bytes(1, t, v, 0)
+    g = torch.Generator().manual_seed(6)
+    logits, parents = 3 * torch.randn(1, t, v, generator=g), list(range(-1, t - 1))
+    tokens, u = torch.zeros(1, t, dtype=torch.int64), torch.rand(1, t, generator=g)
+    tokens[0, 1:] = logits[0, :-1].argmax(dim=-1)
+    if temperature:
+        u[0, 1:990] = 0.0
+    temps = torch.tensor([temperature])
+    want = _oracle(logits, tokens, parents, u, temps)
+    assert want[1][0][989] == 989
+    got = _call(logits, tokens, parents, u, temps)
+    assert (got[0].tolist(), got[2].tolist()) == want
