@@ -131,3 +131,120 @@ def test_more_passes_than_a_word_has_numbers(temperature):
     assert want[1][0][989] == 989
     got = _call(logits, tokens, parents, u, temps)
     assert (got[0].tolist(), got[2].tolist()) == want
+
+
+# Shapes whose first launch takes fewer nodes than the trees have (4 million logits of them, 12 of both kinds): the walk passes
+# over the others with its workgroups together. b, t, v, draft, dtype, reach (1: chains), every which row is greedy (0: none).
+BEYOND = [
+    (8, 12, 128256, True, torch.float32, 2, 3),
+    (8, 12, 128256, False, torch.float32, 3, 3),
+    (8, 12, 128256, False, torch.bfloat16, 1, 1),
+    (32, 6, 128256, True, torch.float16, 2, 4),
+    (32, 6, 128256, False, torch.float16, 2, 4),
+    (32, 6, 128256, False, torch.float16, 1, 1),
+    (32, 6, 128256, False, torch.float32, 5, 0),
+    (2, 70, 151936, True, torch.bfloat16, 2, 0),
+    (2, 70, 100003, False, torch.float16, 4, 2),
+    (600, 3, 8193, False, torch.float16, 1, 2),   # one workgroup a row
+    (600, 5, 4099, True, torch.float16, 2, 3),
+    (70, 40, 2049, False, torch.float32, 2, 3),   # slices of 1032 logits
+    (1, 400, 151936, False, torch.float16, 3, 0),
+]
+
+
+def _likely_paths(seed, b, t, v, dtype, draft, reach, greedy):
+    """Rows whose paths are long: a node's last child has the token that its target (draft) prefers, the ones before it likely
+    ones that are refused often."""
+    g = torch.Generator().manual_seed(seed)
+    parents = [[-1] + [int(torch.randint(max(0, i - reach), i, (1,), generator=g)) for i in range(1, t)] for _ in range(b)]
+    if t > 12:  # every reach-th node goes on, the others have no children
+        parents = [[-1] + [(i - 1) // reach * reach for i in range(1, t)]] * b
+    logits = (3 * torch.randn(b, t, v, generator=g)).to(dtype)
+    q = (logits.float() + 0.5 * torch.randn(b, t, v, generator=g)).to(dtype) if draft else None
+    temps = 0.2 + 0.3 * torch.rand(b, generator=g)
+    if greedy:
+        temps[::greedy] = 0.0
+    tokens, u = torch.zeros(b, t, dtype=torch.int64), torch.rand(b, t, generator=g)
+    top = (logits if q is None else q).float().topk(2, dim=-1).indices
+    if draft and t > 12:  # of the likely ones those which the draft underrates and overrates most
+        many = q.float().topk(8, dim=-1).indices
+        over = q.float().gather(2, many) - logits.float().gather(2, many)
+        top = many.gather(2, torch.stack((over.argmin(dim=-1), over.argmax(dim=-1)), dim=2))
+    for row in range(b):
+        last = {p: i for i, p in enumerate(parents[row])}
+        for i in range(1, t):
+            p = parents[row][i]
+            tokens[row, i] = top[row, p, 0 if last[p] == i else 1]
+            if last[p] == i:
+                u[row, i] *= 0.5 if t <= 12 else 0.02
+            elif t > 12:
+                u[row, i] = 0.9 + 0.09 * u[row, i]
+    return parents, logits, q, tokens, u, temps
+
+
+@pytest.mark.parametrize("case", range(len(BEYOND)))
+def test_nodes_beyond_the_first_launch(case):
+    from runtime_amd.phase2.speculative import DraftTree, verify_draft
+    from oracle import speculative as oracle
+
+    b, t, v, draft, dtype, reach, greedy = BEYOND[case]
+    # The workspace holds a place for every node of the first launch, so it grows with T up to their number.
+    size = [_hip.verify_draft_workspace_bytes(b, n, v, int(draft)) for n in range(1, t + 1)]
+    first = 1 + size.index(size[-1])
+    assert first < t
+    parents, logits, q, tokens, u, temps = _likely_paths(case, b, t, v, dtype, draft, reach, greedy)
+    counts = torch.full((b,), t, dtype=torch.int32)
+    if b > 1:
+        counts[1::5] = t - 1
+        counts[min(3, b - 1)] = 0
+    tree = DraftTree.from_parents(parents, DEV, counts=counts)
+    got = [x.cpu() for x in verify_draft(logits.to(DEV), tokens.to(DEV), tree, u.to(DEV), temps.to(DEV),
+                                         draft_logits=None if q is None else q.to(DEV))]
+    deepest = 0
+    for row in range(b):
+        kept, following = oracle.verify_row(_Rows(logits[row]), tokens[row].tolist(), parents[row], int(counts[row]),
+                                            u[row].tolist(), float(temps[row]), None if q is None else _Rows(q[row]))
+        want = [int(tokens[row, i]) for i in kept[1:]] + ([] if following is None else [following])
+        assert got[2][row].tolist() == kept + [-1] * (t - len(kept)), row
+        assert got[0][row].tolist() == want + [-1] * (t - len(want)), row
+        assert int(got[1][row]) == len(kept)
+        deepest = max(deepest, kept[-1] if kept else 0)
+    assert deepest >= first, "no path reached the nodes beyond"
+
+
+class _Rows:
+    """Logits of a row's nodes in 64 bits, one at a time."""
+
+    def __init__(self, x):
+        self.x = x
+
+    def __getitem__(self, i):
+        return self.x[i].double().numpy()
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+@pytest.mark.parametrize("draft", [False, True])
+def test_nodes_without_a_distribution_beyond_the_first_launch(draft, temperature):
+    """What makes a node of a later pass end its row: a NaN, nothing above -inf, with a temperature +inf."""
+    b, t, v = 8, 14, 128256
+    assert _hip.verify_draft_workspace_bytes(b, t - 1, v, int(draft)) == _hip.verify_draft_workspace_bytes(b, t, v, int(draft))
+    logits, parents = torch.zeros(b, t, v), list(range(-1, t - 1))
+    logits[..., 99999] = 40.0
+    logits[0, 12, 128255] = float("nan")
+    logits[1, 11] = -float("inf")
+    logits[2, 12, 3] = float("inf")
+    logits[3, 11, 0] = -float("inf")          # one token less
+    logits[4, 12] = -float("inf")
+    logits[4, 12, 70000] = -3.0               # one token left
+    tokens, u = torch.full((b, t), 99999, dtype=torch.int64), torch.full((b, t), 0.25)
+    temps, q = torch.full((b,), temperature), logits.clone() if draft else None
+    if draft:
+        q[5, 12, 17] = float("nan")           # a draft without a distribution: its children are not kept
+        q[0:3] = q[6:7]                       # (those rows' drafts have one)
+        q[4] = q[6]
+    want = _oracle(logits, tokens, parents, u, temps, q)
+    got = _call(logits, tokens, parents, u, temps, q)
+    assert (got[0].tolist(), got[2].tolist()) == want
+    greedy = temperature == 0.0
+    assert got[1].tolist() == [13, 12, 13, 14, 13, 13 if draft and not greedy else 14, 14, 14]
+    assert [r[n - 1] for r, n in zip(got[0].tolist(), got[1].tolist())] == [-1, -1, 3 if greedy else -1, 99999, 70000] + [99999] * 3
