@@ -271,7 +271,10 @@ def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, tree: DraftTree, un
     if logits.stride(2) != 1 and v > 1:
         logits = logits.contiguous()
     tokens = _rows_of(tokens, "tokens", (b, t), torch.int64, dev)
+    wide = isinstance(uniforms, torch.Tensor) and uniforms.dtype == torch.float64
     uniforms = _rows_of(uniforms, "uniforms", (b, t), torch.float32, dev)
+    if wide:  # the largest ones would be rounded to 1, at which what is certain is refused
+        uniforms = uniforms.clamp(max=1 - 2.0 ** -24)
     tree.check_batch(b, t, dev)
     if isinstance(temperature, torch.Tensor):
         if temperature.dim() == 0:

@@ -248,3 +248,16 @@ def test_nodes_without_a_distribution_beyond_the_first_launch(draft, temperature
     greedy = temperature == 0.0
     assert got[1].tolist() == [13, 12, 13, 14, 13, 13 if draft and not greedy else 14, 14, 14]
     assert [r[n - 1] for r, n in zip(got[0].tolist(), got[1].tolist())] == [-1, -1, 3 if greedy else -1, 99999, 70000] + [99999] * 3
+
+
+def test_wide_uniform_numbers_stay_below_1():
+    """A token that is certain is kept whatever the number, also one that rounds to 1 in 32 bits."""
+    from runtime_amd.phase2.speculative import DraftTree, verify_draft
+
+    logits = torch.full((1, 3, 500), -float("inf"), device=DEV)
+    logits[..., 7] = 1.0
+    tokens, tree = torch.full((1, 3), 7, dtype=torch.int64, device=DEV), DraftTree.chain(3, DEV)
+    u = torch.full((1, 3), 1 - 2.0 ** -40, dtype=torch.float64, device=DEV)
+    for draft in (None, logits):
+        out = verify_draft(logits, tokens, tree, u, 1.0, draft_logits=draft)
+        assert out.tokens.tolist() == [[7, 7, 7]] and out.counts.tolist() == [3]
