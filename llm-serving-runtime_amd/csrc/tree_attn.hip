@@ -223,17 +223,18 @@ __device__ __forceinline__ int worker_of(int x, int total, int workers) {
                      : "memory");                                                                                         \
     else if constexpr (N == 2)                                                                                            \
         asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off" NT "\n\t"       \
-                     "global_load_lds_dwordx4 %3, off offset:1024" NT "\n\ts_mov_b32 m0, %0"                              \
+                     "global_load_lds_dwordx4 %3, off offset:%4" NT "\n\ts_mov_b32 m0, %0"                                \
                      : "=&s"(was)                                                                                         \
-                     : "s"(at), "v"(from[0]), "v"(from[1] - 1024)                                                         \
+                     : "s"(at), "v"(from[0]), "v"(from[1] - 1024), "n"(1024)                                              \
                      : "memory");                                                                                         \
     else                                                                                                                  \
         asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off" NT "\n\t"       \
-                     "global_load_lds_dwordx4 %3, off offset:1024" NT                                                     \
-                     "\n\tglobal_load_lds_dwordx4 %4, off offset:2048" NT                                                 \
-                     "\n\tglobal_load_lds_dwordx4 %5, off offset:0xc00" NT "\n\ts_mov_b32 m0, %0"                          \
+                     "global_load_lds_dwordx4 %3, off offset:%6" NT                                                       \
+                     "\n\tglobal_load_lds_dwordx4 %4, off offset:%7" NT                                                   \
+                     "\n\tglobal_load_lds_dwordx4 %5, off offset:%8" NT "\n\ts_mov_b32 m0, %0"                            \
                      : "=&s"(was)                                                                                         \
-                     : "s"(at), "v"(from[0]), "v"(from[1] - 1024), "v"(from[2] - 2048), "v"(from[3] - 3 * 1024)               \
+                     : "s"(at), "v"(from[0]), "v"(from[1] - 1024), "v"(from[2] - 2 * 1024), "v"(from[3] - 3 * 1024),          \
+                       "n"(1024), "n"(2 * 1024), "n"(3 * 1024)                                                            \
                      : "memory")
 template <int N, bool STREAM>
 __device__ __forceinline__ void load_to_lds(const char* const (&from)[N], uint32_t to) {
