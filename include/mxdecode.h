@@ -722,7 +722,7 @@ int mx_tree_attn(const uint16_t* q, int64_t q_sb, int64_t q_sh, int64_t q_st, co
  * r = max(r - q, 0) scaled to a sum of 1. Without them q is a point at x: r loses x.
  * Where nothing would remain r stays. Where no child is taken the walk ends: the
  * following token is the first whose running sum of r exceeds uniforms[0] times the
- * whole. All in fp64. path_out (int32 [B, T]): the nodes taken, from node 0, then -1;
+ * whole. All in fp64, of which sums that workgroups exchange keep 44 bits. path_out (int32 [B, T]): the nodes taken, from node 0, then -1;
  * counts_out (int32 [B]): how many; tokens_out (int64 [B, T]): the taken nodes'
  * tokens without node 0's, then the following token, then -1. A token outside [0, V)
  * is never taken. A node whose logits hold a NaN, nothing above -inf or (with a

@@ -240,8 +240,9 @@ struct KeepParams {
 
 // One workgroup per (layer, row). A thread owns 16 bytes of every token of a head's K or V, so what it moves no
 // other thread touches. Paths rise, so token j comes from place j or behind it: a batch of tokens is read before it is
-// written, and no later one comes from a place that was written before. A few dependent loads (path, table, token)
-// and stores; bound by that chain.
+// written, and no later one comes from a place that was written before. What a thread holds of a batch stands in scratch (144
+// bytes of it), so its tokens are read one after the other, each a chain of four loads (path, two pages, token): 5 tokens of one row in
+// 24 layers 4.4 us, 64 rows in 16 layers (23 MB of tokens read and written, 45 by the counters) 16.
 __global__ __launch_bounds__(kThreads) void keep_tokens_kernel(KeepParams p) {
     constexpr int kTogether = 8;
     const int layer = blockIdx.x, b = blockIdx.y;

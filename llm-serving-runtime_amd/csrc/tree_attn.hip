@@ -8,9 +8,9 @@
 //
 // Bound: few query rows read K and V from HBM (4 D bytes a token and head); 256 query rows need as long for the products,
 // and there the softmax, the addresses and the exchange through LDS come on top, since the waves of a SIMD hide little of each other's.
-// Measured, both launches: 32 rows of U[128, 4096] tokens with 16 nodes (G 4, D 128, 279 MB) 65 us, 4.3 TB/s; one row of 131,071
-// tokens with 25 nodes (537 MB) 111 us, 4.8 TB/s; 8 rows of U[4096, 8192] tokens with 64 nodes 78 us, 670 TFLOP/s; two
-// chunks of 509 tokens over U[2048, 4096] 88 us, 690 TFLOP/s; one row of 705 tokens with 5 nodes 16 us.
+// Measured, a call: 32 rows of U[128, 4096] tokens with 16 nodes (G 4, D 128, 279 MB) 65 us, 4.3 TB/s; one row of 131,071
+// tokens with 25 nodes (537 MB) 113 us, 4.7 TB/s; 8 rows of U[4096, 8192] tokens with 64 nodes (52 GFLOP) 80 us, 645 TFLOP/s;
+// two chunks of 509 tokens over U[2048, 4096] (55 GFLOP) 79 us, 700 TFLOP/s; one row of 705 tokens with 5 nodes 16 us.
 //
 // Work decomposition. The G * T query rows of a (row, kv-head) share its K and V. A segment is a (row, kv-head,
 // tile of R query rows), heads of a node next to each other; it holds ceil(visible tokens / 64) tiles. All segments form
@@ -27,7 +27,9 @@
 // dim of the 4 tokens. So probabilities never leave their lane, and V needs no transposed copy.
 //
 // The softmax is the online one in fp32 on the exp2 scale; the reference maximum moves only when it would rise by more than
-// 2^8. p enters the second product rounded to the element type, and l sums the rounded values.
+// 2^8. p enters the second product rounded to the element type, the only operand that the matrix cores take beside such V (in 32 bits
+// a product runs at a sixteenth of the rate), and l sums the rounded values, so the weights still add up to 1: 2.2e-4 to 2.9e-4
+// of the outputs' norm off in fp16 and 1.8e-3 to 2.2e-3 in bf16, where rounding the output alone is 2.1e-4 and 1.7e-3.
 //
 // Masked places have no effect whatever they hold: scores of invisible tokens are replaced by -inf, V of tokens past the end or
 // of blocks outside the pool is staged as 0, and V of a drafted token that is not finite reaches only

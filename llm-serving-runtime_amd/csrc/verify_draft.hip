@@ -8,9 +8,11 @@
 // sum of 1. Where no child is taken the following token is drawn from r. That gives tokens of the target's own
 // distribution whatever the draft was.
 //
-// All of it in 64 bits: an answer is a whole number, and a sum over 10^5 terms in 32 bits would put a border of the
-// running sum on the other side of a uniform number in one draw of some hundred. fp64 arithmetic is what bounds a pass over
-// a vocabulary (about 25 instructions per logit), so only the nodes that a path visits are read.
+// All of it in 64 bits (sums that workgroups exchange keep 44 of their 52): an answer is a whole number, and a sum over 10^5 terms in
+// 32 bits would put a border of the running sum on the other side of a uniform number in one draw of some hundred. A pass over
+// a vocabulary takes 27 vector instructions per logit with everything, 18 of them for the exponential and its sum: 2 to 5 us of
+// its 10 over a slice. The rest is the exchange and the decision behind it (32 rows of 16 nodes: the walk's waves wait in 72 % of
+// their cycles), so only the nodes that a path visits are read.
 //
 // A row of the batch is walked by S workgroups together, each of which owns a slice of the vocabulary. A pass over a
 // node's logits ends in one partial per slice (a sum and what it is relative to); every workgroup reads all partials
@@ -21,8 +23,9 @@
 // past the L2s (relaxed atomics of agent scope), so that a word says by itself whether it is the one waited for: no
 // fence, no counter, one round trip. Words of odd and even passes stand apart, since a workgroup is at most one pass
 // ahead of another of its row, and so do those of passes over a node and of refusals, each numbered by itself: what a word
-// held before is then always two passes older, and a number taken modulo 255 tells the two apart. Every wait ends: workgroups take their row and slice from a counter as they start, so all rows
-// but the last one started have all their workgroups running, finish, and make room for what the last one lacks.
+// held before is then always two passes older, and a number taken modulo 255 tells the two apart. Every wait ends: workgroups
+// take their row and slice from a counter as they start, so all rows but the last one started have all their workgroups
+// running, finish, and make room for what the last one lacks.
 #include "common.h"
 
 namespace mx {
@@ -175,7 +178,7 @@ __device__ __forceinline__ double weight(float l, float ref, double c) {
 }
 
 // The same for whole slices, from a table of 2^(k / 128) in LDS: 2^t = 2^(n / 128) 2^(f / 128), |f| <= 1/2, four terms of the
-// series (the next one is below 2e-15). All instructions cost alike here, fp64 or not: about 19 a logit.
+// series (the next one is below 2e-15). All instructions cost alike here, fp64 or not: 18 a logit with the sum.
 constexpr int kTable = 128;  // 2^7
 struct Exp {
     const double* table;

@@ -250,7 +250,8 @@ def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, tree: DraftTree, un
     ``r = max(r - q, 0)`` (without draft logits: ``r`` without ``x``), scaled to a sum of 1. Where none is kept
     the following token is drawn from ``r``: the first whose running sum exceeds ``uniforms[node 0]``. So the
     tokens are distributed as the target's own samples. At temperature 0 (or below) ``r`` is all at the largest
-    logit, the first on ties: greedy decoding. The arithmetic is in 64 bits.
+    logit, the first on ties: greedy decoding. The arithmetic is in 64 bits (sums over parts of the vocabulary are
+    joined with 44 of their 52).
 
     A drafted token outside the vocabulary is not kept. A node whose logits hold a NaN, nothing above -inf or
     (with a temperature) +inf keeps nothing and is followed by -1.
