@@ -28,7 +28,7 @@
 //
 // The softmax is the online one in fp32 on the exp2 scale; the reference maximum moves only when it would rise by more than
 // 2^8. p enters the second product rounded to the element type, the only operand that the matrix cores take beside such V (in 32 bits
-// a product runs at a sixteenth of the rate), and l sums the rounded values, so the weights still add up to 1: 2.2e-4 to 2.9e-4
+// a product runs at a sixteenth of the rate), and l sums the rounded values, so the weights still add up to 1: 2.2e-4 to 2.8e-4
 // of the outputs' norm off in fp16 and 1.8e-3 to 2.2e-3 in bf16, where rounding the output alone is 2.1e-4 and 1.7e-3.
 //
 // Masked places have no effect whatever they hold: scores of invisible tokens are replaced by -inf, V of tokens past the end or

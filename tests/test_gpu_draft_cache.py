@@ -265,7 +265,7 @@ def test_decode_steps_between_drafts(model):
     cache, want = _prompts(model)
     tree = DraftTree.from_parents([-1, 0, 0, 2], DEV)
     at = 0  # tokens of `want` in the cache
-    for turn in range(3):
+    for _ in range(3):
         # the second branch is the answer, the first one is not; of the answer's two nodes one is kept
         tokens = torch.tensor([[w[at], (w[at + 1] + 1) % 1024, w[at + 1], w[at + 2]] for w in want], device=DEV)
         logits = paged_draft_step(model, cache, tokens, tree)
@@ -336,3 +336,47 @@ def test_a_gradient_is_refused_and_not_lost():
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda x: paged_attention_tree(x, meta, 2, 0.125))(q.unsqueeze(0))
     assert torch.equal(paged_attention_tree(q, meta, 2, 0.125), want)
+
+
+def test_a_captured_step_drafts_verifies_and_keeps(model):
+    """One graph of the whole step over a cache whose lengths advance in place, replayed with eager work between."""
+    from runtime_amd.phase2.hf_decode import paged_draft_step
+    from runtime_amd.phase2.speculative import verify_draft
+
+    cache, want = _prompts(model)
+    cache._graph_safe, cache._cached_seq_len_py = True, None
+    tree = DraftTree.from_parents([-1, 0, 0, 2], DEV)
+    tokens, u = torch.zeros(2, 4, dtype=torch.int64, device=DEV), torch.full((2, 4), 0.5, device=DEV)
+    lens = cache.seq_lens.clone()
+
+    def step():
+        verdict = verify_draft(paged_draft_step(model, cache, tokens, tree), tokens, tree, u, 0.0)
+        cache.keep_drafted(verdict.path, verdict.counts)
+        return verdict
+
+    def draft(at):  # the answer by the second branch; for the second row its last node is another token
+        tokens.copy_(torch.tensor([[w[a], (w[a + 1] + 1) % 1024, w[a + 1], (w[a + 2] + i) % 1024]
+                                   for i, (a, w) in enumerate(zip(at, want))], device=DEV))
+
+    side = torch.cuda.Stream()
+    draft([0, 0])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        step()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            verdict = step()
+    torch.cuda.synchronize()
+    for target in (cache, *cache.layers):
+        getattr(target, "seq_lens" if target is cache else "_row_seq_lens").copy_(lens)
+    at = [0, 0]
+    for _ in range(3):
+        draft(at)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert verdict.counts.tolist() == [3, 2] and verdict.path.tolist() == [[0, 2, 3, -1], [0, 2, -1, -1]]
+        assert verdict.tokens.tolist() == [want[0][at[0] + 1:at[0] + 4] + [-1], want[1][at[1] + 1:at[1] + 3] + [-1, -1]]
+        at = [at[0] + 3, at[1] + 2]
+        assert cache.seq_lens.tolist() == [n + a for n, a in zip(lens.tolist(), at)]
+    cache.pool.check_write_errors()
